@@ -152,6 +152,55 @@ int spaceslug_q4_weights_lora_adamw(spaceslug_q4_weights* w, float learning_rate
 int spaceslug_q4_weights_get_lora(const spaceslug_q4_weights* w, float* a_out, float* b_out, float* da_out,
                                   float* db_out);
 
+/* ---- Training through the frozen weights (no counterpart in the reference) ----
+ * Element type of x, dy and dx in the calls below. */
+#define SPACESLUG_F32 0
+#define SPACESLUG_BF16 1
+
+/* Activations kept in 8 bits between the forward and the backward: x [m x k]
+ * (k % 32 == 0) becomes int8 codes [m x k] and one step byte per 32 values of a
+ * row, exps [m x k/32]; the value kept is codes * 2^(exps - 127).  The step is
+ * the smallest power of two of which the group's largest magnitude takes at
+ * most 127 (never below 2^-126), so a value is off by at most half a step
+ * (magnitudes above 63.5 * 2^122, which would restore as an infinity: by up to
+ * one), and the restored value is exact in bf16.  A group with an infinity or a NaN comes
+ * back as NaN.  Device pointers, x and codes 16-byte aligned, asynchronous on
+ * `stream`, m * k <= 2^40; works in CUDA graph capture. */
+int spaceslug_act8_pack_device(const void* x, int dtype, int8_t* codes, uint8_t* exps, uint32_t m, uint32_t k,
+                               void* stream);
+/* x = codes * 2^(exps - 127), the values the backward uses. */
+int spaceslug_act8_unpack_device(const int8_t* codes, const uint8_t* exps, void* x, int dtype, uint32_t m, uint32_t k,
+                                 void* stream);
+/* spaceslug_q4_weights_lora_backward with X from its 8-bit form (codes [m x k],
+ * exps [m x k/32]) and dY [m x (col_end - col_begin)] in `dtype`; codes and dy
+ * 16-byte aligned.  The gradients (fp32) stay in the handle as there; da
+ * [k x rank] and db [rank x columns], where given (device pointers), receive a
+ * copy.  The first backward of a handle allocates its gradients: make it before
+ * any stream capture. */
+int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps,
+                                            const void* dy, int dtype, uint32_t m, float* da, float* db, void* stream);
+/* dX = dY * dequant(W)^T + (alpha / rank) * (dY * B^T) * A^T [m x k] for the
+ * handle's columns and adapter (if one is attached), dY [m x (col_end -
+ * col_begin)], both of `dtype`, 16-byte aligned; dx must not overlap dy.  For a
+ * column shard dX is this shard's partial sum.  fp32 at fp32-level accuracy;
+ * bf16 products of f16 operands summed in fp32, rounded once. */
+int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, int dtype, uint32_t m,
+                                        void* stream);
+/* Softmax cross entropy of the logits z = X * dequant(W) over the handle's
+ * columns (a whole vocabulary; a handle with an adapter attached is refused),
+ * without keeping the logits:
+ *   lse[i] = log sum_v exp z[i][v],  loss[i] = lse[i] - z[i][targets[i]],
+ *   dx[i] = row_scale[i] * (softmax(z[i]) - onehot(targets[i])) * dequant(W)^T.
+ * x [m x k] and dx [m x k] of `dtype`, 16-byte aligned; targets int64 [m];
+ * row_scale fp32 [m] (the upstream gradient of each row's loss; NULL: all 1);
+ * loss fp32 [m]; lse fp32 [m] or NULL; dx or NULL (the loss alone).  A negative
+ * target takes its row out: loss 0, dx 0 (lse is still written).  A target past
+ * the columns gives NaN in its row's loss and dx.  dx may be x itself.  Device
+ * pointers, asynchronous on `stream`; scratch from the stream-ordered pool. */
+int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, int dtype, const int64_t* targets,
+                                       const float* row_scale, float* loss, float* lse, void* dx, uint32_t m,
+                                       void* stream);
+
 /* The reference's hidden-64 training ABI, same contracts and return codes:
  * dA = X^T dY B^T and dB = (X A)^T dY for X/dY [m x 64], A [64 x rank],
  * B [rank x 64], 1 <= m <= 128, 1 <= rank <= 8 (lora_gradients_api.h:4-6);

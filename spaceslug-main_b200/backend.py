@@ -79,6 +79,11 @@ _SIGNATURES = {
     "spaceslug_q4_weights_lora_sgd": ([_vp, ctypes.c_float, _vp], ctypes.c_int),
     "spaceslug_q4_weights_lora_adamw": ([_vp, ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                          ctypes.c_float, _vp], ctypes.c_int),
+    "spaceslug_act8_pack_device": ([_vp, ctypes.c_int, _vp, _vp, _u32, _u32, _vp], ctypes.c_int),
+    "spaceslug_act8_unpack_device": ([_vp, _vp, _vp, ctypes.c_int, _u32, _u32, _vp], ctypes.c_int),
+    "spaceslug_q4_weights_lora_backward_act8": ([_vp, _vp, _vp, _vp, ctypes.c_int, _u32, _vp, _vp, _vp], ctypes.c_int),
+    "spaceslug_q4_weights_input_gradient": ([_vp, _vp, _vp, ctypes.c_int, _u32, _vp], ctypes.c_int),
+    "spaceslug_q4_weights_cross_entropy": ([_vp, _vp, ctypes.c_int, _vp, _vp, _vp, _vp, _vp, _u32, _vp], ctypes.c_int),
     "spaceslug_q4_weights_get_lora": ([_vp, _f32p, _f32p, _f32p, _f32p], ctypes.c_int),
     "spaceslug_cq4_weights_create": ([_vp, ctypes.c_int, ctypes.POINTER(_vp)], ctypes.c_int),
     "spaceslug_cq4_matmul": ([_vp, _vp, _vp, _u32, _vp], ctypes.c_int),
@@ -102,7 +107,14 @@ _CAPABILITIES = {
     "spaceslug_lora_train_step": "lora_train_step_abi",
     "spaceslug_sgemm": "sgemm",
     "spaceslug_q4_weights_lora_backward": "lora_training",
+    "spaceslug_act8_pack_device": "act8_checkpoint",
+    "spaceslug_q4_weights_lora_backward_act8": "lora_training_act8",
+    "spaceslug_q4_weights_input_gradient": "q4_input_gradient",
+    "spaceslug_q4_weights_cross_entropy": "q4_cross_entropy",
 }
+
+# element types of the training calls (SPACESLUG_F32 / SPACESLUG_BF16)
+_DTYPES = {"f32": 0, "bf16": 1}
 
 
 class CQ4Matrix(ctypes.Structure):
@@ -130,6 +142,12 @@ def _arr(a, dtype) -> np.ndarray:
 
 def _p(a: np.ndarray, typ):
     return a.ctypes.data_as(typ)
+
+
+def _dtype(name: str) -> int:
+    if name not in _DTYPES:
+        raise BackendError(f"dtype must be one of {sorted(_DTYPES)}, not {name!r}")
+    return _DTYPES[name]
 
 
 class BackendSession:
@@ -234,6 +252,15 @@ class BackendSession:
 
     def q4_pack_device(self, w_kn: int, k: int, n: int, packed: int, stream: int = 0) -> None:
         self._call("spaceslug_q4_pack_device", w_kn, k, n, packed, stream or None)
+
+    def act8_pack_device(self, x: int, codes: int, exps: int, m: int, k: int, dtype: str = "f32",
+                         stream: int = 0) -> None:
+        """x [m, k] (dtype) -> int8 codes [m, k] and step bytes [m, k/32]: x is kept as codes * 2^(exps - 127)."""
+        self._call("spaceslug_act8_pack_device", x, _dtype(dtype), codes, exps, m, k, stream or None)
+
+    def act8_unpack_device(self, codes: int, exps: int, x: int, m: int, k: int, dtype: str = "f32",
+                           stream: int = 0) -> None:
+        self._call("spaceslug_act8_unpack_device", codes, exps, x, _dtype(dtype), m, k, stream or None)
 
     def set_operand_type(self, kind: str) -> str:
         prev = self.raw("spaceslug_q4_set_operand_type")({"f16": 0, "bf16": 1}[kind])
@@ -401,6 +428,24 @@ class Q4Weights:
     # ---- LoRA training (device pointers, asynchronous) ----
     def lora_backward(self, x: int, dy: int, m: int, stream: int = 0) -> None:
         self.session._call("spaceslug_q4_weights_lora_backward", self.handle, x, dy, m, stream or None)
+
+    def lora_backward_act8(self, codes: int, exps: int, dy: int, m: int, dtype: str = "f32", da: int = 0, db: int = 0,
+                           stream: int = 0) -> None:
+        """lora_backward with X kept in 8 bits (act8_pack_device) and dY in `dtype`; da [k, r] and db [r, n]
+        (device, fp32) receive a copy of the gradients where given."""
+        self.session._call("spaceslug_q4_weights_lora_backward_act8", self.handle, codes, exps, dy, _dtype(dtype), m,
+                           da or None, db or None, stream or None)
+
+    def input_gradient(self, dy: int, dx: int, m: int, dtype: str = "f32", stream: int = 0) -> None:
+        """dX [m, k] = dY W^T + (alpha/r) (dY B^T) A^T, both of `dtype`."""
+        self.session._call("spaceslug_q4_weights_input_gradient", self.handle, dy, dx, _dtype(dtype), m, stream or None)
+
+    def cross_entropy(self, x: int, targets: int, loss: int, m: int, lse: int = 0, dx: int = 0, row_scale: int = 0,
+                      dtype: str = "f32", stream: int = 0) -> None:
+        """loss [m] (and lse [m], dx [m, k]) of the logits X W over the handle's columns; targets int64 [m], negative:
+        the row is left out; row_scale fp32 [m]: the upstream gradient of each row's loss (0: all 1)."""
+        self.session._call("spaceslug_q4_weights_cross_entropy", self.handle, x, _dtype(dtype), targets,
+                           row_scale or None, loss, lse or None, dx or None, m, stream or None)
 
     def lora_sgd(self, learning_rate: float, stream: int = 0) -> None:
         self.session._call("spaceslug_q4_weights_lora_sgd", self.handle, float(learning_rate), stream or None)

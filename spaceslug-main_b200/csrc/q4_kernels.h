@@ -301,4 +301,26 @@ int launch_sgemm_pair(const SgemmTcArgs& a, int max_pairs, cudaStream_t stream);
 int launch_lora_delta64(const float* x, const float* a, const float* b, float* y, int M, int rank,
                         cudaStream_t stream);
 
+// Activations kept in 8 bits (act8.cu): int8 codes and one step byte (2^(byte - 127)) per 32 values of a contiguous
+// [m][K] matrix, K % 32 == 0, seen as a flat list of groups.
+int launch_act8_pack(const void* x, bool bf16, int8_t* codes, uint8_t* exps, long long groups, cudaStream_t stream);
+int launch_act8_unpack(const int8_t* codes, const uint8_t* exps, void* x, bool bf16, long long groups,
+                       cudaStream_t stream);
+int launch_bf16_to_f32(const void* x, float* y, long long count, cudaStream_t stream);
+// The training operators for a few rows (q4_rows.cu), any M; x, dy and out are fp32 or bf16, 16-byte aligned.
+int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, float* z, long long ld_z,
+                       int M, int N, int K, cudaStream_t stream);
+int rows_wt_splits(int M, int N, int K, int sm_count);
+// partial[splits][M][K] of sum_n d[m][n] w(k, n)
+int launch_rows_wt(const void* d, bool bf16, long long ld_d, const uint32_t* packed, const float* scales,
+                   float* partial, int splits, int M, int N, int K, cudaStream_t stream);
+// lse, loss and (want_grad) d = row_scale (softmax - onehot) of M logit rows, in place
+int launch_rows_softmax(float* z, long long ld_z, const long long* targets, const float* row_scale, float* loss,
+                        float* lse, int M, int N, bool want_grad, cudaStream_t stream);
+// G[m][j] = sum_n dy[m][n] B[j][n]
+int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int M, int N, int rank, cudaStream_t stream);
+// out = sum of the splits in order + s G A^T (A [K][rank]; rank 0: none)
+int launch_rows_finish(const float* partial, int splits, const float* g, const float* a, int rank, float s, void* out,
+                       bool bf16, int M, int K, cudaStream_t stream);
+
 }  // namespace q4

@@ -1100,6 +1100,121 @@ void run_cq4(const spaceslug_cq4_weights& w, const void* a, void* c, int M, cuda
 
 }  // namespace
 
+namespace {
+
+// Makes `device` current for one call and gives the caller's back.
+struct DeviceGuard {
+    int prev = 0;
+    bool moved = false;
+    explicit DeviceGuard(int device) {
+        prev = current_device();
+        if (prev != device) {
+            check(cudaSetDevice(device), "cudaSetDevice");
+            moved = true;
+        }
+    }
+    ~DeviceGuard() {
+        if (moved) cudaSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+// The device that holds p.
+int pointer_device(const void* p) {
+    cudaPointerAttributes a{};
+    check(cudaPointerGetAttributes(&a, p), "cudaPointerGetAttributes");
+    if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) throw CudaError("not device memory");
+    return a.device;
+}
+
+const char* act8_error(const void* x, int dtype, const void* codes, const void* exps, uint32_t m, uint32_t k) {
+    if (!x || !codes || !exps) return "null pointer";
+    if (dtype != SPACESLUG_F32 && dtype != SPACESLUG_BF16) return "dtype must be SPACESLUG_F32 or SPACESLUG_BF16";
+    if (m == 0 || k == 0 || k % 32u) return "m must be positive and k a positive multiple of 32";
+    if (m > (1u << 30) || k > (1u << 30) || static_cast<uint64_t>(m) * k > (uint64_t(1) << 40)) return "m or k too large";
+    if (!aligned16(x) || !aligned16(codes)) return "activations and codes must be 16-byte aligned";
+    return nullptr;
+}
+
+const char* rows_error(const void* in, const void* out, int dtype, uint32_t m) {
+    if (dtype != SPACESLUG_F32 && dtype != SPACESLUG_BF16) return "dtype must be SPACESLUG_F32 or SPACESLUG_BF16";
+    if (m == 0 || m > (1u << 24)) return "m must be 1 .. 2^24";
+    if (!aligned16(in) || !aligned16(out)) return "x, dy and dx must be 16-byte aligned";
+    return nullptr;
+}
+
+// The adapter's gradients of fp32 X and dY into the handle.
+void lora_backward_f32(spaceslug_q4_weights* w, const float* x, const float* dy, int M, cudaStream_t s) {
+    q4::LoraBackwardArgs g{x, dy, w->lora_a, w->lora_b, w->lora_da, w->lora_db, nullptr,
+                           M, w->K, w->N, w->rank, w->alpha / static_cast<float>(w->rank)};
+    if (lora_backward_tc_suits(g)) {
+        DeviceCtx& c = ctx_for(w->device);
+        run_lora_backward_tc(g, c.sm_count, c.status, s);
+    } else {
+        Scratch sc(q4::lora_backward_scratch_floats(M, w->K, w->N, w->rank) * 4, s);
+        g.scratch = static_cast<float*>(sc.p);
+        check_launch(q4::launch_lora_backward(g, s), "lora backward");
+    }
+}
+
+// dX = dY W^T + s (dY B^T) A^T.  The rows go in blocks whose split sums fit 256 MB.
+void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
+    DeviceCtx& c = ctx_for(w->device);
+    const size_t size = bf16 ? 2 : 4;
+    const int block = static_cast<int>(std::clamp<long long>((64ll << 20) / w->K / 8 * 8, 8, 1 << 18));
+    for (int m0 = 0; m0 < M; m0 += block) {
+        const int mc = std::min(block, M - m0);
+        const int splits = q4::rows_wt_splits(mc, w->N, w->K, c.sm_count);
+        Scratch part(static_cast<size_t>(splits) * mc * w->K * 4, s);
+        Scratch gs(static_cast<size_t>(mc) * w->rank * 4, s);
+        const void* d = static_cast<const char*>(dy) + static_cast<size_t>(m0) * w->N * size;
+        if (w->rank > 0)
+            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, static_cast<float*>(gs.p), mc, w->N, w->rank, s),
+                         "dY B^T");
+        check_launch(q4::launch_rows_wt(d, bf16, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, mc,
+                                        w->N, w->K, s),
+                     "dY W^T");
+        check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<float*>(gs.p), w->lora_a,
+                                            w->rank, w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f,
+                                            static_cast<char*>(dx) + static_cast<size_t>(m0) * w->K * size, bf16, mc,
+                                            w->K, s),
+                     "dX");
+    }
+}
+
+// Loss and gradient, the logits of at most 256 MB of rows at a time.
+void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const int64_t* targets,
+                       const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
+    DeviceCtx& c = ctx_for(w->device);
+    const size_t size = bf16 ? 2 : 4;
+    const int block = static_cast<int>(std::clamp<long long>((64ll << 20) / w->N / 8 * 8, 8, 1 << 18));
+    for (int m0 = 0; m0 < M; m0 += block) {
+        const int mc = std::min(block, M - m0);
+        Scratch zs(static_cast<size_t>(mc) * w->N * 4, s);
+        float* z = static_cast<float*>(zs.p);
+        check_launch(q4::launch_rows_logits(static_cast<const char*>(x) + static_cast<size_t>(m0) * w->K * size, bf16,
+                                            w->packed, w->scales, z, w->N, mc, w->N, w->K, s),
+                     "logits");
+        check_launch(q4::launch_rows_softmax(z, w->N, reinterpret_cast<const long long*>(targets) + m0,
+                                             row_scale ? row_scale + m0 : nullptr, loss + m0, lse ? lse + m0 : nullptr,
+                                             mc, w->N, dx != nullptr, s),
+                     "softmax");
+        if (!dx) continue;
+        const int splits = q4::rows_wt_splits(mc, w->N, w->K, c.sm_count);
+        Scratch part(static_cast<size_t>(splits) * mc * w->K * 4, s);
+        check_launch(q4::launch_rows_wt(z, false, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, mc,
+                                        w->N, w->K, s),
+                     "dZ W^T");
+        check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, nullptr, nullptr, 0, 0.0f,
+                                            static_cast<char*>(dx) + static_cast<size_t>(m0) * w->K * size, bf16, mc,
+                                            w->K, s),
+                     "dX");
+    }
+}
+
+}  // namespace
+
 extern "C" {
 
 int spaceslug_vector_add(const float* left, const float* right, float* output, size_t count) {
@@ -1755,16 +1870,85 @@ int spaceslug_q4_weights_lora_backward(spaceslug_q4_weights* w, const float* x, 
         const size_t pa = static_cast<size_t>(w->K) * w->rank * 4, pbb = static_cast<size_t>(w->rank) * w->N * 4;
         if (!w->lora_da) check(cudaMalloc(&w->lora_da, pa), "cudaMalloc dA");
         if (!w->lora_db) check(cudaMalloc(&w->lora_db, pbb), "cudaMalloc dB");
-        q4::LoraBackwardArgs g{x, dy, w->lora_a, w->lora_b, w->lora_da, w->lora_db, nullptr,
-                               static_cast<int>(m), w->K, w->N, w->rank, w->alpha / static_cast<float>(w->rank)};
-        if (lora_backward_tc_suits(g)) {
-            DeviceCtx& c = ctx_for(w->device);
-            run_lora_backward_tc(g, c.sm_count, c.status, s);
-        } else {
-            Scratch sc(q4::lora_backward_scratch_floats(static_cast<int>(m), w->K, w->N, w->rank) * 4, s);
-            g.scratch = static_cast<float*>(sc.p);
-            check_launch(q4::launch_lora_backward(g, s), "lora backward");
-        }
+        lora_backward_f32(w, x, dy, static_cast<int>(m), s);
+        return SPACESLUG_OK;
+    });
+}
+
+int spaceslug_act8_pack_device(const void* x, int dtype, int8_t* codes, uint8_t* exps, uint32_t m, uint32_t k,
+                               void* stream) {
+    if (const char* e = act8_error(x, dtype, codes, exps, m, k)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    return guarded([&] {
+        DeviceGuard dev(pointer_device(x));
+        check_launch(q4::launch_act8_pack(x, dtype == SPACESLUG_BF16, codes, exps,
+                                          static_cast<long long>(m) * (k / 32u), static_cast<cudaStream_t>(stream)),
+                     "act8 pack");
+        return SPACESLUG_OK;
+    });
+}
+
+int spaceslug_act8_unpack_device(const int8_t* codes, const uint8_t* exps, void* x, int dtype, uint32_t m, uint32_t k,
+                                 void* stream) {
+    if (const char* e = act8_error(x, dtype, codes, exps, m, k)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    return guarded([&] {
+        DeviceGuard dev(pointer_device(x));
+        check_launch(q4::launch_act8_unpack(codes, exps, x, dtype == SPACESLUG_BF16,
+                                            static_cast<long long>(m) * (k / 32u), static_cast<cudaStream_t>(stream)),
+                     "act8 unpack");
+        return SPACESLUG_OK;
+    });
+}
+
+int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps,
+                                            const void* dy, int dtype, uint32_t m, float* da, float* db, void* stream) {
+    if (!w || !dy) return fail(SPACESLUG_INVALID_ARGUMENT, "null pointer");
+    if (const char* e = act8_error(dy, dtype, codes, exps, m, static_cast<uint32_t>(w->K)))
+        return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    if (w->rank == 0) return fail(SPACESLUG_INVALID_ARGUMENT, "no LoRA adapter attached");
+    return guarded([&] {
+        DeviceGuard dev(w->device);
+        const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const size_t pa = static_cast<size_t>(w->K) * w->rank * 4, pbb = static_cast<size_t>(w->rank) * w->N * 4;
+        if (!w->lora_da) check(cudaMalloc(&w->lora_da, pa), "cudaMalloc dA");
+        if (!w->lora_db) check(cudaMalloc(&w->lora_db, pbb), "cudaMalloc dB");
+        const int M = static_cast<int>(m);
+        // X (and a bf16 dY) restored in fp32, then the fp32 backward
+        Scratch xs(static_cast<size_t>(M) * w->K * 4, s);
+        Scratch ys(dtype == SPACESLUG_BF16 ? static_cast<size_t>(M) * w->N * 4 : 0, s);
+        check_launch(q4::launch_act8_unpack(codes, exps, xs.p, false, static_cast<long long>(M) * (w->K / 32), s),
+                     "act8 unpack");
+        if (ys.p)
+            check_launch(q4::launch_bf16_to_f32(dy, static_cast<float*>(ys.p), static_cast<long long>(M) * w->N, s),
+                         "bf16 to f32");
+        lora_backward_f32(w, static_cast<const float*>(xs.p), ys.p ? static_cast<const float*>(ys.p)
+                                                                    : static_cast<const float*>(dy), M, s);
+        if (da) check(cudaMemcpyAsync(da, w->lora_da, pa, cudaMemcpyDeviceToDevice, s), "copy dA");
+        if (db) check(cudaMemcpyAsync(db, w->lora_db, pbb, cudaMemcpyDeviceToDevice, s), "copy dB");
+        return SPACESLUG_OK;
+    });
+}
+
+int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, int dtype, uint32_t m,
+                                        void* stream) {
+    if (!w || !dy || !dx) return fail(SPACESLUG_INVALID_ARGUMENT, "null pointer");
+    if (const char* e = rows_error(dy, dx, dtype, m)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    return guarded([&] {
+        DeviceGuard dev(w->device);
+        run_input_gradient(w, dy, dx, dtype == SPACESLUG_BF16, static_cast<int>(m), static_cast<cudaStream_t>(stream));
+        return SPACESLUG_OK;
+    });
+}
+
+int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, int dtype, const int64_t* targets,
+                                       const float* row_scale, float* loss, float* lse, void* dx, uint32_t m,
+                                       void* stream) {
+    if (!w || !x || !targets || !loss) return fail(SPACESLUG_INVALID_ARGUMENT, "null pointer");
+    if (const char* e = rows_error(x, dx, dtype, m)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    if (w->rank != 0) return fail(SPACESLUG_INVALID_ARGUMENT, "cross entropy takes a handle without an adapter");
+    return guarded([&] {
+        DeviceGuard dev(w->device);
+        run_cross_entropy(w, x, dtype == SPACESLUG_BF16, targets, row_scale, loss, lse, dx, static_cast<int>(m),
+                          static_cast<cudaStream_t>(stream));
         return SPACESLUG_OK;
     });
 }

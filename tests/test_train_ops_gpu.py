@@ -1,0 +1,510 @@
+"""GPU: training through frozen int4 weights (activations kept in 8 bits, the adapter's gradients from them, the input
+gradient, softmax cross entropy over a vocabulary) against 64-bit restatements.
+
+Tolerances.  S = sum |a||b| over a product's terms, in 64 bits.
+  fp32: operands to 2^-21, and sums of rounded terms whose chains are at most 255 long: |error| <= 2^-16 S.
+  bf16: one operand rounded to f16 (2^-11 of each term), the result to bf16 (2^-8 of it): 2^-11 S + 2^-8 |y| + 2^-16 S.
+Logits are held to the fp32 bound for both types: dz = 2^-16 max_v S.  Then lse is off by dz + 2^-20 (1 + |lse|), a loss
+by twice that, a probability by 2 dz + 2^-16 of itself.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from spaceslug_b200 import synth
+
+pytestmark = pytest.mark.gpu
+DT = ("f32", "bf16")
+
+
+def _dt(name):
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16}[name]
+
+
+def _w64(packed, scales, k, n, cuda):
+    """W [k, n] in 64 bits from the layout's bytes."""
+    import torch
+    by = torch.from_numpy(np.ascontiguousarray(packed).view(np.uint8).reshape(n, k // 2)).to(cuda).to(torch.int64)
+    v = torch.stack((by % 16, by // 16), -1).flatten(1)
+    v = torch.where(v > 7, v - 16, v).double()
+    sc = torch.from_numpy(np.ascontiguousarray(scales).reshape(n, k // 32)).to(cuda).double()
+    return (v * sc.repeat_interleave(32, 1)).T
+
+
+def _weights(k, n, seed, lo=0.005, hi=0.02):
+    _, packed, scales = synth.make_weights(k, n, lo, hi, seed=seed)
+    return packed, scales
+
+
+def _randn(shape, cuda, seed):
+    import torch
+    return torch.randn(shape, device=cuda, generator=torch.Generator(device=cuda).manual_seed(seed))
+
+
+# ---------------------------------------------------------------------------------------------------- 8-bit copies --
+def _act8_oracle(x):
+    """codes and step bytes of fp32 numpy [m, k] by exact 64-bit arithmetic."""
+    m, k = x.shape
+    g = x.astype(np.float64).reshape(m, k // 32, 32)
+    top = np.abs(g).max(-1)
+    e = np.full(top.shape, -126, np.int64)
+    fin = np.isfinite(top)
+    while True:  # the smallest e >= -126 with top <= 127 2^e
+        more = fin & (top > 127.0 * np.exp2(e.astype(np.float64)))
+        if not more.any():
+            break
+        e[more] += 1
+    codes = np.where(fin[..., None], np.rint(np.where(fin[..., None], g, 0.0) / np.exp2(e.astype(np.float64))[..., None]), 0)
+    codes = np.where((e == 122)[..., None], np.clip(codes, -63, 63), codes)  # 64 * 2^122 is no fp32 value
+    return codes.reshape(m, k).astype(np.int8), np.where(fin, e + 127, 255).astype(np.uint8)
+
+
+def _act8(session, x, dtype):
+    import torch
+    m, k = x.shape
+    codes = torch.full((m, k), 77, dtype=torch.int8, device=x.device)
+    exps = torch.full((m, k // 32), 99, dtype=torch.uint8, device=x.device)
+    session.act8_pack_device(x.data_ptr(), codes.data_ptr(), exps.data_ptr(), m, k, dtype=dtype)
+    back = torch.empty_like(x)
+    session.act8_unpack_device(codes.data_ptr(), exps.data_ptr(), back.data_ptr(), m, k, dtype=dtype)
+    return codes, exps, back
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k", [(1, 32), (3, 64), (1, 4096), (129, 4128), (7, 11008)])
+def test_act8_is_the_exact_rounding(session, cuda, m, k, dtype):
+    import torch
+    x = (_randn((m, k), cuda, m + k) * torch.exp2(torch.randint(-20, 20, (m, k // 32), device=cuda).float())
+         .repeat_interleave(32, 1)).to(_dt(dtype))
+    codes, exps, back = _act8(session, x, dtype)
+    c, e = _act8_oracle(x.float().cpu().numpy())
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(exps.cpu().numpy(), e)
+    step = np.exp2(e.astype(np.float64) - 127).repeat(32, 1)
+    assert np.array_equal(back.double().cpu().numpy(), c * step)  # exact in both types
+    assert np.all(np.abs(back.double().cpu().numpy() - x.double().cpu().numpy()) <= step / 2)
+
+
+def test_act8_edges(session, cuda):
+    """Borders of the step rule, zeros, the smallest and largest magnitudes, infinities and NaN (their group alone)."""
+    import torch
+    rows = np.zeros((12, 64), np.float32)
+    rows[0, :3] = 127.0, -127.0, 0.5
+    rows[1, :3] = np.nextafter(np.float32(127.0), np.float32(200.0)), 1.0, 3.0
+    rows[2, :2] = 127.0 * 2.0 ** -40, 2.0 ** -41
+    rows[3, :2] = np.finfo(np.float32).max, 1.0
+    rows[4, :2] = 2.0 ** -140, -(2.0 ** -126)  # below the least step's half, and one step
+    rows[5, 1], rows[5, 40] = np.inf, 3.0
+    rows[6, 33], rows[6, 2] = np.nan, -5.0
+    rows[7, 5], rows[7, 6] = -np.inf, np.inf
+    rows[8, :4] = 64.0, 63.5, 62.5, -61.5  # ties go to even codes
+    rows[9, :] = -0.0
+    rows[10, :32] = 1e-38
+    rows[11, :] = 2.0 ** 100
+    x = torch.from_numpy(rows).to(cuda)
+    codes, exps, back = _act8(session, x, "f32")
+    c, e = _act8_oracle(rows)
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(exps.cpu().numpy(), e)
+    b = back.cpu().numpy()
+    bad = np.repeat(e == 255, 32, 1)
+    assert bad.sum() == 3 * 32 and np.isnan(b[bad]).all()
+    assert np.array_equal(b[~bad].astype(np.float64), (c * np.exp2(e.astype(np.float64) - 127).repeat(32, 1))[~bad])
+
+
+# ------------------------------------------------------------------------------------------- gradients of the adapter --
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,rank,c0,c1", [
+    (1, 64, 256, 4, 0, 256), (33, 512, 700, 5, 100, 600), (128, 256, 160, 8, 0, 160), (300, 1024, 704, 64, 0, 704),
+    (257, 2080, 1001, 33, 0, 1001), (515, 4096, 640, 16, 32, 616), (128, 32, 32, 1, 0, 32)])
+def test_backward_from_8_bits(session, cuda, m, k, n, rank, c0, c1, dtype):
+    import torch
+    packed, scales = _weights(k, n, 3)
+    rng = np.random.default_rng(m + n)
+    A = (rng.standard_normal((k, rank)) * 0.02).astype(np.float32)
+    B = (rng.standard_normal((rank, n)) * 0.02).astype(np.float32)
+    x = _randn((m, k), cuda, 1)
+    dy = _randn((m, c1 - c0), cuda, 2).to(_dt(dtype))
+    codes, exps, back = _act8(session, x, "f32")
+    da = torch.full((k, rank), float("nan"), device=cuda)
+    db = torch.full((rank, c1 - c0), float("nan"), device=cuda)
+    with session.weights(packed, scales, k, n, c0, c1) as h:
+        h.set_lora(A, B, 2.0 * rank)
+        args = (codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m)
+        h.lora_backward_act8(*args, dtype=dtype, da=da.data_ptr(), db=db.data_ptr())
+        _, _, ha, hb = h.get_lora(rank, grads=True)
+        h.lora_backward_act8(*args, dtype=dtype)
+        _, _, ha2, hb2 = h.get_lora(rank, grads=True)
+    assert np.array_equal(ha, da.cpu().numpy()) and np.array_equal(hb, db.cpu().numpy())
+    assert np.array_equal(ha, ha2) and np.array_equal(hb, hb2)  # sums in a fixed order
+    X, D = back.double(), dy.double()
+    A64, B64 = torch.from_numpy(A).to(cuda).double(), torch.from_numpy(np.ascontiguousarray(B[:, c0:c1])).to(cuda).double()
+    for got, ref, S in ((da, 2.0 * X.T @ (D @ B64.T), 2.0 * X.abs().T @ (D.abs() @ B64.abs().T)),
+                        (db, 2.0 * (X @ A64).T @ D, 2.0 * (X.abs() @ A64.abs()).T @ D.abs())):
+        # two chained products, each to 2^-16 of its S
+        assert ((got.double() - ref).abs() <= 2 * 2.0 ** -16 * S).all()
+        assert (got.double() - ref).norm() <= 1e-5 * ref.norm()
+    assert session.device_status(0) == 0
+
+
+def test_backward_from_8_bits_spreads_nan_and_steps(session, cuda):
+    """A NaN group of X reaches its 32 rows of dA and (through T) dB, no other row of dA; groups whose steps are far
+    apart stay exact."""
+    import torch
+    m, k, n, rank = 160, 256, 96, 8
+    packed, scales = _weights(k, n, 5)
+    A, B = np.full((k, rank), 0.01, np.float32), np.full((rank, n), 0.02, np.float32)
+    x = _randn((m, k), cuda, 3) * torch.exp2(torch.randint(-30, 30, (k // 32,), device=cuda).float()).repeat_interleave(32)
+    clean = x.clone()
+    x[7, 70] = float("nan")
+    dy = _randn((m, n), cuda, 4)
+    out = []
+    with session.weights(packed, scales, k, n) as h:
+        h.set_lora(A, B, float(rank))
+        for v in (clean, x):
+            codes, exps, _ = _act8(session, v, "f32")
+            h.lora_backward_act8(codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m)
+            out.append(h.get_lora(rank, grads=True)[2:])
+        codes, exps, back = _act8(session, clean, "f32")
+    # two chained products, each to 2^-16 of its S (a row's terms may cancel: S, not the result, bounds the error)
+    B64 = torch.from_numpy(B).to(cuda).double()
+    ref = (back.double().T @ (dy.double() @ B64.T)).cpu().numpy()
+    S = (back.double().abs().T @ (dy.double().abs() @ B64.abs().T)).cpu().numpy()
+    assert np.all(np.abs(out[0][0] - ref) <= 2 * 2.0 ** -16 * S)
+    assert np.isnan(out[1][0][64:96]).all() and np.isnan(out[1][1]).all()
+    keep = np.r_[0:64, 96:256]
+    assert np.array_equal(out[1][0][keep], out[0][0][keep])
+
+
+# ------------------------------------------------------------------------------------------------------ dX of a layer --
+def _check_dx(got, dtype, ref, S):
+    import torch
+    err = (got.double() - ref).abs()
+    tol = 2.0 ** -16 * S + 1e-37
+    if dtype == "bf16":
+        tol = tol + 2.0 ** -11 * S + 2.0 ** -8 * ref.abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,rank,c0,c1", [
+    (1, 32, 1, 0, 0, 1), (1, 4096, 4096, 16, 0, 4096), (3, 96, 33, 2, 0, 33), (8, 1024, 257, 64, 0, 257),
+    (9, 64, 256, 0, 0, 256), (128, 512, 700, 5, 100, 600), (257, 2080, 1001, 33, 0, 1001), (300, 1056, 64, 0, 0, 64),
+    (515, 4128, 4099, 8, 0, 4099)])
+def test_input_gradient(session, cuda, m, k, n, rank, c0, c1, dtype):
+    import torch
+    packed, scales = _weights(k, n, 7)
+    rng = np.random.default_rng(m * n)
+    A = (rng.standard_normal((k, max(rank, 1))) * 0.02).astype(np.float32)
+    B = (rng.standard_normal((max(rank, 1), n)) * 0.02).astype(np.float32)
+    dy = _randn((m, c1 - c0), cuda, 5).to(_dt(dtype))
+    dy *= torch.exp2(torch.randint(-12, 3, (m, 1), device=cuda).float()).to(dy.dtype)
+    dx = torch.full((m, k), float("nan"), device=cuda, dtype=_dt(dtype))
+    with session.weights(packed, scales, k, n, c0, c1) as h:
+        if rank:
+            h.set_lora(A, B, 2.0 * rank)
+        h.input_gradient(dy.data_ptr(), dx.data_ptr(), m, dtype=dtype)
+        again = torch.empty_like(dx)
+        h.input_gradient(dy.data_ptr(), again.data_ptr(), m, dtype=dtype)
+    assert torch.equal(dx, again)
+    W, D = _w64(packed, scales, k, n, cuda)[:, c0:c1], dy.double()
+    ref, S = D @ W.T, D.abs() @ W.abs().T
+    if rank:
+        A64, B64 = torch.from_numpy(A).to(cuda).double(), torch.from_numpy(np.ascontiguousarray(B[:, c0:c1])).to(cuda).double()
+        ref, S = ref + 2.0 * (D @ B64.T) @ A64.T, S + 2 * 2.0 * (D.abs() @ B64.abs().T) @ A64.abs().T
+    _check_dx(dx, dtype, ref, S)
+    assert session.device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [4, 40])
+def test_input_gradient_wide_scales_zero_rows_and_nan(session, cuda, m, dtype):
+    """Columns whose scales differ by 2^20, zero rows, zero scales; a row with a NaN and one with an infinity do not
+    reach the others."""
+    import torch
+    k, n = 320, 130
+    packed, scales = _weights(k, n, 11)
+    scales = np.ascontiguousarray(scales.reshape(n, k // 32)) * np.exp2(np.arange(n) % 21 - 20).astype(np.float32)[:, None]
+    scales[5] = 0.0
+    dy = _randn((m, n), cuda, 6)
+    dy[1] = 0.0
+    dy = dy.to(_dt(dtype))
+    dx = torch.empty((m, k), device=cuda, dtype=_dt(dtype))
+    hurt, out = dy.clone(), torch.empty_like(dx)
+    hurt[0, 3], hurt[3, 9] = float("nan"), float("inf")
+    with session.weights(packed, scales, k, n) as h:
+        h.input_gradient(dy.data_ptr(), dx.data_ptr(), m, dtype=dtype)
+        h.input_gradient(hurt.data_ptr(), out.data_ptr(), m, dtype=dtype)
+    W = _w64(packed, scales, k, n, cuda)
+    _check_dx(dx, dtype, dy.double() @ W.T, dy.double().abs() @ W.abs().T)
+    assert not dx[1].any()
+    assert not torch.isfinite(out[0]).any() and not torch.isfinite(out[3][W[:, 9] != 0]).any()
+    keep = [i for i in range(m) if i not in (0, 3)]
+    assert torch.equal(out[keep], dx[keep])
+
+
+# ------------------------------------------------------------------------------------------------------- cross entropy --
+def _loss_ref(x, W, targets, scale):
+    import torch
+    X = x.double()
+    z = X @ W
+    S = (X.abs() @ W.abs()).amax(1)
+    lse = torch.logsumexp(z, 1)
+    used = targets >= 0
+    t = targets.clamp(min=0)
+    loss = torch.where(used, lse - z.gather(1, t[:, None])[:, 0], 0.0)
+    p = torch.exp(z - lse[:, None])
+    hot = torch.zeros_like(p).scatter_(1, t[:, None], 1.0)
+    g = torch.where(used, scale.double(), 0.0)[:, None]
+    return lse, loss, g * ((p - hot) @ W.T), g.abs() * ((p + hot) @ W.abs().T), S
+
+
+def _check_loss(dtype, got, ref):
+    import torch
+    (loss, lse, dx), (rl, rloss, rdx, Sdx, S) = got, ref
+    dz = 2.0 ** -16 * S
+    tol = dz + 2.0 ** -20 * (1 + rl.abs())
+    assert ((lse.double() - rl).abs() <= tol).all(), float(((lse.double() - rl).abs() / tol).max())
+    assert ((loss.double() - rloss).abs() <= 2 * tol).all(), float(((loss.double() - rloss).abs() / tol).max())
+    if dx is not None:
+        tol = (2 * dz[:, None] + 2.0 ** -16) * Sdx + 1e-37
+        if dtype == "bf16":
+            tol = tol + 2.0 ** -10 * Sdx + 2.0 ** -8 * rdx.abs()  # p and W both rounded to f16
+        err = (dx.double() - rdx).abs()
+        assert torch.isfinite(dx).all() and (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n", [(1, 32, 1), (1, 1024, 32003), (5, 64, 259), (8, 2080, 1000), (9, 96, 257),
+                                   (130, 512, 512), (257, 1056, 2049), (300, 256, 33000)])
+def test_cross_entropy(session, cuda, m, k, n, dtype):
+    import torch
+    packed, scales = _weights(k, n, 13)
+    x = _randn((m, k), cuda, 8).to(_dt(dtype))
+    targets = torch.randint(0, n, (m,), device=cuda)
+    if m > 4:
+        targets[2] = -100
+        targets[4] = n - 1
+    scale = torch.rand((m,), device=cuda) + 0.5
+    loss, lse = torch.full((m,), float("nan"), device=cuda), torch.full((m,), float("nan"), device=cuda)
+    dx = torch.full((m, k), float("nan"), device=cuda, dtype=_dt(dtype))
+    alone, inplace = torch.empty_like(loss), x.clone()
+    with session.weights(packed, scales, k, n) as h:
+        h.cross_entropy(x.data_ptr(), targets.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=dx.data_ptr(),
+                        row_scale=scale.data_ptr(), dtype=dtype)
+        h.cross_entropy(x.data_ptr(), targets.data_ptr(), alone.data_ptr(), m, dtype=dtype)
+        l2 = torch.empty_like(loss)
+        h.cross_entropy(inplace.data_ptr(), targets.data_ptr(), l2.data_ptr(), m, dx=inplace.data_ptr(),
+                        row_scale=scale.data_ptr(), dtype=dtype)
+    ref = _loss_ref(x, _w64(packed, scales, k, n, cuda), targets, scale)
+    _check_loss(dtype, (loss, lse, dx), ref)
+    assert torch.equal(alone, loss) and torch.equal(l2, loss) and torch.equal(inplace, dx)
+    if m > 4:
+        assert loss[2] == 0 and not dx[2].any()
+    assert session.device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [6, 70])
+def test_cross_entropy_rows_apart(session, cuda, m, dtype):
+    """All rows ignored; a row of NaN, a target past the vocabulary, logits far from zero and a row of zeros (uniform)."""
+    import torch
+    k, n = 128, 700
+    packed, scales = _weights(k, n, 17)
+    W = _w64(packed, scales, k, n, cuda)
+    x = _randn((m, k), cuda, 9)
+    x[1] = 0.0
+    x[2] *= 400.0
+    x = x.to(_dt(dtype))
+    targets = torch.randint(0, n, (m,), device=cuda)
+    targets[2] = (x[2].double() @ W).argmin()
+    one = torch.ones((m,), device=cuda)
+    loss, lse, dx = torch.empty((m,), device=cuda), torch.empty((m,), device=cuda), torch.empty_like(x)
+    l2, s2, d2 = torch.empty_like(loss), torch.empty_like(lse), torch.empty_like(dx)
+    hurt, t2 = x.clone(), targets.clone()
+    hurt[4, 7] = float("nan")
+    t2[5] = n
+    gone = torch.full((m,), -1, device=cuda)
+    l3, d3 = torch.empty_like(loss), torch.full_like(dx, float("nan"))
+    with session.weights(packed, scales, k, n) as h:
+        call = lambda a, t, l, s, d: h.cross_entropy(a.data_ptr(), t.data_ptr(), l.data_ptr(), m, lse=s.data_ptr(),
+                                                     dx=d.data_ptr(), dtype=dtype)
+        call(x, targets, loss, lse, dx)
+        call(hurt, t2, l2, s2, d2)
+        call(x, gone, l3, s2.clone(), d3)
+    _check_loss(dtype, (loss, lse, dx), _loss_ref(x, W, targets, one))
+    assert abs(float(lse[1]) - np.log(n)) <= 2.0 ** -19 * np.log(n)
+    assert torch.isnan(l2[4]) and torch.isnan(d2[4]).all() and torch.isnan(s2[4])
+    assert torch.isnan(l2[5]) and torch.isnan(d2[5]).all() and s2[5] == lse[5]
+    keep = [i for i in range(m) if i not in (4, 5)]
+    assert torch.equal(l2[keep], loss[keep]) and torch.equal(d2[keep], dx[keep])
+    assert not l3.any() and not d3.any()
+
+
+@pytest.mark.parametrize("m", [5, 64])
+def test_gradients_against_differences(session, cuda, m):
+    """(L(x + h u) - L(x - h u)) / 2h against <dL/dx, u>: the difference is off by h^2/6 |L'''| (third derivatives of a
+    log-sum-exp along u are at most 2 max_v |u W_v|^3 ... bounded here by (2 max|uW|)^3) and by 2^-22 |L| / h in fp32."""
+    import torch
+    k, n, h_ = 256, 500, 2.0 ** -4
+    packed, scales = _weights(k, n, 19)
+    W = _w64(packed, scales, k, n, cuda)
+    x, u = _randn((m, k), cuda, 10), _randn((m, k), cuda, 11)
+    u /= (u.double() @ W).abs().amax(1, keepdim=True).float()  # |uW| <= 1
+    targets = torch.randint(0, n, (m,), device=cuda)
+    out = [torch.empty((m,), device=cuda) for _ in range(3)]
+    dx = torch.empty_like(x)
+    with session.weights(packed, scales, k, n) as h:
+        h.cross_entropy(x.data_ptr(), targets.data_ptr(), out[0].data_ptr(), m, dx=dx.data_ptr())
+        for o, v in ((out[1], x + h_ * u), (out[2], x - h_ * u)):
+            h.cross_entropy(v.data_ptr(), targets.data_ptr(), o.data_ptr(), m)
+    diff = (out[1].double() - out[2].double()) / (2 * h_)
+    S = (x.double().abs() @ W.abs()).amax(1)
+    tol = h_ ** 2 / 6 * 8 + 2 * (2.0 ** -16 * S + 2.0 ** -20 * (1 + out[0].double())) / h_
+    assert ((diff - (dx.double() * u.double()).sum(1)).abs() <= tol).all()
+
+
+def test_input_gradient_is_the_forward_transposed(session, cuda):
+    """<dY, f(x + u) - f(x)> = <dX, u> for the linear layer f with its adapter, f by the fp32 decode path (m <= 8)."""
+    import torch
+    m, k, n, rank = 4, 512, 320, 8
+    packed, scales = _weights(k, n, 23)
+    rng = np.random.default_rng(1)
+    x, u, dy = _randn((m, k), cuda, 12), _randn((m, k), cuda, 13), _randn((m, n), cuda, 14)
+    y0, y1, dx = torch.empty((m, n), device=cuda), torch.empty((m, n), device=cuda), torch.empty((m, k), device=cuda)
+    xu = x + u
+    with session.weights(packed, scales, k, n) as h:
+        h.set_lora(rng.standard_normal((k, rank)).astype(np.float32) * 0.02, rng.standard_normal((rank, n)).astype(np.float32) * 0.02, 16.0)
+        h.run(x.data_ptr(), y0.data_ptr(), m)
+        h.run(xu.data_ptr(), y1.data_ptr(), m)
+        h.input_gradient(dy.data_ptr(), dx.data_ptr(), m)
+    a = (dy.double() * (y1.double() - y0.double())).sum(1)
+    b = (dx.double() * (xu.double() - x.double())).sum(1)
+    W = _w64(packed, scales, k, n, cuda).abs()
+    tol = 2.0 ** -13 * (dy.double().abs() * ((x.double().abs() * 2 + u.double().abs()) @ W)).sum(1)  # forward: 1e-4 class
+    assert ((a - b).abs() <= tol).all()
+
+
+# ------------------------------------------------------------------------------------------------------------ refusals --
+def test_refusals(session, cuda):
+    import torch
+    k, n, m = 64, 96, 4
+    packed, scales = _weights(k, n, 29)
+    x = torch.zeros((m + 1, k), device=cuda)
+    dy = torch.zeros((m + 1, n), device=cuda)
+    t = torch.zeros((m,), dtype=torch.int64, device=cuda)
+    loss = torch.zeros((m,), device=cuda)
+    codes = torch.zeros((m, k), dtype=torch.int8, device=cuda)
+    exps = torch.ones((m, k // 32), dtype=torch.uint8, device=cuda)
+    grad, ce, back = (session.raw("spaceslug_q4_weights_" + s) for s in ("input_gradient", "cross_entropy", "lora_backward_act8"))
+    with session.weights(packed, scales, k, n) as h:
+        w = h.handle
+        X, D, T, L, Q, E = (v.data_ptr() for v in (x, dy, t, loss, codes, exps))
+        for args in ((None, X, 0, m), (D, None, 0, m), (D, X, 2, m), (D, X, 0, 0), (D + 4, X, 0, m), (D, X + 8, 0, m),
+                     (D, X, 0, (1 << 24) + 1)):
+            assert grad(w, *args, None) == 1
+        for args in ((None, 0, T, None, L, None, None, m), (X, 0, None, None, L, None, None, m), (X, 0, T, None, None, None, None, m),
+                     (X, 5, T, None, L, None, None, m), (X, 0, T, None, L, None, None, 0), (X + 4, 0, T, None, L, None, None, m),
+                     (X, 0, T, None, L, None, X + 4, m)):
+            assert ce(w, *args, None) == 1
+        assert back(w, Q, E, D, 0, m, None, None, None) == 1  # no adapter
+        h.set_lora(np.zeros((k, 2), np.float32), np.zeros((2, n), np.float32), 2.0)
+        assert back(w, None, E, D, 0, m, None, None, None) == 1 and back(w, Q, None, D, 0, m, None, None, None) == 1
+        assert back(w, Q, E, None, 0, m, None, None, None) == 1 and back(w, Q, E, D, 3, m, None, None, None) == 1
+        assert back(w, Q, E, D, 0, 0, None, None, None) == 1 and back(w, Q + 8, E, D, 0, m, None, None, None) == 1
+        assert ce(w, X, 0, T, None, L, None, None, m, None) == 1  # an adapter on the vocabulary
+        assert b"adapter" in session._native().spaceslug_last_error()
+    assert not torch.cuda.is_current_stream_capturing() and session.device_status(0) == 0
+
+
+# ------------------------------------------------------------------------------------------------------ used together --
+def _net(session, k, hidden, vocab, rank, seed):
+    rng = np.random.default_rng(seed)
+    out = []
+    for kk, nn in ((k, hidden), (hidden, k)):
+        packed, scales = _weights(kk, nn, seed + kk + nn, 0.01, 0.04)
+        A = (rng.standard_normal((kk, rank)) * 0.05).astype(np.float32)
+        B = (rng.standard_normal((rank, nn)) * 0.05).astype(np.float32)
+        out.append((packed, scales, kk, nn, A, B))
+    packed, scales = _weights(k, vocab, seed + 1, 0.01, 0.04)
+    return out, (packed, scales, k, vocab)
+
+
+@pytest.mark.parametrize("m", [6, 200])
+def test_training_step(session, cuda, m):
+    """Two int4 layers with adapters under a vocabulary: forward, inputs kept in 8 bits, loss, gradients down to the
+    first adapter, on one stream, and once more as a replayed CUDA graph with other inputs."""
+    import torch
+    k, hidden, vocab, rank = 256, 384, 1000, 8
+    layers, head = _net(session, k, hidden, vocab, rank, 31)
+    hs = []
+    for packed, scales, kk, nn, A, B in layers:
+        h = session.weights(packed, scales, kk, nn)
+        h.set_lora(A, B, 2.0 * rank)
+        hs.append(h)
+    hv = session.weights(*head)
+    st = torch.cuda.Stream(cuda)
+    x = _randn((m, k), cuda, 15)
+    t = torch.randint(0, vocab, (m,), device=cuda)
+    scale = torch.full((m,), 1.0 / m, device=cuda)
+    y1, y2 = torch.empty((m, hidden), device=cuda), torch.empty((m, k), device=cuda)
+    c1, e1 = torch.empty((m, k), dtype=torch.int8, device=cuda), torch.empty((m, k // 32), dtype=torch.uint8, device=cuda)
+    c2, e2 = torch.empty((m, hidden), dtype=torch.int8, device=cuda), torch.empty((m, hidden // 32), dtype=torch.uint8, device=cuda)
+    loss, d2, d1 = torch.empty((m,), device=cuda), torch.empty((m, k), device=cuda), torch.empty((m, hidden), device=cuda)
+    g = [(torch.empty((kk, rank), device=cuda), torch.empty((rank, nn), device=cuda)) for _, _, kk, nn, _, _ in layers]
+
+    def step():
+        s = st.cuda_stream
+        session.act8_pack_device(x.data_ptr(), c1.data_ptr(), e1.data_ptr(), m, k, stream=s)
+        hs[0].run(x.data_ptr(), y1.data_ptr(), m, s)
+        session.act8_pack_device(y1.data_ptr(), c2.data_ptr(), e2.data_ptr(), m, hidden, stream=s)
+        hs[1].run(y1.data_ptr(), y2.data_ptr(), m, s)
+        hv.cross_entropy(y2.data_ptr(), t.data_ptr(), loss.data_ptr(), m, dx=d2.data_ptr(), row_scale=scale.data_ptr(), stream=s)
+        hs[1].lora_backward_act8(c2.data_ptr(), e2.data_ptr(), d2.data_ptr(), m, da=g[1][0].data_ptr(), db=g[1][1].data_ptr(), stream=s)
+        hs[1].input_gradient(d2.data_ptr(), d1.data_ptr(), m, stream=s)
+        hs[0].lora_backward_act8(c1.data_ptr(), e1.data_ptr(), d1.data_ptr(), m, da=g[0][0].data_ptr(), db=g[0][1].data_ptr(), stream=s)
+
+    W = [_w64(p, s, kk, nn, cuda) for p, s, kk, nn, _, _ in layers]
+    AB = [(torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()) for *_, A, B in layers]
+    Wv = _w64(*head, cuda)
+
+    def check():
+        torch.cuda.synchronize()
+        # what each call got is what the one before gave; 64-bit restatement of each, and of the whole for the loss
+        Y1 = x.double() @ W[0] + 2.0 * x.double() @ AB[0][0] @ AB[0][1]
+        Y2 = Y1 @ W[1] + 2.0 * Y1 @ AB[1][0] @ AB[1][1]
+        assert (y2.double() - Y2).norm() <= 5e-3 * Y2.norm()
+        _check_loss("f32", (loss, torch.logsumexp(y2.double() @ Wv, 1).float(), d2), _loss_ref(y2, Wv, t, scale))
+        X1 = c1.double() * torch.exp2(e1.double() - 127).repeat_interleave(32, 1)
+        X2 = c2.double() * torch.exp2(e2.double() - 127).repeat_interleave(32, 1)
+        for X, D, (A, B), (da, db) in ((X2, d2.double(), AB[1], g[1]), (X1, d1.double(), AB[0], g[0])):
+            for got, ref in ((da, 2.0 * X.T @ (D @ B.T)), (db, 2.0 * (X @ A).T @ D)):
+                assert (got.double() - ref).norm() <= 1e-5 * ref.norm()
+        ref = d2.double() @ (W[1] + 2.0 * AB[1][0] @ AB[1][1]).T
+        assert (d1.double() - ref).norm() <= 1e-5 * ref.norm()
+        # 8-bit copies: half a step of at most 1/127 of a group's largest value per element
+        assert ((X2 - y1.double()).abs() <= torch.exp2(e2.double() - 128).repeat_interleave(32, 1)).all()
+
+    with torch.cuda.stream(st):
+        step()
+        check()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            step()
+        x.copy_(_randn((m, k), cuda, 16))
+        t.copy_(torch.randint(0, vocab, (m,), device=cuda))
+        for v in (loss, d2, d1):
+            v.fill_(float("nan"))
+        st.synchronize()
+        graph.replay()
+        check()
+        first = [v.clone() for v in (loss, d2, d1, *g[0], *g[1])]
+        step()  # an eager step beside the live graph, then the graph again
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(first, (loss, d2, d1, *g[0], *g[1])))
+    del graph
+    for h in (*hs, hv):
+        h.close()
+    assert session.device_status(0) == 0
