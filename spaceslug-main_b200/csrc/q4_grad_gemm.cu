@@ -1,0 +1,858 @@
+// The two large products of training through frozen int4 weights, on CTA
+// pairs (tcgen05, cta_group::2):
+//
+//   TR = false, logits:  z[m][n]  = sum_k x[m][k] w(k, n)    (softmax cross entropy)
+//   TR = true:           dx[m][k] = sum_n d[m][n] w(k, n)    (input gradient)
+//
+// w(k, n) = float(v) * scale (vulkan-runtime/shaders/q4gemm.comp:104-122).
+// Both read the packed weights as they lie, [n][k/2] bytes, and dequantise
+// them straight into the MMA's shared-memory operand: one packed word becomes
+// 16 bytes (8 f16 of consecutive k) of the 128-byte row of its n, 128-byte
+// swizzled.  That one image is the K-major operand of the logits (rows n,
+// contraction k) and the MN-major operand of the transposed product (64 k
+// contiguous, contraction n): only the descriptors differ.
+//
+// Precision.  The rows of x (or d) enter as f16 planes scaled by a power of
+// two per row, the weights as f16 planes scaled by one power of two per
+// handle.  PA, PB planes each: 1 = the value rounded once to 11 bits, 2 = hi
+// and lo, 22 bits.  (1, 1): bf16 in and out, whose 8 bits are exact in f16,
+// so only w is rounded (2^-12) below the output's own 2^-9.  (1, 2): logits
+// of bf16 x, products to 2^-22, because the loss is fp32.  (2, 2): fp32 (hi
+// hi + hi lo + lo hi).  One scale for the whole handle loses nothing that
+// shows: columns 2^-28 below the largest still have 11 bits.
+//
+// The tensor core adds each MMA into its fp32 accumulator with truncation, so
+// the accumulator is restarted after every chunk of `chunk` 64-wide stages
+// and the chunks are added in registers, rounded to nearest.  The same place
+// rescales: the cross entropy's second product takes p~ = exp(z - max of its
+// 256-column tile) as operand and multiplies each 256-column chunk by
+// exp(tile max - row max), so that no pass over the probabilities is needed
+// between the two products.
+//
+// Roles (16 warps, 4 warpgroups): warp 0 loads the f16 planes of 128 rows per
+// CTA (TMA, 128-byte swizzled boxes of 64), warp 1 of the leader issues the
+// MMAs (M = 256, N = 256, K = 16); warps 4-7 fetch packed words and scales
+// with cp.async into a private ring and dequantise; warps 8-15 hold 128 fp32
+// sums per thread (thread = row, two warps per tensor-memory lane quarter)
+// and run the epilogue while the MMAs fill the other accumulator buffer.
+// Every wait is bounded (status word + abort flag).
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "q4_dequant.cuh"
+#include "q4_kernels.h"
+
+namespace q4 {
+
+namespace {
+
+constexpr int kGgThreads = 512;
+constexpr int kGgRows = 256;   // rows of the pair's tile (128 per CTA, one accumulator lane each)
+constexpr int kGgCols = 256;   // columns of the pair's tile
+constexpr int kGgBK = 64;      // contraction per stage
+constexpr int kGgHalf = 128;
+constexpr int kGgTile = kGgHalf * kGgBK * 2;  // 16 KB: 128 rows of 64 f16
+constexpr int kGgRing = 6;     // stages of packed words and scales in flight per dequant thread
+constexpr int kGgRingBytes = 128 * 40;
+constexpr int kGgDeqWarp0 = 4, kGgDeqWarps = 4;
+constexpr int kGgEpiWarp0 = 8, kGgEpiWarps = 8;
+constexpr int kGgStageOut = 4096;  // one 32 x 128-byte block per epilogue warp
+// Registers per thread after the split: the launch's 512 x 128 cover 128 x 40 + 128 x 64 + 256 x 200.
+constexpr int kGgRegsLaunch = 128, kGgRegsCtl = 40, kGgRegsDeq = 64, kGgRegsEpi = 200;
+static_assert(128 * kGgRegsCtl + 128 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThreads * kGgRegsLaunch, "register split");
+
+template <int PA, int PB>
+struct GgCfg {
+    static constexpr int kStageBytes = (PA + PB) * kGgTile;
+    static constexpr int kStages = PA + PB == 2 ? 5 : PA + PB == 3 ? 3 : 2;
+    static constexpr int kOutOff = kStages * kStageBytes;
+    static constexpr int kRingOff = kOutOff + kGgEpiWarps * kGgStageOut;
+    static constexpr int kXchOff = kRingOff + kGgRing * kGgRingBytes;  // [2 buffers][2 halves][128 rows] floats
+    static constexpr int kBarOff = kXchOff + 2 * 2 * 128 * 4;
+    // full_x[S], full_w[S] (leader), empty[S] (both), acc_full[2] (both), acc_empty[2] (leader), done (leader),
+    // xch[4] (own)
+    static constexpr int kNumBars = 3 * kStages + 9;
+    static constexpr int kMiscOff = kBarOff + kNumBars * 8;
+    static constexpr int kBytes = kMiscOff + 16;
+    static constexpr int kSmem = kBytes + 1024;
+    static_assert(kSmem <= 232448, "shared memory budget");
+};
+
+// K-major: see umma_desc_k_sw128.  MN-major, 128-byte swizzle: 64 elements of
+// the non-contracted dimension per 128-byte row, 8 rows (contraction) per
+// 1024-byte atom; stride-byte-offset 1024 to the next 8 rows, leading-byte-
+// offset to the next 64 elements.
+__device__ __forceinline__ uint64_t gg_desc_mn_sw128(uint32_t addr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// mbar_wait / mbar_wait_warp with the bounded spin in line: a kernel whose
+// warpgroups change their register counts makes no calls, and the epilogue
+// waits with 128 sums in registers.
+__device__ __forceinline__ bool gg_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer_ns();
+    const unsigned long long limit = *static_cast<volatile unsigned long long*>(&g_wait_limit_ns);
+#pragma unroll 1
+    while (true) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > limit) {
+            *abort_flag = 1;
+            if (status) atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool gg_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                             int code) {
+    return __all_sync(0xffffffffu, gg_wait(bar, parity, abort_flag, status, code));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+
+// Eight weights of one word as f16 hi (and, with PB = 2, lo) parts: v exact,
+// hi = RN16(v s_hi + RN16(v s_lo)) as in dequant_word_f16x2, lo = (v s_hi -
+// hi) + RN16(v s_lo), whose bracket is exact, so hi + lo is v s to 2^-22.
+template <int PB>
+__device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_lo, uint4& hi, uint4& lo) {
+    const __half2 mul = __halves2half2(__ushort_as_half(0x3C00u), __ushort_as_half(0x2C00u));  // 1, 1/16
+    const __half2 add = __halves2half2(__ushort_as_half(0xE408u), __ushort_as_half(0xD480u));  // -1032, -72
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint32_t both = __byte_perm(q, 0u, 0x4040u | (static_cast<uint32_t>(b) << 8) | static_cast<uint32_t>(b));
+        const uint32_t t = ((both ^ 0x00800008u) & 0x00F0000Fu) | 0x64006400u;
+        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&t), mul, add);
+        const __half2 c = __hmul2(v, s_lo);
+        const __half2 w = __hfma2(v, s_hi, c);
+        h[b] = *reinterpret_cast<const uint32_t*>(&w);
+        if constexpr (PB == 2) {
+            const __half2 r = __hadd2(__hfma2(v, s_hi, __hneg2(w)), c);
+            l[b] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    if constexpr (PB == 2) lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+struct GgUnit {
+    int mt, ct, z, c0, c1;  // row tile, column tile, split, chunks [c0, c1)
+};
+__device__ __forceinline__ GgUnit gg_unit(const GradGemmArgs& P, int u) {
+    GgUnit w;
+    const int tiles = P.row_tiles * P.col_tiles;
+    const int t = u % tiles;
+    w.z = u / tiles;
+    w.mt = t % P.row_tiles;
+    w.ct = t / P.row_tiles;
+    w.c0 = static_cast<int>(static_cast<long long>(w.z) * P.chunks / P.splits);
+    w.c1 = static_cast<int>(static_cast<long long>(w.z + 1) * P.chunks / P.splits);
+    return w;
+}
+
+// Stores a 128-byte row per lane (eight 16-byte pieces) of a warp's 32-row
+// block, 128-byte swizzled as its tensor map expects.
+__device__ __forceinline__ void gg_stage_row(uint8_t* buf, int lane, int piece, uint4 v) {
+    *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
+}
+
+template <bool TR, int PA, int PB, int EPI>
+__global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_constant__ GradGemmArgs P) {
+    using C = GgCfg<PA, PB>;
+    constexpr int ST = C::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_base = smem_u32(smem_raw);
+    const uint32_t base = (raw_base + 1023u) & ~1023u;
+    uint8_t* smem = smem_raw + (base - raw_base);
+    const uint32_t bar = base + C::kBarOff;
+    auto full_x = [&](int s) { return bar + 8u * s; };
+    auto full_w = [&](int s) { return bar + 8u * (ST + s); };
+    auto empty = [&](int s) { return bar + 8u * (2 * ST + s); };
+    auto acc_full = [&](int b) { return bar + 8u * (3 * ST + b); };
+    auto acc_empty = [&](int b) { return bar + 8u * (3 * ST + 2 + b); };
+    const uint32_t done_bar = bar + 8u * (3 * ST + 4);
+    auto xch_bar = [&](int q) { return bar + 8u * (3 * ST + 5 + q); };
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kMiscOff + 4);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t crank = cluster_ctarank();
+    const bool leader = crank == 0;
+    const int pair = static_cast<int>(blockIdx.x >> 1), npairs = static_cast<int>(gridDim.x >> 1);
+    const int units = P.row_tiles * P.col_tiles * P.splits;
+    int* status = P.status;
+    auto leader_addr = [&](uint32_t a) { return mapa_shared(a, 0); };
+
+    if (tid == 0) {
+        for (int s = 0; s < ST; ++s) {
+            mbar_init(full_x(s), 1);                  // leader's expect_tx (both CTAs' bytes)
+            mbar_init(full_w(s), 2 * kGgDeqWarps);    // dequant warps of both CTAs
+            mbar_init(empty(s), 1);                   // the leader's commit to both
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), 2 * kGgEpiWarps);
+        }
+        mbar_init(done_bar, 1);
+        for (int q = 0; q < 4; ++q) mbar_init(xch_bar(q), 2);  // the two warps of a lane quarter
+        *abort_flag = 0;
+        fence_mbarrier_init();
+        tma_prefetch_desc(&P.tm_a);
+        tma_prefetch_desc(&P.tm_out);
+    }
+    if (warp == 2) {
+        tmem_alloc_pair(smem_u32(tmem_holder), 512);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before_sync();
+    cluster_sync_all();
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp < 4) {
+        regs_dec<kGgRegsCtl>();
+        if (warp == 0 && lane == 0) {
+            // ------------------------------------------------ row planes --
+            int it = 0;
+            bool ok = true;
+            for (int u = pair; u < units && ok; u += npairs) {
+                const GgUnit w = gg_unit(P, u);
+                const int m0 = w.mt * kGgRows + static_cast<int>(crank) * kGgHalf;
+                const int s1 = min(w.c1 * P.chunk, P.stages);
+                for (int st = w.c0 * P.chunk; st < s1; ++st, ++it) {
+                    const int s = it % ST;
+                    if (!gg_wait(empty(s), ((it / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    if (leader) mbar_arrive_expect_tx(full_x(s), 2u * PA * kGgTile);
+                    const uint32_t fx = leader_addr(full_x(s));
+#pragma unroll
+                    for (int p = 0; p < PA; ++p)
+                        tma_load_2d_pair(base + s * C::kStageBytes + p * kGgTile, &P.tm_a, fx, st * kGgBK,
+                                         p * P.plane_rows + m0);
+                }
+            }
+            if (*abort_flag && leader)
+                for (int j = (it > ST ? it - ST : 0); j < it; ++j) mbar_drain(full_x(j % ST), (j / ST) & 1u);
+        } else if (warp == 1 && leader && elect_one()) {
+            // ------------------------------------------------------- MMA --
+            constexpr uint32_t idesc = umma_idesc_f16(0u, kGgRows, kGgCols) | (TR ? (1u << 16) : 0u);
+            int it = 0, cq = 0;
+            bool ok = true;
+            for (int u = pair; u < units && ok; u += npairs) {
+                const GgUnit w = gg_unit(P, u);
+                for (int c = w.c0; c < w.c1 && ok; ++c, ++cq) {
+                    const int b = cq & 1;
+                    if (!gg_wait(acc_empty(b), ((cq >> 1) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t dacc = tmem + static_cast<uint32_t>(b * kGgCols);
+                    const int s1 = min((c + 1) * P.chunk, P.stages);
+                    uint32_t acc = 0;
+                    for (int st = c * P.chunk; st < s1; ++st, ++it) {
+                        const int s = it % ST;
+                        const uint32_t ph = (it / ST) & 1u;
+                        if (!gg_wait(full_x(s), ph, abort_flag, status, kStatusTimeoutMma) ||
+                            !gg_wait(full_w(s), ph, abort_flag, status, kStatusTimeoutMma)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after_sync();
+                        const uint32_t at = base + s * C::kStageBytes, bt = at + PA * kGgTile;
+                        auto mma = [&](int pa, int pb, int kk) {
+                            const uint64_t ad = umma_desc_k_sw128(at + pa * kGgTile + kk * 32);
+                            const uint64_t bd = TR ? gg_desc_mn_sw128(bt + pb * kGgTile + kk * 2048, kGgTile / 2)
+                                                   : umma_desc_k_sw128(bt + pb * kGgTile + kk * 32);
+                            umma_f16_ss_pair(dacc, ad, bd, idesc, acc);
+                            acc = 1;
+                        };
+#pragma unroll
+                        for (int kk = 0; kk < kGgBK / 16; ++kk) {
+                            if constexpr (PA == 2) mma(1, 0, kk);
+                            if constexpr (PB == 2) mma(0, 1, kk);
+                            mma(0, 0, kk);
+                        }
+                        umma_commit_pair_both(empty(s), 0x3);
+                    }
+                    if (ok) umma_commit_pair_both(acc_full(b), 0x3);
+                }
+            }
+            umma_commit_pair(mapa_shared(done_bar, 0));  // tracks every MMA issued above
+            mbar_drain(done_bar, 0u);
+        }
+        __syncwarp();
+    } else if (warp < kGgEpiWarp0) {
+        // ------------------------------------------------------- dequant --
+        // Thread t: logits, column n = t of this CTA's 128 and the stage's 64
+        // k; transposed, n = t % 64 of the stage's 64 and the 64 k t / 64 of
+        // this CTA's 128.  Either way two scale groups of one n: two 16-byte
+        // words and two scales, copied into the thread's own ring slots.
+        regs_dec<kGgRegsDeq>();
+        const int t = tid - kGgDeqWarp0 * 32;
+        const uint32_t ring = base + C::kRingOff;
+        const int groups = P.K / 32;
+        const float cs = exp2i(*P.w_exp);
+        const int row = TR ? (t & 63) : t;  // row of the operand image
+        const uint32_t out_row = static_cast<uint32_t>((TR ? (t >> 6) * (kGgTile / 2) : 0) + row * 128);
+        // the fetch side runs kGgRing - 1 stages ahead of the dequant side
+        int fu = pair, fst = 0, fs1 = 0;
+        GgUnit fw{};
+        bool more = fu < units;
+        auto fetch_unit = [&]() {
+            fw = gg_unit(P, fu);
+            fst = fw.c0 * P.chunk;
+            fs1 = min(fw.c1 * P.chunk, P.stages);
+        };
+        if (more) fetch_unit();
+        auto fetch = [&](int slot) {
+            if (more) {
+                long long n;
+                int g;
+                if constexpr (TR) {
+                    n = static_cast<long long>(fst) * kGgBK + row;
+                    g = (fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64) / 32;
+                } else {
+                    n = static_cast<long long>(fw.ct) * kGgCols + static_cast<int>(crank) * kGgHalf + row;
+                    g = fst * (kGgBK / 32);
+                }
+                const uint32_t dst = ring + slot * kGgRingBytes;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // past the matrix: zeros
+                    const bool in = n < P.N && g + j < groups;
+                    const long long at = in ? n * groups + g + j : 0;
+                    cp_async16(dst + j * 2048 + t * 16, P.packed + at * 4, in ? 16u : 0u);
+                    cp_async4(dst + 4096 + j * 512 + t * 4, P.scales + at, in ? 4u : 0u);
+                }
+                if (++fst >= fs1) {
+                    fu += npairs;
+                    more = fu < units;
+                    if (more) fetch_unit();
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll 1
+        for (int i = 0; i < kGgRing - 1; ++i) fetch(i);
+        int it = 0;
+        bool ok = true;
+        for (int u = pair; u < units && ok; u += npairs) {
+            const GgUnit w = gg_unit(P, u);
+            const int s1 = min(w.c1 * P.chunk, P.stages);
+            for (int st = w.c0 * P.chunk; st < s1; ++st, ++it) {
+                const int slot = it % kGgRing, s = it % ST;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kGgRing - 2) : "memory");
+                const uint8_t* rp = smem + C::kRingOff + slot * kGgRingBytes;
+                const uint4 q[2] = {*reinterpret_cast<const uint4*>(rp + t * 16),
+                                    *reinterpret_cast<const uint4*>(rp + 2048 + t * 16)};
+                const float sc[2] = {*reinterpret_cast<const float*>(rp + 4096 + t * 4) * cs,
+                                     *reinterpret_cast<const float*>(rp + 4608 + t * 4) * cs};
+                fetch((it + kGgRing - 1) % kGgRing);  // the slot read one stage ago
+                if (!gg_wait_warp(empty(s), ((it / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* dst = smem + s * C::kStageBytes + PA * kGgTile + out_row;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    __half2 s_hi, s_lo;
+                    split_scale_f16(sc[j], s_hi, s_lo);
+                    const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 hi, lo;
+                        gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
+                        const int at = ((4 * j + i) ^ (row & 7)) << 4;
+                        *reinterpret_cast<uint4*>(dst + at) = hi;
+                        if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + at) = lo;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(leader_addr(full_w(s)));
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        // ------------------------------------------------------ epilogue --
+        regs_inc<kGgRegsEpi>();
+        const int ew = warp - kGgEpiWarp0, quarter = warp & 3, half = ew >> 2;
+        const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
+        uint8_t* buf = smem + C::kOutOff + ew * kGgStageOut;
+        const uint32_t buf_s = base + C::kOutOff + ew * kGgStageOut;
+        const int row_in = quarter * 32 + lane;  // row of this CTA's 128
+        const int wexp = *P.w_exp;
+        int cq = 0, xq = 0;
+        bool ok = true;
+        for (int u = pair; u < units && ok; u += npairs) {
+            const GgUnit w = gg_unit(P, u);
+            const int row0 = w.mt * kGgRows + static_cast<int>(crank) * kGgHalf + quarter * 32;
+            const int row = row0 + lane;
+            float acc[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
+            for (int c = w.c0; c < w.c1; ++c, ++cq) {
+                const int b = cq & 1;
+                const float f = P.coef != nullptr ? __ldg(P.coef + static_cast<size_t>(c) * P.ld_stat + row) : 1.0f;
+                if (!gg_wait_warp(acc_full(b), (cq >> 1) & 1u, abort_flag, status, kStatusTimeoutEpilogue)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t v[32];
+                    tmem_ld32(t_lane + static_cast<uint32_t>(b * kGgCols + i * 32), v);
+                    tmem_ld_wait_regs(v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[i][j] = fmaf(f, __uint_as_float(v[j]), acc[i][j]);
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote(leader_addr(acc_empty(b)));
+            }
+            if (!ok) break;
+            const int rexp = P.row_exp != nullptr ? (row < P.M ? P.row_exp[row] : 0) : P.fixed_exp;
+            const float scale = exp2i(-(rexp + wexp) / 2) * exp2i(-(rexp + wexp) - (-(rexp + wexp) / 2));
+            const int col0 = w.ct * kGgCols + half * 128;
+            if constexpr (EPI == kGgLoss || EPI == kGgProb) {
+                // In units of log2: z2 = z log2(e); this tile's row maximum over the
+                // columns that exist, the sum of 2^(z2 - max), the target's logit.
+                const float s2 = scale * 1.4426950408889634f;
+                const long long tgt = row < P.M ? P.targets[row] : -1;
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const int col = col0 + i * 32 + j;
+                        if (col == tgt) P.zt[row] = acc[i][j] * scale;
+                        acc[i][j] = col < P.N ? acc[i][j] * s2 : -INFINITY;
+                        top = fmaxf(top, acc[i][j]);
+                    }
+                // the two warps of these rows, through a buffer that alternates: a warp
+                // writes one again only after its partner has arrived for the other
+                float* xch = reinterpret_cast<float*>(smem + C::kXchOff) + (xq & 1) * 256;
+                xch[half * 128 + row_in] = top;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(xch_bar(quarter));
+                if (!gg_wait_warp(xch_bar(quarter), xq & 1u, abort_flag, status, kStatusTimeoutEpilogue)) {
+                    ok = false;
+                    break;
+                }
+                ++xq;
+                top = fmaxf(top, xch[(half ^ 1) * 128 + row_in]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        acc[i][j] = ex2(acc[i][j] - top);  // 2^-inf = 0 past the columns
+                        sum += acc[i][j];
+                    }
+                if (half == 0) P.smax[static_cast<size_t>(w.ct) * P.ld_stat + row] = top;
+                P.ssum[(static_cast<size_t>(w.ct) * 2 + half) * P.ld_stat + row] = sum;
+                if constexpr (EPI == kGgProb) {
+                    constexpr int PP = PA;  // planes of p~: as many as the rows' own
+#pragma unroll
+                    for (int p = 0; p < PP; ++p)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {  // 64 columns = 128 bytes at a time
+                            if (lane == 0) bulk_wait_group_read<0>();
+                            __syncwarp();
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                uint32_t o[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    float& a0 = acc[2 * h + e / 4][(e % 4) * 8 + 2 * j];
+                                    float& a1 = acc[2 * h + e / 4][(e % 4) * 8 + 2 * j + 1];
+                                    const float f0 = p == 0 ? a0 * 16384.0f : a0, f1 = p == 0 ? a1 * 16384.0f : a1;
+                                    const __half2 hv = __floats2half2_rn(f0, f1);
+                                    if (PP == 2 && p == 0) {
+                                        a0 = f0 - __low2float(hv);  // exact: what lo keeps
+                                        a1 = f1 - __high2float(hv);
+                                    }
+                                    o[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                                }
+                                gg_stage_row(buf, lane, e, make_uint4(o[0], o[1], o[2], o[3]));
+                            }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0 && row0 < P.M) {
+                                tma_store_2d(&P.tm_out, buf_s, col0 + h * 64, p * P.out_rows + row0);
+                                bulk_commit_group();
+                            }
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) acc[i][j] *= scale;
+                if (P.rank > 0) {
+                    // + G A^T in fp32: this row's G (scaled by alpha / r), columns of A^T read by the whole warp at once
+                    const float* gr = P.lora_g + static_cast<size_t>(min(row, P.M - 1)) * P.rank;
+                    for (int j = 0; j < P.rank; ++j) {
+                        const float gv = __ldg(gr + j);
+                        const float4* at = reinterpret_cast<const float4*>(P.lora_at + static_cast<size_t>(j) * P.ld_at + col0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 a = __ldg(at + i * 8 + e);
+                                acc[i][4 * e] = fmaf(gv, a.x, acc[i][4 * e]);
+                                acc[i][4 * e + 1] = fmaf(gv, a.y, acc[i][4 * e + 1]);
+                                acc[i][4 * e + 2] = fmaf(gv, a.z, acc[i][4 * e + 2]);
+                                acc[i][4 * e + 3] = fmaf(gv, a.w, acc[i][4 * e + 3]);
+                            }
+                    }
+                }
+                constexpr int kBlocks = EPI == kGgBf16 ? 2 : 4;  // 128 bytes of each row: 64 bf16 or 32 fp32
+                const int orow = w.z * P.out_rows + row0;
+#pragma unroll
+                for (int h = 0; h < kBlocks; ++h) {
+                    if (lane == 0) bulk_wait_group_read<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint4 o;
+                        if constexpr (EPI == kGgBf16) {
+                            uint32_t q[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 hv = __floats2bfloat162_rn(acc[2 * h + e / 4][(e % 4) * 8 + 2 * j],
+                                                                                acc[2 * h + e / 4][(e % 4) * 8 + 2 * j + 1]);
+                                q[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                            }
+                            o = make_uint4(q[0], q[1], q[2], q[3]);
+                        } else {
+                            o = make_uint4(__float_as_uint(acc[h][4 * e]), __float_as_uint(acc[h][4 * e + 1]),
+                                           __float_as_uint(acc[h][4 * e + 2]), __float_as_uint(acc[h][4 * e + 3]));
+                        }
+                        gg_stage_row(buf, lane, e, o);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    const int oc = col0 + h * (128 / kBlocks);
+                    if (lane == 0 && row0 < P.M && oc < P.K) {
+                        tma_store_2d(&P.tm_out, buf_s, oc, orow);
+                        bulk_commit_group();
+                    }
+                }
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();
+    }
+
+    tc_fence_before_sync();
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while its peer may still use its shared memory or tensor memory
+    if (warp == 2) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem, 512);
+    }
+}
+
+template <bool TR, int PA, int PB, int EPI>
+int gg_pairs() {
+    using C = GgCfg<PA, PB>;
+    static int cache[64];
+    static bool known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (known[dev]) return cache[dev];
+    auto kern = grad_gemm_kernel<TR, PA, PB, EPI>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return 0;
+    cudaFuncAttributes fa{};
+    // the register split draws on the launch's registers: refuse a build that was given fewer
+    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs < kGgRegsLaunch) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2, 1, 1);
+    cfg.blockDim = dim3(kGgThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
+    cache[dev] = n;
+    known[dev] = true;
+    return n;
+}
+
+template <bool TR, int PA, int PB, int EPI>
+int gg_launch(const GradGemmArgs& a, cudaStream_t stream) {
+    using C = GgCfg<PA, PB>;
+    auto kern = grad_gemm_kernel<TR, PA, PB, EPI>;
+    const int cap = gg_pairs<TR, PA, PB, EPI>();
+    const long long units = static_cast<long long>(a.row_tiles) * a.col_tiles * a.splits;
+    if (cap < 1 || units < 1 || units > (1ll << 30)) return static_cast<int>(cudaErrorInvalidConfiguration);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * (units < cap ? units : cap)), 1, 1);
+    cfg.blockDim = dim3(kGgThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
+// ------------------------------------------------------------------ helpers --
+__device__ __forceinline__ float gg_in(const float* p) { return *p; }
+__device__ __forceinline__ float gg_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// One block per row: f16 planes of row * 2^e, e such that the row's largest
+// magnitude lies in [2^13, 2^14); lo = the f16 rounding of what hi leaves.
+template <typename T, int PA>
+__global__ void __launch_bounds__(256) cast_planes_kernel(const T* __restrict__ x, __half* __restrict__ planes,
+                                                          int* __restrict__ row_exp, int M, int cols, long long ld) {
+    __shared__ float red[8];
+    const long long m = blockIdx.x;
+    const T* row = x + m * cols;
+    float top = 0.0f;
+    for (int c = threadIdx.x; c < cols; c += 256) top = fmaxf(top, fabsf(gg_in(row + c)));
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+    int e = 0;
+    if (top > 0.0f && isfinite(top)) {
+        int e2;
+        frexpf(top, &e2);
+        e = min(max(14 - e2, -120), 120);
+    }
+    if (threadIdx.x == 0) row_exp[m] = e;
+    const float s = exp2i(e);
+    __half* hi = planes + m * ld;
+    __half* lo = planes + (static_cast<long long>(M) + m) * ld;
+    for (int c = threadIdx.x; c < cols; c += 256) {
+        const float v = gg_in(row + c) * s;
+        const __half h = __float2half_rn(v);
+        hi[c] = h;
+        if constexpr (PA == 2) lo[c] = __float2half_rn(v - __half2float(h));
+    }
+}
+
+// The least of the handle's column exponents, the one for its largest scale.
+__global__ void __launch_bounds__(1024) min_exp_kernel(const int* __restrict__ col_exp, const float* __restrict__ scales,
+                                                       int* __restrict__ out, int N, int groups) {
+    __shared__ int red[32];
+    int e = 1 << 20;
+    for (int n = threadIdx.x; n < N; n += 1024) {
+        bool zero = true;  // an all-zero column has no say (its exponent is 0)
+        const float* s = scales + static_cast<size_t>(n) * groups;
+        for (int g = 0; g < groups && zero; ++g) zero = s[g] == 0.0f;
+        if (!zero) e = min(e, col_exp[n]);
+    }
+    for (int o = 16; o > 0; o >>= 1) e = min(e, __shfl_xor_sync(0xffffffffu, e, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = e;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 32; ++i) e = min(e, red[i]);
+        *out = e == (1 << 20) ? 0 : e;
+    }
+}
+
+// Row statistics of the tiles' (log2 units): row max M2, S = sum over tiles of
+// sums * 2^(tile max - M2), the factor 2^(tile max - M2) of every tile in
+// place of its max, lse and loss.  32 rows x 8 lanes per block.
+__global__ void __launch_bounds__(256) loss_rows_kernel(float* __restrict__ smax, const float* __restrict__ ssum,
+                                                        const float* __restrict__ zt,
+                                                        const long long* __restrict__ targets, float* __restrict__ total,
+                                                        float* __restrict__ loss, float* __restrict__ lse, int M, int N,
+                                                        int tiles, long long ld) {
+    __shared__ float part[8][32];
+    const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + r;
+    const bool in = row < M;
+    float top = -INFINITY;
+    bool bad = false;
+    for (int t = p; t < tiles && in; t += 8) {
+        const float v = smax[static_cast<size_t>(t) * ld + row];
+        bad |= v != v;
+        top = fmaxf(top, v);
+    }
+    part[p][r] = bad ? NAN : top;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, part[i][r]);
+    __syncthreads();
+    float sum = 0.0f;
+    for (int t = p; t < tiles && in; t += 8) {
+        float* at = smax + static_cast<size_t>(t) * ld + row;
+        const float f = exp2f(*at - top);
+        const float* st = ssum + static_cast<size_t>(2 * t) * ld + row;
+        sum += f * (st[0] + st[ld]);
+        *at = f;
+    }
+    part[p][r] = sum;
+    __syncthreads();
+    if (p != 0 || !in) return;
+    for (int i = 1; i < 8; ++i) sum += part[i][r];
+    const float l = 0.69314718055994531f * (top + log2f(sum));
+    const long long t = targets[row];
+    total[row] = sum;
+    if (lse != nullptr) lse[row] = l;
+    loss[row] = t < 0 ? 0.0f : t < N ? l - zt[row] : NAN;
+}
+
+// dx[row][k] = g (sum_z partial[z][row][k] / S - w(k, target)); one block per row.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ partial, int splits, long long out_rows,
+                                                      const float* __restrict__ total,
+                                                      const long long* __restrict__ targets,
+                                                      const float* __restrict__ row_scale,
+                                                      const uint32_t* __restrict__ packed,
+                                                      const float* __restrict__ scales, T* __restrict__ dx, int N, int K) {
+    const long long row = blockIdx.x;
+    const long long t = targets[row];
+    T* out = dx + row * K;
+    const float g = row_scale != nullptr ? row_scale[row] : 1.0f;
+    const float inv = 1.0f / total[row];
+    for (int k = threadIdx.x * 8; k < K; k += 256 * 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (t >= 0) {
+            for (int z = 0; z < splits; ++z) {
+                const float4* p = reinterpret_cast<const float4*>(partial + (z * out_rows + row) * K + k);
+                const float4 a = p[0], b = p[1];
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            }
+            if (t < N) {
+                const uint32_t q = packed[t * (K / 8) + k / 8];
+                const float s = scales[t * (K / 32) + k / 32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int nib = static_cast<int>((q >> (4 * i)) & 15u);
+                    v[i] = g * (v[i] * inv - static_cast<float>((nib ^ 8) - 8) * s);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = NAN;
+            }
+        }
+        if constexpr (std::is_same<T, float>::value) {
+            reinterpret_cast<float4*>(out + k)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(out + k)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                o[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(out + k) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+}
+
+// A [K][r] -> A^T [r][ld], zeros past K.
+__global__ void __launch_bounds__(256) lora_at_kernel(const float* __restrict__ a, float* __restrict__ at, int K,
+                                                      int rank, int ld) {
+    const int k = blockIdx.x * 256 + threadIdx.x;
+    if (k >= ld) return;
+    for (int j = 0; j < rank; ++j) at[static_cast<size_t>(j) * ld + k] = k < K ? a[static_cast<size_t>(k) * rank + j] : 0.0f;
+}
+
+}  // namespace
+
+int grad_gemm_pairs() { return gg_pairs<true, 1, 1, kGgBf16>(); }
+
+int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream) {
+    switch (epi) {
+        case kGgLoss:
+            return planes == 1 ? gg_launch<false, 1, 2, kGgLoss>(a, stream) : gg_launch<false, 2, 2, kGgLoss>(a, stream);
+        case kGgProb:
+            return planes == 1 ? gg_launch<false, 1, 2, kGgProb>(a, stream) : gg_launch<false, 2, 2, kGgProb>(a, stream);
+        case kGgF32:
+            return planes == 1 ? gg_launch<true, 1, 1, kGgF32>(a, stream) : gg_launch<true, 2, 2, kGgF32>(a, stream);
+        case kGgBf16:
+            if (planes == 1) return gg_launch<true, 1, 1, kGgBf16>(a, stream);
+    }
+    return static_cast<int>(cudaErrorInvalidValue);
+}
+
+int launch_cast_planes(const void* x, bool bf16, int planes, void* out, int* row_exp, int M, int cols, long long ld,
+                       cudaStream_t stream) {
+    __half* o = static_cast<__half*>(out);
+    if (bf16)
+        cast_planes_kernel<__nv_bfloat16, 1><<<M, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), o, row_exp, M,
+                                                                    cols, ld);
+    else if (planes == 2)
+        cast_planes_kernel<float, 2><<<M, 256, 0, stream>>>(static_cast<const float*>(x), o, row_exp, M, cols, ld);
+    else
+        return static_cast<int>(cudaErrorInvalidValue);
+    return static_cast<int>(cudaGetLastError());
+}
+
+int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int K, cudaStream_t stream) {
+    min_exp_kernel<<<1, 1024, 0, stream>>>(col_exp, scales, out, N, K / 32);
+    return static_cast<int>(cudaGetLastError());
+}
+
+int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
+                     float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream) {
+    loss_rows_kernel<<<(M + 31) / 32, 256, 0, stream>>>(smax, ssum, zt, targets, total, loss, lse, M, N, tiles, ld);
+    return static_cast<int>(cudaGetLastError());
+}
+
+int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const long long* targets,
+                   const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
+                   int N, int K, cudaStream_t stream) {
+    if (bf16)
+        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, targets, row_scale, packed, scales,
+                                              static_cast<__nv_bfloat16*>(dx), N, K);
+    else
+        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, targets, row_scale, packed, scales,
+                                              static_cast<float*>(dx), N, K);
+    return static_cast<int>(cudaGetLastError());
+}
+
+int launch_lora_at(const float* a, float* at, int K, int rank, int ld, cudaStream_t stream) {
+    lora_at_kernel<<<(ld + 255) / 256, 256, 0, stream>>>(a, at, K, rank, ld);
+    return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace q4

@@ -317,10 +317,52 @@ int launch_rows_wt(const void* d, bool bf16, long long ld_d, const uint32_t* pac
 // lse, loss and (want_grad) d = row_scale (softmax - onehot) of M logit rows, in place
 int launch_rows_softmax(float* z, long long ld_z, const long long* targets, const float* row_scale, float* loss,
                         float* lse, int M, int N, bool want_grad, cudaStream_t stream);
-// G[m][j] = sum_n dy[m][n] B[j][n]
-int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int M, int N, int rank, cudaStream_t stream);
-// out = sum of the splits in order + s G A^T (A [K][rank]; rank 0: none)
-int launch_rows_finish(const float* partial, int splits, const float* g, const float* a, int rank, float s, void* out,
-                       bool bf16, int M, int K, cudaStream_t stream);
+// G[m][j] = scale sum_n dy[m][n] B[j][n]
+int launch_rows_proj(const void* dy, bool bf16, const float* b, float scale, float* g, int M, int N, int rank,
+                     cudaStream_t stream);
+// out [M][K] = sum in order of the splits (split_floats apart) + G A^T (A [K][rank]; rank 0: none)
+int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, const float* a,
+                       int rank, void* out, bool bf16, int M, int K, cudaStream_t stream);
+
+// The large products of training through the frozen weights (q4_grad_gemm.cu).  Epilogues: the logits' tile statistics
+// (kGgLoss), those and the planes of p~ = exp(z - tile max) 2^14 (kGgProb), the transposed product in fp32 (kGgF32:
+// split z at row z * out_rows) or bf16 (kGgBf16).
+enum : int { kGgLoss = 0, kGgProb = 1, kGgF32 = 2, kGgBf16 = 3 };
+struct GradGemmArgs {
+    CUtensorMap tm_a;        // f16 planes of the rows: [planes * plane_rows][contraction], box 64 x 128, 128B swizzle
+    CUtensorMap tm_out;      // p~ planes or the output: box 128 bytes x 32 rows, 128B swizzle (not read by kGgLoss)
+    const uint32_t* packed;  // [N][K/8]
+    const float* scales;     // [N][K/32]
+    const int* w_exp;        // the handle's power of two (device)
+    const int* row_exp;      // [M], or nullptr: fixed_exp for every row
+    int fixed_exp;
+    int M, N, K;
+    int plane_rows, out_rows;  // rows between planes of the input, and between planes or splits of the output
+    int row_tiles, col_tiles, splits;
+    int stages, chunk, chunks;  // 64-wide stages of the contraction, stages per accumulator chunk, chunks
+    const float* coef;       // [chunks][ld_stat] factor of a row's chunk, or nullptr
+    const float* lora_g;     // [M][rank] (scaled), lora_at [rank][ld_at]; rank 0: none
+    const float* lora_at;
+    int rank, ld_at;
+    const long long* targets;  // logits: [M]
+    float* zt;               // [M] the target's logit
+    float* smax;             // [col_tiles][ld_stat]
+    float* ssum;             // [2 col_tiles][ld_stat]
+    long long ld_stat;
+    int* status;
+};
+int grad_gemm_pairs();  // co-resident CTA pairs on the current device
+int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream);
+// f16 planes [planes][M][ld] of fp32 (2 planes) or bf16 (1) rows scaled by 2^row_exp
+int launch_cast_planes(const void* x, bool bf16, int planes, void* out, int* row_exp, int M, int cols, long long ld,
+                       cudaStream_t stream);
+int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int K, cudaStream_t stream);
+// tile statistics -> chunk factors (in smax), row sums, loss and lse
+int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
+                     float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream);
+int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const long long* targets,
+                   const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
+                   int N, int K, cudaStream_t stream);
+int launch_lora_at(const float* a, float* at, int K, int rank, int ld, cudaStream_t stream);
 
 }  // namespace q4

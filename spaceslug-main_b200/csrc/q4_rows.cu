@@ -5,8 +5,8 @@
 //   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n)        (logits)
 //   rows_wt_kernel       dx[m][k] = sum_n d[m][n] w(k, n)        (the transposed product)
 //   rows_softmax_kernel  lse, loss and d = g (softmax(z) - onehot) of logit rows, in place
-//   rows_proj_kernel     G[m][j]  = sum_n dy[m][n] B[j][n]       (the adapter's side)
-//   rows_finish_kernel   sums the splits of n in order, adds s G A^T, rounds once to the output's type
+//   rows_proj_kernel     G[m][j]  = s sum_n dy[m][n] B[j][n]     (the adapter's side)
+//   rows_finish_kernel   sums the splits of n in order, adds G A^T, rounds once to the output's type
 //
 // w(k, n) = float(v) * scale as everywhere (vulkan-runtime/shaders/q4gemm.comp:104-122),
 // one rounding.  With one to eight rows these products are bound by the
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(512) rows_softmax_kernel(float* __restrict__ z
 constexpr int kProjRows = 4, kProjRanks = 16;
 template <typename T>
 __global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy, const float* __restrict__ b,
-                                                        float* __restrict__ g, int M, int N, int rank) {
+                                                        float scale, float* __restrict__ g, int M, int N, int rank) {
     __shared__ float red[8][64];
     const int m0 = blockIdx.x * kProjRows, j0 = blockIdx.y * kProjRanks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -231,25 +231,25 @@ __global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy
         float t = 0.0f;
         for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
         const int r = threadIdx.x / kProjRanks, j = threadIdx.x % kProjRanks;
-        if (m0 + r < M && j0 + j < rank) g[static_cast<size_t>(m0 + r) * rank + j0 + j] = t;
+        if (m0 + r < M && j0 + j < rank) g[static_cast<size_t>(m0 + r) * rank + j0 + j] = scale * t;
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) rows_finish_kernel(const float* __restrict__ partial, int splits,
-                                                          const float* __restrict__ g, const float* __restrict__ a,
-                                                          int rank, float s, T* __restrict__ out, long long count,
-                                                          int K) {
+                                                          long long split_floats, const float* __restrict__ g,
+                                                          const float* __restrict__ a, int rank, T* __restrict__ out,
+                                                          long long count, int K) {
     const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= count) return;
     float v = 0.0f;
-    for (int z = 0; z < splits; ++z) v += partial[z * count + i];
+    for (int z = 0; z < splits; ++z) v += partial[z * split_floats + i];
     if (rank > 0) {
         const long long m = i / K;
         const int k = static_cast<int>(i % K);
         float l = 0.0f;
         for (int j = 0; j < rank; ++j) l = fmaf(g[m * rank + j], __ldg(a + static_cast<size_t>(k) * rank + j), l);
-        v = fmaf(s, l, v);
+        v += l;
     }
     row_store(out + i, v);
 }
@@ -315,25 +315,27 @@ int launch_rows_softmax(float* z, long long ld_z, const long long* targets, cons
     return static_cast<int>(cudaGetLastError());
 }
 
-int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int M, int N, int rank, cudaStream_t stream) {
+int launch_rows_proj(const void* dy, bool bf16, const float* b, float scale, float* g, int M, int N, int rank,
+                     cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>((M + kProjRows - 1) / kProjRows),
                     static_cast<unsigned>((rank + kProjRanks - 1) / kProjRanks));
     if (bf16)
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), b, g, M, N, rank);
+        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), b, scale, g, M, N, rank);
     else
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(dy), b, g, M, N, rank);
+        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(dy), b, scale, g, M, N, rank);
     return static_cast<int>(cudaGetLastError());
 }
 
-int launch_rows_finish(const float* partial, int splits, const float* g, const float* a, int rank, float s, void* out,
-                       bool bf16, int M, int K, cudaStream_t stream) {
+int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, const float* a,
+                       int rank, void* out, bool bf16, int M, int K, cudaStream_t stream) {
     const long long count = static_cast<long long>(M) * K;
     const unsigned blocks = static_cast<unsigned>((count + 255) / 256);
     if (bf16)
-        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, g, a, rank, s, static_cast<__nv_bfloat16*>(out),
-                                                       count, K);
+        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, split_floats, g, a, rank,
+                                                       static_cast<__nv_bfloat16*>(out), count, K);
     else
-        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, g, a, rank, s, static_cast<float*>(out), count, K);
+        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, split_floats, g, a, rank, static_cast<float*>(out),
+                                                       count, K);
     return static_cast<int>(cudaGetLastError());
 }
 

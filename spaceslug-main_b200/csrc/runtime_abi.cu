@@ -1158,57 +1158,220 @@ void lora_backward_f32(spaceslug_q4_weights* w, const float* x, const float* dy,
     }
 }
 
-// dX = dY W^T + s (dY B^T) A^T.  The rows go in blocks whose split sums fit 256 MB.
-void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
+// Rows up to which the training products stream the weights on the CUDA cores
+// (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
+constexpr int kRowsKernelMax = 8;
+constexpr long long kTrainScratch = 512ll << 20;  // bytes of operand planes per block of rows
+
+// Splits of the contraction of a product of `tiles` 256 x 256 tiles and
+// `chunks` accumulator chunks of `cost` cycles: the least of waves x (chunks
+// per split) plus each unit's fill and epilogue (about 4000 cycles) plus, for
+// more than one split, the partial sums' way through HBM (write and read, at
+// about 3400 bytes per cycle) and the launch that adds them.
+int grad_splits(long long tiles, int chunks, long long cost, int pairs, long long out_floats, bool partial_anyway) {
+    int best = 1;
+    long long least = -1;
+    for (int z = 1; z <= std::min(chunks, 64); ++z) {
+        long long t = (tiles * z + pairs - 1) / pairs * ((chunks + z - 1) / z * cost + 4000);
+        if (z > 1 || partial_anyway) t += z * out_floats * 8 / 3400;
+        if (z > 1 && !partial_anyway) t += 6000;
+        if (least < 0 || t < least) {
+            least = t;
+            best = z;
+        }
+    }
+    return best;
+}
+
+int pairs_or_throw() {
+    const int pairs = q4::grad_gemm_pairs();
+    if (pairs < 1) throw CudaError("the training product does not fit this device");
+    return pairs;
+}
+
+// dX = dY W^T + s (dY B^T) A^T for at most kRowsKernelMax rows.
+void run_input_gradient_rows(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
+    const int splits = q4::rows_wt_splits(M, w->N, w->K, c.sm_count);
+    Scratch part(static_cast<size_t>(splits) * M * w->K * 4, s);
+    Scratch gs(static_cast<size_t>(M) * w->rank * 4, s);
+    const float lscale = w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f;
+    if (w->rank > 0)
+        check_launch(q4::launch_rows_proj(dy, bf16, w->lora_b, lscale, static_cast<float*>(gs.p), M, w->N, w->rank, s),
+                     "dY B^T");
+    check_launch(q4::launch_rows_wt(dy, bf16, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, M, w->N,
+                                    w->K, s),
+                 "dY W^T");
+    check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<long long>(M) * w->K,
+                                        static_cast<float*>(gs.p), w->lora_a, w->rank, dx, bf16, M, w->K, s),
+                 "dX");
+}
+
+void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
+    if (M <= kRowsKernelMax) {
+        run_input_gradient_rows(w, dy, dx, bf16, M, s);
+        return;
+    }
+    DeviceCtx& c = ctx_for(w->device);
+    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
     const size_t size = bf16 ? 2 : 4;
-    const int block = static_cast<int>(std::clamp<long long>((64ll << 20) / w->K / 8 * 8, 8, 1 << 18));
+    const long long ld = (static_cast<long long>(N) + 7) / 8 * 8, ld_at = (static_cast<long long>(K) + 255) / 256 * 256;
+    const float lscale = w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f;
+    Scratch at(w->rank > 0 ? static_cast<size_t>(w->rank) * ld_at * 4 : 0, s);
+    if (w->rank > 0)
+        check_launch(q4::launch_lora_at(w->lora_a, static_cast<float*>(at.p), K, w->rank, static_cast<int>(ld_at), s), "A^T");
+    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0);
-        const int splits = q4::rows_wt_splits(mc, w->N, w->K, c.sm_count);
-        Scratch part(static_cast<size_t>(splits) * mc * w->K * 4, s);
+        const void* d = static_cast<const char*>(dy) + static_cast<size_t>(m0) * N * size;
+        void* out = static_cast<char*>(dx) + static_cast<size_t>(m0) * K * size;
+        q4::GradGemmArgs g{};
+        g.M = mc; g.N = N; g.K = K;
+        g.row_tiles = (mc + 255) / 256;
+        g.col_tiles = (K + 255) / 256;
+        g.stages = (N + 63) / 64;
+        g.chunk = 8;
+        g.chunks = (g.stages + g.chunk - 1) / g.chunk;
+        g.splits = grad_splits(static_cast<long long>(g.row_tiles) * g.col_tiles, g.chunks,
+                               (planes == 1 ? 512 : 1536) * g.chunk, pairs, static_cast<long long>(mc) * K, false);
+        g.out_rows = g.row_tiles * 256;
+        g.plane_rows = mc;
+        Scratch x16(static_cast<size_t>(planes) * mc * ld * 2, s);
+        Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
         Scratch gs(static_cast<size_t>(mc) * w->rank * 4, s);
-        const void* d = static_cast<const char*>(dy) + static_cast<size_t>(m0) * w->N * size;
+        Scratch part(g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0, s);
+        check_launch(q4::launch_cast_planes(d, bf16, planes, x16.p, static_cast<int*>(rexp.p), mc, N, ld, s), "dY planes");
         if (w->rank > 0)
-            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, static_cast<float*>(gs.p), mc, w->N, w->rank, s),
+            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, lscale, static_cast<float*>(gs.p), mc, N, w->rank, s),
                          "dY B^T");
-        check_launch(q4::launch_rows_wt(d, bf16, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, mc,
-                                        w->N, w->K, s),
-                     "dY W^T");
-        check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<float*>(gs.p), w->lora_a,
-                                            w->rank, w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f,
-                                            static_cast<char*>(dx) + static_cast<size_t>(m0) * w->K * size, bf16, mc,
-                                            w->K, s),
-                     "dX");
+        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(N),
+                  static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(ld) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+        const bool direct16 = bf16 && g.splits == 1;
+        if (direct16)
+            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
+                      static_cast<uint64_t>(K) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        else
+            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, part.p ? part.p : out, static_cast<uint64_t>(K),
+                      part.p ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc),
+                      static_cast<uint64_t>(K) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        g.packed = w->packed; g.scales = w->scales; g.w_exp = w->col_exp + N;
+        g.row_exp = static_cast<int*>(rexp.p);
+        if (g.splits == 1 && w->rank > 0) {
+            g.rank = w->rank;
+            g.lora_g = static_cast<float*>(gs.p);
+            g.lora_at = static_cast<float*>(at.p);
+            g.ld_at = static_cast<int>(ld_at);
+        }
+        g.status = c.status;
+        check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, s), "dY W^T");
+        if (g.splits > 1)
+            check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), g.splits, static_cast<long long>(g.out_rows) * K,
+                                                static_cast<float*>(gs.p), w->lora_a, w->rank, out, bf16, mc, K, s),
+                         "dX");
     }
 }
 
-// Loss and gradient, the logits of at most 256 MB of rows at a time.
-void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const int64_t* targets,
-                       const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
+// Loss and gradient of at most kRowsKernelMax rows, their logits in scratch.
+void run_cross_entropy_rows(spaceslug_q4_weights* w, const void* x, bool bf16, const long long* targets,
+                            const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
+    Scratch zs(static_cast<size_t>(M) * w->N * 4, s);
+    float* z = static_cast<float*>(zs.p);
+    check_launch(q4::launch_rows_logits(x, bf16, w->packed, w->scales, z, w->N, M, w->N, w->K, s), "logits");
+    check_launch(q4::launch_rows_softmax(z, w->N, targets, row_scale, loss, lse, M, w->N, dx != nullptr, s), "softmax");
+    if (!dx) return;
+    const int splits = q4::rows_wt_splits(M, w->N, w->K, c.sm_count);
+    Scratch part(static_cast<size_t>(splits) * M * w->K * 4, s);
+    check_launch(q4::launch_rows_wt(z, false, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, M, w->N,
+                                    w->K, s),
+                 "dZ W^T");
+    check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<long long>(M) * w->K, nullptr,
+                                        nullptr, 0, dx, bf16, M, w->K, s),
+                 "dX");
+}
+
+// Loss and gradient.  Per block of rows: the f16 planes of X; the logits'
+// product, whose epilogue leaves each 256-column tile's max, sum and (for the
+// gradient) exp(z - max) as f16 planes; the rows' lse, loss and tile factors;
+// the transposed product of those planes; its splits' sum, normalised, with
+// the target's column taken off.  The logits themselves are never stored.
+void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const int64_t* targets64,
+                       const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
+    static_assert(sizeof(long long) == sizeof(int64_t), "targets are int64");
+    const long long* targets = reinterpret_cast<const long long*>(targets64);
+    if (M <= kRowsKernelMax) {
+        run_cross_entropy_rows(w, x, bf16, targets, row_scale, loss, lse, dx, M, s);
+        return;
+    }
+    DeviceCtx& c = ctx_for(w->device);
+    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
     const size_t size = bf16 ? 2 : 4;
-    const int block = static_cast<int>(std::clamp<long long>((64ll << 20) / w->N / 8 * 8, 8, 1 << 18));
+    const int tiles = (N + 255) / 256;
+    const long long ld_p = static_cast<long long>(tiles) * 256;
+    const long long row_bytes = 2ll * planes * (dx ? ld_p : K);
+    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20));
     for (int m0 = 0; m0 < M; m0 += block) {
-        const int mc = std::min(block, M - m0);
-        Scratch zs(static_cast<size_t>(mc) * w->N * 4, s);
-        float* z = static_cast<float*>(zs.p);
-        check_launch(q4::launch_rows_logits(static_cast<const char*>(x) + static_cast<size_t>(m0) * w->K * size, bf16,
-                                            w->packed, w->scales, z, w->N, mc, w->N, w->K, s),
-                     "logits");
-        check_launch(q4::launch_rows_softmax(z, w->N, reinterpret_cast<const long long*>(targets) + m0,
-                                             row_scale ? row_scale + m0 : nullptr, loss + m0, lse ? lse + m0 : nullptr,
-                                             mc, w->N, dx != nullptr, s),
-                     "softmax");
+        const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
+        Scratch x16(static_cast<size_t>(planes) * mc * K * 2, s);
+        Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
+        Scratch stat((static_cast<size_t>(3) * tiles + 2) * mp * 4, s);
+        Scratch prob(dx ? static_cast<size_t>(planes) * mp * ld_p * 2 : 0, s);
+        float* smax = static_cast<float*>(stat.p);
+        float* ssum = smax + static_cast<size_t>(tiles) * mp;
+        float* zt = ssum + static_cast<size_t>(2) * tiles * mp;
+        float* total = zt + mp;
+        check_launch(q4::launch_cast_planes(static_cast<const char*>(x) + static_cast<size_t>(m0) * K * size, bf16, planes,
+                                            x16.p, static_cast<int*>(rexp.p), mc, K, K, s),
+                     "X planes");
+        q4::GradGemmArgs g{};
+        g.M = mc; g.N = N; g.K = K;
+        g.row_tiles = mp / 256;
+        g.col_tiles = tiles;
+        g.splits = 1;
+        g.stages = (K + 63) / 64;
+        g.chunk = 8;
+        g.chunks = (g.stages + g.chunk - 1) / g.chunk;
+        g.plane_rows = mc;
+        g.out_rows = mp;
+        g.packed = w->packed; g.scales = w->scales; g.w_exp = w->col_exp + N;
+        g.row_exp = static_cast<int*>(rexp.p);
+        g.targets = targets + m0;
+        g.zt = zt; g.smax = smax; g.ssum = ssum;
+        g.ld_stat = mp;
+        g.status = c.status;
+        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(K),
+                  static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (dx)
+            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
+                      static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 32,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+        else
+            g.tm_out = g.tm_a;  // not read
+        check_launch(q4::launch_grad_gemm(g, planes, dx ? q4::kGgProb : q4::kGgLoss, s), "logits");
+        check_launch(q4::launch_loss_rows(smax, ssum, zt, targets + m0, total, loss + m0, lse ? lse + m0 : nullptr, mc, N,
+                                          tiles, mp, s),
+                     "loss rows");
         if (!dx) continue;
-        const int splits = q4::rows_wt_splits(mc, w->N, w->K, c.sm_count);
-        Scratch part(static_cast<size_t>(splits) * mc * w->K * 4, s);
-        check_launch(q4::launch_rows_wt(z, false, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, mc,
-                                        w->N, w->K, s),
-                     "dZ W^T");
-        check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, nullptr, nullptr, 0, 0.0f,
-                                            static_cast<char*>(dx) + static_cast<size_t>(m0) * w->K * size, bf16, mc,
-                                            w->K, s),
+        q4::GradGemmArgs d = g;
+        d.col_tiles = (K + 255) / 256;
+        d.stages = tiles * 4;
+        d.chunk = 4;  // one 256-column tile of the logits: one factor per row
+        d.chunks = tiles;
+        d.splits = grad_splits(static_cast<long long>(d.row_tiles) * d.col_tiles, tiles, (planes == 1 ? 512 : 1536) * 4,
+                               pairs, static_cast<long long>(mp) * K, true);
+        d.plane_rows = mp;
+        d.row_exp = nullptr;
+        d.fixed_exp = 14;  // p~ carries 2^14
+        d.coef = smax;
+        Scratch part(static_cast<size_t>(d.splits) * mp * K * 4, s);
+        encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
+                  static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+        encode_2d(&d.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, part.p, static_cast<uint64_t>(K),
+                  static_cast<uint64_t>(d.splits) * mp, static_cast<uint64_t>(K) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, s), "P W^T");
+        check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, targets + m0,
+                                        row_scale ? row_scale + m0 : nullptr, w->packed, w->scales,
+                                        static_cast<char*>(dx) + static_cast<size_t>(m0) * K * size, bf16, mc, N, K, s),
                      "dX");
     }
 }
@@ -1389,11 +1552,13 @@ int spaceslug_q4_weights_create(const uint32_t* packed, const float* scales, uin
         try {
             check(cudaMalloc(&w->packed, pb), "cudaMalloc packed");
             check(cudaMalloc(&w->scales, sb), "cudaMalloc scales");
-            check(cudaMalloc(&w->col_exp, static_cast<size_t>(w->N) * sizeof(int)), "cudaMalloc col_exp");
+            // the columns' exponents and, behind them, their least
+            check(cudaMalloc(&w->col_exp, (static_cast<size_t>(w->N) + 1) * sizeof(int)), "cudaMalloc col_exp");
             std::lock_guard<std::mutex> lk(c.host_mu);
             q4up::staged_h2d(device, w->packed, packed + static_cast<size_t>(col_begin) * (k / 8u), pb, c.stream);
             q4up::staged_h2d(device, w->scales, scales + static_cast<size_t>(col_begin) * G, sb, c.stream);
             check_launch(q4::launch_col_exp(w->scales, w->col_exp, w->N, w->K, c.stream), "col_exp");
+            check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, c.stream), "min_exp");
             check(cudaStreamSynchronize(c.stream), "cudaStreamSynchronize");
         } catch (...) {
             spaceslug_q4_weights_destroy(w);
@@ -1424,11 +1589,13 @@ int spaceslug_q4_weights_create_logical(const int8_t* w_kn, const float* scales,
         try {
             check(cudaMalloc(&w->packed, pb), "cudaMalloc packed");
             check(cudaMalloc(&w->scales, sb), "cudaMalloc scales");
-            check(cudaMalloc(&w->col_exp, static_cast<size_t>(w->N) * sizeof(int)), "cudaMalloc col_exp");
+            // the columns' exponents and, behind them, their least
+            check(cudaMalloc(&w->col_exp, (static_cast<size_t>(w->N) + 1) * sizeof(int)), "cudaMalloc col_exp");
             std::lock_guard<std::mutex> lk(c.host_mu);
             q4up::staged_pack_logical(device, w->packed, w_kn, k, n, col_begin, static_cast<uint32_t>(w->N), c.stream);
             q4up::staged_h2d(device, w->scales, scales + static_cast<size_t>(col_begin) * G, sb, c.stream);
             check_launch(q4::launch_col_exp(w->scales, w->col_exp, w->N, w->K, c.stream), "col_exp");
+            check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, c.stream), "min_exp");
             check(cudaStreamSynchronize(c.stream), "cudaStreamSynchronize");
         } catch (...) {
             spaceslug_q4_weights_destroy(w);
