@@ -324,60 +324,69 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
         const float cs = exp2i(*P.w_exp);
         const int row = TR ? (t & 63) : t;  // row of the operand image
         const uint32_t out_row = static_cast<uint32_t>((TR ? (t >> 6) * (kGgTile / 2) : 0) + row * 128);
-        // the fetch side runs kGgRing - 1 stages ahead of the dequant side
-        int fu = pair, fst = 0, fs1 = 0;
-        GgUnit fw{};
-        bool more = fu < units;
-        auto fetch_unit = [&]() {
-            fw = gg_unit(P, fu);
-            fst = fw.c0 * P.chunk;
-            fs1 = min(fw.c1 * P.chunk, P.stages);
-        };
-        if (more) fetch_unit();
+        // The fetch side runs kGgRing - 1 stages ahead of the dequant side.  Within
+        // a unit its element index `at` (n * groups + g) moves by a constant.
+        int fu = pair, left = 0, fn = 0, fg = 0;
+        long long at = 0;
+        const long long at_step = TR ? static_cast<long long>(kGgBK) * groups : kGgBK / 32;
         auto fetch = [&](int slot) {
-            if (more) {
-                long long n;
-                int g;
-                if constexpr (TR) {
-                    n = static_cast<long long>(fst) * kGgBK + row;
-                    g = (fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64) / 32;
-                } else {
-                    n = static_cast<long long>(fw.ct) * kGgCols + static_cast<int>(crank) * kGgHalf + row;
-                    g = fst * (kGgBK / 32);
-                }
+            if (left == 0 && fu < units) {
+                const GgUnit fw = gg_unit(P, fu);
+                fu += npairs;
+                const int st0 = fw.c0 * P.chunk;
+                left = min(fw.c1 * P.chunk, P.stages) - st0;
+                fn = TR ? st0 * kGgBK + row : fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + row;
+                fg = TR ? (fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64) / 32 : st0 * (kGgBK / 32);
+                at = static_cast<long long>(fn) * groups + fg;
+            }
+            if (left > 0) {
                 const uint32_t dst = ring + slot * kGgRingBytes;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {  // past the matrix: zeros
-                    const bool in = n < P.N && g + j < groups;
-                    const long long at = in ? n * groups + g + j : 0;
-                    cp_async16(dst + j * 2048 + t * 16, P.packed + at * 4, in ? 16u : 0u);
-                    cp_async4(dst + 4096 + j * 512 + t * 4, P.scales + at, in ? 4u : 0u);
+                    const bool in = fn < P.N && fg + j < groups;
+                    const long long e = in ? at + j : 0;
+                    cp_async16(dst + j * 2048 + t * 16, P.packed + e * 4, in ? 16u : 0u);
+                    cp_async4(dst + 4096 + j * 512 + t * 4, P.scales + e, in ? 4u : 0u);
                 }
-                if (++fst >= fs1) {
-                    fu += npairs;
-                    more = fu < units;
-                    if (more) fetch_unit();
+                --left;
+                at += at_step;
+                if constexpr (TR) {
+                    fn += kGgBK;
+                } else {
+                    fg += kGgBK / 32;
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        // Words and scales of a stage, ring -> registers, one stage ahead of their use.
+        uint4 q[2];
+        float sc[2];
+        auto load = [&](int slot) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kGgRing - 2) : "memory");
+            const uint8_t* rp = smem + C::kRingOff + slot * kGgRingBytes;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                q[j] = *reinterpret_cast<const uint4*>(rp + j * 2048 + t * 16);
+                sc[j] = *reinterpret_cast<const float*>(rp + 4096 + j * 512 + t * 4);
+            }
+        };
 #pragma unroll 1
         for (int i = 0; i < kGgRing - 1; ++i) fetch(i);
-        int it = 0;
+        load(0);
+        fetch(kGgRing - 1);
+        int slot = 1, s = 0;
+        uint32_t ph = 1;
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
             const GgUnit w = gg_unit(P, u);
             const int s1 = min(w.c1 * P.chunk, P.stages);
-            for (int st = w.c0 * P.chunk; st < s1; ++st, ++it) {
-                const int slot = it % kGgRing, s = it % ST;
-                asm volatile("cp.async.wait_group %0;" ::"n"(kGgRing - 2) : "memory");
-                const uint8_t* rp = smem + C::kRingOff + slot * kGgRingBytes;
-                const uint4 q[2] = {*reinterpret_cast<const uint4*>(rp + t * 16),
-                                    *reinterpret_cast<const uint4*>(rp + 2048 + t * 16)};
-                const float sc[2] = {*reinterpret_cast<const float*>(rp + 4096 + t * 4) * cs,
-                                     *reinterpret_cast<const float*>(rp + 4608 + t * 4) * cs};
-                fetch((it + kGgRing - 1) % kGgRing);  // the slot read one stage ago
-                if (!gg_wait_warp(empty(s), ((it / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
+            for (int st = w.c0 * P.chunk; st < s1; ++st) {
+                const uint4 qc[2] = {q[0], q[1]};
+                const float sv[2] = {sc[0] * cs, sc[1] * cs};
+                load(slot);  // of the next stage (past the last one: stale words that nothing uses)
+                fetch(slot == 0 ? kGgRing - 1 : slot - 1);  // the slot whose words are in qc
+                slot = slot + 1 == kGgRing ? 0 : slot + 1;
+                if (!gg_wait_warp(empty(s), ph, abort_flag, status, kStatusTimeoutDequant)) {
                     ok = false;
                     break;
                 }
@@ -385,20 +394,24 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     __half2 s_hi, s_lo;
-                    split_scale_f16(sc[j], s_hi, s_lo);
-                    const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+                    split_scale_f16(sv[j], s_hi, s_lo);
+                    const uint32_t words[4] = {qc[j].x, qc[j].y, qc[j].z, qc[j].w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint4 hi, lo;
                         gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
-                        const int at = ((4 * j + i) ^ (row & 7)) << 4;
-                        *reinterpret_cast<uint4*>(dst + at) = hi;
-                        if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + at) = lo;
+                        const int o = ((4 * j + i) ^ (row & 7)) << 4;
+                        *reinterpret_cast<uint4*>(dst + o) = hi;
+                        if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
                     }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_remote(leader_addr(full_w(s)));
+                if (++s == ST) {
+                    s = 0;
+                    ph ^= 1u;
+                }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
