@@ -437,11 +437,11 @@ int lora_tc_rp(int rank) {
 // number of stages (t) and the launch's units fill whole waves of the SMs:
 // the cost of a candidate is waves x (longest unit + about two stages of
 // fill and store).
-void lora_tc_plan(int count, const int* R, const int* L, int sm_count, int* splits) {
+void lora_tc_plan(int count, const int* R, const int* L, int sm_count, int* splits, int stage_l) {
     int tiles[2], NS[2], nsmax = 1;
     for (int i = 0; i < count; ++i) {
         tiles[i] = (R[i] + kLtRows - 1) / kLtRows;
-        NS[i] = (L[i] + kLtL - 1) / kLtL;
+        NS[i] = (L[i] + stage_l - 1) / stage_l;
         if (NS[i] > nsmax) nsmax = NS[i];
         splits[i] = 1;
     }

@@ -253,8 +253,8 @@ struct LoraTcPass {
     int* status;
 };
 int lora_tc_rp(int rank);  // padded rank: 8, 16, 32 or 64
-// l ranges per 128-row tile for `count` problems sharing one launch
-void lora_tc_plan(int count, const int* R, const int* L, int sm_count, int* splits);
+// l ranges per 128-row tile for `count` problems sharing one launch, in stages of stage_l
+void lora_tc_plan(int count, const int* R, const int* L, int sm_count, int* splits, int stage_l = 32);
 int launch_lora_tc_pass(const LoraTcPass& p, cudaStream_t stream);
 // v[row][j] = sum of the splits in order; mode 0: stacked TF32 planes of the
 // transpose ([2 rp][ld]); mode 1: s * transpose ([r][ld]); mode 2: s * rows
@@ -364,5 +364,36 @@ int launch_loss_dx(const float* partial, int splits, long long out_rows, const f
                    const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream);
 int launch_lora_at(const float* a, float* at, int K, int rank, int ld, cudaStream_t stream);
+
+// LoRA gradients with wide operands exact in bf16 (lora16.cu): a problem is partial[split][row][rp] of D[R x r] = sum
+// over l < L of Aop[row][l] Bop[j][l].  tm_a: bf16 (K-major box 64 l x 128 rows, 128B swizzle; MN-major box 128 rows x
+// 64 l, unswizzled) or, with act8, int8 codes (64 l x 128 rows, 64B swizzle; 128 rows x 64 l, unswizzled) with their
+// step bytes exps [source row][groups]; tm_b: Bop's stacked bf16 planes, dims {L, 3 rp}, box 64 x 3 rp, 128B swizzle.
+struct Lora16Problem {
+    CUtensorMap tm_a, tm_b;
+    const uint8_t* exps;
+    float* partial;
+    int R, L, splits, act8, groups;
+};
+struct Lora16Pass {
+    Lora16Problem prob[2];
+    int count, mn_major, rp, sm_count;
+    int* status;
+};
+int lora16_rp(int rank);  // padded rank: 16, 32 or 64
+int lora16_stage();       // contraction elements per stage
+int launch_lora16_pass(const Lora16Pass& p, cudaStream_t stream);
+// v[row][j] = sum of the splits in order (pitch between rows of src), or with from_rows src[j][row]; written as stacked
+// bf16 planes [3 rp][ld] or TF32 planes [2 rp][ld] of v^T, or as s v^T [r][ld] or s v [R][ld] (and the same to out2).
+enum : int { kL16Planes16 = 0, kL16PlanesTf32 = 1, kL16Transposed = 2, kL16AsRows = 3 };
+struct Lora16Finish {
+    const float* src;
+    int splits, R, pitch, r, rp, mode, from_rows;
+    float s;
+    void* out;
+    float* out2;
+    long long ld;
+};
+int launch_lora16_finish(const Lora16Finish* f, int count, cudaStream_t stream);
 
 }  // namespace q4

@@ -1158,6 +1158,120 @@ void lora_backward_f32(spaceslug_q4_weights* w, const float* x, const float* dy,
     }
 }
 
+// The adapter's gradients with X in 8 bits, into the handle (and to da, db):
+// all four products in bf16 passes (lora16.cu) when dY is bf16 too, with rows
+// of 16 bytes; for fp32 dY the two products of X there and the two of dY in
+// the TF32 passes of lora_tc.cu.
+bool lora_backward_act8_suits(int K, int N, bool bf16) { return K >= 32 && N >= 32 && N % (bf16 ? 8 : 4) == 0; }
+
+void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps, const void* dy, bool bf16,
+                            int M, float* da, float* db, cudaStream_t s) {
+    DeviceCtx& c = ctx_for(w->device);
+    const int K = w->K, N = w->N, r = w->rank, rp = q4::lora16_rp(r), rt = q4::lora_tc_rp(r), G = K / 32;
+    const float scale = w->alpha / static_cast<float>(r);
+    auto round8 = [](int v) { return (static_cast<long long>(v) + 7) / 8 * 8; };
+    const long long Kp = round8(K), Np = round8(N), Mp = round8(M);
+    const int R1[2] = {M, M}, L1[2] = {K, N}, R2[2] = {K, N}, L2[2] = {M, M};
+    int s1[2], s2[2];  // splits of {T, G} and {dA, dB}
+    const int st = q4::lora16_stage();
+    if (bf16) {
+        q4::lora_tc_plan(2, R1, L1, c.sm_count, s1, st);
+        q4::lora_tc_plan(2, R2, L2, c.sm_count, s2, st);
+    } else {
+        q4::lora_tc_plan(1, R1, L1, c.sm_count, s1, st);
+        q4::lora_tc_plan(1, R1 + 1, L1 + 1, c.sm_count, s1 + 1);
+        q4::lora_tc_plan(1, R2, L2, c.sm_count, s2, st);
+        q4::lora_tc_plan(1, R2 + 1, L2 + 1, c.sm_count, s2 + 1);
+    }
+    const int rg = bf16 ? rp : rt;  // padded rank of the dY passes
+    // planes: A^T and G^T (bf16), B and T^T (bf16 or TF32); partial sums of both passes
+    const size_t pl16 = static_cast<size_t>(3) * rp * 2, plY = bf16 ? pl16 : static_cast<size_t>(2) * rt * 4;
+    auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+    const size_t bA = up(pl16 * Kp), bG = up(pl16 * Mp), bB = up(plY * Np), bT = up(plY * Mp);
+    const size_t pT = up(static_cast<size_t>(s1[0]) * M * rp * 4), pG = up(static_cast<size_t>(s1[1]) * M * rg * 4);
+    const size_t pA = up(static_cast<size_t>(s2[0]) * K * rp * 4), pB = up(static_cast<size_t>(s2[1]) * N * rg * 4);
+    Scratch sc(bA + bG + bB + bT + std::max(pT + pG, pA + pB), s);
+    char* at = static_cast<char*>(sc.p);
+    char *gt = at + bA, *bt = gt + bG, *tt = bt + bB, *part = tt + bT;
+    float *partT = reinterpret_cast<float*>(part), *partG = reinterpret_cast<float*>(part + pT);
+    float *partA = reinterpret_cast<float*>(part), *partB = reinterpret_cast<float*>(part + pA);
+    const auto I8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const auto B16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const auto F32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    const auto SW = CU_TENSOR_MAP_SWIZZLE_128B;
+    auto planes16 = [&](q4::Lora16Problem& q, const void* plane, int L) {
+        encode_2d(&q.tm_b, B16, plane, static_cast<uint64_t>(L), static_cast<uint64_t>(3 * rp), round8(L) * 2, 64,
+                  static_cast<uint32_t>(3 * rp), SW);
+    };
+    auto x_problem = [&](q4::Lora16Problem& q, bool mn, const void* plane, int splits, float* partial) {
+        q = {};
+        encode_2d(&q.tm_a, I8, codes, static_cast<uint64_t>(K), static_cast<uint64_t>(M), static_cast<uint64_t>(K),
+                  mn ? 128 : 64, mn ? 64 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B);
+        planes16(q, plane, mn ? M : K);
+        q.exps = exps;
+        q.partial = partial;
+        q.R = mn ? K : M;
+        q.L = mn ? M : K;
+        q.splits = splits;
+        q.act8 = 1;
+        q.groups = G;
+    };
+    auto y16_problem = [&](q4::Lora16Problem& q, bool mn, const void* plane, int splits, float* partial) {
+        q = {};
+        encode_2d(&q.tm_a, B16, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(N) * 2,
+                  mn ? 128 : 64, mn ? 64 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
+        planes16(q, plane, mn ? M : N);
+        q.partial = partial;
+        q.R = mn ? N : M;
+        q.L = mn ? M : N;
+        q.splits = splits;
+    };
+    auto y32_pass = [&](bool mn, const void* plane, int splits, float* partial) {
+        q4::LoraTcPass p{};
+        p.count = 1;
+        p.rp = rt;
+        p.sm_count = c.sm_count;
+        p.status = c.status;
+        p.mn_major = mn ? 1 : 0;
+        q4::LoraTcProblem& q = p.prob[0];
+        encode_2d(&q.tm_a, F32, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(N) * 4,
+                  mn ? 128 : 32, mn ? 32 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
+        const int L = mn ? M : N;
+        encode_2d(&q.tm_b, F32, plane, static_cast<uint64_t>(L), static_cast<uint64_t>(2 * rt), round8(L) * 4, 32,
+                  static_cast<uint32_t>(2 * rt), SW);
+        q.partial = partial;
+        q.R = mn ? N : M;
+        q.L = L;
+        q.splits = splits;
+        check_launch(q4::launch_lora_tc_pass(p, s), "lora pass (fp32 dY)");
+    };
+    const int planesY = bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32;
+    q4::Lora16Finish f[2];
+    f[0] = {w->lora_a, 1, K, r, r, rp, q4::kL16Planes16, 0, 1.0f, at, nullptr, Kp};
+    f[1] = {w->lora_b, 1, N, N, r, rg, planesY, 1, 1.0f, bt, nullptr, Np};
+    check_launch(q4::launch_lora16_finish(f, 2, s), "lora A / B planes");
+    q4::Lora16Pass p{};
+    p.rp = rp;
+    p.sm_count = c.sm_count;
+    p.status = c.status;
+    p.count = bf16 ? 2 : 1;
+    x_problem(p.prob[0], false, at, s1[0], partT);
+    if (bf16) y16_problem(p.prob[1], false, bt, s1[1], partG);
+    check_launch(q4::launch_lora16_pass(p, s), "lora T / G pass");
+    if (!bf16) y32_pass(false, bt, s1[1], partG);
+    f[0] = {partT, s1[0], M, rp, r, rg, planesY, 0, 1.0f, tt, nullptr, Mp};
+    f[1] = {partG, s1[1], M, rg, r, rp, q4::kL16Planes16, 0, 1.0f, gt, nullptr, Mp};
+    check_launch(q4::launch_lora16_finish(f, 2, s), "lora T / G planes");
+    p.mn_major = 1;
+    x_problem(p.prob[0], true, gt, s2[0], partA);
+    if (bf16) y16_problem(p.prob[1], true, tt, s2[1], partB);
+    check_launch(q4::launch_lora16_pass(p, s), "lora dA / dB pass");
+    if (!bf16) y32_pass(true, tt, s2[1], partB);
+    f[0] = {partA, s2[0], K, rp, r, rp, q4::kL16AsRows, 0, scale, w->lora_da, da, r};
+    f[1] = {partB, s2[1], N, rg, r, rg, q4::kL16Transposed, 0, scale, w->lora_db, db, N};
+    check_launch(q4::launch_lora16_finish(f, 2, s), "lora dA / dB");
+}
+
 // Rows up to which the training products stream the weights on the CUDA cores
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
 constexpr int kRowsKernelMax = 8;
@@ -2079,7 +2193,11 @@ int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_
         if (!w->lora_da) check(cudaMalloc(&w->lora_da, pa), "cudaMalloc dA");
         if (!w->lora_db) check(cudaMalloc(&w->lora_db, pbb), "cudaMalloc dB");
         const int M = static_cast<int>(m);
-        // X (and a bf16 dY) restored in fp32, then the fp32 backward
+        if (lora_backward_act8_suits(w->K, w->N, dtype == SPACESLUG_BF16)) {
+            run_lora_backward_act8(w, codes, exps, dy, dtype == SPACESLUG_BF16, M, da, db, s);
+            return SPACESLUG_OK;
+        }
+        // rows of dY that no 16-byte copy can follow: X (and a bf16 dY) restored in fp32, then the fp32 backward
         Scratch xs(static_cast<size_t>(M) * w->K * 4, s);
         Scratch ys(dtype == SPACESLUG_BF16 ? static_cast<size_t>(M) * w->N * 4 : 0, s);
         check_launch(q4::launch_act8_unpack(codes, exps, xs.p, false, static_cast<long long>(M) * (w->K / 32), s),
