@@ -137,19 +137,29 @@ __device__ __forceinline__ void regs_inc() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
 }
 
-// Eight weights of one word as f16 hi (and, with PB = 2, lo) parts: v exact,
+// Eight weights of one word as four f16 pairs of hi (and, with PB = 2, lo)
+// parts.  With every nibble's sign bit flipped (v + 8), one LOP3 puts nibbles
+// i and i + 4 under f16's 1024 in the two halves of a register, so a pair
+// holds k = (0, 4), (1, 5), (2, 6), (3, 7): the operands' order within each 8
+// is 0 4 1 5 2 6 3 7 (18 instructions per word; keeping k in order takes a
+// byte permute and a second LOP3 per pair, 24).  The logits' rows are stored
+// in that order by the cast; of the transposed product it is the order of the
+// accumulator's columns, undone by the epilogue's choice of registers.
 // hi = RN16(v s_hi + RN16(v s_lo)) as in dequant_word_f16x2, lo = (v s_hi -
 // hi) + RN16(v s_lo), whose bracket is exact, so hi + lo is v s to 2^-22.
 template <int PB>
 __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_lo, uint4& hi, uint4& lo) {
-    const __half2 mul = __halves2half2(__ushort_as_half(0x3C00u), __ushort_as_half(0x2C00u));  // 1, 1/16
-    const __half2 add = __halves2half2(__ushort_as_half(0xE408u), __ushort_as_half(0xD480u));  // -1032, -72
+    const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00u));  // 1/16
+    const __half2 bias0 = __half2half2(__ushort_as_half(0xE408u));      // -1032: 1024 + (v + 8)
+    const __half2 bias1 = __half2half2(__ushort_as_half(0xD480u));      // -72: (1024 + 16 (v + 8)) / 16
+    const uint32_t x = q ^ 0x88888888u, y = x >> 8;
+    uint32_t t[4] = {(x & 0x000F000Fu) | 0x64006400u, (x & 0x00F000F0u) | 0x64006400u,
+                     (y & 0x000F000Fu) | 0x64006400u, (y & 0x00F000F0u) | 0x64006400u};
     uint32_t h[4], l[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-        const uint32_t both = __byte_perm(q, 0u, 0x4040u | (static_cast<uint32_t>(b) << 8) | static_cast<uint32_t>(b));
-        const uint32_t t = ((both ^ 0x00800008u) & 0x00F0000Fu) | 0x64006400u;
-        const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&t), mul, add);
+        const __half2 u = *reinterpret_cast<const __half2*>(&t[b]);
+        const __half2 v = (b & 1) ? __hfma2(u, sixteenth, bias1) : __hadd2(u, bias0);
         const __half2 c = __hmul2(v, s_lo);
         const __half2 w = __hfma2(v, s_hi, c);
         h[b] = *reinterpret_cast<const uint32_t*>(&w);
@@ -161,6 +171,8 @@ __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_l
     hi = make_uint4(h[0], h[1], h[2], h[3]);
     if constexpr (PB == 2) lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
+// Place of k (0..7) in that order.
+__host__ __device__ constexpr int gg_place(int k) { return k < 4 ? 2 * k : 2 * (k - 4) + 1; }
 
 struct GgUnit {
     int mt, ct, z, c0, c1;  // row tile, column tile, split, chunks [c0, c1)
@@ -391,6 +403,17 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                     break;
                 }
                 uint8_t* dst = smem + s * C::kStageBytes + PA * kGgTile + out_row;
+                if (TR && st == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
+                    const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
+#pragma unroll
+                    for (int p = 0; p < PB; ++p) {
+                        const uint4* src = reinterpret_cast<const uint4*>(
+                            static_cast<const __half*>(P.lora_at) + static_cast<size_t>(p * 64 + row) * P.ld_at + k0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint4*>(dst + p * kGgTile + ((i ^ (row & 7)) << 4)) = __ldg(src + i);
+                    }
+                } else
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     __half2 s_hi, s_lo;
@@ -534,24 +557,6 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[i][j] *= scale;
-                if (P.rank > 0) {
-                    // + G A^T in fp32: this row's G (scaled by alpha / r), columns of A^T read by the whole warp at once
-                    const float* gr = P.lora_g + static_cast<size_t>(min(row, P.M - 1)) * P.rank;
-                    for (int j = 0; j < P.rank; ++j) {
-                        const float gv = __ldg(gr + j);
-                        const float4* at = reinterpret_cast<const float4*>(P.lora_at + static_cast<size_t>(j) * P.ld_at + col0);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 a = __ldg(at + i * 8 + e);
-                                acc[i][4 * e] = fmaf(gv, a.x, acc[i][4 * e]);
-                                acc[i][4 * e + 1] = fmaf(gv, a.y, acc[i][4 * e + 1]);
-                                acc[i][4 * e + 2] = fmaf(gv, a.z, acc[i][4 * e + 2]);
-                                acc[i][4 * e + 3] = fmaf(gv, a.w, acc[i][4 * e + 3]);
-                            }
-                    }
-                }
                 constexpr int kBlocks = EPI == kGgBf16 ? 2 : 4;  // 128 bytes of each row: 64 bf16 or 32 fp32
                 const int orow = w.z * P.out_rows + row0;
 #pragma unroll
@@ -565,14 +570,18 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                             uint32_t q[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 hv = __floats2bfloat162_rn(acc[2 * h + e / 4][(e % 4) * 8 + 2 * j],
-                                                                                acc[2 * h + e / 4][(e % 4) * 8 + 2 * j + 1]);
+                                const __nv_bfloat162 hv =
+                                    __floats2bfloat162_rn(acc[2 * h + e / 4][(e % 4) * 8 + gg_place(2 * j)],
+                                                          acc[2 * h + e / 4][(e % 4) * 8 + gg_place(2 * j + 1)]);
                                 q[j] = *reinterpret_cast<const uint32_t*>(&hv);
                             }
                             o = make_uint4(q[0], q[1], q[2], q[3]);
                         } else {
-                            o = make_uint4(__float_as_uint(acc[h][4 * e]), __float_as_uint(acc[h][4 * e + 1]),
-                                           __float_as_uint(acc[h][4 * e + 2]), __float_as_uint(acc[h][4 * e + 3]));
+                            const int g8 = (e / 2) * 8, k4 = (e % 2) * 4;
+                            o = make_uint4(__float_as_uint(acc[h][g8 + gg_place(k4)]),
+                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 1)]),
+                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 2)]),
+                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 3)]));
                         }
                         gg_stage_row(buf, lane, e, o);
                     }
@@ -654,17 +663,80 @@ int gg_launch(const GradGemmArgs& a, cudaStream_t stream) {
 // ------------------------------------------------------------------ helpers --
 __device__ __forceinline__ float gg_in(const float* p) { return *p; }
 __device__ __forceinline__ float gg_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void gg_in8(const float* p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void gg_in8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
 
-// One block per row: f16 planes of row * 2^e, e such that the row's largest
-// magnitude lies in [2^13, 2^14); lo = the f16 rounding of what hi leaves.
+// One block per row: f16 planes [planes][M][ld] of row * 2^e, e such that the
+// largest magnitude lies in [2^13, 2^14); lo = the f16 rounding of what hi
+// leaves.  Columns past the row are zero.  With an adapter the last 64 columns
+// are the row's G = s dY B^T (the sum of its partial products) times 2^gexp[j],
+// the exponents that A^T's planes were scaled down by, so that G A^T is 64
+// more terms of the same contraction; the row's exponent covers them too.
+// Thread t takes pieces of 8 columns t, t + 256, ...; the first kCastKeep of
+// them stay in registers between the maximum and the rounding.
+constexpr int kCastKeep = 6;
 template <typename T, int PA>
-__global__ void __launch_bounds__(256) cast_planes_kernel(const T* __restrict__ x, __half* __restrict__ planes,
-                                                          int* __restrict__ row_exp, int M, int cols, long long ld) {
+__global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     __shared__ float red[8];
+    __shared__ float gs[64];
+    pdl_launch_dependents();
+    pdl_wait();
     const long long m = blockIdx.x;
-    const T* row = x + m * cols;
+    const T* row = static_cast<const T*>(A.x) + m * A.cols;
+    const bool vec = A.cols % 8 == 0;
+    const int pieces = (A.cols + 7) / 8;
+    auto get = [&](int p, float (&v)[8]) {
+        if (vec) {
+            gg_in8(row + p * 8, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < A.cols ? gg_in(row + p * 8 + i) : 0.0f;
+        }
+    };
+    float keep[kCastKeep][8];
     float top = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += 256) top = fmaxf(top, fabsf(gg_in(row + c)));
+#pragma unroll
+    for (int k = 0; k < kCastKeep; ++k) {
+        const int p = threadIdx.x + 256 * k;
+        if (p < pieces) {
+            get(p, keep[k]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) keep[k][i] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kCastKeep; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(keep[k][i]));
+    for (int p = threadIdx.x + 256 * kCastKeep; p < pieces; p += 256) {
+        float v[8];
+        get(p, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    }
+    if (A.rank > 0 && threadIdx.x < 64) {
+        float g = 0.0f;
+        if (threadIdx.x < A.rank) {
+            for (int z = 0; z < A.gsplits; ++z)
+                g += A.gpart[(static_cast<long long>(z) * A.M + m) * A.gpitch + threadIdx.x];
+            g = ldexpf(g * A.gscale, A.gexp[threadIdx.x]);
+        }
+        gs[threadIdx.x] = g;
+        top = fmaxf(top, fabsf(g));
+    }
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -675,15 +747,42 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const T* __restrict__ 
         frexpf(top, &e2);
         e = min(max(14 - e2, -120), 120);
     }
-    if (threadIdx.x == 0) row_exp[m] = e;
+    if (threadIdx.x == 0) A.row_exp[m] = e;
     const float s = exp2i(e);
-    __half* hi = planes + m * ld;
-    __half* lo = planes + (static_cast<long long>(M) + m) * ld;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-        const float v = gg_in(row + c) * s;
-        const __half h = __float2half_rn(v);
-        hi[c] = h;
-        if constexpr (PA == 2) lo[c] = __float2half_rn(v - __half2float(h));
+    __half* hi = static_cast<__half*>(A.out) + m * A.ld;
+    auto put = [&](int p, const float (&v)[8]) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // in order, or as (0, 4), (1, 5), (2, 6), (3, 7): the order of the dequantised words
+            const float a = (A.by_word ? v[i] : v[2 * i]) * s, b = (A.by_word ? v[i + 4] : v[2 * i + 1]) * s;
+            const __half2 hv = __floats2half2_rn(a, b);
+            h[i] = *reinterpret_cast<const uint32_t*>(&hv);
+            if constexpr (PA == 2) {
+                const __half2 lv = __floats2half2_rn(a - __low2float(hv), b - __high2float(hv));
+                l[i] = *reinterpret_cast<const uint32_t*>(&lv);
+            }
+        }
+        *reinterpret_cast<uint4*>(hi + p * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+        if constexpr (PA == 2)
+            *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+#pragma unroll
+    for (int k = 0; k < kCastKeep; ++k) {
+        const int p = threadIdx.x + 256 * k;
+        if (p < pieces) put(p, keep[k]);
+    }
+    for (int p = threadIdx.x + 256 * kCastKeep; p < pieces; p += 256) {
+        float v[8];
+        get(p, v);
+        put(p, v);
+    }
+    const int end = static_cast<int>(A.ld / 8), gp = A.rank > 0 ? end - 8 : end;
+    for (int p = pieces + threadIdx.x; p < end; p += 256) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = p >= gp ? gs[(p - gp) * 8 + i] : 0.0f;
+        put(p, v);
     }
 }
 
@@ -801,12 +900,51 @@ __global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ 
     }
 }
 
-// A [K][r] -> A^T [r][ld], zeros past K.
-__global__ void __launch_bounds__(256) lora_at_kernel(const float* __restrict__ a, float* __restrict__ at, int K,
-                                                      int rank, int ld) {
-    const int k = blockIdx.x * 256 + threadIdx.x;
-    if (k >= ld) return;
-    for (int j = 0; j < rank; ++j) at[static_cast<size_t>(j) * ld + k] = k < K ? a[static_cast<size_t>(k) * rank + j] : 0.0f;
+// One block per rank j < 64: f16 planes [planes][64][ld] of A^T's row j times
+// 2^E_j, E_j such that its largest magnitude lies in [2^13, 2^14) (k in the
+// dequantised words' order, zeros past K and past the rank), and the exponent
+// w_exp - E_j that G's column j carries in exchange.
+__global__ void __launch_bounds__(256) lora_at_kernel(const float* __restrict__ a, __half* __restrict__ at,
+                                                      int* __restrict__ gexp, const int* __restrict__ w_exp, int K,
+                                                      int rank, int ld, int planes) {
+    __shared__ float red[8];
+    const int j = blockIdx.x;
+    float top = 0.0f;
+    if (j < rank)
+        for (int k = threadIdx.x; k < K; k += 256) top = fmaxf(top, fabsf(a[static_cast<size_t>(k) * rank + j]));
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, red[i]);
+    int e = 0;
+    if (top > 0.0f && isfinite(top)) {
+        int e2;
+        frexpf(top, &e2);
+        e = min(max(14 - e2, -120), 120);
+    }
+    if (threadIdx.x == 0) gexp[j] = *w_exp - e;
+    const float s = exp2i(e);
+    for (int i = threadIdx.x; i < ld; i += 256) {
+        const int k = (i & ~7) + (i & 1) * 4 + ((i & 7) >> 1);  // place i holds k
+        const float v = j < rank && k < K ? a[static_cast<size_t>(k) * rank + j] * s : 0.0f;
+        const __half h = __float2half_rn(v);
+        at[static_cast<size_t>(j) * ld + i] = h;
+        if (planes == 2) at[static_cast<size_t>(64 + j) * ld + i] = __float2half_rn(v - __half2float(h));
+    }
+}
+
+template <typename Kern, typename Arg>
+int gg_launch_pdl(Kern kern, unsigned grid, cudaStream_t stream, const Arg& arg) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, arg));
 }
 
 }  // namespace
@@ -827,17 +965,11 @@ int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t st
     return static_cast<int>(cudaErrorInvalidValue);
 }
 
-int launch_cast_planes(const void* x, bool bf16, int planes, void* out, int* row_exp, int M, int cols, long long ld,
-                       cudaStream_t stream) {
-    __half* o = static_cast<__half*>(out);
-    if (bf16)
-        cast_planes_kernel<__nv_bfloat16, 1><<<M, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), o, row_exp, M,
-                                                                    cols, ld);
-    else if (planes == 2)
-        cast_planes_kernel<float, 2><<<M, 256, 0, stream>>>(static_cast<const float*>(x), o, row_exp, M, cols, ld);
-    else
-        return static_cast<int>(cudaErrorInvalidValue);
-    return static_cast<int>(cudaGetLastError());
+int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream) {
+    if (a.M < 1 || a.ld % 8 != 0 || a.ld < a.cols || a.rank > 64) return static_cast<int>(cudaErrorInvalidValue);
+    if (bf16) return gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1>, static_cast<unsigned>(a.M), stream, a);
+    if (planes == 2) return gg_launch_pdl(cast_planes_kernel<float, 2>, static_cast<unsigned>(a.M), stream, a);
+    return static_cast<int>(cudaErrorInvalidValue);
 }
 
 int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int K, cudaStream_t stream) {
@@ -863,8 +995,9 @@ int launch_loss_dx(const float* partial, int splits, long long out_rows, const f
     return static_cast<int>(cudaGetLastError());
 }
 
-int launch_lora_at(const float* a, float* at, int K, int rank, int ld, cudaStream_t stream) {
-    lora_at_kernel<<<(ld + 255) / 256, 256, 0, stream>>>(a, at, K, rank, ld);
+int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K, int rank, int ld, int planes,
+                   cudaStream_t stream) {
+    lora_at_kernel<<<64, 256, 0, stream>>>(a, static_cast<__half*>(at), gexp, w_exp, K, rank, ld, planes);
     return static_cast<int>(cudaGetLastError());
 }
 

@@ -341,9 +341,8 @@ struct GradGemmArgs {
     int row_tiles, col_tiles, splits;
     int stages, chunk, chunks;  // 64-wide stages of the contraction, stages per accumulator chunk, chunks
     const float* coef;       // [chunks][ld_stat] factor of a row's chunk, or nullptr
-    const float* lora_g;     // [M][rank] (scaled), lora_at [rank][ld_at]; rank 0: none
-    const float* lora_at;
-    int rank, ld_at;
+    const void* lora_at;     // transposed product with an adapter: f16 planes [planes][64][ld_at] of A^T, the operand
+    int lora_stage, ld_at;   // of stage lora_stage (-1: none), whose 64 row columns hold G
     const long long* targets;  // logits: [M]
     float* zt;               // [M] the target's logit
     float* smax;             // [col_tiles][ld_stat]
@@ -353,9 +352,21 @@ struct GradGemmArgs {
 };
 int grad_gemm_pairs();  // co-resident CTA pairs on the current device
 int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream);
-// f16 planes [planes][M][ld] of fp32 (2 planes) or bf16 (1) rows scaled by 2^row_exp
-int launch_cast_planes(const void* x, bool bf16, int planes, void* out, int* row_exp, int M, int cols, long long ld,
-                       cudaStream_t stream);
+// f16 planes [planes][M][ld] of fp32 (2 planes) or bf16 (1) rows scaled by 2^row_exp; by_word: each 8 columns in the
+// order 0 4 1 5 2 6 3 7; with an adapter (rank > 0) the last 64 columns hold gscale * sum of gpart [gsplits][M][gpitch].
+struct CastArgs {
+    const void* x;
+    void* out;
+    int* row_exp;
+    int M, cols;
+    long long ld;
+    int by_word;
+    const float* gpart;
+    const int* gexp;
+    int rank, gsplits, gpitch;
+    float gscale;
+};
+int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream);
 int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int K, cudaStream_t stream);
 // tile statistics -> chunk factors (in smax), row sums, loss and lse
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
@@ -363,7 +374,8 @@ int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long
 int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const long long* targets,
                    const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream);
-int launch_lora_at(const float* a, float* at, int K, int rank, int ld, cudaStream_t stream);
+int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K, int rank, int ld, int planes,
+                   cudaStream_t stream);
 
 // LoRA gradients with wide operands exact in bf16 (lora16.cu): a problem is partial[split][row][rp] of D[R x r] = sum
 // over l < L of Aop[row][l] Bop[j][l].  tm_a: bf16 (K-major box 64 l x 128 rows, 128B swizzle; MN-major box 128 rows x

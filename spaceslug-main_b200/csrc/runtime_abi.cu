@@ -1327,13 +1327,26 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         return;
     }
     DeviceCtx& c = ctx_for(w->device);
-    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
+    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
     const size_t size = bf16 ? 2 : 4;
-    const long long ld = (static_cast<long long>(N) + 7) / 8 * 8, ld_at = (static_cast<long long>(K) + 255) / 256 * 256;
-    const float lscale = w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f;
-    Scratch at(w->rank > 0 ? static_cast<size_t>(w->rank) * ld_at * 4 : 0, s);
-    if (w->rank > 0)
-        check_launch(q4::launch_lora_at(w->lora_a, static_cast<float*>(at.p), K, w->rank, static_cast<int>(ld_at), s), "A^T");
+    // contraction: N padded to whole 64-wide stages, and one more stage for the adapter's G A^T
+    const int wstages = (N + 63) / 64;
+    const long long ld = 64ll * (wstages + (r > 0 ? 1 : 0)), ld_at = (static_cast<long long>(K) + 255) / 256 * 256;
+    Scratch at(r > 0 ? static_cast<size_t>(planes) * 64 * ld_at * 2 : 0, s);
+    Scratch gexp(r > 0 ? 64 * sizeof(int) : 0, s);
+    const bool gt = r > 0 && N >= 32 && N % (bf16 ? 8 : 4) == 0;  // G by the tensor-core passes
+    const int rp = gt ? (bf16 ? q4::lora16_rp(r) : q4::lora_tc_rp(r)) : r;
+    const long long np = (static_cast<long long>(N) + 7) / 8 * 8;
+    Scratch bp(gt ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0, s);
+    if (r > 0)
+        check_launch(q4::launch_lora_at(w->lora_a, at.p, static_cast<int*>(gexp.p), w->col_exp + N, K, r,
+                                        static_cast<int>(ld_at), planes, s),
+                     "A^T planes");
+    if (gt) {
+        const q4::Lora16Finish f{w->lora_b, 1, N, N, r, rp, bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32, 1, 1.0f, bp.p,
+                                 nullptr, np};
+        check_launch(q4::launch_lora16_finish(&f, 1, s), "B planes");
+    }
     const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0);
@@ -1343,7 +1356,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.M = mc; g.N = N; g.K = K;
         g.row_tiles = (mc + 255) / 256;
         g.col_tiles = (K + 255) / 256;
-        g.stages = (N + 63) / 64;
+        g.stages = static_cast<int>(ld / 64);
         g.chunk = 8;
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.splits = grad_splits(static_cast<long long>(g.row_tiles) * g.col_tiles, g.chunks,
@@ -1352,13 +1365,46 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.plane_rows = mc;
         Scratch x16(static_cast<size_t>(planes) * mc * ld * 2, s);
         Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
-        Scratch gs(static_cast<size_t>(mc) * w->rank * 4, s);
         Scratch part(g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0, s);
-        check_launch(q4::launch_cast_planes(d, bf16, planes, x16.p, static_cast<int*>(rexp.p), mc, N, ld, s), "dY planes");
-        if (w->rank > 0)
-            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, lscale, static_cast<float*>(gs.p), mc, N, w->rank, s),
-                         "dY B^T");
-        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(N),
+        int gsplits = 1;
+        if (gt) q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
+        Scratch gs(r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0, s);
+        float* gpart = static_cast<float*>(gs.p);
+        if (gt && bf16) {
+            q4::Lora16Pass p{};
+            p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
+            q4::Lora16Problem& q = p.prob[0];
+            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
+                      static_cast<uint64_t>(N) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, bp.p, static_cast<uint64_t>(N),
+                      static_cast<uint64_t>(3 * rp), static_cast<uint64_t>(np) * 2, 64, static_cast<uint32_t>(3 * rp),
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+            q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
+            check_launch(q4::launch_lora16_pass(p, s), "dY B^T");
+        } else if (gt) {
+            q4::LoraTcPass p{};
+            p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
+            q4::LoraTcProblem& q = p.prob[0];
+            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
+                      static_cast<uint64_t>(N) * 4, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, bp.p, static_cast<uint64_t>(N),
+                      static_cast<uint64_t>(2 * rp), static_cast<uint64_t>(np) * 4, 32, static_cast<uint32_t>(2 * rp),
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+            q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
+            check_launch(q4::launch_lora_tc_pass(p, s), "dY B^T");
+        } else if (r > 0) {
+            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, 1.0f, gpart, mc, N, r, s), "dY B^T");
+        }
+        q4::CastArgs ca{};
+        ca.x = d; ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
+        ca.M = mc; ca.cols = N; ca.ld = ld;
+        if (r > 0) {
+            ca.gpart = gpart; ca.gexp = static_cast<int*>(gexp.p);
+            ca.rank = r; ca.gsplits = gsplits; ca.gpitch = rp;
+            ca.gscale = w->alpha / static_cast<float>(r);
+        }
+        check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "dY planes");
+        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(ld),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(ld) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         const bool direct16 = bf16 && g.splits == 1;
         if (direct16)
@@ -1370,17 +1416,14 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
                       static_cast<uint64_t>(K) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
         g.packed = w->packed; g.scales = w->scales; g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
-        if (g.splits == 1 && w->rank > 0) {
-            g.rank = w->rank;
-            g.lora_g = static_cast<float*>(gs.p);
-            g.lora_at = static_cast<float*>(at.p);
-            g.ld_at = static_cast<int>(ld_at);
-        }
+        g.lora_at = at.p;
+        g.ld_at = static_cast<int>(ld_at);
+        g.lora_stage = r > 0 ? wstages : -1;
         g.status = c.status;
         check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, s), "dY W^T");
         if (g.splits > 1)
             check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), g.splits, static_cast<long long>(g.out_rows) * K,
-                                                static_cast<float*>(gs.p), w->lora_a, w->rank, out, bf16, mc, K, s),
+                                                nullptr, nullptr, 0, out, bf16, mc, K, s),
                          "dX");
     }
 }
@@ -1434,9 +1477,12 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         float* ssum = smax + static_cast<size_t>(tiles) * mp;
         float* zt = ssum + static_cast<size_t>(2) * tiles * mp;
         float* total = zt + mp;
-        check_launch(q4::launch_cast_planes(static_cast<const char*>(x) + static_cast<size_t>(m0) * K * size, bf16, planes,
-                                            x16.p, static_cast<int*>(rexp.p), mc, K, K, s),
-                     "X planes");
+        q4::CastArgs ca{};
+        ca.x = static_cast<const char*>(x) + static_cast<size_t>(m0) * K * size;
+        ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
+        ca.M = mc; ca.cols = K; ca.ld = K;
+        ca.by_word = 1;
+        check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "X planes");
         q4::GradGemmArgs g{};
         g.M = mc; g.N = N; g.K = K;
         g.row_tiles = mp / 256;
@@ -1452,6 +1498,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.targets = targets + m0;
         g.zt = zt; g.smax = smax; g.ssum = ssum;
         g.ld_stat = mp;
+        g.lora_stage = -1;
         g.status = c.status;
         encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(K),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
