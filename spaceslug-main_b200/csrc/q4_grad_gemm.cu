@@ -31,8 +31,9 @@
 //
 // Roles (16 warps, 4 warpgroups): warp 0 loads the f16 planes of 128 rows per
 // CTA (TMA, 128-byte swizzled boxes of 64), warp 1 of the leader issues the
-// MMAs (M = 256, N = 256, K = 16); warps 4-7 fetch packed words and scales
-// with cp.async into a private ring and dequantise; warps 8-15 hold 128 fp32
+// MMAs (M = 256, N = 256, K = 16); warp 3 loads packed words and scales (TMA:
+// as cp.async copies, 16 or 4 bytes from a different row per lane, they took
+// 512 of a stage's shared-memory cycles); warps 4-7 dequantise; warps 8-15 hold 128 fp32
 // sums per thread (thread = row, two warps per tensor-memory lane quarter)
 // and run the epilogue while the MMAs fill the other accumulator buffer.
 // Every wait is bounded (status word + abort flag).
@@ -58,11 +59,13 @@ constexpr int kGgCols = 256;   // columns of the pair's tile
 constexpr int kGgBK = 64;      // contraction per stage
 constexpr int kGgHalf = 128;
 constexpr int kGgTile = kGgHalf * kGgBK * 2;  // 16 KB: 128 rows of 64 f16
-constexpr int kGgRing = 6;     // stages of packed words and scales in flight per dequant thread
-constexpr int kGgRingBytes = 128 * 40;
+constexpr int kGgOutBytes = 4096;  // one block of 32 rows x 128 bytes per epilogue warp
+// Raw weights: blocks of 128 n x 128 k (two stages of either product), 64
+// bytes of words per n (64-byte swizzled) and 4 scales.
+constexpr int kGgRaw = 3;
+constexpr int kGgRawWords = 128 * 64, kGgRawBytes = kGgRawWords + 128 * 16;
 constexpr int kGgDeqWarp0 = 4, kGgDeqWarps = 4;
 constexpr int kGgEpiWarp0 = 8, kGgEpiWarps = 8;
-constexpr int kGgStageOut = 4096;  // one 32 x 128-byte block per epilogue warp
 // Registers per thread after the split: the launch's 512 x 128 cover 128 x 40 + 128 x 64 + 256 x 200.
 constexpr int kGgRegsLaunch = 128, kGgRegsCtl = 40, kGgRegsDeq = 64, kGgRegsEpi = 200;
 static_assert(128 * kGgRegsCtl + 128 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThreads * kGgRegsLaunch, "register split");
@@ -72,12 +75,12 @@ struct GgCfg {
     static constexpr int kStageBytes = (PA + PB) * kGgTile;
     static constexpr int kStages = PA + PB == 2 ? 5 : PA + PB == 3 ? 3 : 2;
     static constexpr int kOutOff = kStages * kStageBytes;
-    static constexpr int kRingOff = kOutOff + kGgEpiWarps * kGgStageOut;
-    static constexpr int kXchOff = kRingOff + kGgRing * kGgRingBytes;  // [2 buffers][2 halves][128 rows] floats
+    static constexpr int kRawOff = kOutOff + kGgEpiWarps * kGgOutBytes;
+    static constexpr int kXchOff = kRawOff + kGgRaw * kGgRawBytes;  // [2 buffers][2 halves][128 rows] floats
     static constexpr int kBarOff = kXchOff + 2 * 2 * 128 * 4;
     // full_x[S], full_w[S] (leader), empty[S] (both), acc_full[2] (both), acc_empty[2] (leader), done (leader),
-    // xch[4] (own)
-    static constexpr int kNumBars = 3 * kStages + 9;
+    // xch[4], full_r[R], empty_r[R] (own)
+    static constexpr int kNumBars = 3 * kStages + 9 + 2 * kGgRaw;
     static constexpr int kMiscOff = kBarOff + kNumBars * 8;
     static constexpr int kBytes = kMiscOff + 16;
     static constexpr int kSmem = kBytes + 1024;
@@ -98,9 +101,6 @@ __device__ __forceinline__ uint64_t gg_desc_mn_sw128(uint32_t addr, uint32_t lbo
     return d;
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -189,7 +189,7 @@ __device__ __forceinline__ GgUnit gg_unit(const GradGemmArgs& P, int u) {
     return w;
 }
 
-// Stores a 128-byte row per lane (eight 16-byte pieces) of a warp's 32-row
+// Stores 16-byte piece `piece` of lane's 128-byte row of a warp's 32-row
 // block, 128-byte swizzled as its tensor map expects.
 __device__ __forceinline__ void gg_stage_row(uint8_t* buf, int lane, int piece, uint4 v) {
     *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
@@ -211,6 +211,8 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
     auto acc_empty = [&](int b) { return bar + 8u * (3 * ST + 2 + b); };
     const uint32_t done_bar = bar + 8u * (3 * ST + 4);
     auto xch_bar = [&](int q) { return bar + 8u * (3 * ST + 5 + q); };
+    auto full_r = [&](int r) { return bar + 8u * (3 * ST + 9 + r); };
+    auto empty_r = [&](int r) { return bar + 8u * (3 * ST + 9 + kGgRaw + r); };
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kMiscOff + 4);
 
@@ -232,11 +234,17 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
             mbar_init(acc_full(b), 1);
             mbar_init(acc_empty(b), 2 * kGgEpiWarps);
         }
+        for (int r = 0; r < kGgRaw; ++r) {
+            mbar_init(full_r(r), 1);
+            mbar_init(empty_r(r), kGgDeqWarps);
+        }
         mbar_init(done_bar, 1);
         for (int q = 0; q < 4; ++q) mbar_init(xch_bar(q), 2);  // the two warps of a lane quarter
         *abort_flag = 0;
         fence_mbarrier_init();
         tma_prefetch_desc(&P.tm_a);
+        tma_prefetch_desc(&P.tm_w);
+        tma_prefetch_desc(&P.tm_s);
         tma_prefetch_desc(&P.tm_out);
     }
     if (warp == 2) {
@@ -274,6 +282,30 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
             }
             if (*abort_flag && leader)
                 for (int j = (it > ST ? it - ST : 0); j < it; ++j) mbar_drain(full_x(j % ST), (j / ST) & 1u);
+        } else if (warp == 3 && lane == 0) {
+            // ---------------------------------------------- raw weights --
+            int it = 0;
+            bool ok = true;
+            for (int u = pair; u < units && ok; u += npairs) {
+                const GgUnit w = gg_unit(P, u);
+                const int tile0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf;
+                const int s1 = min(w.c1 * P.chunk, P.stages);
+                for (int st = w.c0 * P.chunk; st < s1; st += 2, ++it) {
+                    const int r = it % kGgRaw;
+                    if (!gg_wait(empty_r(r), ((it / kGgRaw) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    const int k0 = TR ? tile0 : st * kGgBK, n0 = TR ? st * kGgBK : tile0;
+                    const uint32_t dst = base + C::kRawOff + r * kGgRawBytes;
+                    mbar_arrive_expect_tx(full_r(r), kGgRawBytes);
+                    tma_load_2d(dst, &P.tm_w, full_r(r), k0 / 8, n0);
+                    tma_load_2d(dst + kGgRawWords, &P.tm_s, full_r(r), k0 / 32, n0);
+                }
+            }
+            if (*abort_flag)
+                for (int j = (it > kGgRaw ? it - kGgRaw : 0); j < it; ++j)
+                    mbar_drain(full_r(j % kGgRaw), (j / kGgRaw) & 1u);
         } else if (warp == 1 && leader && elect_one()) {
             // ------------------------------------------------------- MMA --
             constexpr uint32_t idesc = umma_idesc_f16(0u, kGgRows, kGgCols) | (TR ? (1u << 16) : 0u);
@@ -327,124 +359,91 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
         // ------------------------------------------------------- dequant --
         // Thread t: logits, column n = t of this CTA's 128 and the stage's 64
         // k; transposed, n = t % 64 of the stage's 64 and the 64 k t / 64 of
-        // this CTA's 128.  Either way two scale groups of one n: two 16-byte
-        // words and two scales, copied into the thread's own ring slots.
+        // this CTA's 128.  Either way two scale groups of one n per stage, from
+        // a raw block that holds two stages: the k halves or the n halves.
         regs_dec<kGgRegsDeq>();
         const int t = tid - kGgDeqWarp0 * 32;
-        const uint32_t ring = base + C::kRingOff;
-        const int groups = P.K / 32;
         const float cs = exp2i(*P.w_exp);
         const int row = TR ? (t & 63) : t;  // row of the operand image
         const uint32_t out_row = static_cast<uint32_t>((TR ? (t >> 6) * (kGgTile / 2) : 0) + row * 128);
-        // The fetch side runs kGgRing - 1 stages ahead of the dequant side.  Within
-        // a unit its element index `at` (n * groups + g) moves by a constant.
-        int fu = pair, left = 0, fn = 0, fg = 0;
-        long long at = 0;
-        const long long at_step = TR ? static_cast<long long>(kGgBK) * groups : kGgBK / 32;
-        auto fetch = [&](int slot) {
-            if (left == 0 && fu < units) {
-                const GgUnit fw = gg_unit(P, fu);
-                fu += npairs;
-                const int st0 = fw.c0 * P.chunk;
-                left = min(fw.c1 * P.chunk, P.stages) - st0;
-                fn = TR ? st0 * kGgBK + row : fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + row;
-                fg = TR ? (fw.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64) / 32 : st0 * (kGgBK / 32);
-                at = static_cast<long long>(fn) * groups + fg;
-            }
-            if (left > 0) {
-                const uint32_t dst = ring + slot * kGgRingBytes;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {  // past the matrix: zeros
-                    const bool in = fn < P.N && fg + j < groups;
-                    const long long e = in ? at + j : 0;
-                    cp_async16(dst + j * 2048 + t * 16, P.packed + e * 4, in ? 16u : 0u);
-                    cp_async4(dst + 4096 + j * 512 + t * 4, P.scales + e, in ? 4u : 0u);
-                }
-                --left;
-                at += at_step;
-                if constexpr (TR) {
-                    fn += kGgBK;
-                } else {
-                    fg += kGgBK / 32;
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        // Words and scales of a stage, ring -> registers, one stage ahead of their use.
-        uint4 q[2];
-        float sc[2];
-        auto load = [&](int slot) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kGgRing - 2) : "memory");
-            const uint8_t* rp = smem + C::kRingOff + slot * kGgRingBytes;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                q[j] = *reinterpret_cast<const uint4*>(rp + j * 2048 + t * 16);
-                sc[j] = *reinterpret_cast<const float*>(rp + 4096 + j * 512 + t * 4);
-            }
-        };
-#pragma unroll 1
-        for (int i = 0; i < kGgRing - 1; ++i) fetch(i);
-        load(0);
-        fetch(kGgRing - 1);
-        int slot = 1, s = 0;
+        int it = 0, s = 0;
         uint32_t ph = 1;
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
             const GgUnit w = gg_unit(P, u);
             const int s1 = min(w.c1 * P.chunk, P.stages);
-            for (int st = w.c0 * P.chunk; st < s1; ++st) {
-                const uint4 qc[2] = {q[0], q[1]};
-                const float sv[2] = {sc[0] * cs, sc[1] * cs};
-                load(slot);  // of the next stage (past the last one: stale words that nothing uses)
-                fetch(slot == 0 ? kGgRing - 1 : slot - 1);  // the slot whose words are in qc
-                slot = slot + 1 == kGgRing ? 0 : slot + 1;
-                if (!gg_wait_warp(empty(s), ph, abort_flag, status, kStatusTimeoutDequant)) {
+            for (int st0 = w.c0 * P.chunk; st0 < s1; st0 += 2, ++it) {
+                const int r = it % kGgRaw;
+                if (!gg_wait_warp(full_r(r), (it / kGgRaw) & 1u, abort_flag, status, kStatusTimeoutDequant)) {
                     ok = false;
                     break;
                 }
-                uint8_t* dst = smem + s * C::kStageBytes + PA * kGgTile + out_row;
-                if (TR && st == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
-                    const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
+                const uint8_t* raw = smem + C::kRawOff + r * kGgRawBytes;
+                uint4 q[2][2];
+                float2 sc[2];
 #pragma unroll
-                    for (int p = 0; p < PB; ++p) {
-                        const uint4* src = reinterpret_cast<const uint4*>(
-                            static_cast<const __half*>(P.lora_at) + static_cast<size_t>(p * 64 + row) * P.ld_at + k0);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            *reinterpret_cast<uint4*>(dst + p * kGgTile + ((i ^ (row & 7)) << 4)) = __ldg(src + i);
-                    }
-                } else
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    __half2 s_hi, s_lo;
-                    split_scale_f16(sv[j], s_hi, s_lo);
-                    const uint32_t words[4] = {qc[j].x, qc[j].y, qc[j].z, qc[j].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 hi, lo;
-                        gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
-                        const int o = ((4 * j + i) ^ (row & 7)) << 4;
-                        *reinterpret_cast<uint4*>(dst + o) = hi;
-                        if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
-                    }
+                for (int g = 0; g < 2; ++g) {
+                    const int n = TR ? g * 64 + row : row, h = TR ? t >> 6 : g;  // row and 64-k half of the block
+                    const uint8_t* wr = raw + n * 64;
+                    const int key = (n >> 1) & 3;
+                    q[g][0] = *reinterpret_cast<const uint4*>(wr + (((2 * h) ^ key) << 4));
+                    q[g][1] = *reinterpret_cast<const uint4*>(wr + (((2 * h + 1) ^ key) << 4));
+                    sc[g] = *reinterpret_cast<const float2*>(raw + kGgRawWords + n * 16 + h * 8);
                 }
-                fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_remote(leader_addr(full_w(s)));
-                if (++s == ST) {
-                    s = 0;
-                    ph ^= 1u;
+                if (lane == 0) mbar_arrive(empty_r(r));
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    if (st0 + g >= s1) break;
+                    if (!gg_wait_warp(empty(s), ph, abort_flag, status, kStatusTimeoutDequant)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* dst = smem + s * C::kStageBytes + PA * kGgTile + out_row;
+                    if (TR && st0 + g == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
+                        const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
+#pragma unroll
+                        for (int p = 0; p < PB; ++p) {
+                            const uint4* src = reinterpret_cast<const uint4*>(
+                                static_cast<const __half*>(P.lora_at) + static_cast<size_t>(p * 64 + row) * P.ld_at + k0);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<uint4*>(dst + p * kGgTile + ((i ^ (row & 7)) << 4)) = __ldg(src + i);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            __half2 s_hi, s_lo;
+                            split_scale_f16((j == 0 ? sc[g].x : sc[g].y) * cs, s_hi, s_lo);
+                            const uint32_t words[4] = {q[g][j].x, q[g][j].y, q[g][j].z, q[g][j].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                uint4 hi, lo;
+                                gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
+                                const int o = ((4 * j + i) ^ (row & 7)) << 4;
+                                *reinterpret_cast<uint4*>(dst + o) = hi;
+                                if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_remote(leader_addr(full_w(s)));
+                    if (++s == ST) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
                 }
+                if (!ok) break;
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ------------------------------------------------------ epilogue --
         regs_inc<kGgRegsEpi>();
         const int ew = warp - kGgEpiWarp0, quarter = warp & 3, half = ew >> 2;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
-        uint8_t* buf = smem + C::kOutOff + ew * kGgStageOut;
-        const uint32_t buf_s = base + C::kOutOff + ew * kGgStageOut;
+        uint8_t* buf = smem + C::kOutOff + ew * kGgOutBytes;
+        const uint32_t buf_s = base + C::kOutOff + ew * kGgOutBytes;
         const int row_in = quarter * 32 + lane;  // row of this CTA's 128
         const int wexp = *P.w_exp;
         int cq = 0, xq = 0;
@@ -557,37 +556,38 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) acc[i][j] *= scale;
-                constexpr int kBlocks = EPI == kGgBf16 ? 2 : 4;  // 128 bytes of each row: 64 bf16 or 32 fp32
+                constexpr int kOutCols = EPI == kGgBf16 ? 64 : 32;  // columns of a 128-byte block row
                 const int orow = w.z * P.out_rows + row0;
 #pragma unroll
-                for (int h = 0; h < kBlocks; ++h) {
+                for (int h = 0; h < 128 / kOutCols; ++h) {
                     if (lane == 0) bulk_wait_group_read<0>();
                     __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         uint4 o;
                         if constexpr (EPI == kGgBf16) {
+                            const int c8 = h * kOutCols + e * 8;
                             uint32_t q[4];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const __nv_bfloat162 hv =
-                                    __floats2bfloat162_rn(acc[2 * h + e / 4][(e % 4) * 8 + gg_place(2 * j)],
-                                                          acc[2 * h + e / 4][(e % 4) * 8 + gg_place(2 * j + 1)]);
+                                    __floats2bfloat162_rn(acc[c8 / 32][c8 % 32 + gg_place(2 * j)],
+                                                          acc[c8 / 32][c8 % 32 + gg_place(2 * j + 1)]);
                                 q[j] = *reinterpret_cast<const uint32_t*>(&hv);
                             }
                             o = make_uint4(q[0], q[1], q[2], q[3]);
                         } else {
-                            const int g8 = (e / 2) * 8, k4 = (e % 2) * 4;
-                            o = make_uint4(__float_as_uint(acc[h][g8 + gg_place(k4)]),
-                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 1)]),
-                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 2)]),
-                                           __float_as_uint(acc[h][g8 + gg_place(k4 + 3)]));
+                            const int c4 = h * kOutCols + e * 4, c8 = c4 & ~7, k4 = c4 & 4;
+                            o = make_uint4(__float_as_uint(acc[c8 / 32][c8 % 32 + gg_place(k4)]),
+                                           __float_as_uint(acc[c8 / 32][c8 % 32 + gg_place(k4 + 1)]),
+                                           __float_as_uint(acc[c8 / 32][c8 % 32 + gg_place(k4 + 2)]),
+                                           __float_as_uint(acc[c8 / 32][c8 % 32 + gg_place(k4 + 3)]));
                         }
                         gg_stage_row(buf, lane, e, o);
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
-                    const int oc = col0 + h * (128 / kBlocks);
+                    const int oc = col0 + h * kOutCols;
                     if (lane == 0 && row0 < P.M && oc < P.K) {
                         tma_store_2d(&P.tm_out, buf_s, oc, orow);
                         bulk_commit_group();
@@ -684,9 +684,9 @@ __device__ __forceinline__ void gg_in8(const __nv_bfloat16* p, float (&v)[8]) {
 // are the row's G = s dY B^T (the sum of its partial products) times 2^gexp[j],
 // the exponents that A^T's planes were scaled down by, so that G A^T is 64
 // more terms of the same contraction; the row's exponent covers them too.
-// Thread t takes pieces of 8 columns t, t + 256, ...; the first kCastKeep of
-// them stay in registers between the maximum and the rounding.
-constexpr int kCastKeep = 6;
+// The row is read twice, the second time from L1 / L2: keeping it in registers
+// (48 floats a thread) halves the blocks per SM and measured slower (24 against
+// 16 us at 4096 x 4096 bf16).
 template <typename T, int PA>
 __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     __shared__ float red[8];
@@ -705,23 +705,8 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
             for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < A.cols ? gg_in(row + p * 8 + i) : 0.0f;
         }
     };
-    float keep[kCastKeep][8];
     float top = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kCastKeep; ++k) {
-        const int p = threadIdx.x + 256 * k;
-        if (p < pieces) {
-            get(p, keep[k]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) keep[k][i] = 0.0f;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < kCastKeep; ++k)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(keep[k][i]));
-    for (int p = threadIdx.x + 256 * kCastKeep; p < pieces; p += 256) {
+    for (int p = threadIdx.x; p < pieces; p += 256) {
         float v[8];
         get(p, v);
 #pragma unroll
@@ -767,12 +752,7 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
         if constexpr (PA == 2)
             *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
     };
-#pragma unroll
-    for (int k = 0; k < kCastKeep; ++k) {
-        const int p = threadIdx.x + 256 * k;
-        if (p < pieces) put(p, keep[k]);
-    }
-    for (int p = threadIdx.x + 256 * kCastKeep; p < pieces; p += 256) {
+    for (int p = threadIdx.x; p < pieces; p += 256) {
         float v[8];
         get(p, v);
         put(p, v);

@@ -331,8 +331,8 @@ enum : int { kGgLoss = 0, kGgProb = 1, kGgF32 = 2, kGgBf16 = 3 };
 struct GradGemmArgs {
     CUtensorMap tm_a;        // f16 planes of the rows: [planes * plane_rows][contraction], box 64 x 128, 128B swizzle
     CUtensorMap tm_out;      // p~ planes or the output: box 128 bytes x 32 rows, 128B swizzle (not read by kGgLoss)
-    const uint32_t* packed;  // [N][K/8]
-    const float* scales;     // [N][K/32]
+    CUtensorMap tm_w;        // packed words uint32 [N][K/8], box 16 x 128, 64B swizzle
+    CUtensorMap tm_s;        // scales fp32 [N][groups], rows of 16-byte multiples, box 4 x 128
     const int* w_exp;        // the handle's power of two (device)
     const int* row_exp;      // [M], or nullptr: fixed_exp for every row
     int fixed_exp;

@@ -953,6 +953,7 @@ struct spaceslug_q4_weights {
     uint32_t col_begin = 0, n_total = 0;
     uint32_t* packed = nullptr;
     float* scales = nullptr;
+    float* scales_pad = nullptr;  // scales with rows of 16-byte multiples (training products, k % 128 != 0)
     int* col_exp = nullptr;
     float* lora_a = nullptr;
     float* lora_b = nullptr;
@@ -982,6 +983,21 @@ struct spaceslug_q4_weights {
     float* adam = nullptr;  // first and second moments of A then of B: 2 * (K*r + r*N)
     int adam_step = 0;
 };
+
+// What the training products need beside a handle's words and scales, laid out
+// once: the least column exponent (one power of two for the whole handle) and,
+// where k % 128 != 0, a copy of the scales whose rows are 16-byte multiples, as
+// TMA asks.  On the context's stream.
+void prepare_training(spaceslug_q4_weights* w, cudaStream_t s) {
+    check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, s), "min_exp");
+    const size_t G = static_cast<size_t>(w->K) / 32, Gp = (G + 3) / 4 * 4;
+    if (G == Gp) return;
+    check(cudaMalloc(&w->scales_pad, w->N * Gp * 4), "cudaMalloc padded scales");
+    check(cudaMemsetAsync(w->scales_pad, 0, w->N * Gp * 4, s), "cudaMemset padded scales");
+    check(cudaMemcpy2DAsync(w->scales_pad, Gp * 4, w->scales, G * 4, G * 4, static_cast<size_t>(w->N),
+                            cudaMemcpyDeviceToDevice, s),
+          "cudaMemcpy2D padded scales");
+}
 
 // Caller holds the device's host_mu (or owns the handle exclusively).
 void drop_host_graphs(spaceslug_q4_weights* w) {
@@ -1297,6 +1313,23 @@ int grad_splits(long long tiles, int chunks, long long cost, int pairs, long lon
     return best;
 }
 
+// fp32 rows of the transposed product, in blocks of 32 x 32.
+void encode_grad_out(CUtensorMap* map, const void* out, uint64_t rows, int K) {
+    encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, out, static_cast<uint64_t>(K), rows, static_cast<uint64_t>(K) * 4, 32,
+              32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The handle's words and scales as the training products load them: blocks of
+// 128 columns x 128 k.
+void encode_grad_weights(spaceslug_q4_weights* w, q4::GradGemmArgs& g) {
+    const int K = w->K, N = w->N, G = K / 32, Gp = (G + 3) / 4 * 4;
+    const float* scales = w->scales_pad ? w->scales_pad : w->scales;
+    encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, w->packed, static_cast<uint64_t>(K) / 8, static_cast<uint64_t>(N),
+              static_cast<uint64_t>(K) / 2, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
+    encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, scales, static_cast<uint64_t>(G), static_cast<uint64_t>(N),
+              static_cast<uint64_t>(Gp) * 4, 4, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 int pairs_or_throw() {
     const int pairs = q4::grad_gemm_pairs();
     if (pairs < 1) throw CudaError("the training product does not fit this device");
@@ -1411,10 +1444,10 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
             encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
                       static_cast<uint64_t>(K) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
         else
-            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, part.p ? part.p : out, static_cast<uint64_t>(K),
-                      part.p ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc),
-                      static_cast<uint64_t>(K) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
-        g.packed = w->packed; g.scales = w->scales; g.w_exp = w->col_exp + N;
+            encode_grad_out(&g.tm_out, part.p ? part.p : out,
+                            part.p ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc), K);
+        encode_grad_weights(w, g);
+        g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
         g.lora_at = at.p;
         g.ld_at = static_cast<int>(ld_at);
@@ -1493,7 +1526,8 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.plane_rows = mc;
         g.out_rows = mp;
-        g.packed = w->packed; g.scales = w->scales; g.w_exp = w->col_exp + N;
+        encode_grad_weights(w, g);
+        g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
         g.targets = targets + m0;
         g.zt = zt; g.smax = smax; g.ssum = ssum;
@@ -1527,8 +1561,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         Scratch part(static_cast<size_t>(d.splits) * mp * K * 4, s);
         encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
                   static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-        encode_2d(&d.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, part.p, static_cast<uint64_t>(K),
-                  static_cast<uint64_t>(d.splits) * mp, static_cast<uint64_t>(K) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        encode_grad_out(&d.tm_out, part.p, static_cast<uint64_t>(d.splits) * mp, K);
         check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, s), "P W^T");
         check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, targets + m0,
                                         row_scale ? row_scale + m0 : nullptr, w->packed, w->scales,
@@ -1719,7 +1752,7 @@ int spaceslug_q4_weights_create(const uint32_t* packed, const float* scales, uin
             q4up::staged_h2d(device, w->packed, packed + static_cast<size_t>(col_begin) * (k / 8u), pb, c.stream);
             q4up::staged_h2d(device, w->scales, scales + static_cast<size_t>(col_begin) * G, sb, c.stream);
             check_launch(q4::launch_col_exp(w->scales, w->col_exp, w->N, w->K, c.stream), "col_exp");
-            check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, c.stream), "min_exp");
+            prepare_training(w, c.stream);
             check(cudaStreamSynchronize(c.stream), "cudaStreamSynchronize");
         } catch (...) {
             spaceslug_q4_weights_destroy(w);
@@ -1756,7 +1789,7 @@ int spaceslug_q4_weights_create_logical(const int8_t* w_kn, const float* scales,
             q4up::staged_pack_logical(device, w->packed, w_kn, k, n, col_begin, static_cast<uint32_t>(w->N), c.stream);
             q4up::staged_h2d(device, w->scales, scales + static_cast<size_t>(col_begin) * G, sb, c.stream);
             check_launch(q4::launch_col_exp(w->scales, w->col_exp, w->N, w->K, c.stream), "col_exp");
-            check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, c.stream), "min_exp");
+            prepare_training(w, c.stream);
             check(cudaStreamSynchronize(c.stream), "cudaStreamSynchronize");
         } catch (...) {
             spaceslug_q4_weights_destroy(w);
@@ -2089,6 +2122,7 @@ int spaceslug_q4_weights_destroy(spaceslug_q4_weights* w) {
     }
     cudaFree(w->packed);
     cudaFree(w->scales);
+    cudaFree(w->scales_pad);
     cudaFree(w->col_exp);
     cudaFree(w->lora_a);
     cudaFree(w->lora_b);
