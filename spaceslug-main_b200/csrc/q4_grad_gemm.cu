@@ -29,11 +29,11 @@
 // exp(tile max - row max), so that no pass over the probabilities is needed
 // between the two products.
 //
-// Roles (16 warps, 4 warpgroups): warp 0 loads the f16 planes of 128 rows per
+// Roles (20 warps, 5 warpgroups): warp 0 loads the f16 planes of 128 rows per
 // CTA (TMA, 128-byte swizzled boxes of 64), warp 1 of the leader issues the
 // MMAs (M = 256, N = 256, K = 16); warp 3 loads packed words and scales (TMA:
 // as cp.async copies, 16 or 4 bytes from a different row per lane, they took
-// 512 of a stage's shared-memory cycles); warps 4-7 dequantise; warps 8-15 hold 128 fp32
+// 512 of a stage's shared-memory cycles); warps 4-11 dequantise; warps 12-19 hold 128 fp32
 // sums per thread (thread = row, two warps per tensor-memory lane quarter)
 // and run the epilogue while the MMAs fill the other accumulator buffer.
 // Every wait is bounded (status word + abort flag).
@@ -53,7 +53,7 @@ namespace q4 {
 
 namespace {
 
-constexpr int kGgThreads = 512;
+constexpr int kGgThreads = 640;
 constexpr int kGgRows = 256;   // rows of the pair's tile (128 per CTA, one accumulator lane each)
 constexpr int kGgCols = 256;   // columns of the pair's tile
 constexpr int kGgBK = 64;      // contraction per stage
@@ -64,11 +64,11 @@ constexpr int kGgOutBytes = 4096;  // one block of 32 rows x 128 bytes per epilo
 // bytes of words per n (64-byte swizzled) and 4 scales.
 constexpr int kGgRaw = 3;
 constexpr int kGgRawWords = 128 * 64, kGgRawBytes = kGgRawWords + 128 * 16;
-constexpr int kGgDeqWarp0 = 4, kGgDeqWarps = 4;
-constexpr int kGgEpiWarp0 = 8, kGgEpiWarps = 8;
-// Registers per thread after the split: the launch's 512 x 128 cover 128 x 40 + 128 x 64 + 256 x 200.
-constexpr int kGgRegsLaunch = 128, kGgRegsCtl = 40, kGgRegsDeq = 64, kGgRegsEpi = 200;
-static_assert(128 * kGgRegsCtl + 128 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThreads * kGgRegsLaunch, "register split");
+constexpr int kGgDeqWarp0 = 4, kGgDeqWarps = 8;  // two warpgroups, one per stage of a raw block
+constexpr int kGgEpiWarp0 = 12, kGgEpiWarps = 8;
+// Registers per thread after the split: the launch's 640 x 96 cover 128 x 32 + 256 x 56 + 256 x 168.
+constexpr int kGgRegsLaunch = 96, kGgRegsCtl = 32, kGgRegsDeq = 56, kGgRegsEpi = 168;
+static_assert(128 * kGgRegsCtl + 256 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThreads * kGgRegsLaunch, "register split");
 
 template <int PA, int PB>
 struct GgCfg {
@@ -127,6 +127,14 @@ __device__ __forceinline__ bool gg_wait(uint32_t bar, uint32_t parity, volatile 
 __device__ __forceinline__ bool gg_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
                                              int code) {
     return __all_sync(0xffffffffu, gg_wait(bar, parity, abort_flag, status, code));
+}
+// tcgen05.wait::ld that takes the loaded registers along, so that they are not read before it.
+__device__ __forceinline__ void gg_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 template <int R>
 __device__ __forceinline__ void regs_dec() {
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
     if (tid == 0) {
         for (int s = 0; s < ST; ++s) {
             mbar_init(full_x(s), 1);                  // leader's expect_tx (both CTAs' bytes)
-            mbar_init(full_w(s), 2 * kGgDeqWarps);    // dequant warps of both CTAs
+            mbar_init(full_w(s), kGgDeqWarps);        // one dequant warpgroup of each CTA
             mbar_init(empty(s), 1);                   // the leader's commit to both
         }
         for (int b = 0; b < 2; ++b) {
@@ -357,45 +365,40 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
         __syncwarp();
     } else if (warp < kGgEpiWarp0) {
         // ------------------------------------------------------- dequant --
-        // Thread t: logits, column n = t of this CTA's 128 and the stage's 64
-        // k; transposed, n = t % 64 of the stage's 64 and the 64 k t / 64 of
-        // this CTA's 128.  Either way two scale groups of one n per stage, from
-        // a raw block that holds two stages: the k halves or the n halves.
+        // Warpgroup g dequantises stage g of each raw block, which holds two: the
+        // k halves (logits) or the n halves (transposed).  Its thread t: logits,
+        // column n = t of this CTA's 128 and the stage's 64 k; transposed, n = t
+        // % 64 of the stage's 64 and the 64 k t / 64 of this CTA's 128: either
+        // way two scale groups of one n.
         regs_dec<kGgRegsDeq>();
-        const int t = tid - kGgDeqWarp0 * 32;
+        const int g = (warp - kGgDeqWarp0) >> 2, t = (tid - kGgDeqWarp0 * 32) & 127;
         const float cs = exp2i(*P.w_exp);
         const int row = TR ? (t & 63) : t;  // row of the operand image
         const uint32_t out_row = static_cast<uint32_t>((TR ? (t >> 6) * (kGgTile / 2) : 0) + row * 128);
-        int it = 0, s = 0;
-        uint32_t ph = 1;
+        const int rn = TR ? g * 64 + row : row, rh = TR ? t >> 6 : g;  // row and 64-k half of the raw block
+        const int rkey = (rn >> 1) & 3;
+        const uint32_t at0 = static_cast<uint32_t>(rn * 64 + (((2 * rh) ^ rkey) << 4));
+        const uint32_t at1 = static_cast<uint32_t>(rn * 64 + (((2 * rh + 1) ^ rkey) << 4));
+        const uint32_t ats = static_cast<uint32_t>(kGgRawWords + rn * 16 + rh * 8);
+        int it = 0, sq = 0;  // raw block and stage counters
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
             const GgUnit w = gg_unit(P, u);
             const int s1 = min(w.c1 * P.chunk, P.stages);
             for (int st0 = w.c0 * P.chunk; st0 < s1; st0 += 2, ++it) {
-                const int r = it % kGgRaw;
+                const int r = it % kGgRaw, n = min(2, s1 - st0);
                 if (!gg_wait_warp(full_r(r), (it / kGgRaw) & 1u, abort_flag, status, kStatusTimeoutDequant)) {
                     ok = false;
                     break;
                 }
                 const uint8_t* raw = smem + C::kRawOff + r * kGgRawBytes;
-                uint4 q[2][2];
-                float2 sc[2];
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const int n = TR ? g * 64 + row : row, h = TR ? t >> 6 : g;  // row and 64-k half of the block
-                    const uint8_t* wr = raw + n * 64;
-                    const int key = (n >> 1) & 3;
-                    q[g][0] = *reinterpret_cast<const uint4*>(wr + (((2 * h) ^ key) << 4));
-                    q[g][1] = *reinterpret_cast<const uint4*>(wr + (((2 * h + 1) ^ key) << 4));
-                    sc[g] = *reinterpret_cast<const float2*>(raw + kGgRawWords + n * 16 + h * 8);
-                }
+                const uint4 q[2] = {*reinterpret_cast<const uint4*>(raw + at0), *reinterpret_cast<const uint4*>(raw + at1)};
+                const float2 sc = *reinterpret_cast<const float2*>(raw + ats);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty_r(r));
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    if (st0 + g >= s1) break;
-                    if (!gg_wait_warp(empty(s), ph, abort_flag, status, kStatusTimeoutDequant)) {
+                if (g < n) {
+                    const int s = (sq + g) % ST;
+                    if (!gg_wait_warp(empty(s), (((sq + g) / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
                         ok = false;
                         break;
                     }
@@ -414,8 +417,8 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             __half2 s_hi, s_lo;
-                            split_scale_f16((j == 0 ? sc[g].x : sc[g].y) * cs, s_hi, s_lo);
-                            const uint32_t words[4] = {q[g][j].x, q[g][j].y, q[g][j].z, q[g][j].w};
+                            split_scale_f16((j == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
+                            const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 uint4 hi, lo;
@@ -429,12 +432,8 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_remote(leader_addr(full_w(s)));
-                    if (++s == ST) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
                 }
-                if (!ok) break;
+                sq += n;
             }
         }
     } else {
@@ -466,12 +465,13 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                 }
                 tc_fence_after_sync();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t v[32];
-                    tmem_ld32(t_lane + static_cast<uint32_t>(b * kGgCols + i * 32), v);
-                    tmem_ld_wait_regs(v);
+                for (int i = 0; i < 8; ++i) {
+                    uint32_t v[16];
+                    tmem_ld16(t_lane + static_cast<uint32_t>(b * kGgCols + i * 16), v);
+                    gg_ld_wait(v);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) acc[i][j] = fmaf(f, __uint_as_float(v[j]), acc[i][j]);
+                    for (int j = 0; j < 16; ++j)
+                        acc[i / 2][(i % 2) * 16 + j] = fmaf(f, __uint_as_float(v[j]), acc[i / 2][(i % 2) * 16 + j]);
                 }
                 tc_fence_before_sync();
                 __syncwarp();
