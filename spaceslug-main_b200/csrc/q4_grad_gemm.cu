@@ -19,7 +19,12 @@
 // so only w is rounded (2^-12) below the output's own 2^-9.  (1, 2): logits
 // of bf16 x, products to 2^-22, because the loss is fp32.  (2, 2): fp32 (hi
 // hi + hi lo + lo hi).  One scale for the whole handle loses nothing that
-// shows: columns 2^-28 below the largest still have 11 bits.
+// shows: columns 2^-28 below the largest still have 11 bits.  In (1, 2) the lo
+// product only has to be right to a few bits (it is 2^-12 of the whole), so it
+// runs in fp8 at half the cost: e4m3 copies of the rows and of 64 lo, whose
+// 2^-4 leaves logits right to about 2^-16 of their terms.  The target's own
+// logit comes from an fp32 product and its term is kept out of the sums, so
+// that a loss near zero keeps its digits.
 //
 // The tensor core adds each MMA into its fp32 accumulator with truncation, so
 // the accumulator is restarted after every chunk of `chunk` 64-wide stages
@@ -72,7 +77,12 @@ static_assert(128 * kGgRegsCtl + 256 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThrea
 
 template <int PA, int PB>
 struct GgCfg {
-    static constexpr int kStageBytes = (PA + PB) * kGgTile;
+    // (1, 2): the lo plane of w in fp8, against an fp8 copy of the rows
+    static constexpr bool kLo8 = PA == 1 && PB == 2;
+    static constexpr int kA8 = PA * kGgTile;                       // fp8 rows: 128 x 64 bytes
+    static constexpr int kB = kA8 + (kLo8 ? kGgTile / 2 : 0);      // w hi
+    static constexpr int kBLo = kB + kGgTile;                      // w lo (f16, or 128 x 64 bytes of fp8)
+    static constexpr int kStageBytes = kLo8 ? kBLo + kGgTile / 2 : (PA + PB) * kGgTile;
     static constexpr int kStages = PA + PB == 2 ? 5 : PA + PB == 3 ? 3 : 2;
     static constexpr int kOutOff = kStages * kStageBytes;
     static constexpr int kRawOff = kOutOff + kGgEpiWarps * kGgOutBytes;
@@ -101,6 +111,32 @@ __device__ __forceinline__ uint64_t gg_desc_mn_sw128(uint32_t addr, uint32_t lbo
     return d;
 }
 
+// K-major operand of 64-byte rows (64 fp8), 64-byte swizzled: 8-row atoms of 512 bytes.
+__device__ __forceinline__ uint64_t gg_desc_k_sw64(uint32_t addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(1u) << 16;
+    d |= static_cast<uint64_t>(512u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(4u) << 61;  // SWIZZLE_64B
+    return d;
+}
+// Pair MMA on e4m3 operands (K = 32), fp32 accumulate.
+__device__ __forceinline__ void umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Two f16 as two e4m3 bytes (round to nearest, clamped to +-448).
+__device__ __forceinline__ uint32_t gg_e4m3x2(__half2 v) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
+    return r;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -155,7 +191,8 @@ __device__ __forceinline__ void regs_inc() {
 // accumulator's columns, undone by the epilogue's choice of registers.
 // hi = RN16(v s_hi + RN16(v s_lo)) as in dequant_word_f16x2, lo = (v s_hi -
 // hi) + RN16(v s_lo), whose bracket is exact, so hi + lo is v s to 2^-22.
-template <int PB>
+// With LO8, lo is 64 times that in e4m3: eight bytes in lo.x and lo.y.
+template <int PB, bool LO8>
 __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_lo, uint4& hi, uint4& lo) {
     const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00u));  // 1/16
     const __half2 bias0 = __half2half2(__ushort_as_half(0xE408u));      // -1032: 1024 + (v + 8)
@@ -173,11 +210,15 @@ __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_l
         h[b] = *reinterpret_cast<const uint32_t*>(&w);
         if constexpr (PB == 2) {
             const __half2 r = __hadd2(__hfma2(v, s_hi, __hneg2(w)), c);
-            l[b] = *reinterpret_cast<const uint32_t*>(&r);
+            if constexpr (LO8) {
+                l[b] = gg_e4m3x2(__hmul2(r, __half2half2(__ushort_as_half(0x5400u))));  // 64 r
+            } else {
+                l[b] = *reinterpret_cast<const uint32_t*>(&r);
+            }
         }
     }
     hi = make_uint4(h[0], h[1], h[2], h[3]);
-    if constexpr (PB == 2) lo = make_uint4(l[0], l[1], l[2], l[3]);
+    if constexpr (PB == 2) lo = LO8 ? make_uint4(l[0] | (l[1] << 16), l[2] | (l[3] << 16), 0, 0) : make_uint4(l[0], l[1], l[2], l[3]);
 }
 // Place of k (0..7) in that order.
 __host__ __device__ constexpr int gg_place(int k) { return k < 4 ? 2 * k : 2 * (k - 4) + 1; }
@@ -280,12 +321,14 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                         ok = false;
                         break;
                     }
-                    if (leader) mbar_arrive_expect_tx(full_x(s), 2u * PA * kGgTile);
+                    if (leader) mbar_arrive_expect_tx(full_x(s), 2u * static_cast<uint32_t>(C::kB));
                     const uint32_t fx = leader_addr(full_x(s));
 #pragma unroll
                     for (int p = 0; p < PA; ++p)
                         tma_load_2d_pair(base + s * C::kStageBytes + p * kGgTile, &P.tm_a, fx, st * kGgBK,
                                          p * P.plane_rows + m0);
+                    if constexpr (C::kLo8)
+                        tma_load_2d_pair(base + s * C::kStageBytes + C::kA8, &P.tm_a8, fx, st * kGgBK, m0);
                 }
             }
             if (*abort_flag && leader)
@@ -340,7 +383,15 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                             break;
                         }
                         tc_fence_after_sync();
-                        const uint32_t at = base + s * C::kStageBytes, bt = at + PA * kGgTile;
+                        const uint32_t at = base + s * C::kStageBytes, bt = at + C::kB;
+                        if constexpr (C::kLo8) {
+#pragma unroll
+                            for (int kk = 0; kk < kGgBK / 32; ++kk) {
+                                umma_f8_ss_pair(dacc, gg_desc_k_sw64(at + C::kA8 + kk * 32),
+                                                gg_desc_k_sw64(at + C::kBLo + kk * 32), idesc, acc);
+                                acc = 1;
+                            }
+                        }
                         auto mma = [&](int pa, int pb, int kk) {
                             const uint64_t ad = umma_desc_k_sw128(at + pa * kGgTile + kk * 32);
                             const uint64_t bd = TR ? gg_desc_mn_sw128(bt + pb * kGgTile + kk * 2048, kGgTile / 2)
@@ -351,7 +402,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
 #pragma unroll
                         for (int kk = 0; kk < kGgBK / 16; ++kk) {
                             if constexpr (PA == 2) mma(1, 0, kk);
-                            if constexpr (PB == 2) mma(0, 1, kk);
+                            if constexpr (PB == 2 && !C::kLo8) mma(0, 1, kk);
                             mma(0, 0, kk);
                         }
                         umma_commit_pair_both(empty(s), 0x3);
@@ -402,7 +453,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                         ok = false;
                         break;
                     }
-                    uint8_t* dst = smem + s * C::kStageBytes + PA * kGgTile + out_row;
+                    uint8_t* dst = smem + s * C::kStageBytes + C::kB + out_row;
                     if (TR && st0 + g == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
                         const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
 #pragma unroll
@@ -422,10 +473,17 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 uint4 hi, lo;
-                                gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
+                                gg_dequant<PB, C::kLo8>(words[i], s_hi, s_lo, hi, lo);
                                 const int o = ((4 * j + i) ^ (row & 7)) << 4;
                                 *reinterpret_cast<uint4*>(dst + o) = hi;
-                                if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
+                                if constexpr (C::kLo8) {
+                                    // 64-byte rows: 16-byte piece of two words, 64-byte swizzled
+                                    uint8_t* d8 = smem + s * C::kStageBytes + C::kBLo + row * 64 +
+                                                  (((2 * j + i / 2) ^ ((row >> 1) & 3)) << 4) + (i & 1) * 8;
+                                    *reinterpret_cast<uint2*>(d8) = make_uint2(lo.x, lo.y);
+                                } else if constexpr (PB == 2) {
+                                    *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
+                                }
                             }
                         }
                     }
@@ -483,17 +541,18 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
             const int col0 = w.ct * kGgCols + half * 128;
             if constexpr (EPI == kGgLoss || EPI == kGgProb) {
                 // In units of log2: z2 = z log2(e); this tile's row maximum over the
-                // columns that exist, the sum of 2^(z2 - max), the target's logit.
+                // columns that exist other than the target's (whose logit the
+                // cast has from an fp32 product), and the sum of 2^(z2 - max).
                 const float s2 = scale * 1.4426950408889634f;
                 const long long tgt = row < P.M ? P.targets[row] : -1;
+                const int tcol = tgt >= col0 && tgt < col0 + 128 ? static_cast<int>(tgt) - col0 : -1;
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        const int col = col0 + i * 32 + j;
-                        if (col == tgt) P.zt[row] = acc[i][j] * scale;
-                        acc[i][j] = col < P.N ? acc[i][j] * s2 : -INFINITY;
+                        const int c = i * 32 + j;
+                        acc[i][j] = col0 + c < P.N && c != tcol ? acc[i][j] * s2 : -INFINITY;
                         top = fmaxf(top, acc[i][j]);
                     }
                 // the two warps of these rows, through a buffer that alternates: a warp
@@ -508,12 +567,13 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                 }
                 ++xq;
                 top = fmaxf(top, xch[(half ^ 1) * 128 + row_in]);
+                const float ref = top == -INFINITY ? 0.0f : top;  // a tile of the target alone: all terms 0
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        acc[i][j] = ex2(acc[i][j] - top);  // 2^-inf = 0 past the columns
+                        acc[i][j] = ex2(acc[i][j] - ref);  // 2^-inf = 0 where there is no term
                         sum += acc[i][j];
                     }
                 if (half == 0) P.smax[static_cast<size_t>(w.ct) * P.ld_stat + row] = top;
@@ -684,6 +744,8 @@ __device__ __forceinline__ void gg_in8(const __nv_bfloat16* p, float (&v)[8]) {
 // are the row's G = s dY B^T (the sum of its partial products) times 2^gexp[j],
 // the exponents that A^T's planes were scaled down by, so that G A^T is 64
 // more terms of the same contraction; the row's exponent covers them too.
+// For the loss it also forms the target's logit in fp32, and (bf16) the e4m3
+// copy of the row.
 // The row is read twice, the second time from L1 / L2: keeping it in registers
 // (48 floats a thread) halves the blocks per SM and measured slower (24 against
 // 16 us at 4096 x 4096 bf16).
@@ -705,12 +767,22 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
             for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < A.cols ? gg_in(row + p * 8 + i) : 0.0f;
         }
     };
-    float top = 0.0f;
+    float top = 0.0f, dot = 0.0f;
+    const long long tgt = A.targets != nullptr ? A.targets[m] : -1;
+    const bool want_dot = tgt >= 0 && tgt < A.N;
     for (int p = threadIdx.x; p < pieces; p += 256) {
         float v[8];
         get(p, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+        if (want_dot) {  // the target's logit, w = v s in fp32
+            const uint32_t q = __ldg(A.packed + tgt * (A.cols / 8) + p);
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                part = fmaf(v[i], static_cast<float>((static_cast<int>((q >> (4 * i)) & 15u) ^ 8) - 8), part);
+            dot = fmaf(part, __ldg(A.scales + tgt * (A.cols / 32) + (p >> 2)), dot);
+        }
     }
     if (A.rank > 0 && threadIdx.x < 64) {
         float g = 0.0f;
@@ -734,6 +806,17 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     }
     if (threadIdx.x == 0) A.row_exp[m] = e;
     const float s = exp2i(e);
+    if (A.targets != nullptr) {
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        __syncthreads();  // red has been read
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float z = 0.0f;
+            for (int i = 0; i < 8; ++i) z += red[i];
+            A.zt[m] = z;
+        }
+    }
     __half* hi = static_cast<__half*>(A.out) + m * A.ld;
     auto put = [&](int p, const float (&v)[8]) {
         uint32_t h[4], l[4];
@@ -749,6 +832,14 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
             }
         }
         *reinterpret_cast<uint4*>(hi + p * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (PA == 1 && A.out8 != nullptr) {  // the row * 2^(e - 6) in e4m3, to go with 64 w_lo
+            const __half2 down = __half2half2(__ushort_as_half(0x2400u));  // 1/64
+            uint32_t q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = gg_e4m3x2(__hmul2(*reinterpret_cast<const __half2*>(&h[i]), down));
+            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(A.out8) + m * A.ld + p * 8) =
+                make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+        }
         if constexpr (PA == 2)
             *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
     };
@@ -786,52 +877,56 @@ __global__ void __launch_bounds__(1024) min_exp_kernel(const int* __restrict__ c
     }
 }
 
-// Row statistics of the tiles' (log2 units): row max M2, S = sum over tiles of
-// sums * 2^(tile max - M2), the factor 2^(tile max - M2) of every tile in
-// place of its max, lse and loss.  32 rows x 8 lanes per block.
-__global__ void __launch_bounds__(256) loss_rows_kernel(float* __restrict__ smax, const float* __restrict__ ssum,
-                                                        const float* __restrict__ zt,
-                                                        const long long* __restrict__ targets, float* __restrict__ total,
-                                                        float* __restrict__ loss, float* __restrict__ lse, int M, int N,
-                                                        int tiles, long long ld) {
-    __shared__ float part[8][32];
+// Row statistics of the tiles' (log2 units, target excluded) and the target's
+// logit: row max M2 with the target, S = sum over tiles of sums * 2^(tile max -
+// M2) + 2^(target - M2), the factor 2^(tile max - M2) of every tile in place of
+// its max, lse and loss.  The loss of a likely target is log1p(others /
+// target), which does not cancel.  32 rows x 32 lanes per block.
+__global__ void __launch_bounds__(1024) loss_rows_kernel(float* __restrict__ smax, const float* __restrict__ ssum,
+                                                         const float* __restrict__ zt,
+                                                         const long long* __restrict__ targets,
+                                                         float* __restrict__ total, float* __restrict__ loss,
+                                                         float* __restrict__ lse, int M, int N, int tiles, long long ld) {
+    __shared__ float part[32][33];
     const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
     const int row = blockIdx.x * 32 + r;
     const bool in = row < M;
-    float top = -INFINITY;
-    bool bad = false;
-    for (int t = p; t < tiles && in; t += 8) {
-        const float v = smax[static_cast<size_t>(t) * ld + row];
-        bad |= v != v;
-        top = fmaxf(top, v);
-    }
-    part[p][r] = bad ? NAN : top;
+    const long long t = in ? targets[row] : -1;
+    const float t2 = t >= 0 && t < N ? zt[row] * 1.4426950408889634f : -INFINITY;
+    float top = t2;
+#pragma unroll 4
+    for (int i = p; i < tiles && in; i += 32) top = fmaxf(top, smax[static_cast<size_t>(i) * ld + row]);
+    part[p][r] = top;
     __syncthreads();
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, part[i][r]);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i][r]);
     __syncthreads();
     float sum = 0.0f;
-    for (int t = p; t < tiles && in; t += 8) {
-        float* at = smax + static_cast<size_t>(t) * ld + row;
+#pragma unroll 4
+    for (int i = p; i < tiles && in; i += 32) {
+        float* at = smax + static_cast<size_t>(i) * ld + row;
         const float f = exp2f(*at - top);
-        const float* st = ssum + static_cast<size_t>(2 * t) * ld + row;
+        const float* st = ssum + static_cast<size_t>(2 * i) * ld + row;
         sum += f * (st[0] + st[ld]);
         *at = f;
     }
     part[p][r] = sum;
     __syncthreads();
     if (p != 0 || !in) return;
-    for (int i = 1; i < 8; ++i) sum += part[i][r];
-    const float l = 0.69314718055994531f * (top + log2f(sum));
-    const long long t = targets[row];
-    total[row] = sum;
+    for (int i = 1; i < 32; ++i) sum += part[i][r];
+    const float et = exp2f(t2 - top), all = sum + et;
+    total[row] = all;
+    const float l = 0.69314718055994531f * (top + log2f(all));
     if (lse != nullptr) lse[row] = l;
-    loss[row] = t < 0 ? 0.0f : t < N ? l - zt[row] : NAN;
+    loss[row] = t < 0 ? 0.0f : t >= N ? NAN : et > 0.0009765625f ? log1pf(sum / et) : l - zt[row];
 }
 
-// dx[row][k] = g (sum_z partial[z][row][k] / S - w(k, target)); one block per row.
+// dx[row][k] = g (sum_z partial[z][row][k] / S + (p_t - 1) w(k, target)), p_t - 1 =
+// expm1(-loss); one block per row.
 template <typename T>
 __global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ partial, int splits, long long out_rows,
                                                       const float* __restrict__ total,
+                                                      const float* __restrict__ loss,
                                                       const long long* __restrict__ targets,
                                                       const float* __restrict__ row_scale,
                                                       const uint32_t* __restrict__ packed,
@@ -840,7 +935,7 @@ __global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ 
     const long long t = targets[row];
     T* out = dx + row * K;
     const float g = row_scale != nullptr ? row_scale[row] : 1.0f;
-    const float inv = 1.0f / total[row];
+    const float inv = 1.0f / total[row], hot = expm1f(-loss[row]);
     for (int k = threadIdx.x * 8; k < K; k += 256 * 8) {
         float v[8];
 #pragma unroll
@@ -858,7 +953,7 @@ __global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int nib = static_cast<int>((q >> (4 * i)) & 15u);
-                    v[i] = g * (v[i] * inv - static_cast<float>((nib ^ 8) - 8) * s);
+                    v[i] = g * (v[i] * inv + hot * (static_cast<float>((nib ^ 8) - 8) * s));
                 }
             } else {
 #pragma unroll
@@ -959,18 +1054,18 @@ int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int
 
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
                      float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream) {
-    loss_rows_kernel<<<(M + 31) / 32, 256, 0, stream>>>(smax, ssum, zt, targets, total, loss, lse, M, N, tiles, ld);
+    loss_rows_kernel<<<(M + 31) / 32, 1024, 0, stream>>>(smax, ssum, zt, targets, total, loss, lse, M, N, tiles, ld);
     return static_cast<int>(cudaGetLastError());
 }
 
-int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const long long* targets,
-                   const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
+int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,
+                   const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream) {
     if (bf16)
-        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, targets, row_scale, packed, scales,
+        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, loss, targets, row_scale, packed, scales,
                                               static_cast<__nv_bfloat16*>(dx), N, K);
     else
-        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, targets, row_scale, packed, scales,
+        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, loss, targets, row_scale, packed, scales,
                                               static_cast<float*>(dx), N, K);
     return static_cast<int>(cudaGetLastError());
 }

@@ -330,6 +330,7 @@ int launch_rows_finish(const float* partial, int splits, long long split_floats,
 enum : int { kGgLoss = 0, kGgProb = 1, kGgF32 = 2, kGgBf16 = 3 };
 struct GradGemmArgs {
     CUtensorMap tm_a;        // f16 planes of the rows: [planes * plane_rows][contraction], box 64 x 128, 128B swizzle
+    CUtensorMap tm_a8;       // logits of one plane: the rows in e4m3 [rows][contraction], box 64 x 128, 64B swizzle
     CUtensorMap tm_out;      // p~ planes or the output: box 128 bytes x 32 rows, 128B swizzle (not read by kGgLoss)
     CUtensorMap tm_w;        // packed words uint32 [N][K/8], box 16 x 128, 64B swizzle
     CUtensorMap tm_s;        // scales fp32 [N][groups], rows of 16-byte multiples, box 4 x 128
@@ -344,7 +345,6 @@ struct GradGemmArgs {
     const void* lora_at;     // transposed product with an adapter: f16 planes [planes][64][ld_at] of A^T, the operand
     int lora_stage, ld_at;   // of stage lora_stage (-1: none), whose 64 row columns hold G
     const long long* targets;  // logits: [M]
-    float* zt;               // [M] the target's logit
     float* smax;             // [col_tiles][ld_stat]
     float* ssum;             // [2 col_tiles][ld_stat]
     long long ld_stat;
@@ -354,9 +354,16 @@ int grad_gemm_pairs();  // co-resident CTA pairs on the current device
 int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream);
 // f16 planes [planes][M][ld] of fp32 (2 planes) or bf16 (1) rows scaled by 2^row_exp; by_word: each 8 columns in the
 // order 0 4 1 5 2 6 3 7; with an adapter (rank > 0) the last 64 columns hold gscale * sum of gpart [gsplits][M][gpitch].
+// targets (logits): the target column's logit of each row in fp32 to zt, and to out8 the e4m3 copy of bf16 rows.
 struct CastArgs {
     const void* x;
     void* out;
+    void* out8;
+    const long long* targets;
+    const uint32_t* packed;
+    const float* scales;
+    float* zt;
+    int N;
     int* row_exp;
     int M, cols;
     long long ld;
@@ -371,8 +378,8 @@ int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int
 // tile statistics -> chunk factors (in smax), row sums, loss and lse
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
                      float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream);
-int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const long long* targets,
-                   const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
+int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,
+                   const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream);
 int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K, int rank, int ld, int planes,
                    cudaStream_t stream);

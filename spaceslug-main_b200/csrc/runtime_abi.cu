@@ -1390,7 +1390,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.row_tiles = (mc + 255) / 256;
         g.col_tiles = (K + 255) / 256;
         g.stages = static_cast<int>(ld / 64);
-        g.chunk = 8;
+        g.chunk = bf16 ? 8 : 2;  // truncated sums of 512 or 128 terms
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.splits = grad_splits(static_cast<long long>(g.row_tiles) * g.col_tiles, g.chunks,
                                (planes == 1 ? 512 : 1536) * g.chunk, pairs, static_cast<long long>(mc) * K, false);
@@ -1503,6 +1503,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
         Scratch x16(static_cast<size_t>(planes) * mc * K * 2, s);
+        Scratch x8(bf16 ? static_cast<size_t>(mc) * K : 0, s);
         Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
         Scratch stat((static_cast<size_t>(3) * tiles + 2) * mp * 4, s);
         Scratch prob(dx ? static_cast<size_t>(planes) * mp * ld_p * 2 : 0, s);
@@ -1515,6 +1516,8 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
         ca.M = mc; ca.cols = K; ca.ld = K;
         ca.by_word = 1;
+        ca.out8 = x8.p;
+        ca.targets = targets + m0; ca.packed = w->packed; ca.scales = w->scales; ca.zt = zt; ca.N = N;
         check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "X planes");
         q4::GradGemmArgs g{};
         g.M = mc; g.N = N; g.K = K;
@@ -1522,7 +1525,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.col_tiles = tiles;
         g.splits = 1;
         g.stages = (K + 63) / 64;
-        g.chunk = 8;
+        g.chunk = bf16 ? 4 : 2;  // truncated sums of 256 or 128 terms
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.plane_rows = mc;
         g.out_rows = mp;
@@ -1530,12 +1533,16 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
         g.targets = targets + m0;
-        g.zt = zt; g.smax = smax; g.ssum = ssum;
+        g.smax = smax; g.ssum = ssum;
         g.ld_stat = mp;
         g.lora_stage = -1;
         g.status = c.status;
         encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(K),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+        g.tm_a8 = g.tm_a;  // not read without an e4m3 copy
+        if (bf16)
+            encode_2d(&g.tm_a8, CU_TENSOR_MAP_DATA_TYPE_UINT8, x8.p, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
+                      static_cast<uint64_t>(K), 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
         if (dx)
             encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
                       static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 32,
@@ -1563,7 +1570,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
                   static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         encode_grad_out(&d.tm_out, part.p, static_cast<uint64_t>(d.splits) * mp, K);
         check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, s), "P W^T");
-        check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, targets + m0,
+        check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, loss + m0, targets + m0,
                                         row_scale ? row_scale + m0 : nullptr, w->packed, w->scales,
                                         static_cast<char*>(dx) + static_cast<size_t>(m0) * K * size, bf16, mc, N, K, s),
                      "dX");

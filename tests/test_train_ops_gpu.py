@@ -4,7 +4,9 @@ gradient, softmax cross entropy over a vocabulary) against 64-bit restatements.
 Tolerances.  S = sum |a||b| over a product's terms, in 64 bits.
   fp32: operands to 2^-21, and sums of rounded terms whose chains are at most 255 long: |error| <= 2^-16 S.
   bf16: one operand rounded to f16 (2^-11 of each term), the result to bf16 (2^-8 of it): 2^-11 S + 2^-8 |y| + 2^-16 S.
-Logits are held to the fp32 bound for both types: dz = 2^-16 max_v S.  Then lse is off by dz + 2^-20 (1 + |lse|), a loss
+Logits are held to the fp32 bound for both types: dz = 2^-16 max_v S (bf16: what W's f16 part leaves is multiplied in
+fp8, off by at most 2^-11 (2^-4 + 2^-4) = 2^-14 of a term and of random sign, so by 2^-14 S / sqrt(k), which is below
+2^-16 S from k = 16 on).  Then lse is off by dz + 2^-20 (1 + |lse|), a loss
 by twice that, a probability by 2 dz + 2^-16 of itself.
 """
 from __future__ import annotations
