@@ -471,18 +471,20 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                             split_scale_f16((j == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
                             const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                uint4 hi, lo;
-                                gg_dequant<PB, C::kLo8>(words[i], s_hi, s_lo, hi, lo);
-                                const int o = ((4 * j + i) ^ (row & 7)) << 4;
-                                *reinterpret_cast<uint4*>(dst + o) = hi;
-                                if constexpr (C::kLo8) {
-                                    // 64-byte rows: 16-byte piece of two words, 64-byte swizzled
-                                    uint8_t* d8 = smem + s * C::kStageBytes + C::kBLo + row * 64 +
-                                                  (((2 * j + i / 2) ^ ((row >> 1) & 3)) << 4) + (i & 1) * 8;
-                                    *reinterpret_cast<uint2*>(d8) = make_uint2(lo.x, lo.y);
+                            for (int i = 0; i < 4; i += 2) {
+                                uint4 hi0, hi1, lo0, lo1;
+                                gg_dequant<PB, C::kLo8>(words[i], s_hi, s_lo, hi0, lo0);
+                                gg_dequant<PB, C::kLo8>(words[i + 1], s_hi, s_lo, hi1, lo1);
+                                const int o0 = ((4 * j + i) ^ (row & 7)) << 4, o1 = ((4 * j + i + 1) ^ (row & 7)) << 4;
+                                *reinterpret_cast<uint4*>(dst + o0) = hi0;
+                                *reinterpret_cast<uint4*>(dst + o1) = hi1;
+                                if constexpr (C::kLo8) {  // 64-byte rows: a 16-byte piece holds two words
+                                    *reinterpret_cast<uint4*>(smem + s * C::kStageBytes + C::kBLo + row * 64 +
+                                                              (((2 * j + i / 2) ^ ((row >> 1) & 3)) << 4)) =
+                                        make_uint4(lo0.x, lo0.y, lo1.x, lo1.y);
                                 } else if constexpr (PB == 2) {
-                                    *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
+                                    *reinterpret_cast<uint4*>(dst + kGgTile + o0) = lo0;
+                                    *reinterpret_cast<uint4*>(dst + kGgTile + o1) = lo1;
                                 }
                             }
                         }

@@ -1390,7 +1390,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.row_tiles = (mc + 255) / 256;
         g.col_tiles = (K + 255) / 256;
         g.stages = static_cast<int>(ld / 64);
-        g.chunk = bf16 ? 8 : 2;  // truncated sums of 512 or 128 terms
+        g.chunk = bf16 ? 8 : 4;  // truncated sums of 512 or 256 terms
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.splits = grad_splits(static_cast<long long>(g.row_tiles) * g.col_tiles, g.chunks,
                                (planes == 1 ? 512 : 1536) * g.chunk, pairs, static_cast<long long>(mc) * K, false);
@@ -1525,7 +1525,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.col_tiles = tiles;
         g.splits = 1;
         g.stages = (K + 63) / 64;
-        g.chunk = bf16 ? 4 : 2;  // truncated sums of 256 or 128 terms
+        g.chunk = bf16 ? 8 : 4;  // truncated sums of 512 or 256 terms
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.plane_rows = mc;
         g.out_rows = mp;
