@@ -307,23 +307,26 @@ int launch_act8_pack(const void* x, bool bf16, int8_t* codes, uint8_t* exps, lon
 int launch_act8_unpack(const int8_t* codes, const uint8_t* exps, void* x, bool bf16, long long groups,
                        cudaStream_t stream);
 int launch_bf16_to_f32(const void* x, float* y, long long count, cudaStream_t stream);
-// The training operators for a few rows (q4_rows.cu), any M; x, dy and out are fp32 or bf16, 16-byte aligned.
-int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, float* z, long long ld_z,
-                       int M, int N, int K, cudaStream_t stream);
-int rows_wt_splits(int M, int N, int K, int sm_count);
-// partial[splits][M][K] of sum_n d[m][n] w(k, n)
-int launch_rows_wt(const void* d, bool bf16, long long ld_d, const uint32_t* packed, const float* scales,
-                   float* partial, int splits, int M, int N, int K, cudaStream_t stream);
-// lse, loss and (want_grad) d = row_scale (softmax - onehot) of M logit rows, in place
-int launch_rows_softmax(float* z, long long ld_z, const long long* targets, const float* row_scale, float* loss,
-                        float* lse, int M, int N, bool want_grad, cudaStream_t stream);
-// G[m][j] = scale sum_n dy[m][n] B[j][n]
-int launch_rows_proj(const void* dy, bool bf16, const float* b, float scale, float* g, int M, int N, int rank,
+// The training operators for 1 <= M <= 8 rows (q4_rows.cu); x, dy and out are fp32 or bf16, 16-byte aligned.
+int rows_logits_tiles(int N);  // blocks of columns with one max and sum each
+// logits z [M][N], the target's zt [M], smax and ssum [M][tiles] (log2 units, without the target)
+int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, const long long* targets,
+                       float* z, float* zt, float* smax, float* ssum, int M, int N, int K, cudaStream_t stream);
+// lse, loss and coef [M][3]: the row's max, g / S and g (p_target - 1)
+int launch_rows_loss(const float* smax, const float* ssum, const float* zt, const long long* targets,
+                     const float* row_scale, float* loss, float* lse, float* coef, int M, int N, cudaStream_t stream);
+int rows_wt_splits(int N, int K, int sm_count);
+// partial[splits][M][K] of sum_n d[m][n] w(k, n); with coef, d holds logits and stands for g (softmax - onehot)
+int launch_rows_wt(const void* d, bool bf16, const float* coef, const long long* targets, const uint32_t* packed,
+                   const float* scales, float* partial, int splits, int M, int N, int K, cudaStream_t stream);
+// G[z][m][j] = sum over range z of n of dy[m][n] B[j][n], any M
+int rows_proj_splits(int M, int N, int rank, int sm_count);
+int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int splits, int M, int N, int rank,
                      cudaStream_t stream);
-// out [M][K] = sum in order of the splits (split_floats apart) + G A^T (A [K][rank]; rank 0: none)
-int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, const float* a,
-                       int rank, void* out, bool bf16, int M, int K, cudaStream_t stream);
-
+// out [M][K] = sum in order of the splits (split_floats apart) + scale (sum of G's ranges) A^T (A [K][rank]; rank 0:
+// none), any M without an adapter
+int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, int gsplits,
+                       const float* a, int rank, float scale, void* out, bool bf16, int M, int K, cudaStream_t stream);
 // The large products of training through the frozen weights (q4_grad_gemm.cu).  Epilogues: the logits' tile statistics
 // (kGgLoss), those and the planes of p~ = exp(z - tile max) 2^14 (kGgProb), the transposed product in fp32 (kGgF32:
 // split z at row z * out_rows) or bf16 (kGgBf16).

@@ -1,16 +1,16 @@
-// The training operators on the frozen int4 weights for a few rows, on the
-// CUDA cores in fp32: products that stream the packed weights once per block
-// of at most eight rows.
+// The training operators on the frozen int4 weights for one to eight rows, on
+// the CUDA cores in fp32: products that stream the packed weights once.
 //
-//   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n)        (logits)
-//   rows_wt_kernel       dx[m][k] = sum_n d[m][n] w(k, n)        (the transposed product)
-//   rows_softmax_kernel  lse, loss and d = g (softmax(z) - onehot) of logit rows, in place
-//   rows_proj_kernel     G[m][j]  = s sum_n dy[m][n] B[j][n]     (the adapter's side)
-//   rows_finish_kernel   sums the splits of n in order, adds G A^T, rounds once to the output's type
+//   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n), and each 32 columns' max and sum of exponentials
+//   rows_loss_kernel     lse, loss and the rows' coefficients of the gradient
+//   rows_wt_kernel       dx[m][k] = sum_n d[m][n] w(k, n), d given or formed from z and the coefficients
+//   rows_proj_kernel     G[m][j]  = sum_n dy[m][n] B[j][n] (the adapter's side, any number of rows)
+//   rows_finish_kernel   sums the splits of n in order, adds s G A^T, rounds once to the output's type
 //
 // w(k, n) = float(v) * scale as everywhere (vulkan-runtime/shaders/q4gemm.comp:104-122),
-// one rounding.  With one to eight rows these products are bound by the
-// weights' bytes (0.625 B per weight) or by their unpacking.
+// one rounding.  With a row or two these products are bound by the weights'
+// bytes (0.625 B per weight), with eight by their unpacking and fp32 FMAs; so
+// the row count is a template constant.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -55,160 +55,255 @@ __device__ __forceinline__ void word_weights(uint32_t q, float s, float (&w)[8])
     }
 }
 
-// One warp per four columns; lanes take the words of k in turn, MR rows of x
-// are held in registers against the four columns' weights.
-constexpr int kRowsCols = 4;
-template <int MR, typename T>
-__global__ void __launch_bounds__(256) rows_logits_kernel(const T* __restrict__ x, const uint32_t* __restrict__ packed,
-                                                          const float* __restrict__ scales, float* __restrict__ z,
-                                                          long long ld_z, int M, int N, int K) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n0 = (blockIdx.x * 8 + warp) * kRowsCols, m0 = blockIdx.y * MR;
-    if (n0 >= N) return;
-    const int words = K / 8, groups = K / 32;
-    float acc[kRowsCols * MR];
-#pragma unroll
-    for (int i = 0; i < kRowsCols * MR; ++i) acc[i] = 0.0f;
-#pragma unroll 2
-    for (int w = lane; w < words; w += 32) {
-        uint32_t q[kRowsCols];
-        float s[kRowsCols];
-#pragma unroll
-        for (int c = 0; c < kRowsCols; ++c) {
-            const size_t n = static_cast<size_t>(min(n0 + c, N - 1));
-            q[c] = __ldg(packed + n * words + w);
-            s[c] = __ldg(scales + n * groups + (w >> 2));
-        }
-        float xv[MR][8];
-#pragma unroll
-        for (int r = 0; r < MR; ++r) row_load8(x + static_cast<size_t>(min(m0 + r, M - 1)) * K + w * 8, xv[r]);
-#pragma unroll
-        for (int c = 0; c < kRowsCols; ++c) {
-            float wv[8];
-            word_weights(q[c], s[c], wv);
-#pragma unroll
-            for (int r = 0; r < MR; ++r)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[c * MR + r] = fmaf(xv[r][i], wv[i], acc[c * MR + r]);
-        }
-    }
-    const float total = warp_reduce_scatter<kRowsCols * MR>(acc, lane);
-    constexpr int kShare = 32 / (kRowsCols * MR);  // lanes that hold the same value
-    const int i = value_index<kRowsCols * MR>(lane), c = i / MR, r = i % MR;
-    if (lane % kShare == 0 && n0 + c < N && m0 + r < M) z[static_cast<long long>(m0 + r) * ld_z + n0 + c] = total;
-}
+// z2 += a * b for two packed k.
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 
-// One thread per word of k (8 outputs) and MR rows; n in blockIdx.y's range.
-// The rows' d values of 256 n at a time sit in shared memory.
-constexpr int kWtThreads = 128, kWtTile = 256;
+// 32 columns per block, one per lane; the eight warps share k: each takes four
+// of the 32 groups of a 1024-k chunk, whose words (16 bytes per group) and
+// scales are all loaded before the chunk's x, which every lane reads from
+// shared memory at once (one wavefront per four k of a row).  Keeping x in
+// registers against four columns per warp instead took 150 registers, eight
+// warps per SM and 39 us at 5 x 1024 x 32003.  The warps' sums meet in shared
+// memory, and per row the 32 columns give their maximum and the sum of
+// exp(z - max), both without the target's column (log2 units: smax, ssum).
+constexpr int kRowsCols = 32, kRowsChunk = 1024, kRowsBatch = kRowsChunk / 32 / 8;
 template <int MR, typename T>
-__global__ void __launch_bounds__(kWtThreads) rows_wt_kernel(const T* __restrict__ d, long long ld_d,
-                                                             const uint32_t* __restrict__ packed,
+__global__ void __launch_bounds__(256, 3) rows_logits_kernel(const T* __restrict__ x, const uint32_t* __restrict__ packed,
                                                              const float* __restrict__ scales,
-                                                             float* __restrict__ partial, int M, int N, int K) {
-    __shared__ float ds[kWtTile][MR];
-    const int kw = blockIdx.x * kWtThreads + threadIdx.x, words = K / 8, groups = K / 32;
-    const int m0 = blockIdx.z * MR;
-    const int nb = static_cast<int>(static_cast<long long>(N) * blockIdx.y / gridDim.y);
-    const int ne = static_cast<int>(static_cast<long long>(N) * (blockIdx.y + 1) / gridDim.y);
-    float acc[MR][8];
+                                                             const long long* __restrict__ targets,
+                                                             float* __restrict__ z, float* __restrict__ zt,
+                                                             float* __restrict__ smax, float* __restrict__ ssum, int N,
+                                                             int K) {
+    __shared__ __align__(16) float xs[MR * kRowsChunk];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = blockIdx.x * kRowsCols + lane, groups = K / 32;
+    const size_t row_g = static_cast<size_t>(min(n, N - 1)) * groups;
+    float2 acc[MR];
 #pragma unroll
-    for (int r = 0; r < MR; ++r)
+    for (int r = 0; r < MR; ++r) acc[r] = make_float2(0.0f, 0.0f);
+    for (int k0 = 0; k0 < K; k0 += kRowsChunk) {
+        const int g0 = k0 / 32 + warp * kRowsBatch, kn = min(kRowsChunk, K - k0);
+        uint4 q[kRowsBatch];
+        float s[kRowsBatch];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[r][i] = 0.0f;
-    for (int n0 = nb; n0 < ne; n0 += kWtTile) {
-        const int cnt = min(kWtTile, ne - n0);
-        __syncthreads();
-        for (int i = threadIdx.x; i < MR * kWtTile; i += kWtThreads) {
-            const int r = i / kWtTile, j = i % kWtTile;
-            ds[j][r] = (j < cnt && m0 + r < M) ? row_load(d + static_cast<long long>(m0 + r) * ld_d + n0 + j) : 0.0f;
+        for (int b = 0; b < kRowsBatch; ++b) {
+            const bool in = g0 + b < groups;
+            q[b] = in ? __ldg(reinterpret_cast<const uint4*>(packed) + row_g + g0 + b) : make_uint4(0, 0, 0, 0);
+            s[b] = in ? __ldg(scales + row_g + g0 + b) : 0.0f;
+        }
+        __syncthreads();  // the chunk before has been read
+        for (int i = threadIdx.x * 8; i < MR * kRowsChunk; i += 256 * 8) {
+            const int r = i / kRowsChunk, k = i % kRowsChunk;
+            float v[8];
+            if (k < kn) {
+                row_load8(x + static_cast<size_t>(r) * K + k0 + k, v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+            }
+            *reinterpret_cast<float4*>(xs + i) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(xs + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
         }
         __syncthreads();
-        if (kw < words) {
-            const uint32_t* pw = packed + static_cast<size_t>(n0) * words + kw;
-            const float* ps = scales + static_cast<size_t>(n0) * groups + (kw >> 2);
-#pragma unroll 8
-            for (int j = 0; j < cnt; ++j) {
+#pragma unroll
+        for (int b = 0; b < kRowsBatch; ++b) {
+            if (g0 + b >= groups) break;  // an infinite x may not meet a group that does not exist
+            const uint32_t words[4] = {q[b].x, q[b].y, q[b].z, q[b].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
                 float wv[8];
-                word_weights(__ldg(pw + static_cast<size_t>(j) * words), __ldg(ps + static_cast<size_t>(j) * groups), wv);
+                word_weights(words[i], s[b], wv);
+                const float* xp = xs + (warp * kRowsBatch + b) * 32 + i * 8;
 #pragma unroll
                 for (int r = 0; r < MR; ++r) {
-                    const float dv = ds[j][r];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[r][i] = fmaf(dv, wv[i], acc[r][i]);
+                    const float4 u = *reinterpret_cast<const float4*>(xp + r * kRowsChunk);
+                    const float4 v = *reinterpret_cast<const float4*>(xp + r * kRowsChunk + 4);
+                    acc[r] = ffma2(make_float2(u.x, u.y), make_float2(wv[0], wv[1]), acc[r]);
+                    acc[r] = ffma2(make_float2(u.z, u.w), make_float2(wv[2], wv[3]), acc[r]);
+                    acc[r] = ffma2(make_float2(v.x, v.y), make_float2(wv[4], wv[5]), acc[r]);
+                    acc[r] = ffma2(make_float2(v.z, v.w), make_float2(wv[6], wv[7]), acc[r]);
                 }
             }
         }
     }
-    if (kw >= words) return;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < MR; ++r) xs[(r * 8 + warp) * 32 + lane] = acc[r].x + acc[r].y;
+    __syncthreads();
+    for (int r = warp; r < MR; r += 8) {  // one warp per row, one column per lane
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) total += xs[(r * 8 + w) * 32 + lane];
+        const bool hot = targets[r] == n;
+        if (n < N) z[static_cast<long long>(r) * N + n] = total;
+        if (hot && n < N) zt[r] = total;
+        const float z2 = n < N && !hot ? total * 1.4426950408889634f : -INFINITY;
+        float top = z2;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float sum = exp2f(z2 - (top == -INFINITY ? 0.0f : top));
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+            smax[static_cast<size_t>(r) * gridDim.x + blockIdx.x] = top;
+            ssum[static_cast<size_t>(r) * gridDim.x + blockIdx.x] = sum;
+        }
+    }
+}
+
+// One block per row of the blocks' statistics: lse, loss, and for the
+// gradient M2, g / S and g (p_target - 1) (coef[3 row ..]).  A negative target
+// takes the row out of the loss (loss 0, gradient 0); one past the columns
+// gives NaN.
+__global__ void __launch_bounds__(512) rows_loss_kernel(const float* __restrict__ smax, const float* __restrict__ ssum,
+                                                        const float* __restrict__ zt,
+                                                        const long long* __restrict__ targets,
+                                                        const float* __restrict__ row_scale, float* __restrict__ loss,
+                                                        float* __restrict__ lse, float* __restrict__ coef, int N,
+                                                        int tiles) {
+    __shared__ float red[16];
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float* sm = smax + static_cast<size_t>(row) * tiles;
+    const float* ss = ssum + static_cast<size_t>(row) * tiles;
+    const long long t = targets[row];
+    const float t2 = t >= 0 && t < N ? zt[row] * 1.4426950408889634f : -INFINITY;
+    float top = t2;
+    for (int i = threadIdx.x; i < tiles; i += 512) top = fmaxf(top, sm[i]);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, red[i]);
+    __syncthreads();
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < tiles; i += 512) sum += exp2f(sm[i] - top) * ss[i];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    sum = 0.0f;
+    for (int i = 0; i < 16; ++i) sum += red[i];
+    const float et = exp2f(t2 - top), all = sum + et;
+    const float l = 0.69314718055994531f * (top + log2f(all));
+    const float v = t < 0 ? 0.0f : t >= N ? NAN : et > 0.0009765625f ? log1pf(sum / et) : l - zt[row];
+    if (lse != nullptr) lse[row] = l;
+    loss[row] = v;
+    const float g = t < 0 ? 0.0f : row_scale != nullptr ? row_scale[row] : 1.0f;
+    coef[3 * row] = top;
+    coef[3 * row + 1] = t < N ? g / all : NAN;
+    coef[3 * row + 2] = t < 0 ? 0.0f : g * expm1f(-v);
+}
+
+// Thread (word of k, part p of 4): 8 outputs of MR rows over a quarter of
+// blockIdx.y's range of n; the quarters are added through shared memory.  The
+// rows' d values of 256 n at a time sit in shared memory: d itself, or with
+// `coef` (the loss) g p = coef[1] exp2(z2 - coef[0]) and coef[2] at the target.
+// The words of eight n per thread are in flight while d is staged.
+constexpr int kWtWords = 64, kWtParts = 4, kWtThreads = kWtWords * kWtParts, kWtTile = 128, kWtBatch = 8;
+template <int MR, typename T>
+__global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(const T* __restrict__ d, const float* __restrict__ coef,
+                                                             const long long* __restrict__ targets,
+                                                             const uint32_t* __restrict__ packed,
+                                                             const float* __restrict__ scales,
+                                                             float* __restrict__ partial, int N, int K) {
+    __shared__ __align__(16) float ds[kWtTile][MR];
+    __shared__ __align__(16) float sums[kWtParts - 1][kWtWords][8];
+    const int wl = threadIdx.x % kWtWords, part = threadIdx.x / kWtWords;
+    const int kw = blockIdx.x * kWtWords + wl, words = K / 8, groups = K / 32;
+    const int nb = static_cast<int>(static_cast<long long>(N) * blockIdx.y / gridDim.y);
+    const int ne = static_cast<int>(static_cast<long long>(N) * (blockIdx.y + 1) / gridDim.y);
+    float2 acc[MR][4];
 #pragma unroll
     for (int r = 0; r < MR; ++r)
-        if (m0 + r < M) {
-            float4* out = reinterpret_cast<float4*>(
-                partial + (static_cast<size_t>(blockIdx.y) * M + m0 + r) * K + static_cast<size_t>(kw) * 8);
-            out[0] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
-            out[1] = make_float4(acc[r][4], acc[r][5], acc[r][6], acc[r][7]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][i] = make_float2(0.0f, 0.0f);
+    for (int n0 = nb; n0 < ne; n0 += kWtTile) {
+        const int cnt = min(kWtTile, ne - n0);
+        const uint32_t* pw = packed + static_cast<size_t>(n0) * words + kw;
+        const float* ps = scales + static_cast<size_t>(n0) * groups + (kw >> 2);
+        uint32_t q[kWtBatch];
+        float s[kWtBatch];
+        auto load = [&](int j0) {
+#pragma unroll
+            for (int b = 0; b < kWtBatch; ++b) {
+                const int j = j0 + b * kWtParts;
+                const bool in = j < cnt && kw < words;
+                q[b] = in ? __ldg(pw + static_cast<size_t>(j) * words) : 0u;
+                s[b] = in ? __ldg(ps + static_cast<size_t>(j) * groups) : 0.0f;
+            }
+        };
+        load(part);
+        __syncthreads();  // the tile before has been read
+        for (int i = threadIdx.x; i < MR * kWtTile; i += kWtThreads) {
+            const int r = i / kWtTile, j = i % kWtTile;
+            float v = 0.0f;
+            if (j < cnt) {
+                v = row_load(d + static_cast<size_t>(r) * N + n0 + j);
+                if (coef != nullptr) {
+                    const float inv = coef[3 * r + 1];
+                    v = targets[r] < 0 ? 0.0f
+                                       : targets[r] == n0 + j ? coef[3 * r + 2]
+                                                              : inv * exp2f(v * 1.4426950408889634f - coef[3 * r]);
+                }
+            }
+            ds[j][r] = v;
         }
-}
-
-__device__ __forceinline__ float rows_block_sum(float v, float* red) {
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.0f;
-    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) t += red[i];  // the same order in every thread
-    return t;
-}
-
-// One block per row of logits.  A negative target takes the row out of the
-// loss (loss 0, gradient 0); one past the columns gives NaN, never a read
-// outside the row.
-__global__ void __launch_bounds__(512) rows_softmax_kernel(float* __restrict__ z, long long ld_z,
-                                                           const long long* __restrict__ targets,
-                                                           const float* __restrict__ row_scale,
-                                                           float* __restrict__ loss, float* __restrict__ lse, int N,
-                                                           int want_grad) {
-    __shared__ float red[16];
-    float* row = z + static_cast<long long>(blockIdx.x) * ld_z;
-    float top = -INFINITY;
-    for (int n = threadIdx.x; n < N; n += blockDim.x) top = fmaxf(top, row[n]);
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-    __syncthreads();
-    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) top = fmaxf(top, red[i]);
-    float sum = 0.0f;
-    for (int n = threadIdx.x; n < N; n += blockDim.x) sum += expf(row[n] - top);
-    sum = rows_block_sum(sum, red);
-    const float l = top + logf(sum);
-    const long long t = targets[blockIdx.x];
-    const bool used = t >= 0;
-    const float zt = t >= 0 && t < N ? row[t] : NAN;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        if (lse != nullptr) lse[blockIdx.x] = l;
-        loss[blockIdx.x] = used ? l - zt : 0.0f;
+        __syncthreads();
+        for (int j0 = part; j0 < cnt; j0 += kWtBatch * kWtParts) {
+            if (j0 != part) load(j0);
+#pragma unroll
+            for (int b = 0; b < kWtBatch; ++b) {
+                const int j = j0 + b * kWtParts;
+                if (j >= cnt) break;
+                float wv[8];
+                word_weights(q[b], s[b], wv);
+#pragma unroll
+                for (int r = 0; r < MR; ++r) {
+                    const float2 dv = make_float2(ds[j][r], ds[j][r]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[r][i] = ffma2(dv, make_float2(wv[2 * i], wv[2 * i + 1]), acc[r][i]);
+                }
+            }
+        }
     }
-    if (!want_grad) return;
-    const float g = used ? (row_scale != nullptr ? row_scale[blockIdx.x] : 1.0f) : 0.0f;
-    const float bad = used && t >= N ? NAN : 0.0f;
-    for (int n = threadIdx.x; n < N; n += blockDim.x)
-        row[n] = used ? g * (expf(row[n] - top) / sum - (n == t ? 1.0f : 0.0f)) + bad : 0.0f;
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        float4* mine = part > 0 ? reinterpret_cast<float4*>(&sums[part - 1][wl][0]) : nullptr;
+        __syncthreads();
+        if (part > 0) {
+            mine[0] = make_float4(acc[r][0].x, acc[r][0].y, acc[r][1].x, acc[r][1].y);
+            mine[1] = make_float4(acc[r][2].x, acc[r][2].y, acc[r][3].x, acc[r][3].y);
+        }
+        __syncthreads();
+        if (part == 0 && kw < words) {
+            float4 a = make_float4(acc[r][0].x, acc[r][0].y, acc[r][1].x, acc[r][1].y);
+            float4 b = make_float4(acc[r][2].x, acc[r][2].y, acc[r][3].x, acc[r][3].y);
+#pragma unroll
+            for (int p = 0; p < kWtParts - 1; ++p) {
+                const float4 u = *reinterpret_cast<const float4*>(&sums[p][wl][0]);
+                const float4 v = *reinterpret_cast<const float4*>(&sums[p][wl][4]);
+                a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+                b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+            }
+            float4* out = reinterpret_cast<float4*>(partial + (static_cast<size_t>(blockIdx.y) * MR + r) * K +
+                                                    static_cast<size_t>(kw) * 8);
+            out[0] = a;
+            out[1] = b;
+        }
+    }
 }
 
-// Four rows x 16 ranks per block; the threads take n in turn and the 64 sums
-// are added over the block in a fixed order.
+// Four rows x 16 ranks per block and range of n (blockIdx.z): partial[z][M][rank].
 constexpr int kProjRows = 4, kProjRanks = 16;
 template <typename T>
 __global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy, const float* __restrict__ b,
-                                                        float scale, float* __restrict__ g, int M, int N, int rank) {
+                                                        float* __restrict__ g, int M, int N, int rank) {
     __shared__ float red[8][64];
     const int m0 = blockIdx.x * kProjRows, j0 = blockIdx.y * kProjRanks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nb = static_cast<int>(static_cast<long long>(N) * blockIdx.z / gridDim.z);
+    const int ne = static_cast<int>(static_cast<long long>(N) * (blockIdx.z + 1) / gridDim.z);
     float acc[64];
 #pragma unroll
     for (int i = 0; i < 64; ++i) acc[i] = 0.0f;
-    for (int n = threadIdx.x; n < N; n += 256) {
+    for (int n = nb + threadIdx.x; n < ne; n += 256) {
         float dv[kProjRows];
 #pragma unroll
         for (int r = 0; r < kProjRows; ++r) dv[r] = row_load(dy + static_cast<size_t>(min(m0 + r, M - 1)) * N + n);
@@ -231,111 +326,147 @@ __global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy
         float t = 0.0f;
         for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
         const int r = threadIdx.x / kProjRanks, j = threadIdx.x % kProjRanks;
-        if (m0 + r < M && j0 + j < rank) g[static_cast<size_t>(m0 + r) * rank + j0 + j] = scale * t;
+        if (m0 + r < M && j0 + j < rank) g[(static_cast<size_t>(blockIdx.z) * M + m0 + r) * rank + j0 + j] = t;
     }
 }
 
+// One row's 128 k per block (blockIdx.y: row): the splits' sum, half of them
+// per thread of a pair of warps, each in order; and with an adapter
+// scale * (sum of G's ranges) A^T.
 template <typename T>
 __global__ void __launch_bounds__(256) rows_finish_kernel(const float* __restrict__ partial, int splits,
                                                           long long split_floats, const float* __restrict__ g,
-                                                          const float* __restrict__ a, int rank, T* __restrict__ out,
-                                                          long long count, int K) {
-    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= count) return;
+                                                          int gsplits, const float* __restrict__ a, int rank,
+                                                          float scale, T* __restrict__ out, int M, int K) {
+    __shared__ float gs[64];
+    __shared__ float half[128];
+    const long long row = blockIdx.y;
+    const int c = threadIdx.x & 127, h = threadIdx.x >> 7, k = blockIdx.x * 128 + c;
+    if (threadIdx.x < rank) {
+        float t = 0.0f;
+#pragma unroll 8
+        for (int z = 0; z < gsplits; ++z) t += g[(static_cast<size_t>(z) * M + row) * rank + threadIdx.x];
+        gs[threadIdx.x] = scale * t;
+    }
     float v = 0.0f;
-    for (int z = 0; z < splits; ++z) v += partial[z * split_floats + i];
+    if (k < K) {
+        const float* p = partial + row * K + k;
+        const int z1 = h == 0 ? (splits + 1) / 2 : splits;
+#pragma unroll 8
+        for (int z = h == 0 ? 0 : (splits + 1) / 2; z < z1; ++z) v += p[z * split_floats];
+    }
+    if (h == 1) half[c] = v;
+    __syncthreads();
+    if (h == 1 || k >= K) return;
+    v += half[c];
     if (rank > 0) {
-        const long long m = i / K;
-        const int k = static_cast<int>(i % K);
+        const float* ar = a + static_cast<size_t>(k) * rank;
         float l = 0.0f;
-        for (int j = 0; j < rank; ++j) l = fmaf(g[m * rank + j], __ldg(a + static_cast<size_t>(k) * rank + j), l);
+#pragma unroll 8
+        for (int j = 0; j < rank; ++j) l = fmaf(gs[j], __ldg(ar + j), l);
         v += l;
     }
-    row_store(out + i, v);
+    row_store(out + row * K + k, v);
 }
 
+// f with the row count as a constant, 1..8.
 template <typename F>
-void rows_dispatch(int M, F&& f) {
-    if (M >= 5)
-        f(std::integral_constant<int, 8>());
-    else if (M >= 3)
-        f(std::integral_constant<int, 4>());
-    else if (M == 2)
-        f(std::integral_constant<int, 2>());
-    else
-        f(std::integral_constant<int, 1>());
+int rows_dispatch(int M, F&& f) {
+    switch (M) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        case 6: return f(std::integral_constant<int, 6>());
+        case 7: return f(std::integral_constant<int, 7>());
+        case 8: return f(std::integral_constant<int, 8>());
+    }
+    return static_cast<int>(cudaErrorInvalidValue);
 }
 
 }  // namespace
 
-int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, float* z, long long ld_z,
-                       int M, int N, int K, cudaStream_t stream) {
-    rows_dispatch(M, [&](auto mr) {
+int rows_logits_tiles(int N) { return (N + kRowsCols - 1) / kRowsCols; }
+
+int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, const long long* targets,
+                       float* z, float* zt, float* smax, float* ssum, int M, int N, int K, cudaStream_t stream) {
+    const unsigned grid = static_cast<unsigned>(rows_logits_tiles(N));
+    return rows_dispatch(M, [&](auto mr) {
         constexpr int MR = decltype(mr)::value;
-        const dim3 grid(static_cast<unsigned>((N + 8 * kRowsCols - 1) / (8 * kRowsCols)),
-                        static_cast<unsigned>((M + MR - 1) / MR));
         if (bf16)
-            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), packed, scales, z,
-                                                             ld_z, M, N, K);
+            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), packed, scales, targets,
+                                                             z, zt, smax, ssum, N, K);
         else
-            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), packed, scales, z, ld_z, M,
-                                                             N, K);
+            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), packed, scales, targets, z, zt,
+                                                             smax, ssum, N, K);
+        return static_cast<int>(cudaGetLastError());
     });
+}
+
+int launch_rows_loss(const float* smax, const float* ssum, const float* zt, const long long* targets,
+                     const float* row_scale, float* loss, float* lse, float* coef, int M, int N, cudaStream_t stream) {
+    rows_loss_kernel<<<static_cast<unsigned>(M), 512, 0, stream>>>(smax, ssum, zt, targets, row_scale, loss, lse, coef, N,
+                                                                   rows_logits_tiles(N));
     return static_cast<int>(cudaGetLastError());
 }
 
-// Splits of n: enough blocks for the SMs, at least 64 n each.
-int rows_wt_splits(int M, int N, int K, int sm_count) {
-    const long long blocks = static_cast<long long>((K / 8 + kWtThreads - 1) / kWtThreads) * ((M + 7) / 8);
-    long long s = (8ll * sm_count + blocks - 1) / blocks;
-    if (s > (N + 63) / 64) s = (N + 63) / 64;
+// Splits of n: about two blocks per SM (one wave), at least 32 n each.
+int rows_wt_splits(int N, int K, int sm_count) {
+    const long long blocks = (K / 8 + kWtWords - 1) / kWtWords;
+    long long s = 2ll * sm_count / blocks;
+    if (s > (N + 31) / 32) s = (N + 31) / 32;
     return static_cast<int>(s < 1 ? 1 : s);
 }
 
-int launch_rows_wt(const void* d, bool bf16, long long ld_d, const uint32_t* packed, const float* scales,
-                   float* partial, int splits, int M, int N, int K, cudaStream_t stream) {
-    rows_dispatch(M, [&](auto mr) {
+int launch_rows_wt(const void* d, bool bf16, const float* coef, const long long* targets, const uint32_t* packed,
+                   const float* scales, float* partial, int splits, int M, int N, int K, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>((K / 8 + kWtWords - 1) / kWtWords), static_cast<unsigned>(splits));
+    return rows_dispatch(M, [&](auto mr) {
         constexpr int MR = decltype(mr)::value;
-        const dim3 grid(static_cast<unsigned>((K / 8 + kWtThreads - 1) / kWtThreads), static_cast<unsigned>(splits),
-                        static_cast<unsigned>((M + MR - 1) / MR));
         if (bf16)
-            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(d), ld_d, packed,
-                                                                scales, partial, M, N, K);
+            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(d), coef, targets, packed,
+                                                                scales, partial, N, K);
         else
-            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const float*>(d), ld_d, packed, scales,
-                                                                partial, M, N, K);
+            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const float*>(d), coef, targets, packed, scales,
+                                                                partial, N, K);
+        return static_cast<int>(cudaGetLastError());
     });
-    return static_cast<int>(cudaGetLastError());
 }
 
-int launch_rows_softmax(float* z, long long ld_z, const long long* targets, const float* row_scale, float* loss,
-                        float* lse, int M, int N, bool want_grad, cudaStream_t stream) {
-    rows_softmax_kernel<<<static_cast<unsigned>(M), 512, 0, stream>>>(z, ld_z, targets, row_scale, loss, lse, N,
-                                                                       want_grad ? 1 : 0);
-    return static_cast<int>(cudaGetLastError());
+// Ranges of n per block of rows: enough blocks for the SMs, at least 256 n each.
+int rows_proj_splits(int M, int N, int rank, int sm_count) {
+    const long long blocks = static_cast<long long>((M + kProjRows - 1) / kProjRows) * ((rank + kProjRanks - 1) / kProjRanks);
+    long long s = sm_count / blocks;
+    if (s > N / 256) s = N / 256;
+    return static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
-int launch_rows_proj(const void* dy, bool bf16, const float* b, float scale, float* g, int M, int N, int rank,
+int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int splits, int M, int N, int rank,
                      cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>((M + kProjRows - 1) / kProjRows),
-                    static_cast<unsigned>((rank + kProjRanks - 1) / kProjRanks));
+                    static_cast<unsigned>((rank + kProjRanks - 1) / kProjRanks), static_cast<unsigned>(splits));
     if (bf16)
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), b, scale, g, M, N, rank);
+        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), b, g, M, N, rank);
     else
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(dy), b, scale, g, M, N, rank);
+        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(dy), b, g, M, N, rank);
     return static_cast<int>(cudaGetLastError());
 }
 
-int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, const float* a,
-                       int rank, void* out, bool bf16, int M, int K, cudaStream_t stream) {
-    const long long count = static_cast<long long>(M) * K;
-    const unsigned blocks = static_cast<unsigned>((count + 255) / 256);
-    if (bf16)
-        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, split_floats, g, a, rank,
-                                                       static_cast<__nv_bfloat16*>(out), count, K);
-    else
-        rows_finish_kernel<<<blocks, 256, 0, stream>>>(partial, splits, split_floats, g, a, rank, static_cast<float*>(out),
-                                                       count, K);
+int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, int gsplits,
+                       const float* a, int rank, float scale, void* out, bool bf16, int M, int K, cudaStream_t stream) {
+    for (int m0 = 0; m0 < M; m0 += 32768) {  // rows are blockIdx.y
+        const int mc = M - m0 < 32768 ? M - m0 : 32768;
+        if (rank > 0 && m0 > 0) return static_cast<int>(cudaErrorInvalidValue);  // an adapter here has few rows
+        const dim3 grid(static_cast<unsigned>((K + 127) / 128), static_cast<unsigned>(mc));
+        const float* p = partial + static_cast<long long>(m0) * K;
+        if (bf16)
+            rows_finish_kernel<<<grid, 256, 0, stream>>>(p, splits, split_floats, g, gsplits, a, rank, scale,
+                                                         static_cast<__nv_bfloat16*>(out) + static_cast<long long>(m0) * K, mc, K);
+        else
+            rows_finish_kernel<<<grid, 256, 0, stream>>>(p, splits, split_floats, g, gsplits, a, rank, scale,
+                                                         static_cast<float*>(out) + static_cast<long long>(m0) * K, mc, K);
+    }
     return static_cast<int>(cudaGetLastError());
 }
 

@@ -1339,18 +1339,16 @@ int pairs_or_throw() {
 // dX = dY W^T + s (dY B^T) A^T for at most kRowsKernelMax rows.
 void run_input_gradient_rows(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
-    const int splits = q4::rows_wt_splits(M, w->N, w->K, c.sm_count);
-    Scratch part(static_cast<size_t>(splits) * M * w->K * 4, s);
-    Scratch gs(static_cast<size_t>(M) * w->rank * 4, s);
-    const float lscale = w->rank > 0 ? w->alpha / static_cast<float>(w->rank) : 0.0f;
-    if (w->rank > 0)
-        check_launch(q4::launch_rows_proj(dy, bf16, w->lora_b, lscale, static_cast<float*>(gs.p), M, w->N, w->rank, s),
-                     "dY B^T");
-    check_launch(q4::launch_rows_wt(dy, bf16, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, M, w->N,
-                                    w->K, s),
+    const int splits = q4::rows_wt_splits(w->N, w->K, c.sm_count), r = w->rank;
+    const int gsplits = r > 0 ? q4::rows_proj_splits(M, w->N, r, c.sm_count) : 0;
+    const size_t pf = static_cast<size_t>(splits) * M * w->K;
+    Scratch sc((pf + static_cast<size_t>(gsplits) * M * r) * 4, s);
+    float *part = static_cast<float*>(sc.p), *gs = part + pf;
+    if (r > 0) check_launch(q4::launch_rows_proj(dy, bf16, w->lora_b, gs, gsplits, M, w->N, r, s), "dY B^T");
+    check_launch(q4::launch_rows_wt(dy, bf16, nullptr, nullptr, w->packed, w->scales, part, splits, M, w->N, w->K, s),
                  "dY W^T");
-    check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<long long>(M) * w->K,
-                                        static_cast<float*>(gs.p), w->lora_a, w->rank, dx, bf16, M, w->K, s),
+    check_launch(q4::launch_rows_finish(part, splits, static_cast<long long>(M) * w->K, gs, gsplits, w->lora_a, r,
+                                        r > 0 ? w->alpha / static_cast<float>(r) : 0.0f, dx, bf16, M, w->K, s),
                  "dX");
 }
 
@@ -1400,7 +1398,10 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
         Scratch part(g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0, s);
         int gsplits = 1;
-        if (gt) q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
+        if (gt)
+            q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
+        else if (r > 0)
+            gsplits = q4::rows_proj_splits(mc, N, r, c.sm_count);
         Scratch gs(r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0, s);
         float* gpart = static_cast<float*>(gs.p);
         if (gt && bf16) {
@@ -1426,7 +1427,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
             q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
             check_launch(q4::launch_lora_tc_pass(p, s), "dY B^T");
         } else if (r > 0) {
-            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, 1.0f, gpart, mc, N, r, s), "dY B^T");
+            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, gpart, gsplits, mc, N, r, s), "dY B^T");
         }
         q4::CastArgs ca{};
         ca.x = d; ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
@@ -1456,7 +1457,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, s), "dY W^T");
         if (g.splits > 1)
             check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), g.splits, static_cast<long long>(g.out_rows) * K,
-                                                nullptr, nullptr, 0, out, bf16, mc, K, s),
+                                                nullptr, 0, nullptr, 0, 0.0f, out, bf16, mc, K, s),
                          "dX");
     }
 }
@@ -1465,18 +1466,19 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
 void run_cross_entropy_rows(spaceslug_q4_weights* w, const void* x, bool bf16, const long long* targets,
                             const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
-    Scratch zs(static_cast<size_t>(M) * w->N * 4, s);
-    float* z = static_cast<float*>(zs.p);
-    check_launch(q4::launch_rows_logits(x, bf16, w->packed, w->scales, z, w->N, M, w->N, w->K, s), "logits");
-    check_launch(q4::launch_rows_softmax(z, w->N, targets, row_scale, loss, lse, M, w->N, dx != nullptr, s), "softmax");
+    const int N = w->N, K = w->K, tiles = q4::rows_logits_tiles(N);
+    const int splits = dx ? q4::rows_wt_splits(N, K, c.sm_count) : 0;
+    const size_t zf = (static_cast<size_t>(M) * N + 3) / 4 * 4, sf = static_cast<size_t>(M) * tiles;
+    const size_t pf = static_cast<size_t>(splits) * M * K;  // 16-byte aligned: behind z
+    Scratch sc((zf + pf + 2 * sf + static_cast<size_t>(4) * M) * 4, s);
+    float* z = static_cast<float*>(sc.p);
+    float *part = z + zf, *smax = part + pf, *ssum = smax + sf, *zt = ssum + sf, *coef = zt + M;
+    check_launch(q4::launch_rows_logits(x, bf16, w->packed, w->scales, targets, z, zt, smax, ssum, M, N, K, s), "logits");
+    check_launch(q4::launch_rows_loss(smax, ssum, zt, targets, row_scale, loss, lse, coef, M, N, s), "loss rows");
     if (!dx) return;
-    const int splits = q4::rows_wt_splits(M, w->N, w->K, c.sm_count);
-    Scratch part(static_cast<size_t>(splits) * M * w->K * 4, s);
-    check_launch(q4::launch_rows_wt(z, false, w->N, w->packed, w->scales, static_cast<float*>(part.p), splits, M, w->N,
-                                    w->K, s),
-                 "dZ W^T");
-    check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), splits, static_cast<long long>(M) * w->K, nullptr,
-                                        nullptr, 0, dx, bf16, M, w->K, s),
+    check_launch(q4::launch_rows_wt(z, false, coef, targets, w->packed, w->scales, part, splits, M, N, K, s), "P W^T");
+    check_launch(q4::launch_rows_finish(part, splits, static_cast<long long>(M) * K, nullptr, 0, nullptr, 0, 0.0f, dx, bf16,
+                                        M, K, s),
                  "dX");
 }
 
