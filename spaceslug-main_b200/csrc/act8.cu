@@ -15,7 +15,10 @@
 // reader turns into NaN (0 * inf).
 //
 // K is a multiple of 32, so a contiguous [m][K] matrix is a flat list of
-// groups: both kernels give 8 values to a thread and 4 lanes to a group.
+// groups.  A thread takes 16 bytes of x at a time (4 fp32 or 8 bf16 values, 8
+// or 4 lanes per group), so a warp's loads and stores are whole lines, and four
+// such pieces a block apart, all loaded before the first is used: both kernels
+// are bound by HBM, and one piece per thread leaves too few bytes in flight.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -28,90 +31,119 @@ namespace q4 {
 
 namespace {
 
-constexpr int kActThreads = 256;
+constexpr int kActThreads = 256, kActPieces = 4;
 constexpr int kActLargest = 249;  // step byte of magnitudes above 127 * 2^121
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+template <typename T>
+struct ActIo;  // a 16-byte piece of x as V values
+template <>
+struct ActIo<float> {
+    static constexpr int V = 4;
+    using Codes = uint32_t;
+    static __device__ __forceinline__ void values(uint4 q, float (&v)[4]) {
+        v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y);
+        v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
     }
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);  // exact for restored values
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    static __device__ __forceinline__ uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-}
+    static __device__ __forceinline__ Codes codes(const uint32_t (&w)[2]) { return w[0]; }
+    static __device__ __forceinline__ void words(Codes c, uint32_t (&w)[2]) { w[0] = c; }
+};
+template <>
+struct ActIo<__nv_bfloat16> {
+    static constexpr int V = 8;
+    using Codes = uint2;
+    static __device__ __forceinline__ void values(uint4 q, float (&v)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[8]) {
+        uint32_t w[4];  // restored values are exact in bf16
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __byte_perm(__float_as_uint(v[2 * i]), __float_as_uint(v[2 * i + 1]), 0x7632);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ Codes codes(const uint32_t (&w)[2]) { return make_uint2(w[0], w[1]); }
+    static __device__ __forceinline__ void words(Codes c, uint32_t (&w)[2]) { w[0] = c.x; w[1] = c.y; }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kActThreads) act8_pack_kernel(const T* __restrict__ x, int8_t* __restrict__ codes,
-                                                                uint8_t* __restrict__ exps, long long groups) {
-    const long long t = static_cast<long long>(blockIdx.x) * kActThreads + threadIdx.x;
-    const long long g = t >> 2;
-    const bool in = g < groups;  // a group's four lanes agree
-    float v[8];
-    if (in) {
-        load8(x + t * 8, v);
-    } else {
+                                                                uint8_t* __restrict__ exps, long long pieces) {
+    using Io = ActIo<T>;
+    constexpr int V = Io::V, kLanes = 32 / V;  // lanes per group
+    const long long t0 = static_cast<long long>(blockIdx.x) * (kActThreads * kActPieces) + threadIdx.x;
+    uint4 q[kActPieces];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int i = 0; i < kActPieces; ++i) {
+        const long long t = t0 + i * kActThreads;
+        q[i] = t < pieces ? __ldcs(reinterpret_cast<const uint4*>(x) + t) : make_uint4(0, 0, 0, 0);
     }
-    // magnitudes compared as bits: an infinity or a NaN is above every finite value
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const bool bad = top >= 0x7F800000u;
-    const int step = max(1, static_cast<int>(top >> 23) - 6 + ((top & 0x7FFFFFu) > 0x7E0000u ? 1 : 0));
-    const float inv = __uint_as_float(static_cast<uint32_t>(254 - step) << 23);  // 2^-e
-    if (step == kActLargest && !bad) {  // 64 steps would restore as an infinity
+    for (int i = 0; i < kActPieces; ++i) {
+        const long long t = t0 + i * kActThreads;  // a group's lanes agree on t < pieces
+        float v[V];
+        Io::values(q[i], v);
+        // magnitudes compared as bits: an infinity or a NaN is above every finite value
+        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -0x1.f8p+127f), 0x1.f8p+127f);
-    }
-    uint32_t w[2] = {0, 0};
+        for (int j = 0; j < V; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t c = bad ? 0u : static_cast<uint32_t>(__float2int_rn(v[i] * inv)) & 0xFFu;
-        w[i >> 2] |= c << (8 * (i & 3));
-    }
-    if (in) {
-        *reinterpret_cast<uint2*>(codes + t * 8) = make_uint2(w[0], w[1]);
-        if ((t & 3) == 0) exps[g] = static_cast<uint8_t>(bad ? 255 : step);
+        for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool bad = top >= 0x7F800000u;
+        const int step = max(1, static_cast<int>(top >> 23) - 6 + ((top & 0x7FFFFFu) > 0x7E0000u ? 1 : 0));
+        const float inv = __uint_as_float(static_cast<uint32_t>(254 - step) << 23);  // 2^-e
+        if (step == kActLargest && !bad) {  // 64 steps would restore as an infinity
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = fminf(fmaxf(v[j], -0x1.f8p+127f), 0x1.f8p+127f);
+        }
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint32_t c = bad ? 0u : static_cast<uint32_t>(__float2int_rn(v[j] * inv)) & 0xFFu;
+            w[j >> 2] |= c << (8 * (j & 3));
+        }
+        if (t < pieces) {
+            reinterpret_cast<typename Io::Codes*>(codes)[t] = Io::codes(w);
+            if (t % kLanes == 0) exps[t / kLanes] = static_cast<uint8_t>(bad ? 255 : step);
+        }
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kActThreads) act8_unpack_kernel(const int8_t* __restrict__ codes,
                                                                   const uint8_t* __restrict__ exps, T* __restrict__ x,
-                                                                  long long groups) {
-    const long long t = static_cast<long long>(blockIdx.x) * kActThreads + threadIdx.x;
-    const long long g = t >> 2;
-    if (g >= groups) return;
-    const uint2 q = __ldcs(reinterpret_cast<const uint2*>(codes + t * 8));
-    const float step = __uint_as_float(static_cast<uint32_t>(exps[g]) << 23);
-    const uint32_t w[2] = {q.x, q.y};
-    float v[8];
+                                                                  long long pieces) {
+    using Io = ActIo<T>;
+    constexpr int V = Io::V, kLanes = 32 / V;
+    const long long t0 = static_cast<long long>(blockIdx.x) * (kActThreads * kActPieces) + threadIdx.x;
+    typename Io::Codes c[kActPieces] = {};
+    uint32_t e[kActPieces] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = static_cast<float>(static_cast<int8_t>((w[i >> 2] >> (8 * (i & 3))) & 0xFFu)) * step;
-    store8(x + t * 8, v);
+    for (int i = 0; i < kActPieces; ++i) {
+        const long long t = t0 + i * kActThreads;
+        if (t < pieces) {
+            c[i] = __ldcs(reinterpret_cast<const typename Io::Codes*>(codes) + t);
+            e[i] = __ldg(exps + t / kLanes);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kActPieces; ++i) {
+        const long long t = t0 + i * kActThreads;
+        const float step = __uint_as_float(e[i] << 23);
+        uint32_t w[2];
+        Io::words(c[i], w);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            v[j] = static_cast<float>(static_cast<int8_t>((w[j >> 2] >> (8 * (j & 3))) & 0xFFu)) * step;
+        if (t < pieces) reinterpret_cast<uint4*>(x)[t] = Io::pack(v);
+    }
 }
 
 __global__ void __launch_bounds__(256) bf16_to_f32_kernel(const __nv_bfloat16* __restrict__ x, float* __restrict__ y,
@@ -128,22 +160,31 @@ int launch_bf16_to_f32(const void* x, float* y, long long count, cudaStream_t st
     return static_cast<int>(cudaGetLastError());
 }
 
+namespace {
+unsigned act8_blocks(long long pieces) {
+    const long long per = static_cast<long long>(kActThreads) * kActPieces;
+    return static_cast<unsigned>((pieces + per - 1) / per);
+}
+}  // namespace
+
 int launch_act8_pack(const void* x, bool bf16, int8_t* codes, uint8_t* exps, long long groups, cudaStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>((groups * 4 + kActThreads - 1) / kActThreads);
+    const long long pieces = groups * (bf16 ? 4 : 8);
     if (bf16)
-        act8_pack_kernel<<<blocks, kActThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), codes, exps, groups);
+        act8_pack_kernel<<<act8_blocks(pieces), kActThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), codes, exps,
+                                                                          pieces);
     else
-        act8_pack_kernel<<<blocks, kActThreads, 0, stream>>>(static_cast<const float*>(x), codes, exps, groups);
+        act8_pack_kernel<<<act8_blocks(pieces), kActThreads, 0, stream>>>(static_cast<const float*>(x), codes, exps, pieces);
     return static_cast<int>(cudaGetLastError());
 }
 
 int launch_act8_unpack(const int8_t* codes, const uint8_t* exps, void* x, bool bf16, long long groups,
                        cudaStream_t stream) {
-    const unsigned blocks = static_cast<unsigned>((groups * 4 + kActThreads - 1) / kActThreads);
+    const long long pieces = groups * (bf16 ? 4 : 8);
     if (bf16)
-        act8_unpack_kernel<<<blocks, kActThreads, 0, stream>>>(codes, exps, static_cast<__nv_bfloat16*>(x), groups);
+        act8_unpack_kernel<<<act8_blocks(pieces), kActThreads, 0, stream>>>(codes, exps, static_cast<__nv_bfloat16*>(x),
+                                                                            pieces);
     else
-        act8_unpack_kernel<<<blocks, kActThreads, 0, stream>>>(codes, exps, static_cast<float*>(x), groups);
+        act8_unpack_kernel<<<act8_blocks(pieces), kActThreads, 0, stream>>>(codes, exps, static_cast<float*>(x), pieces);
     return static_cast<int>(cudaGetLastError());
 }
 
