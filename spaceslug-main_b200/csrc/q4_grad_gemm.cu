@@ -58,7 +58,6 @@ namespace q4 {
 
 namespace {
 
-constexpr int kGgThreads = 640;
 constexpr int kGgRows = 256;   // rows of the pair's tile (128 per CTA, one accumulator lane each)
 constexpr int kGgCols = 256;   // columns of the pair's tile
 constexpr int kGgBK = 64;      // contraction per stage
@@ -70,13 +69,18 @@ constexpr int kGgOutBytes = 4096;  // one block of 32 rows x 128 bytes per epilo
 constexpr int kGgRaw = 3;
 constexpr int kGgRawWords = 128 * 64, kGgRawBytes = kGgRawWords + 128 * 16;
 constexpr int kGgDeqWarp0 = 4, kGgDeqWarps = 8;  // two warpgroups, one per stage of a raw block
-constexpr int kGgEpiWarp0 = 12, kGgEpiWarps = 8;
+constexpr int kGgEpiWarps = 8;
 // Registers per thread after the split: the launch's 640 x 96 cover 128 x 32 + 256 x 56 + 256 x 168.
 constexpr int kGgRegsLaunch = 96, kGgRegsCtl = 32, kGgRegsDeq = 56, kGgRegsEpi = 168;
-static_assert(128 * kGgRegsCtl + 256 * kGgRegsDeq + 256 * kGgRegsEpi <= kGgThreads * kGgRegsLaunch, "register split");
+static_assert(128 * kGgRegsCtl + 256 * kGgRegsDeq + 256 * kGgRegsEpi <= 640 * kGgRegsLaunch, "register split");
 
-template <int PA, int PB>
+// WT: the weights come dequantised from planes in memory (TMA), without dequant
+// warps and without a register split (384 threads of up to 168 registers).
+template <int PA, int PB, bool WT>
 struct GgCfg {
+    static constexpr int kThreads = WT ? 384 : 640;
+    static constexpr int kEpiWarp0 = WT ? 4 : 12;
+    static constexpr int kRegsLaunch = WT ? 0 : kGgRegsLaunch;  // least the launch must have
     // (1, 2): the lo plane of w in fp8, against an fp8 copy of the rows
     static constexpr bool kLo8 = PA == 1 && PB == 2;
     static constexpr int kA8 = PA * kGgTile;                       // fp8 rows: 128 x 64 bytes
@@ -244,9 +248,9 @@ __device__ __forceinline__ void gg_stage_row(uint8_t* buf, int lane, int piece, 
     *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
 }
 
-template <bool TR, int PA, int PB, int EPI>
-__global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_constant__ GradGemmArgs P) {
-    using C = GgCfg<PA, PB>;
+template <bool TR, int PA, int PB, int EPI, bool WT>
+__global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __grid_constant__ GradGemmArgs P) {
+    using C = GgCfg<PA, PB, WT>;
     constexpr int ST = C::kStages;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = smem_u32(smem_raw);
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
     const uint32_t tmem = *tmem_holder;
 
     if (warp < 4) {
-        regs_dec<kGgRegsCtl>();
+        if constexpr (!WT) regs_dec<kGgRegsCtl>();
         if (warp == 0 && lane == 0) {
             // ------------------------------------------------ row planes --
             int it = 0;
@@ -321,8 +325,26 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                         ok = false;
                         break;
                     }
-                    if (leader) mbar_arrive_expect_tx(full_x(s), 2u * static_cast<uint32_t>(C::kB));
+                    if (leader) mbar_arrive_expect_tx(full_x(s), 2u * static_cast<uint32_t>(WT ? C::kStageBytes : C::kB));
                     const uint32_t fx = leader_addr(full_x(s));
+                    if constexpr (WT) {
+                        const uint32_t b = base + s * C::kStageBytes + C::kB;
+                        const int tile0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf;
+                        if constexpr (TR) {  // 64 n x 128 k as two boxes of 64 k; the adapter's stage from A^T's planes
+                            const bool at = st == P.lora_stage;
+#pragma unroll
+                            for (int p = 0; p < PB; ++p)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    tma_load_2d_pair(b + p * kGgTile + h * (kGgTile / 2),
+                                                     at ? &P.tm_at : p == 0 ? &P.tm_w : &P.tm_s, fx, tile0 + 64 * h,
+                                                     at ? 64 * p : st * kGgBK);
+                        } else {
+                            tma_load_2d_pair(b, &P.tm_w, fx, st * kGgBK, tile0);
+                            if constexpr (PB == 2)
+                                tma_load_2d_pair(base + s * C::kStageBytes + C::kBLo, &P.tm_s, fx, st * kGgBK, tile0);
+                        }
+                    }
 #pragma unroll
                     for (int p = 0; p < PA; ++p)
                         tma_load_2d_pair(base + s * C::kStageBytes + p * kGgTile, &P.tm_a, fx, st * kGgBK,
@@ -333,7 +355,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
             }
             if (*abort_flag && leader)
                 for (int j = (it > ST ? it - ST : 0); j < it; ++j) mbar_drain(full_x(j % ST), (j / ST) & 1u);
-        } else if (warp == 3 && lane == 0) {
+        } else if (!WT && warp == 3 && lane == 0) {
             // ---------------------------------------------- raw weights --
             int it = 0;
             bool ok = true;
@@ -378,7 +400,7 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
                         const int s = it % ST;
                         const uint32_t ph = (it / ST) & 1u;
                         if (!gg_wait(full_x(s), ph, abort_flag, status, kStatusTimeoutMma) ||
-                            !gg_wait(full_w(s), ph, abort_flag, status, kStatusTimeoutMma)) {
+                            (!WT && !gg_wait(full_w(s), ph, abort_flag, status, kStatusTimeoutMma))) {
                             ok = false;
                             break;
                         }
@@ -414,14 +436,14 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
             mbar_drain(done_bar, 0u);
         }
         __syncwarp();
-    } else if (warp < kGgEpiWarp0) {
+    } else if (!WT && warp < C::kEpiWarp0) {
         // ------------------------------------------------------- dequant --
         // Warpgroup g dequantises stage g of each raw block, which holds two: the
         // k halves (logits) or the n halves (transposed).  Its thread t: logits,
         // column n = t of this CTA's 128 and the stage's 64 k; transposed, n = t
         // % 64 of the stage's 64 and the 64 k t / 64 of this CTA's 128: either
         // way two scale groups of one n.
-        regs_dec<kGgRegsDeq>();
+        if constexpr (!WT) regs_dec<kGgRegsDeq>();
         const int g = (warp - kGgDeqWarp0) >> 2, t = (tid - kGgDeqWarp0 * 32) & 127;
         const float cs = exp2i(*P.w_exp);
         const int row = TR ? (t & 63) : t;  // row of the operand image
@@ -498,8 +520,8 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
         }
     } else {
         // ------------------------------------------------------ epilogue --
-        regs_inc<kGgRegsEpi>();
-        const int ew = warp - kGgEpiWarp0, quarter = warp & 3, half = ew >> 2;
+        if constexpr (!WT) regs_inc<kGgRegsEpi>();
+        const int ew = warp - C::kEpiWarp0, quarter = warp & 3, half = ew >> 2;
         const uint32_t t_lane = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(half * 128);
         uint8_t* buf = smem + C::kOutOff + ew * kGgOutBytes;
         const uint32_t buf_s = base + C::kOutOff + ew * kGgOutBytes;
@@ -669,22 +691,22 @@ __global__ void __launch_bounds__(kGgThreads, 1) grad_gemm_kernel(const __grid_c
     }
 }
 
-template <bool TR, int PA, int PB, int EPI>
+template <bool TR, int PA, int PB, int EPI, bool WT>
 int gg_pairs() {
-    using C = GgCfg<PA, PB>;
+    using C = GgCfg<PA, PB, WT>;
     static int cache[64];
     static bool known[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
     if (known[dev]) return cache[dev];
-    auto kern = grad_gemm_kernel<TR, PA, PB, EPI>;
+    auto kern = grad_gemm_kernel<TR, PA, PB, EPI, WT>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return 0;
     cudaFuncAttributes fa{};
     // the register split draws on the launch's registers: refuse a build that was given fewer
-    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs < kGgRegsLaunch) return 0;
+    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs < C::kRegsLaunch) return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2, 1, 1);
-    cfg.blockDim = dim3(kGgThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -700,16 +722,16 @@ int gg_pairs() {
     return n;
 }
 
-template <bool TR, int PA, int PB, int EPI>
+template <bool TR, int PA, int PB, int EPI, bool WT>
 int gg_launch(const GradGemmArgs& a, cudaStream_t stream) {
-    using C = GgCfg<PA, PB>;
-    auto kern = grad_gemm_kernel<TR, PA, PB, EPI>;
-    const int cap = gg_pairs<TR, PA, PB, EPI>();
+    using C = GgCfg<PA, PB, WT>;
+    auto kern = grad_gemm_kernel<TR, PA, PB, EPI, WT>;
+    const int cap = gg_pairs<TR, PA, PB, EPI, WT>();
     const long long units = static_cast<long long>(a.row_tiles) * a.col_tiles * a.splits;
     if (cap < 1 || units < 1 || units > (1ll << 30)) return static_cast<int>(cudaErrorInvalidConfiguration);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (units < cap ? units : cap)), 1, 1);
-    cfg.blockDim = dim3(kGgThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -856,6 +878,41 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = p >= gp ? gs[(p - gp) * 8 + i] : 0.0f;
         put(p, v);
+    }
+}
+
+// The dequantised planes [N][K] of a handle's weights, in the dequantised
+// words' order: what the products' dequant warps write to shared memory, once
+// for all row tiles.  Four words per thread, a block apart.
+template <int PB, bool LO8>
+__global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __restrict__ packed,
+                                                            const float* __restrict__ scales,
+                                                            const int* __restrict__ w_exp, __half* __restrict__ hi,
+                                                            __half* __restrict__ lo, long long words) {
+    const float cs = exp2i(*w_exp);
+    const long long i0 = static_cast<long long>(blockIdx.x) * 1024 + threadIdx.x;
+    uint32_t q[4];
+    float s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const long long i = i0 + u * 256;
+        q[u] = i < words ? __ldcs(packed + i) : 0u;
+        s[u] = i < words ? __ldg(scales + (i >> 2)) : 0.0f;  // a row has K / 8 words and K / 32 scales
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const long long i = i0 + u * 256;
+        if (i >= words) break;
+        __half2 s_hi, s_lo;
+        split_scale_f16(s[u] * cs, s_hi, s_lo);
+        uint4 h, l;
+        gg_dequant<PB, LO8>(q[u], s_hi, s_lo, h, l);
+        reinterpret_cast<uint4*>(hi)[i] = h;
+        if constexpr (LO8) {
+            reinterpret_cast<uint2*>(lo)[i] = make_uint2(l.x, l.y);
+        } else if constexpr (PB == 2) {
+            reinterpret_cast<uint4*>(lo)[i] = l;
+        }
     }
 }
 
@@ -1026,20 +1083,41 @@ int gg_launch_pdl(Kern kern, unsigned grid, cudaStream_t stream, const Arg& arg)
 
 }  // namespace
 
-int grad_gemm_pairs() { return gg_pairs<true, 1, 1, kGgBf16>(); }
+int grad_gemm_pairs() { return gg_pairs<true, 1, 1, kGgBf16, false>(); }
 
-int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream) {
+namespace {
+template <bool WT>
+int gg_dispatch(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream) {
     switch (epi) {
         case kGgLoss:
-            return planes == 1 ? gg_launch<false, 1, 2, kGgLoss>(a, stream) : gg_launch<false, 2, 2, kGgLoss>(a, stream);
+            return planes == 1 ? gg_launch<false, 1, 2, kGgLoss, WT>(a, stream) : gg_launch<false, 2, 2, kGgLoss, WT>(a, stream);
         case kGgProb:
-            return planes == 1 ? gg_launch<false, 1, 2, kGgProb>(a, stream) : gg_launch<false, 2, 2, kGgProb>(a, stream);
+            return planes == 1 ? gg_launch<false, 1, 2, kGgProb, WT>(a, stream) : gg_launch<false, 2, 2, kGgProb, WT>(a, stream);
         case kGgF32:
-            return planes == 1 ? gg_launch<true, 1, 1, kGgF32>(a, stream) : gg_launch<true, 2, 2, kGgF32>(a, stream);
+            return planes == 1 ? gg_launch<true, 1, 1, kGgF32, WT>(a, stream) : gg_launch<true, 2, 2, kGgF32, WT>(a, stream);
         case kGgBf16:
-            if (planes == 1) return gg_launch<true, 1, 1, kGgBf16>(a, stream);
+            if (planes == 1) return gg_launch<true, 1, 1, kGgBf16, WT>(a, stream);
     }
     return static_cast<int>(cudaErrorInvalidValue);
+}
+}  // namespace
+
+int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_planes, cudaStream_t stream) {
+    return from_planes ? gg_dispatch<true>(a, planes, epi, stream) : gg_dispatch<false>(a, planes, epi, stream);
+}
+
+int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo, bool lo8,
+                         int N, int K, cudaStream_t stream) {
+    const long long words = static_cast<long long>(N) * (K / 8);
+    const unsigned blocks = static_cast<unsigned>((words + 1023) / 1024);
+    __half *h = static_cast<__half*>(hi), *l = static_cast<__half*>(lo);
+    if (lo == nullptr)
+        weight_planes_kernel<1, false><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
+    else if (lo8)
+        weight_planes_kernel<2, true><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
+    else
+        weight_planes_kernel<2, false><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
+    return static_cast<int>(cudaGetLastError());
 }
 
 int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream) {

@@ -1292,6 +1292,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
 constexpr int kRowsKernelMax = 8;
 constexpr long long kTrainScratch = 512ll << 20;  // bytes of operand planes per block of rows
+constexpr int kPlaneRows = 1024;  // rows from which the weights are dequantised once into planes
 
 // Splits of the contraction of a product of `tiles` 256 x 256 tiles and
 // `chunks` accumulator chunks of `cost` cycles: the least of waves x (chunks
@@ -1319,16 +1320,43 @@ void encode_grad_out(CUtensorMap* map, const void* out, uint64_t rows, int K) {
               32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// The handle's words and scales as the training products load them: blocks of
-// 128 columns x 128 k.
-void encode_grad_weights(spaceslug_q4_weights* w, q4::GradGemmArgs& g) {
-    const int K = w->K, N = w->N, G = K / 32, Gp = (G + 3) / 4 * 4;
-    const float* scales = w->scales_pad ? w->scales_pad : w->scales;
-    encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, w->packed, static_cast<uint64_t>(K) / 8, static_cast<uint64_t>(N),
-              static_cast<uint64_t>(K) / 2, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
-    encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, scales, static_cast<uint64_t>(G), static_cast<uint64_t>(N),
-              static_cast<uint64_t>(Gp) * 4, 4, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
-}
+// The weights of one training call: the handle's words and scales, dequantised
+// by the products themselves, or (many row tiles, whose every one would
+// dequantise them again) planes that one kernel writes into scratch first.
+struct TrainWeights {
+    spaceslug_q4_weights* w;
+    int planes;       // f16 planes of the rows (1: bf16, 2: fp32)
+    bool from_planes;
+    Scratch hi, lo;
+    TrainWeights(spaceslug_q4_weights* h, int row_planes, bool logits, int M, cudaStream_t s)
+        : w(h), planes(row_planes), from_planes(M >= kPlaneRows),
+          hi(from_planes ? static_cast<size_t>(h->N) * h->K * 2 : 0, s),
+          lo(!from_planes ? 0 : static_cast<size_t>(h->N) * h->K * (row_planes == 2 ? 2 : logits ? 1 : 0), s) {
+        if (from_planes)
+            check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, hi.p, lo.p, planes == 1, w->N,
+                                                  w->K, s),
+                         "weight planes");
+    }
+    // tensor maps of the logits' (or, transposed, the second) product
+    void encode(q4::GradGemmArgs& g, bool transposed) const {
+        const uint64_t K = static_cast<uint64_t>(w->K), N = static_cast<uint64_t>(w->N);
+        if (from_planes) {
+            const uint32_t rows = transposed ? 64 : 128;
+            const bool lo8 = planes == 1;
+            encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, hi.p, K, N, K * 2, 64, rows, CU_TENSOR_MAP_SWIZZLE_128B);
+            g.tm_s = g.tm_w;  // not read by a product of one plane of the weights
+            if (lo.p && !(lo8 && transposed))
+                encode_2d(&g.tm_s, lo8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, lo.p, K, N,
+                          lo8 ? K : K * 2, 64, rows, lo8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+            g.tm_at = g.tm_w;  // read with an adapter only
+            return;
+        }
+        const uint64_t G = K / 32, Gp = (G + 3) / 4 * 4;
+        const float* scales = w->scales_pad ? w->scales_pad : w->scales;
+        encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, w->packed, K / 8, N, K / 2, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
+        encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, scales, G, N, Gp * 4, 4, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+};
 
 int pairs_or_throw() {
     const int pairs = q4::grad_gemm_pairs();
@@ -1378,6 +1406,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
                                  nullptr, np};
         check_launch(q4::launch_lora16_finish(&f, 1, s), "B planes");
     }
+    const TrainWeights weights(w, planes, false, M, s);
     const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0);
@@ -1447,14 +1476,18 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         else
             encode_grad_out(&g.tm_out, part.p ? part.p : out,
                             part.p ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc), K);
-        encode_grad_weights(w, g);
+        weights.encode(g, true);
+        if (weights.from_planes && r > 0)
+            encode_2d(&g.tm_at, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, at.p, static_cast<uint64_t>(ld_at),
+                      static_cast<uint64_t>(planes) * 64, static_cast<uint64_t>(ld_at) * 2, 64, 64,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
         g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
         g.lora_at = at.p;
         g.ld_at = static_cast<int>(ld_at);
         g.lora_stage = r > 0 ? wstages : -1;
         g.status = c.status;
-        check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, s), "dY W^T");
+        check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, weights.from_planes, s), "dY W^T");
         if (g.splits > 1)
             check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), g.splits, static_cast<long long>(g.out_rows) * K,
                                                 nullptr, 0, nullptr, 0, 0.0f, out, bf16, mc, K, s),
@@ -1502,6 +1535,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     const long long ld_p = static_cast<long long>(tiles) * 256;
     const long long row_bytes = 2ll * planes * (dx ? ld_p : K);
     const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20));
+    const TrainWeights weights(w, planes, true, M, s);
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
         Scratch x16(static_cast<size_t>(planes) * mc * K * 2, s);
@@ -1531,7 +1565,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.chunks = (g.stages + g.chunk - 1) / g.chunk;
         g.plane_rows = mc;
         g.out_rows = mp;
-        encode_grad_weights(w, g);
+        weights.encode(g, false);
         g.w_exp = w->col_exp + N;
         g.row_exp = static_cast<int*>(rexp.p);
         g.targets = targets + m0;
@@ -1551,7 +1585,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
                       CU_TENSOR_MAP_SWIZZLE_128B);
         else
             g.tm_out = g.tm_a;  // not read
-        check_launch(q4::launch_grad_gemm(g, planes, dx ? q4::kGgProb : q4::kGgLoss, s), "logits");
+        check_launch(q4::launch_grad_gemm(g, planes, dx ? q4::kGgProb : q4::kGgLoss, weights.from_planes, s), "logits");
         check_launch(q4::launch_loss_rows(smax, ssum, zt, targets + m0, total, loss + m0, lse ? lse + m0 : nullptr, mc, N,
                                           tiles, mp, s),
                      "loss rows");
@@ -1571,7 +1605,8 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
                   static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         encode_grad_out(&d.tm_out, part.p, static_cast<uint64_t>(d.splits) * mp, K);
-        check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, s), "P W^T");
+        weights.encode(d, true);
+        check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, weights.from_planes, s), "P W^T");
         check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, loss + m0, targets + m0,
                                         row_scale ? row_scale + m0 : nullptr, w->packed, w->scales,
                                         static_cast<char*>(dx) + static_cast<size_t>(m0) * K * size, bf16, mc, N, K, s),
