@@ -264,6 +264,13 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 // predecessor finished must wait here before touching data the predecessor
 // writes; a kernel signals its dependents may start their prologue.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// p after a pdl_wait, opaque to the compiler: a load through a read-only
+// (__restrict__ or __ldg) pointer may otherwise be moved above the wait.
+template <typename T>
+__device__ __forceinline__ T* after_wait(T* p) {
+    asm volatile("" : "+l"(p)::"memory");
+    return p;
+}
 __device__ __forceinline__ void pdl_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

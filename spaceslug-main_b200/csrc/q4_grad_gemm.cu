@@ -308,11 +308,13 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_holder;
+    pdl_launch_dependents();
 
     if (warp < 4) {
         if constexpr (!WT) regs_dec<kGgRegsCtl>();
         if (warp == 0 && lane == 0) {
             // ------------------------------------------------ row planes --
+            pdl_wait();
             int it = 0;
             bool ok = true;
             for (int u = pair; u < units && ok; u += npairs) {
@@ -477,11 +479,13 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                     }
                     uint8_t* dst = smem + s * C::kStageBytes + C::kB + out_row;
                     if (TR && st0 + g == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
+                        pdl_wait();
+                        const __half* lora_at = after_wait(static_cast<const __half*>(P.lora_at));
                         const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
 #pragma unroll
                         for (int p = 0; p < PB; ++p) {
                             const uint4* src = reinterpret_cast<const uint4*>(
-                                static_cast<const __half*>(P.lora_at) + static_cast<size_t>(p * 64 + row) * P.ld_at + k0);
+                                lora_at + static_cast<size_t>(p * 64 + row) * P.ld_at + k0);
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
                                 *reinterpret_cast<uint4*>(dst + p * kGgTile + ((i ^ (row & 7)) << 4)) = __ldg(src + i);
@@ -527,6 +531,10 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
         const uint32_t buf_s = base + C::kOutOff + ew * kGgOutBytes;
         const int row_in = quarter * 32 + lane;  // row of this CTA's 128
         const int wexp = *P.w_exp;
+        pdl_wait();
+        const float* coef = after_wait(P.coef);
+        const int* row_exp = after_wait(P.row_exp);
+        const long long* targets = after_wait(P.targets);
         int cq = 0, xq = 0;
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
@@ -540,7 +548,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
             for (int c = w.c0; c < w.c1; ++c, ++cq) {
                 const int b = cq & 1;
-                const float f = P.coef != nullptr ? __ldg(P.coef + static_cast<size_t>(c) * P.ld_stat + row) : 1.0f;
+                const float f = coef != nullptr ? __ldg(coef + static_cast<size_t>(c) * P.ld_stat + row) : 1.0f;
                 if (!gg_wait_warp(acc_full(b), (cq >> 1) & 1u, abort_flag, status, kStatusTimeoutEpilogue)) {
                     ok = false;
                     break;
@@ -560,7 +568,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 if (lane == 0) mbar_arrive_remote(leader_addr(acc_empty(b)));
             }
             if (!ok) break;
-            const int rexp = P.row_exp != nullptr ? (row < P.M ? P.row_exp[row] : 0) : P.fixed_exp;
+            const int rexp = row_exp != nullptr ? (row < P.M ? row_exp[row] : 0) : P.fixed_exp;
             const float scale = exp2i(-(rexp + wexp) / 2) * exp2i(-(rexp + wexp) - (-(rexp + wexp) / 2));
             const int col0 = w.ct * kGgCols + half * 128;
             if constexpr (EPI == kGgLoss || EPI == kGgProb) {
@@ -568,7 +576,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 // columns that exist other than the target's (whose logit the
                 // cast has from an fp32 product), and the sum of 2^(z2 - max).
                 const float s2 = scale * 1.4426950408889634f;
-                const long long tgt = row < P.M ? P.targets[row] : -1;
+                const long long tgt = row < P.M ? targets[row] : -1;
                 const int tcol = tgt >= col0 && tgt < col0 + 128 ? static_cast<int>(tgt) - col0 : -1;
                 float top = -INFINITY;
 #pragma unroll
@@ -734,17 +742,35 @@ int gg_launch(const GradGemmArgs& a, cudaStream_t stream) {
     cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, a));
 }
 
 // ------------------------------------------------------------------ helpers --
+// Every kernel of this file starts under the tail of the one before
+// (programmatic dependent launch) and waits for it before it touches memory
+// that a call writes.
+template <typename... Params, typename... Args>
+int gg_launch_pdl(void (*kern)(Params...), unsigned grid, unsigned threads, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...));
+}
 __device__ __forceinline__ float gg_in(const float* p) { return *p; }
 __device__ __forceinline__ float gg_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void gg_in8(const float* p, float (&v)[8]) {
@@ -780,7 +806,10 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     pdl_launch_dependents();
     pdl_wait();
     const long long m = blockIdx.x;
-    const T* row = static_cast<const T*>(A.x) + m * A.cols;
+    const T* row = after_wait(static_cast<const T*>(A.x)) + m * A.cols;
+    const long long* targets = after_wait(A.targets);
+    const float* gpart = after_wait(A.gpart);
+    const int* gexp = after_wait(A.gexp);
     const bool vec = A.cols % 8 == 0;
     const int pieces = (A.cols + 7) / 8;
     auto get = [&](int p, float (&v)[8]) {
@@ -792,7 +821,7 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
         }
     };
     float top = 0.0f, dot = 0.0f;
-    const long long tgt = A.targets != nullptr ? A.targets[m] : -1;
+    const long long tgt = targets != nullptr ? targets[m] : -1;
     const bool want_dot = tgt >= 0 && tgt < A.N;
     for (int p = threadIdx.x; p < pieces; p += 256) {
         float v[8];
@@ -812,8 +841,8 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
         float g = 0.0f;
         if (threadIdx.x < A.rank) {
             for (int z = 0; z < A.gsplits; ++z)
-                g += A.gpart[(static_cast<long long>(z) * A.M + m) * A.gpitch + threadIdx.x];
-            g = ldexpf(g * A.gscale, A.gexp[threadIdx.x]);
+                g += gpart[(static_cast<long long>(z) * A.M + m) * A.gpitch + threadIdx.x];
+            g = ldexpf(g * A.gscale, gexp[threadIdx.x]);
         }
         gs[threadIdx.x] = g;
         top = fmaxf(top, fabsf(g));
@@ -830,7 +859,7 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     }
     if (threadIdx.x == 0) A.row_exp[m] = e;
     const float s = exp2i(e);
-    if (A.targets != nullptr) {
+    if (targets != nullptr) {
         for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
         __syncthreads();  // red has been read
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = dot;
@@ -884,11 +913,12 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
 // The dequantised planes [N][K] of a handle's weights, in the dequantised
 // words' order: what the products' dequant warps write to shared memory, once
 // for all row tiles.  Four words per thread, a block apart.
-template <int PB, bool LO8>
+template <bool LO8>
 __global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __restrict__ packed,
                                                             const float* __restrict__ scales,
                                                             const int* __restrict__ w_exp, __half* __restrict__ hi,
-                                                            __half* __restrict__ lo, long long words) {
+                                                            uint2* __restrict__ lo8, long long words) {
+    pdl_launch_dependents();
     const float cs = exp2i(*w_exp);
     const long long i0 = static_cast<long long>(blockIdx.x) * 1024 + threadIdx.x;
     uint32_t q[4];
@@ -899,6 +929,7 @@ __global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __re
         q[u] = i < words ? __ldcs(packed + i) : 0u;
         s[u] = i < words ? __ldg(scales + (i >> 2)) : 0.0f;  // a row has K / 8 words and K / 32 scales
     }
+    pdl_wait();  // the scratch may still be read by the launch before
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const long long i = i0 + u * 256;
@@ -906,13 +937,9 @@ __global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __re
         __half2 s_hi, s_lo;
         split_scale_f16(s[u] * cs, s_hi, s_lo);
         uint4 h, l;
-        gg_dequant<PB, LO8>(q[u], s_hi, s_lo, h, l);
+        gg_dequant<LO8 ? 2 : 1, LO8>(q[u], s_hi, s_lo, h, l);
         reinterpret_cast<uint4*>(hi)[i] = h;
-        if constexpr (LO8) {
-            reinterpret_cast<uint2*>(lo)[i] = make_uint2(l.x, l.y);
-        } else if constexpr (PB == 2) {
-            reinterpret_cast<uint4*>(lo)[i] = l;
-        }
+        if constexpr (LO8) lo8[i] = make_uint2(l.x, l.y);
     }
 }
 
@@ -941,12 +968,17 @@ __global__ void __launch_bounds__(1024) min_exp_kernel(const int* __restrict__ c
 // M2) + 2^(target - M2), the factor 2^(tile max - M2) of every tile in place of
 // its max, lse and loss.  The loss of a likely target is log1p(others /
 // target), which does not cancel.  32 rows x 32 lanes per block.
-__global__ void __launch_bounds__(1024) loss_rows_kernel(float* __restrict__ smax, const float* __restrict__ ssum,
-                                                         const float* __restrict__ zt,
-                                                         const long long* __restrict__ targets,
+__global__ void __launch_bounds__(1024) loss_rows_kernel(float* smax, const float* ssum, const float* zt,
+                                                         const long long* targets,
                                                          float* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ lse, int M, int N, int tiles, long long ld) {
     __shared__ float part[32][33];
+    pdl_launch_dependents();
+    pdl_wait();
+    smax = after_wait(smax);
+    ssum = after_wait(ssum);
+    zt = after_wait(zt);
+    targets = after_wait(targets);
     const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
     const int row = blockIdx.x * 32 + r;
     const bool in = row < M;
@@ -983,13 +1015,18 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(float* __restrict__ sma
 // dx[row][k] = g (sum_z partial[z][row][k] / S + (p_t - 1) w(k, target)), p_t - 1 =
 // expm1(-loss); one block per row.
 template <typename T>
-__global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ partial, int splits, long long out_rows,
-                                                      const float* __restrict__ total,
-                                                      const float* __restrict__ loss,
-                                                      const long long* __restrict__ targets,
-                                                      const float* __restrict__ row_scale,
+__global__ void __launch_bounds__(256) loss_dx_kernel(const float* partial, int splits, long long out_rows,
+                                                      const float* total, const float* loss,
+                                                      const long long* targets, const float* row_scale,
                                                       const uint32_t* __restrict__ packed,
                                                       const float* __restrict__ scales, T* __restrict__ dx, int N, int K) {
+    pdl_launch_dependents();
+    pdl_wait();
+    partial = after_wait(partial);
+    total = after_wait(total);
+    loss = after_wait(loss);
+    targets = after_wait(targets);
+    row_scale = after_wait(row_scale);
     const long long row = blockIdx.x;
     const long long t = targets[row];
     T* out = dx + row * K;
@@ -1038,10 +1075,13 @@ __global__ void __launch_bounds__(256) loss_dx_kernel(const float* __restrict__ 
 // 2^E_j, E_j such that its largest magnitude lies in [2^13, 2^14) (k in the
 // dequantised words' order, zeros past K and past the rank), and the exponent
 // w_exp - E_j that G's column j carries in exchange.
-__global__ void __launch_bounds__(256) lora_at_kernel(const float* __restrict__ a, __half* __restrict__ at,
+__global__ void __launch_bounds__(256) lora_at_kernel(const float* a, __half* __restrict__ at,
                                                       int* __restrict__ gexp, const int* __restrict__ w_exp, int K,
                                                       int rank, int ld, int planes) {
     __shared__ float red[8];
+    pdl_launch_dependents();
+    pdl_wait();  // A may come from an optimizer step, the planes may still be read
+    a = after_wait(a);
     const int j = blockIdx.x;
     float top = 0.0f;
     if (j < rank)
@@ -1067,63 +1107,48 @@ __global__ void __launch_bounds__(256) lora_at_kernel(const float* __restrict__ 
     }
 }
 
-template <typename Kern, typename Arg>
-int gg_launch_pdl(Kern kern, unsigned grid, cudaStream_t stream, const Arg& arg) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, arg));
-}
-
 }  // namespace
 
 int grad_gemm_pairs() { return gg_pairs<true, 1, 1, kGgBf16, false>(); }
 
-namespace {
-template <bool WT>
-int gg_dispatch(const GradGemmArgs& a, int planes, int epi, cudaStream_t stream) {
+int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_planes, cudaStream_t stream) {
+    if (from_planes && planes != 1) return static_cast<int>(cudaErrorInvalidValue);
     switch (epi) {
         case kGgLoss:
-            return planes == 1 ? gg_launch<false, 1, 2, kGgLoss, WT>(a, stream) : gg_launch<false, 2, 2, kGgLoss, WT>(a, stream);
+            return from_planes   ? gg_launch<false, 1, 2, kGgLoss, true>(a, stream)
+                   : planes == 1 ? gg_launch<false, 1, 2, kGgLoss, false>(a, stream)
+                                 : gg_launch<false, 2, 2, kGgLoss, false>(a, stream);
         case kGgProb:
-            return planes == 1 ? gg_launch<false, 1, 2, kGgProb, WT>(a, stream) : gg_launch<false, 2, 2, kGgProb, WT>(a, stream);
+            return from_planes   ? gg_launch<false, 1, 2, kGgProb, true>(a, stream)
+                   : planes == 1 ? gg_launch<false, 1, 2, kGgProb, false>(a, stream)
+                                 : gg_launch<false, 2, 2, kGgProb, false>(a, stream);
         case kGgF32:
-            return planes == 1 ? gg_launch<true, 1, 1, kGgF32, WT>(a, stream) : gg_launch<true, 2, 2, kGgF32, WT>(a, stream);
+            return from_planes   ? gg_launch<true, 1, 1, kGgF32, true>(a, stream)
+                   : planes == 1 ? gg_launch<true, 1, 1, kGgF32, false>(a, stream)
+                                 : gg_launch<true, 2, 2, kGgF32, false>(a, stream);
         case kGgBf16:
-            if (planes == 1) return gg_launch<true, 1, 1, kGgBf16, WT>(a, stream);
+            if (planes != 1) break;
+            return from_planes ? gg_launch<true, 1, 1, kGgBf16, true>(a, stream)
+                               : gg_launch<true, 1, 1, kGgBf16, false>(a, stream);
     }
     return static_cast<int>(cudaErrorInvalidValue);
 }
-}  // namespace
 
-int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_planes, cudaStream_t stream) {
-    return from_planes ? gg_dispatch<true>(a, planes, epi, stream) : gg_dispatch<false>(a, planes, epi, stream);
-}
-
-int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo, bool lo8,
-                         int N, int K, cudaStream_t stream) {
+int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo8, int N, int K,
+                         cudaStream_t stream) {
     const long long words = static_cast<long long>(N) * (K / 8);
     const unsigned blocks = static_cast<unsigned>((words + 1023) / 1024);
-    __half *h = static_cast<__half*>(hi), *l = static_cast<__half*>(lo);
-    if (lo == nullptr)
-        weight_planes_kernel<1, false><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
-    else if (lo8)
-        weight_planes_kernel<2, true><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
-    else
-        weight_planes_kernel<2, false><<<blocks, 256, 0, stream>>>(packed, scales, w_exp, h, l, words);
-    return static_cast<int>(cudaGetLastError());
+    if (lo8 == nullptr)
+        return gg_launch_pdl(weight_planes_kernel<false>, blocks, 256, stream, packed, scales, w_exp, static_cast<__half*>(hi),
+                             static_cast<uint2*>(lo8), words);
+    return gg_launch_pdl(weight_planes_kernel<true>, blocks, 256, stream, packed, scales, w_exp, static_cast<__half*>(hi),
+                         static_cast<uint2*>(lo8), words);
 }
 
 int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream) {
     if (a.M < 1 || a.ld % 8 != 0 || a.ld < a.cols || a.rank > 64) return static_cast<int>(cudaErrorInvalidValue);
-    if (bf16) return gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1>, static_cast<unsigned>(a.M), stream, a);
-    if (planes == 2) return gg_launch_pdl(cast_planes_kernel<float, 2>, static_cast<unsigned>(a.M), stream, a);
+    if (bf16) return gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1>, static_cast<unsigned>(a.M), 256, stream, a);
+    if (planes == 2) return gg_launch_pdl(cast_planes_kernel<float, 2>, static_cast<unsigned>(a.M), 256, stream, a);
     return static_cast<int>(cudaErrorInvalidValue);
 }
 
@@ -1134,26 +1159,23 @@ int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int
 
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
                      float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream) {
-    loss_rows_kernel<<<(M + 31) / 32, 1024, 0, stream>>>(smax, ssum, zt, targets, total, loss, lse, M, N, tiles, ld);
-    return static_cast<int>(cudaGetLastError());
+    return gg_launch_pdl(loss_rows_kernel, static_cast<unsigned>((M + 31) / 32), 1024, stream, smax, ssum, zt, targets,
+                         total, loss, lse, M, N, tiles, ld);
 }
 
 int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,
-                   const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
-                   int N, int K, cudaStream_t stream) {
+                   const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx,
+                   bool bf16, int M, int N, int K, cudaStream_t stream) {
     if (bf16)
-        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, loss, targets, row_scale, packed, scales,
-                                              static_cast<__nv_bfloat16*>(dx), N, K);
-    else
-        loss_dx_kernel<<<M, 256, 0, stream>>>(partial, splits, out_rows, total, loss, targets, row_scale, packed, scales,
-                                              static_cast<float*>(dx), N, K);
-    return static_cast<int>(cudaGetLastError());
+        return gg_launch_pdl(loss_dx_kernel<__nv_bfloat16>, static_cast<unsigned>(M), 256, stream, partial, splits, out_rows,
+                             total, loss, targets, row_scale, packed, scales, static_cast<__nv_bfloat16*>(dx), N, K);
+    return gg_launch_pdl(loss_dx_kernel<float>, static_cast<unsigned>(M), 256, stream, partial, splits, out_rows, total, loss,
+                         targets, row_scale, packed, scales, static_cast<float*>(dx), N, K);
 }
 
 int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K, int rank, int ld, int planes,
                    cudaStream_t stream) {
-    lora_at_kernel<<<64, 256, 0, stream>>>(a, static_cast<__half*>(at), gexp, w_exp, K, rank, ld, planes);
-    return static_cast<int>(cudaGetLastError());
+    return gg_launch_pdl(lora_at_kernel, 64, 256, stream, a, static_cast<__half*>(at), gexp, w_exp, K, rank, ld, planes);
 }
 
 }  // namespace q4

@@ -68,13 +68,16 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) { return _
 // exp(z - max), both without the target's column (log2 units: smax, ssum).
 constexpr int kRowsCols = 32, kRowsChunk = 1024, kRowsBatch = kRowsChunk / 32 / 8;
 template <int MR, typename T>
-__global__ void __launch_bounds__(256, 3) rows_logits_kernel(const T* __restrict__ x, const uint32_t* __restrict__ packed,
-                                                             const float* __restrict__ scales,
-                                                             const long long* __restrict__ targets,
+__global__ void __launch_bounds__(256, 3) rows_logits_kernel(const T* x, const uint32_t* __restrict__ packed,
+                                                             const float* __restrict__ scales, const long long* targets,
                                                              float* __restrict__ z, float* __restrict__ zt,
                                                              float* __restrict__ smax, float* __restrict__ ssum, int N,
                                                              int K) {
     __shared__ __align__(16) float xs[MR * kRowsChunk];
+    pdl_launch_dependents();
+    pdl_wait();
+    x = after_wait(x);
+    targets = after_wait(targets);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int n = blockIdx.x * kRowsCols + lane, groups = K / 32;
     const size_t row_g = static_cast<size_t>(min(n, N - 1)) * groups;
@@ -153,13 +156,18 @@ __global__ void __launch_bounds__(256, 3) rows_logits_kernel(const T* __restrict
 // gradient M2, g / S and g (p_target - 1) (coef[3 row ..]).  A negative target
 // takes the row out of the loss (loss 0, gradient 0); one past the columns
 // gives NaN.
-__global__ void __launch_bounds__(512) rows_loss_kernel(const float* __restrict__ smax, const float* __restrict__ ssum,
-                                                        const float* __restrict__ zt,
-                                                        const long long* __restrict__ targets,
-                                                        const float* __restrict__ row_scale, float* __restrict__ loss,
+__global__ void __launch_bounds__(512) rows_loss_kernel(const float* smax, const float* ssum, const float* zt,
+                                                        const long long* targets, const float* row_scale, float* __restrict__ loss,
                                                         float* __restrict__ lse, float* __restrict__ coef, int N,
                                                         int tiles) {
     __shared__ float red[16];
+    pdl_launch_dependents();
+    pdl_wait();
+    smax = after_wait(smax);
+    ssum = after_wait(ssum);
+    zt = after_wait(zt);
+    targets = after_wait(targets);
+    row_scale = after_wait(row_scale);
     const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* sm = smax + static_cast<size_t>(row) * tiles;
     const float* ss = ssum + static_cast<size_t>(row) * tiles;
@@ -198,13 +206,13 @@ __global__ void __launch_bounds__(512) rows_loss_kernel(const float* __restrict_
 // The words of eight n per thread are in flight while d is staged.
 constexpr int kWtWords = 64, kWtParts = 4, kWtThreads = kWtWords * kWtParts, kWtTile = 128, kWtBatch = 8;
 template <int MR, typename T>
-__global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(const T* __restrict__ d, const float* __restrict__ coef,
-                                                             const long long* __restrict__ targets,
+__global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(const T* d, const float* coef, const long long* targets,
                                                              const uint32_t* __restrict__ packed,
                                                              const float* __restrict__ scales,
                                                              float* __restrict__ partial, int N, int K) {
     __shared__ __align__(16) float ds[kWtTile][MR];
     __shared__ __align__(16) float sums[kWtParts - 1][kWtWords][8];
+    pdl_launch_dependents();
     const int wl = threadIdx.x % kWtWords, part = threadIdx.x / kWtWords;
     const int kw = blockIdx.x * kWtWords + wl, words = K / 8, groups = K / 32;
     const int nb = static_cast<int>(static_cast<long long>(N) * blockIdx.y / gridDim.y);
@@ -230,6 +238,12 @@ __global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(co
             }
         };
         load(part);
+        if (n0 == nb) {
+            pdl_wait();  // d, and the partial sums' memory
+            d = after_wait(d);
+            coef = after_wait(coef);
+            targets = after_wait(targets);
+        }
         __syncthreads();  // the tile before has been read
         for (int i = threadIdx.x; i < MR * kWtTile; i += kWtThreads) {
             const int r = i / kWtTile, j = i % kWtTile;
@@ -293,9 +307,13 @@ __global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(co
 // Four rows x 16 ranks per block and range of n (blockIdx.z): partial[z][M][rank].
 constexpr int kProjRows = 4, kProjRanks = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy, const float* __restrict__ b,
+__global__ void __launch_bounds__(256) rows_proj_kernel(const T* dy, const float* b,
                                                         float* __restrict__ g, int M, int N, int rank) {
     __shared__ float red[8][64];
+    pdl_launch_dependents();
+    pdl_wait();
+    dy = after_wait(dy);
+    b = after_wait(b);
     const int m0 = blockIdx.x * kProjRows, j0 = blockIdx.y * kProjRanks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nb = static_cast<int>(static_cast<long long>(N) * blockIdx.z / gridDim.z);
@@ -334,12 +352,16 @@ __global__ void __launch_bounds__(256) rows_proj_kernel(const T* __restrict__ dy
 // per thread of a pair of warps, each in order; and with an adapter
 // scale * (sum of G's ranges) A^T.
 template <typename T>
-__global__ void __launch_bounds__(256) rows_finish_kernel(const float* __restrict__ partial, int splits,
-                                                          long long split_floats, const float* __restrict__ g,
-                                                          int gsplits, const float* __restrict__ a, int rank,
+__global__ void __launch_bounds__(256) rows_finish_kernel(const float* partial, int splits, long long split_floats,
+                                                          const float* g, int gsplits, const float* a, int rank,
                                                           float scale, T* __restrict__ out, int M, int K) {
     __shared__ float gs[64];
     __shared__ float half[128];
+    pdl_launch_dependents();
+    pdl_wait();
+    partial = after_wait(partial);
+    g = after_wait(g);
+    a = after_wait(a);
     const long long row = blockIdx.y;
     const int c = threadIdx.x & 127, h = threadIdx.x >> 7, k = blockIdx.x * 128 + c;
     if (threadIdx.x < rank) {
@@ -369,6 +391,21 @@ __global__ void __launch_bounds__(256) rows_finish_kernel(const float* __restric
     row_store(out + row * K + k, v);
 }
 
+// Launch under the tail of the kernel before (programmatic dependent launch).
+template <typename... Params, typename... Args>
+int rows_launch(void (*kern)(Params...), dim3 grid, unsigned threads, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...));
+}
+
 // f with the row count as a constant, 1..8.
 template <typename F>
 int rows_dispatch(int M, F&& f) {
@@ -391,24 +428,20 @@ int rows_logits_tiles(int N) { return (N + kRowsCols - 1) / kRowsCols; }
 
 int launch_rows_logits(const void* x, bool bf16, const uint32_t* packed, const float* scales, const long long* targets,
                        float* z, float* zt, float* smax, float* ssum, int M, int N, int K, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(rows_logits_tiles(N));
+    const dim3 grid(static_cast<unsigned>(rows_logits_tiles(N)));
     return rows_dispatch(M, [&](auto mr) {
         constexpr int MR = decltype(mr)::value;
-        if (bf16)
-            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), packed, scales, targets,
-                                                             z, zt, smax, ssum, N, K);
-        else
-            rows_logits_kernel<MR><<<grid, 256, 0, stream>>>(static_cast<const float*>(x), packed, scales, targets, z, zt,
-                                                             smax, ssum, N, K);
-        return static_cast<int>(cudaGetLastError());
+        return bf16 ? rows_launch(rows_logits_kernel<MR, __nv_bfloat16>, grid, 256, stream,
+                                  static_cast<const __nv_bfloat16*>(x), packed, scales, targets, z, zt, smax, ssum, N, K)
+                    : rows_launch(rows_logits_kernel<MR, float>, grid, 256, stream, static_cast<const float*>(x), packed,
+                                  scales, targets, z, zt, smax, ssum, N, K);
     });
 }
 
 int launch_rows_loss(const float* smax, const float* ssum, const float* zt, const long long* targets,
                      const float* row_scale, float* loss, float* lse, float* coef, int M, int N, cudaStream_t stream) {
-    rows_loss_kernel<<<static_cast<unsigned>(M), 512, 0, stream>>>(smax, ssum, zt, targets, row_scale, loss, lse, coef, N,
-                                                                   rows_logits_tiles(N));
-    return static_cast<int>(cudaGetLastError());
+    return rows_launch(rows_loss_kernel, dim3(static_cast<unsigned>(M)), 512, stream, smax, ssum, zt, targets, row_scale,
+                       loss, lse, coef, N, rows_logits_tiles(N));
 }
 
 // Splits of n: about two blocks per SM (one wave), at least 32 n each.
@@ -424,13 +457,10 @@ int launch_rows_wt(const void* d, bool bf16, const float* coef, const long long*
     const dim3 grid(static_cast<unsigned>((K / 8 + kWtWords - 1) / kWtWords), static_cast<unsigned>(splits));
     return rows_dispatch(M, [&](auto mr) {
         constexpr int MR = decltype(mr)::value;
-        if (bf16)
-            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const __nv_bfloat16*>(d), coef, targets, packed,
-                                                                scales, partial, N, K);
-        else
-            rows_wt_kernel<MR><<<grid, kWtThreads, 0, stream>>>(static_cast<const float*>(d), coef, targets, packed, scales,
-                                                                partial, N, K);
-        return static_cast<int>(cudaGetLastError());
+        return bf16 ? rows_launch(rows_wt_kernel<MR, __nv_bfloat16>, grid, kWtThreads, stream,
+                                  static_cast<const __nv_bfloat16*>(d), coef, targets, packed, scales, partial, N, K)
+                    : rows_launch(rows_wt_kernel<MR, float>, grid, kWtThreads, stream, static_cast<const float*>(d), coef,
+                                  targets, packed, scales, partial, N, K);
     });
 }
 
@@ -446,28 +476,25 @@ int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int sp
                      cudaStream_t stream) {
     const dim3 grid(static_cast<unsigned>((M + kProjRows - 1) / kProjRows),
                     static_cast<unsigned>((rank + kProjRanks - 1) / kProjRanks), static_cast<unsigned>(splits));
-    if (bf16)
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(dy), b, g, M, N, rank);
-    else
-        rows_proj_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(dy), b, g, M, N, rank);
-    return static_cast<int>(cudaGetLastError());
+    return bf16 ? rows_launch(rows_proj_kernel<__nv_bfloat16>, grid, 256, stream, static_cast<const __nv_bfloat16*>(dy), b, g,
+                              M, N, rank)
+                : rows_launch(rows_proj_kernel<float>, grid, 256, stream, static_cast<const float*>(dy), b, g, M, N, rank);
 }
 
 int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, int gsplits,
                        const float* a, int rank, float scale, void* out, bool bf16, int M, int K, cudaStream_t stream) {
-    for (int m0 = 0; m0 < M; m0 += 32768) {  // rows are blockIdx.y
+    int rc = 0;
+    for (int m0 = 0; m0 < M && rc == 0; m0 += 32768) {  // rows are blockIdx.y
         const int mc = M - m0 < 32768 ? M - m0 : 32768;
         if (rank > 0 && m0 > 0) return static_cast<int>(cudaErrorInvalidValue);  // an adapter here has few rows
         const dim3 grid(static_cast<unsigned>((K + 127) / 128), static_cast<unsigned>(mc));
-        const float* p = partial + static_cast<long long>(m0) * K;
-        if (bf16)
-            rows_finish_kernel<<<grid, 256, 0, stream>>>(p, splits, split_floats, g, gsplits, a, rank, scale,
-                                                         static_cast<__nv_bfloat16*>(out) + static_cast<long long>(m0) * K, mc, K);
-        else
-            rows_finish_kernel<<<grid, 256, 0, stream>>>(p, splits, split_floats, g, gsplits, a, rank, scale,
-                                                         static_cast<float*>(out) + static_cast<long long>(m0) * K, mc, K);
+        const long long at = static_cast<long long>(m0) * K;
+        rc = bf16 ? rows_launch(rows_finish_kernel<__nv_bfloat16>, grid, 256, stream, partial + at, splits, split_floats, g,
+                                gsplits, a, rank, scale, static_cast<__nv_bfloat16*>(out) + at, mc, K)
+                  : rows_launch(rows_finish_kernel<float>, grid, 256, stream, partial + at, splits, split_floats, g, gsplits,
+                                a, rank, scale, static_cast<float*>(out) + at, mc, K);
     }
-    return static_cast<int>(cudaGetLastError());
+    return rc;
 }
 
 }  // namespace q4

@@ -1292,7 +1292,6 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
 constexpr int kRowsKernelMax = 8;
 constexpr long long kTrainScratch = 512ll << 20;  // bytes of operand planes per block of rows
-constexpr int kPlaneRows = 1024;  // rows from which the weights are dequantised once into planes
 
 // Splits of the contraction of a product of `tiles` 256 x 256 tiles and
 // `chunks` accumulator chunks of `cost` cycles: the least of waves x (chunks
@@ -1321,40 +1320,57 @@ void encode_grad_out(CUtensorMap* map, const void* out, uint64_t rows, int K) {
 }
 
 // The weights of one training call: the handle's words and scales, dequantised
-// by the products themselves, or (many row tiles, whose every one would
-// dequantise them again) planes that one kernel writes into scratch first.
+// by the products themselves, or, where many row tiles would each do that
+// again, planes that one kernel writes into scratch first.  Measured on B200
+// (planes / words): bf16 dX at k = 4096, n = 11008: 113 / 98 us at 1024 rows, 207
+// / 199 at 1536, 192 / 196 at 2048, 363 / 406 at 4096; bf16 loss at k = 4096, n =
+// 32000: 689 / 654, 980 / 961, 1248 / 1291 and 2409 / 2541 us.  fp32 products,
+// three MMAs per weight, are not bound by the dequantisation: 5337 / 5131 us at
+// 4096 rows, words always.
+constexpr int kPlaneRows = 2048;
 struct TrainWeights {
     spaceslug_q4_weights* w;
-    int planes;       // f16 planes of the rows (1: bf16, 2: fp32)
     bool from_planes;
-    Scratch hi, lo;
-    TrainWeights(spaceslug_q4_weights* h, int row_planes, bool logits, int M, cudaStream_t s)
-        : w(h), planes(row_planes), from_planes(M >= kPlaneRows),
-          hi(from_planes ? static_cast<size_t>(h->N) * h->K * 2 : 0, s),
-          lo(!from_planes ? 0 : static_cast<size_t>(h->N) * h->K * (row_planes == 2 ? 2 : logits ? 1 : 0), s) {
-        if (from_planes)
-            check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, hi.p, lo.p, planes == 1, w->N,
-                                                  w->K, s),
-                         "weight planes");
+    Scratch planes;  // hi [N][K] f16, and for the logits 64 lo [N][K] e4m3
+    void* lo8 = nullptr;
+    TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s)
+        : w(h), from_planes(bf16 && M >= kPlaneRows),
+          planes(from_planes ? static_cast<size_t>(h->N) * h->K * (logits ? 3 : 2) : 0, s) {
+        if (!from_planes) return;
+        if (logits) lo8 = static_cast<char*>(planes.p) + static_cast<size_t>(w->N) * w->K * 2;
+        check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, planes.p, lo8, w->N, w->K, s),
+                     "weight planes");
     }
-    // tensor maps of the logits' (or, transposed, the second) product
+    // tensor maps of the logits' or the transposed product
     void encode(q4::GradGemmArgs& g, bool transposed) const {
         const uint64_t K = static_cast<uint64_t>(w->K), N = static_cast<uint64_t>(w->N);
         if (from_planes) {
-            const uint32_t rows = transposed ? 64 : 128;
-            const bool lo8 = planes == 1;
-            encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, hi.p, K, N, K * 2, 64, rows, CU_TENSOR_MAP_SWIZZLE_128B);
-            g.tm_s = g.tm_w;  // not read by a product of one plane of the weights
-            if (lo.p && !(lo8 && transposed))
-                encode_2d(&g.tm_s, lo8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, lo.p, K, N,
-                          lo8 ? K : K * 2, 64, rows, lo8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
-            g.tm_at = g.tm_w;  // read with an adapter only
+            encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes.p, K, N, K * 2, 64, transposed ? 64 : 128,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+            g.tm_s = g.tm_w;  // not read by the transposed product
+            if (!transposed)
+                encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_UINT8, lo8, K, N, K, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
             return;
         }
         const uint64_t G = K / 32, Gp = (G + 3) / 4 * 4;
         const float* scales = w->scales_pad ? w->scales_pad : w->scales;
         encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, w->packed, K / 8, N, K / 2, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
         encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, scales, G, N, Gp * 4, 4, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
+    }
+};
+
+// Pieces of one scratch buffer, each 256-byte aligned: add() every size, then
+// take() them in the same order.
+struct Carve {
+    size_t total = 0, at = 0;
+    char* base = nullptr;
+    static size_t up(size_t b) { return (b + 255) / 256 * 256; }
+    void add(size_t bytes) { total += up(bytes); }
+    template <typename T>
+    T* take(size_t bytes) {
+        T* p = bytes ? reinterpret_cast<T*>(base + at) : nullptr;
+        at += up(bytes);
+        return p;
     }
 };
 
@@ -1391,23 +1407,28 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     // contraction: N padded to whole 64-wide stages, and one more stage for the adapter's G A^T
     const int wstages = (N + 63) / 64;
     const long long ld = 64ll * (wstages + (r > 0 ? 1 : 0)), ld_at = (static_cast<long long>(K) + 255) / 256 * 256;
-    Scratch at(r > 0 ? static_cast<size_t>(planes) * 64 * ld_at * 2 : 0, s);
-    Scratch gexp(r > 0 ? 64 * sizeof(int) : 0, s);
+    const long long np = (static_cast<long long>(N) + 7) / 8 * 8;
     const bool gt = r > 0 && N >= 32 && N % (bf16 ? 8 : 4) == 0;  // G by the tensor-core passes
     const int rp = gt ? (bf16 ? q4::lora16_rp(r) : q4::lora_tc_rp(r)) : r;
-    const long long np = (static_cast<long long>(N) + 7) / 8 * 8;
-    Scratch bp(gt ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0, s);
+    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
+    const size_t b_at = r > 0 ? static_cast<size_t>(planes) * 64 * ld_at * 2 : 0, b_exp = r > 0 ? 64 * sizeof(int) : 0;
+    const size_t b_bp = gt ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0;
+    Carve fixed;
+    for (size_t b : {b_at, b_exp, b_bp}) fixed.add(b);
+    Scratch fixed_mem(fixed.total, s);
+    fixed.base = static_cast<char*>(fixed_mem.p);
+    void* at = fixed.take<void>(b_at);
+    int* gexp = fixed.take<int>(b_exp);
+    void* bp = fixed.take<void>(b_bp);
+    const TrainWeights weights(w, bf16, false, M, s);
     if (r > 0)
-        check_launch(q4::launch_lora_at(w->lora_a, at.p, static_cast<int*>(gexp.p), w->col_exp + N, K, r,
-                                        static_cast<int>(ld_at), planes, s),
+        check_launch(q4::launch_lora_at(w->lora_a, at, gexp, w->col_exp + N, K, r, static_cast<int>(ld_at), planes, s),
                      "A^T planes");
     if (gt) {
-        const q4::Lora16Finish f{w->lora_b, 1, N, N, r, rp, bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32, 1, 1.0f, bp.p,
+        const q4::Lora16Finish f{w->lora_b, 1, N, N, r, rp, bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32, 1, 1.0f, bp,
                                  nullptr, np};
         check_launch(q4::launch_lora16_finish(&f, 1, s), "B planes");
     }
-    const TrainWeights weights(w, planes, false, M, s);
-    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0);
         const void* d = static_cast<const char*>(dy) + static_cast<size_t>(m0) * N * size;
@@ -1423,23 +1444,29 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
                                (planes == 1 ? 512 : 1536) * g.chunk, pairs, static_cast<long long>(mc) * K, false);
         g.out_rows = g.row_tiles * 256;
         g.plane_rows = mc;
-        Scratch x16(static_cast<size_t>(planes) * mc * ld * 2, s);
-        Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
-        Scratch part(g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0, s);
         int gsplits = 1;
         if (gt)
             q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
         else if (r > 0)
             gsplits = q4::rows_proj_splits(mc, N, r, c.sm_count);
-        Scratch gs(r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0, s);
-        float* gpart = static_cast<float*>(gs.p);
+        const size_t b_x = static_cast<size_t>(planes) * mc * ld * 2, b_re = static_cast<size_t>(mc) * sizeof(int);
+        const size_t b_part = g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0;
+        const size_t b_g = r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0;
+        Carve cut;
+        for (size_t b : {b_x, b_re, b_part, b_g}) cut.add(b);
+        Scratch mem(cut.total, s);
+        cut.base = static_cast<char*>(mem.p);
+        void* x16 = cut.take<void>(b_x);
+        int* rexp = cut.take<int>(b_re);
+        float* part = cut.take<float>(b_part);
+        float* gpart = cut.take<float>(b_g);
         if (gt && bf16) {
             q4::Lora16Pass p{};
             p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
             q4::Lora16Problem& q = p.prob[0];
             encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
                       static_cast<uint64_t>(N) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, bp.p, static_cast<uint64_t>(N),
+            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, bp, static_cast<uint64_t>(N),
                       static_cast<uint64_t>(3 * rp), static_cast<uint64_t>(np) * 2, 64, static_cast<uint32_t>(3 * rp),
                       CU_TENSOR_MAP_SWIZZLE_128B);
             q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
@@ -1450,7 +1477,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
             q4::LoraTcProblem& q = p.prob[0];
             encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
                       static_cast<uint64_t>(N) * 4, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, bp.p, static_cast<uint64_t>(N),
+            encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, bp, static_cast<uint64_t>(N),
                       static_cast<uint64_t>(2 * rp), static_cast<uint64_t>(np) * 4, 32, static_cast<uint32_t>(2 * rp),
                       CU_TENSOR_MAP_SWIZZLE_128B);
             q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
@@ -1459,38 +1486,38 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
             check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, gpart, gsplits, mc, N, r, s), "dY B^T");
         }
         q4::CastArgs ca{};
-        ca.x = d; ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
+        ca.x = d; ca.out = x16; ca.row_exp = rexp;
         ca.M = mc; ca.cols = N; ca.ld = ld;
         if (r > 0) {
-            ca.gpart = gpart; ca.gexp = static_cast<int*>(gexp.p);
+            ca.gpart = gpart; ca.gexp = gexp;
             ca.rank = r; ca.gsplits = gsplits; ca.gpitch = rp;
             ca.gscale = w->alpha / static_cast<float>(r);
         }
         check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "dY planes");
-        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(ld),
+        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(ld),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(ld) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         const bool direct16 = bf16 && g.splits == 1;
         if (direct16)
             encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, out, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
                       static_cast<uint64_t>(K) * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
         else
-            encode_grad_out(&g.tm_out, part.p ? part.p : out,
-                            part.p ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc), K);
+            encode_grad_out(&g.tm_out, part ? part : out,
+                            part ? static_cast<uint64_t>(g.splits) * g.out_rows : static_cast<uint64_t>(mc), K);
         weights.encode(g, true);
+        g.tm_at = g.tm_w;  // read with an adapter only
         if (weights.from_planes && r > 0)
-            encode_2d(&g.tm_at, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, at.p, static_cast<uint64_t>(ld_at),
-                      static_cast<uint64_t>(planes) * 64, static_cast<uint64_t>(ld_at) * 2, 64, 64,
-                      CU_TENSOR_MAP_SWIZZLE_128B);
+            encode_2d(&g.tm_at, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, at, static_cast<uint64_t>(ld_at), 64,
+                      static_cast<uint64_t>(ld_at) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
         g.w_exp = w->col_exp + N;
-        g.row_exp = static_cast<int*>(rexp.p);
-        g.lora_at = at.p;
+        g.row_exp = rexp;
+        g.lora_at = at;
         g.ld_at = static_cast<int>(ld_at);
         g.lora_stage = r > 0 ? wstages : -1;
         g.status = c.status;
         check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, weights.from_planes, s), "dY W^T");
         if (g.splits > 1)
-            check_launch(q4::launch_rows_finish(static_cast<float*>(part.p), g.splits, static_cast<long long>(g.out_rows) * K,
-                                                nullptr, 0, nullptr, 0, 0.0f, out, bf16, mc, K, s),
+            check_launch(q4::launch_rows_finish(part, g.splits, static_cast<long long>(g.out_rows) * K, nullptr, 0, nullptr,
+                                                0, 0.0f, out, bf16, mc, K, s),
                          "dX");
     }
 }
@@ -1535,24 +1562,35 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     const long long ld_p = static_cast<long long>(tiles) * 256;
     const long long row_bytes = 2ll * planes * (dx ? ld_p : K);
     const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20));
-    const TrainWeights weights(w, planes, true, M, s);
+    const TrainWeights weights(w, bf16, true, M, s);
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
-        Scratch x16(static_cast<size_t>(planes) * mc * K * 2, s);
-        Scratch x8(bf16 ? static_cast<size_t>(mc) * K : 0, s);
-        Scratch rexp(static_cast<size_t>(mc) * sizeof(int), s);
-        Scratch stat((static_cast<size_t>(3) * tiles + 2) * mp * 4, s);
-        Scratch prob(dx ? static_cast<size_t>(planes) * mp * ld_p * 2 : 0, s);
-        float* smax = static_cast<float*>(stat.p);
-        float* ssum = smax + static_cast<size_t>(tiles) * mp;
-        float* zt = ssum + static_cast<size_t>(2) * tiles * mp;
-        float* total = zt + mp;
+        const size_t b_x = static_cast<size_t>(planes) * mc * K * 2, b_x8 = bf16 ? static_cast<size_t>(mc) * K : 0;
+        const size_t b_re = static_cast<size_t>(mc) * sizeof(int), b_t = static_cast<size_t>(tiles) * mp * 4;
+        const size_t b_row = static_cast<size_t>(mp) * 4, b_prob = dx ? static_cast<size_t>(planes) * mp * ld_p * 2 : 0;
+        const int splits = dx ? grad_splits(static_cast<long long>(mp / 256) * ((K + 255) / 256), tiles,
+                                            (planes == 1 ? 512 : 1536) * 4, pairs, static_cast<long long>(mp) * K, true)
+                              : 0;
+        const size_t b_part = static_cast<size_t>(splits) * mp * K * 4;
+        Carve cut;
+        for (size_t b : {b_x, b_x8, b_re, b_t, 2 * b_t, b_row, b_row, b_prob, b_part}) cut.add(b);
+        Scratch mem(cut.total, s);
+        cut.base = static_cast<char*>(mem.p);
+        void* x16 = cut.take<void>(b_x);
+        void* x8 = cut.take<void>(b_x8);
+        int* rexp = cut.take<int>(b_re);
+        float* smax = cut.take<float>(b_t);
+        float* ssum = cut.take<float>(2 * b_t);
+        float* zt = cut.take<float>(b_row);
+        float* total = cut.take<float>(b_row);
+        void* prob = cut.take<void>(b_prob);
+        float* part = cut.take<float>(b_part);
         q4::CastArgs ca{};
         ca.x = static_cast<const char*>(x) + static_cast<size_t>(m0) * K * size;
-        ca.out = x16.p; ca.row_exp = static_cast<int*>(rexp.p);
+        ca.out = x16; ca.row_exp = rexp;
         ca.M = mc; ca.cols = K; ca.ld = K;
         ca.by_word = 1;
-        ca.out8 = x8.p;
+        ca.out8 = x8;
         ca.targets = targets + m0; ca.packed = w->packed; ca.scales = w->scales; ca.zt = zt; ca.N = N;
         check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "X planes");
         q4::GradGemmArgs g{};
@@ -1566,21 +1604,22 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.plane_rows = mc;
         g.out_rows = mp;
         weights.encode(g, false);
+        g.tm_at = g.tm_w;  // not read
         g.w_exp = w->col_exp + N;
-        g.row_exp = static_cast<int*>(rexp.p);
+        g.row_exp = rexp;
         g.targets = targets + m0;
         g.smax = smax; g.ssum = ssum;
         g.ld_stat = mp;
         g.lora_stage = -1;
         g.status = c.status;
-        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16.p, static_cast<uint64_t>(K),
+        encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(K),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
         g.tm_a8 = g.tm_a;  // not read without an e4m3 copy
         if (bf16)
-            encode_2d(&g.tm_a8, CU_TENSOR_MAP_DATA_TYPE_UINT8, x8.p, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
+            encode_2d(&g.tm_a8, CU_TENSOR_MAP_DATA_TYPE_UINT8, x8, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
                       static_cast<uint64_t>(K), 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
         if (dx)
-            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
+            encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob, static_cast<uint64_t>(ld_p),
                       static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 32,
                       CU_TENSOR_MAP_SWIZZLE_128B);
         else
@@ -1595,19 +1634,17 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         d.stages = tiles * 4;
         d.chunk = 4;  // one 256-column tile of the logits: one factor per row
         d.chunks = tiles;
-        d.splits = grad_splits(static_cast<long long>(d.row_tiles) * d.col_tiles, tiles, (planes == 1 ? 512 : 1536) * 4,
-                               pairs, static_cast<long long>(mp) * K, true);
+        d.splits = splits;
         d.plane_rows = mp;
         d.row_exp = nullptr;
         d.fixed_exp = 14;  // p~ carries 2^14
         d.coef = smax;
-        Scratch part(static_cast<size_t>(d.splits) * mp * K * 4, s);
-        encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob.p, static_cast<uint64_t>(ld_p),
+        encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob, static_cast<uint64_t>(ld_p),
                   static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-        encode_grad_out(&d.tm_out, part.p, static_cast<uint64_t>(d.splits) * mp, K);
+        encode_grad_out(&d.tm_out, part, static_cast<uint64_t>(d.splits) * mp, K);
         weights.encode(d, true);
         check_launch(q4::launch_grad_gemm(d, planes, q4::kGgF32, weights.from_planes, s), "P W^T");
-        check_launch(q4::launch_loss_dx(static_cast<float*>(part.p), d.splits, mp, total, loss + m0, targets + m0,
+        check_launch(q4::launch_loss_dx(part, d.splits, mp, total, loss + m0, targets + m0,
                                         row_scale ? row_scale + m0 : nullptr, w->packed, w->scales,
                                         static_cast<char*>(dx) + static_cast<size_t>(m0) * K * size, bf16, mc, N, K, s),
                      "dX");
