@@ -308,7 +308,6 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_holder;
-    pdl_launch_dependents();
 
     if (warp < 4) {
         if constexpr (!WT) regs_dec<kGgRegsCtl>();
@@ -532,9 +531,6 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
         const int row_in = quarter * 32 + lane;  // row of this CTA's 128
         const int wexp = *P.w_exp;
         pdl_wait();
-        const float* coef = after_wait(P.coef);
-        const int* row_exp = after_wait(P.row_exp);
-        const long long* targets = after_wait(P.targets);
         int cq = 0, xq = 0;
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
@@ -548,7 +544,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 for (int j = 0; j < 32; ++j) acc[i][j] = 0.0f;
             for (int c = w.c0; c < w.c1; ++c, ++cq) {
                 const int b = cq & 1;
-                const float f = coef != nullptr ? __ldg(coef + static_cast<size_t>(c) * P.ld_stat + row) : 1.0f;
+                const float f = P.coef != nullptr ? after_wait(P.coef)[static_cast<size_t>(c) * P.ld_stat + row] : 1.0f;
                 if (!gg_wait_warp(acc_full(b), (cq >> 1) & 1u, abort_flag, status, kStatusTimeoutEpilogue)) {
                     ok = false;
                     break;
@@ -568,7 +564,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 if (lane == 0) mbar_arrive_remote(leader_addr(acc_empty(b)));
             }
             if (!ok) break;
-            const int rexp = row_exp != nullptr ? (row < P.M ? row_exp[row] : 0) : P.fixed_exp;
+            const int rexp = P.row_exp != nullptr ? (row < P.M ? after_wait(P.row_exp)[row] : 0) : P.fixed_exp;
             const float scale = exp2i(-(rexp + wexp) / 2) * exp2i(-(rexp + wexp) - (-(rexp + wexp) / 2));
             const int col0 = w.ct * kGgCols + half * 128;
             if constexpr (EPI == kGgLoss || EPI == kGgProb) {
@@ -576,7 +572,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                 // columns that exist other than the target's (whose logit the
                 // cast has from an fp32 product), and the sum of 2^(z2 - max).
                 const float s2 = scale * 1.4426950408889634f;
-                const long long tgt = row < P.M ? targets[row] : -1;
+                const long long tgt = row < P.M ? after_wait(P.targets)[row] : -1;
                 const int tcol = tgt >= col0 && tgt < col0 + 128 ? static_cast<int>(tgt) - col0 : -1;
                 float top = -INFINITY;
 #pragma unroll
@@ -690,6 +686,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
         if (lane == 0) bulk_wait_group_all();
     }
 
+    pdl_launch_dependents();  // here: blocks of the next launch that wait beside this one's cost it 3%
     tc_fence_before_sync();
     __syncwarp();
     cluster_sync_all();  // no CTA leaves while its peer may still use its shared memory or tensor memory
