@@ -87,17 +87,20 @@ struct GgCfg {
     static constexpr int kB = kA8 + (kLo8 ? kGgTile / 2 : 0);      // w hi
     static constexpr int kBLo = kB + kGgTile;                      // w lo (f16, or 128 x 64 bytes of fp8)
     static constexpr int kStageBytes = kLo8 ? kBLo + kGgTile / 2 : (PA + PB) * kGgTile;
-    static constexpr int kStages = PA + PB == 2 ? 5 : PA + PB == 3 ? 3 : 2;
+    static constexpr int kStages = PA + PB == 2 ? (WT ? 6 : 5) : PA + PB == 3 ? (WT ? 4 : 3) : 2;
     static constexpr int kOutOff = kStages * kStageBytes;
     static constexpr int kRawOff = kOutOff + kGgEpiWarps * kGgOutBytes;
-    static constexpr int kXchOff = kRawOff + kGgRaw * kGgRawBytes;  // [2 buffers][2 halves][128 rows] floats
+    static constexpr int kXchOff = kRawOff + (WT ? 0 : kGgRaw * kGgRawBytes);  // [2 buffers][2 halves][128 rows] floats
     static constexpr int kBarOff = kXchOff + 2 * 2 * 128 * 4;
     // full_x[S], full_w[S] (leader), empty[S] (both), acc_full[2] (both), acc_empty[2] (leader), done (leader),
     // xch[4], full_r[R], empty_r[R] (own)
     static constexpr int kNumBars = 3 * kStages + 9 + 2 * kGgRaw;
     static constexpr int kMiscOff = kBarOff + kNumBars * 8;
     static constexpr int kBytes = kMiscOff + 16;
-    static constexpr int kSmem = kBytes + 1024;
+    // Dynamic shared memory starts 1024-aligned; with no room for slack a
+    // window that does not is reported and nothing is loaded.
+    static constexpr int kSlack = WT ? 0 : 1024;
+    static constexpr int kSmem = kBytes + kSlack;
     static_assert(kSmem <= 232448, "shared memory budget");
 };
 
@@ -252,9 +255,13 @@ template <bool TR, int PA, int PB, int EPI, bool WT>
 __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __grid_constant__ GradGemmArgs P) {
     using C = GgCfg<PA, PB, WT>;
     constexpr int ST = C::kStages;
-    extern __shared__ uint8_t smem_raw[];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t raw_base = smem_u32(smem_raw);
     const uint32_t base = (raw_base + 1023u) & ~1023u;
+    if (base - raw_base > static_cast<uint32_t>(C::kSlack)) {  // the same in every CTA
+        if (threadIdx.x == 0 && P.status) atomicCAS(P.status, 0, kStatusBadLaunch);
+        return;
+    }
     uint8_t* smem = smem_raw + (base - raw_base);
     const uint32_t bar = base + C::kBarOff;
     auto full_x = [&](int s) { return bar + 8u * s; };
