@@ -54,7 +54,9 @@ struct L16Cfg {
     static constexpr int kTmemStages = (512 - kACol) / 32;
     static constexpr int kSmemStages = 200 * 1024 / kStageBytes;
     static constexpr int kStages0 = kSmemStages < kTmemStages ? kSmemStages : kTmemStages;
-    static constexpr int kStages = kStages0 > 8 ? 8 : kStages0;
+    // even: a slot then belongs to one group of split warps and one MMA warp,
+    // which see each of its phases (a parity only tells two successive ones apart)
+    static constexpr int kStages = (kStages0 > 8 ? 8 : kStages0) / 2 * 2;
     static_assert(kStages > 2, "the epilogue waits on the stages' commits: it must not fall a phase behind");
     static constexpr int kStepOff = kStages * kStageBytes;      // 8 split warps x 64 steps
     static constexpr int kBarOff = kStepOff + 8 * 64 * 4;

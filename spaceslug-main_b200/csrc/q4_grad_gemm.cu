@@ -446,21 +446,24 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
         __syncwarp();
     } else if (!WT && warp < C::kEpiWarp0) {
         // ------------------------------------------------------- dequant --
-        // Warpgroup g dequantises stage g of each raw block, which holds two: the
-        // k halves (logits) or the n halves (transposed).  Its thread t: logits,
-        // column n = t of this CTA's 128 and the stage's 64 k; transposed, n = t
-        // % 64 of the stage's 64 and the 64 k t / 64 of this CTA's 128: either
-        // way two scale groups of one n.
+        // A raw block holds two stages: the k halves (logits) or the n halves
+        // (transposed).  The two warpgroups take the stages of the whole
+        // sequence in turn, so each waits for every second stage's slot, at most
+        // kStages after the one before: a parity then cannot mistake the phase
+        // before the last for the one waited for (as it could if a warpgroup
+        // always took the same half and skipped the odd stage at a unit's end).
+        // Thread t of a warpgroup: logits, column n = t of this CTA's 128 and
+        // the stage's 64 k; transposed, n = t % 64 of the stage's 64 and the 64
+        // k t / 64 of this CTA's 128: either way two scale groups of one n.
         if constexpr (!WT) regs_dec<kGgRegsDeq>();
-        const int g = (warp - kGgDeqWarp0) >> 2, t = (tid - kGgDeqWarp0 * 32) & 127;
+        const int wg = (warp - kGgDeqWarp0) >> 2, t = (tid - kGgDeqWarp0 * 32) & 127;
         const float cs = exp2i(*P.w_exp);
-        const int row = TR ? (t & 63) : t;  // row of the operand image
+        const int row = TR ? (t & 63) : t;  // row of the operand image, and of the block's first half
         const uint32_t out_row = static_cast<uint32_t>((TR ? (t >> 6) * (kGgTile / 2) : 0) + row * 128);
-        const int rn = TR ? g * 64 + row : row, rh = TR ? t >> 6 : g;  // row and 64-k half of the raw block
-        const int rkey = (rn >> 1) & 3;
-        const uint32_t at0 = static_cast<uint32_t>(rn * 64 + (((2 * rh) ^ rkey) << 4));
-        const uint32_t at1 = static_cast<uint32_t>(rn * 64 + (((2 * rh + 1) ^ rkey) << 4));
-        const uint32_t ats = static_cast<uint32_t>(kGgRawWords + rn * 16 + rh * 8);
+        const int rh = TR ? t >> 6 : 0, rkey = (row >> 1) & 3;  // 64-k half of the block's first half
+        const uint32_t at0 = static_cast<uint32_t>(row * 64 + (((2 * rh) ^ rkey) << 4));
+        const uint32_t at1 = static_cast<uint32_t>(row * 64 + (((2 * rh + 1) ^ rkey) << 4));
+        const uint32_t ats = static_cast<uint32_t>(kGgRawWords + row * 16 + rh * 8);
         int it = 0, sq = 0;  // raw block and stage counters
         bool ok = true;
         for (int u = pair; u < units && ok; u += npairs) {
@@ -473,18 +476,22 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                     break;
                 }
                 const uint8_t* raw = smem + C::kRawOff + r * kGgRawBytes;
-                const uint4 q[2] = {*reinterpret_cast<const uint4*>(raw + at0), *reinterpret_cast<const uint4*>(raw + at1)};
-                const float2 sc = *reinterpret_cast<const float2*>(raw + ats);
+                const int j = (sq ^ wg) & 1;  // this warpgroup's half
+                // second half: 64 rows on (transposed), or the other 32 bytes of the row
+                const uint32_t add = TR ? j * 64 * 64 : 0, flip = TR ? 0 : j * 32;
+                const uint4 q[2] = {*reinterpret_cast<const uint4*>(raw + (at0 ^ flip) + add),
+                                    *reinterpret_cast<const uint4*>(raw + (at1 ^ flip) + add)};
+                const float2 sc = *reinterpret_cast<const float2*>(raw + ats + (TR ? j * 64 * 16 : j * 8));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty_r(r));
-                if (g < n) {
-                    const int s = (sq + g) % ST;
-                    if (!gg_wait_warp(empty(s), (((sq + g) / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
+                if (j < n) {
+                    const int s = (sq + j) % ST;
+                    if (!gg_wait_warp(empty(s), (((sq + j) / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
                         ok = false;
                         break;
                     }
                     uint8_t* dst = smem + s * C::kStageBytes + C::kB + out_row;
-                    if (TR && st0 + g == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
+                    if (TR && st0 + j == P.lora_stage) {  // A^T: row = rank, 64 k of this half, planes as prepared
                         pdl_wait();
                         const __half* lora_at = after_wait(static_cast<const __half*>(P.lora_at));
                         const int k0 = w.ct * kGgCols + static_cast<int>(crank) * kGgHalf + (t >> 6) * 64;
@@ -498,21 +505,21 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
+                        for (int h = 0; h < 2; ++h) {
                             __half2 s_hi, s_lo;
-                            split_scale_f16((j == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
-                            const uint32_t words[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+                            split_scale_f16((h == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
+                            const uint32_t words[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
 #pragma unroll
                             for (int i = 0; i < 4; i += 2) {
                                 uint4 hi0, hi1, lo0, lo1;
                                 gg_dequant<PB, C::kLo8>(words[i], s_hi, s_lo, hi0, lo0);
                                 gg_dequant<PB, C::kLo8>(words[i + 1], s_hi, s_lo, hi1, lo1);
-                                const int o0 = ((4 * j + i) ^ (row & 7)) << 4, o1 = ((4 * j + i + 1) ^ (row & 7)) << 4;
+                                const int o0 = ((4 * h + i) ^ (row & 7)) << 4, o1 = ((4 * h + i + 1) ^ (row & 7)) << 4;
                                 *reinterpret_cast<uint4*>(dst + o0) = hi0;
                                 *reinterpret_cast<uint4*>(dst + o1) = hi1;
                                 if constexpr (C::kLo8) {  // 64-byte rows: a 16-byte piece holds two words
                                     *reinterpret_cast<uint4*>(smem + s * C::kStageBytes + C::kBLo + row * 64 +
-                                                              (((2 * j + i / 2) ^ ((row >> 1) & 3)) << 4)) =
+                                                              (((2 * h + i / 2) ^ ((row >> 1) & 3)) << 4)) =
                                         make_uint4(lo0.x, lo0.y, lo1.x, lo1.y);
                                 } else if constexpr (PB == 2) {
                                     *reinterpret_cast<uint4*>(dst + kGgTile + o0) = lo0;

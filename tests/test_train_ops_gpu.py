@@ -118,7 +118,8 @@ def test_act8_edges(session, cuda):
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("m,k,n,rank,c0,c1", [
     (1, 64, 256, 4, 0, 256), (33, 512, 700, 5, 100, 600), (128, 256, 160, 8, 0, 160), (300, 1024, 704, 64, 0, 704),
-    (257, 2080, 1001, 33, 0, 1001), (515, 4096, 640, 16, 32, 616), (128, 32, 32, 1, 0, 32)])
+    (257, 2080, 1001, 33, 0, 1001), (515, 4096, 640, 16, 32, 616), (128, 32, 32, 1, 0, 32),
+    (1500, 1056, 2048, 32, 0, 2048)])
 def test_backward_from_8_bits(session, cuda, m, k, n, rank, c0, c1, dtype):
     import torch
     packed, scales = _weights(k, n, 3)
@@ -193,7 +194,9 @@ def _check_dx(got, dtype, ref, S):
 @pytest.mark.parametrize("m,k,n,rank,c0,c1", [
     (1, 32, 1, 0, 0, 1), (1, 4096, 4096, 16, 0, 4096), (3, 96, 33, 2, 0, 33), (8, 1024, 257, 64, 0, 257),
     (9, 64, 256, 0, 0, 256), (128, 512, 700, 5, 100, 600), (257, 2080, 1001, 33, 0, 1001), (300, 1056, 64, 0, 0, 64),
-    (515, 4128, 4099, 8, 0, 4099), (1100, 288, 515, 6, 0, 515), (2048, 512, 640, 0, 64, 640), (1057, 96, 65, 64, 0, 65)])
+    (515, 4128, 4099, 8, 0, 4099), (1100, 288, 515, 6, 0, 515), (2048, 512, 640, 0, 64, 640), (1057, 96, 65, 64, 0, 65),
+    # an odd number of 64-wide stages and several tiles per CTA pair; an adapter on weights taken from planes
+    (2000, 4096, 130, 0, 0, 130), (2050, 2592, 264, 20, 0, 264)])
 def test_input_gradient(session, cuda, m, k, n, rank, c0, c1, dtype):
     import torch
     packed, scales = _weights(k, n, 7)
@@ -280,7 +283,7 @@ def _check_loss(dtype, got, ref):
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("m,k,n", [(1, 32, 1), (1, 1024, 32003), (5, 64, 259), (8, 2080, 1000), (9, 96, 257),
                                    (130, 512, 512), (257, 1056, 2049), (300, 256, 33000), (1030, 160, 777),
-                                   (1025, 32, 5), (2100, 512, 3001)])
+                                   (1025, 32, 5), (2100, 512, 3001), (300, 160, 40000)])
 def test_cross_entropy(session, cuda, m, k, n, dtype):
     import torch
     packed, scales = _weights(k, n, 13)
