@@ -146,19 +146,7 @@ __global__ void __launch_bounds__(kActThreads) act8_unpack_kernel(const int8_t* 
     }
 }
 
-__global__ void __launch_bounds__(256) bf16_to_f32_kernel(const __nv_bfloat16* __restrict__ x, float* __restrict__ y,
-                                                          long long count) {
-    const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (i < count) y[i] = __bfloat162float(x[i]);
-}
-
 }  // namespace
-
-int launch_bf16_to_f32(const void* x, float* y, long long count, cudaStream_t stream) {
-    bf16_to_f32_kernel<<<static_cast<unsigned>((count + 255) / 256), 256, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(x), y, count);
-    return static_cast<int>(cudaGetLastError());
-}
 
 namespace {
 unsigned act8_blocks(long long pieces) {

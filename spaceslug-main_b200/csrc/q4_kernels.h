@@ -306,7 +306,6 @@ int launch_lora_delta64(const float* x, const float* a, const float* b, float* y
 int launch_act8_pack(const void* x, bool bf16, int8_t* codes, uint8_t* exps, long long groups, cudaStream_t stream);
 int launch_act8_unpack(const int8_t* codes, const uint8_t* exps, void* x, bool bf16, long long groups,
                        cudaStream_t stream);
-int launch_bf16_to_f32(const void* x, float* y, long long count, cudaStream_t stream);
 // The training operators for 1 <= M <= 8 rows (q4_rows.cu); x, dy and out are fp32 or bf16, 16-byte aligned.
 int rows_logits_tiles(int N);  // blocks of columns with one max and sum each
 // logits z [M][N], the target's zt [M], smax and ssum [M][tiles] (log2 units, without the target)

@@ -1160,26 +1160,11 @@ const char* rows_error(const void* in, const void* out, int dtype, uint32_t m) {
     return nullptr;
 }
 
-// The adapter's gradients of fp32 X and dY into the handle.
-void lora_backward_f32(spaceslug_q4_weights* w, const float* x, const float* dy, int M, cudaStream_t s) {
-    q4::LoraBackwardArgs g{x, dy, w->lora_a, w->lora_b, w->lora_da, w->lora_db, nullptr,
-                           M, w->K, w->N, w->rank, w->alpha / static_cast<float>(w->rank)};
-    if (lora_backward_tc_suits(g)) {
-        DeviceCtx& c = ctx_for(w->device);
-        run_lora_backward_tc(g, c.sm_count, c.status, s);
-    } else {
-        Scratch sc(q4::lora_backward_scratch_floats(M, w->K, w->N, w->rank) * 4, s);
-        g.scratch = static_cast<float*>(sc.p);
-        check_launch(q4::launch_lora_backward(g, s), "lora backward");
-    }
-}
-
 // The adapter's gradients with X in 8 bits, into the handle (and to da, db):
-// all four products in bf16 passes (lora16.cu) when dY is bf16 too, with rows
-// of 16 bytes; for fp32 dY the two products of X there and the two of dY in
-// the TF32 passes of lora_tc.cu.
-bool lora_backward_act8_suits(int K, int N, bool bf16) { return K >= 32 && N >= 32 && N % (bf16 ? 8 : 4) == 0; }
-
+// all four products in bf16 passes (lora16.cu) when dY is bf16 too; for fp32 dY
+// the two products of X there and the two of dY in the TF32 passes of
+// lora_tc.cu.  TMA wants rows of dY whose length is a multiple of 16 bytes:
+// others are copied once into such rows.
 void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps, const void* dy, bool bf16,
                             int M, float* da, float* db, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
@@ -1187,6 +1172,15 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     const float scale = w->alpha / static_cast<float>(r);
     auto round8 = [](int v) { return (static_cast<long long>(v) + 7) / 8 * 8; };
     const long long Kp = round8(K), Np = round8(N), Mp = round8(M);
+    const size_t size = bf16 ? 2 : 4;
+    const bool copy = N * size % 16 != 0;
+    const size_t ld_y = (copy ? static_cast<size_t>(Np) : static_cast<size_t>(N)) * size;
+    Scratch rows(copy ? ld_y * M : 0, s);
+    if (copy) {
+        check(cudaMemcpy2DAsync(rows.p, ld_y, dy, N * size, N * size, static_cast<size_t>(M), cudaMemcpyDeviceToDevice, s),
+              "cudaMemcpy2DAsync (dY rows)");
+        dy = rows.p;
+    }
     const int R1[2] = {M, M}, L1[2] = {K, N}, R2[2] = {K, N}, L2[2] = {M, M};
     int s1[2], s2[2];  // splits of {T, G} and {dA, dB}
     const int st = q4::lora16_stage();
@@ -1234,7 +1228,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     };
     auto y16_problem = [&](q4::Lora16Problem& q, bool mn, const void* plane, int splits, float* partial) {
         q = {};
-        encode_2d(&q.tm_a, B16, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(N) * 2,
+        encode_2d(&q.tm_a, B16, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), ld_y,
                   mn ? 128 : 64, mn ? 64 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
         planes16(q, plane, mn ? M : N);
         q.partial = partial;
@@ -1250,7 +1244,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
         p.status = c.status;
         p.mn_major = mn ? 1 : 0;
         q4::LoraTcProblem& q = p.prob[0];
-        encode_2d(&q.tm_a, F32, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), static_cast<uint64_t>(N) * 4,
+        encode_2d(&q.tm_a, F32, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), ld_y,
                   mn ? 128 : 32, mn ? 32 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
         const int L = mn ? M : N;
         encode_2d(&q.tm_b, F32, plane, static_cast<uint64_t>(L), static_cast<uint64_t>(2 * rt), round8(L) * 4, 32,
@@ -2313,7 +2307,16 @@ int spaceslug_q4_weights_lora_backward(spaceslug_q4_weights* w, const float* x, 
         const size_t pa = static_cast<size_t>(w->K) * w->rank * 4, pbb = static_cast<size_t>(w->rank) * w->N * 4;
         if (!w->lora_da) check(cudaMalloc(&w->lora_da, pa), "cudaMalloc dA");
         if (!w->lora_db) check(cudaMalloc(&w->lora_db, pbb), "cudaMalloc dB");
-        lora_backward_f32(w, x, dy, static_cast<int>(m), s);
+        q4::LoraBackwardArgs g{x, dy, w->lora_a, w->lora_b, w->lora_da, w->lora_db, nullptr,
+                               static_cast<int>(m), w->K, w->N, w->rank, w->alpha / static_cast<float>(w->rank)};
+        if (lora_backward_tc_suits(g)) {
+            DeviceCtx& c = ctx_for(w->device);
+            run_lora_backward_tc(g, c.sm_count, c.status, s);
+        } else {
+            Scratch sc(q4::lora_backward_scratch_floats(static_cast<int>(m), w->K, w->N, w->rank) * 4, s);
+            g.scratch = static_cast<float*>(sc.p);
+            check_launch(q4::launch_lora_backward(g, s), "lora backward");
+        }
         return SPACESLUG_OK;
     });
 }
@@ -2354,23 +2357,7 @@ int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_
         const size_t pa = static_cast<size_t>(w->K) * w->rank * 4, pbb = static_cast<size_t>(w->rank) * w->N * 4;
         if (!w->lora_da) check(cudaMalloc(&w->lora_da, pa), "cudaMalloc dA");
         if (!w->lora_db) check(cudaMalloc(&w->lora_db, pbb), "cudaMalloc dB");
-        const int M = static_cast<int>(m);
-        if (lora_backward_act8_suits(w->K, w->N, dtype == SPACESLUG_BF16)) {
-            run_lora_backward_act8(w, codes, exps, dy, dtype == SPACESLUG_BF16, M, da, db, s);
-            return SPACESLUG_OK;
-        }
-        // rows of dY that no 16-byte copy can follow: X (and a bf16 dY) restored in fp32, then the fp32 backward
-        Scratch xs(static_cast<size_t>(M) * w->K * 4, s);
-        Scratch ys(dtype == SPACESLUG_BF16 ? static_cast<size_t>(M) * w->N * 4 : 0, s);
-        check_launch(q4::launch_act8_unpack(codes, exps, xs.p, false, static_cast<long long>(M) * (w->K / 32), s),
-                     "act8 unpack");
-        if (ys.p)
-            check_launch(q4::launch_bf16_to_f32(dy, static_cast<float*>(ys.p), static_cast<long long>(M) * w->N, s),
-                         "bf16 to f32");
-        lora_backward_f32(w, static_cast<const float*>(xs.p), ys.p ? static_cast<const float*>(ys.p)
-                                                                    : static_cast<const float*>(dy), M, s);
-        if (da) check(cudaMemcpyAsync(da, w->lora_da, pa, cudaMemcpyDeviceToDevice, s), "copy dA");
-        if (db) check(cudaMemcpyAsync(db, w->lora_db, pbb, cudaMemcpyDeviceToDevice, s), "copy dB");
+        run_lora_backward_act8(w, codes, exps, dy, dtype == SPACESLUG_BF16, static_cast<int>(m), da, db, s);
         return SPACESLUG_OK;
     });
 }

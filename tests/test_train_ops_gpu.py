@@ -119,7 +119,7 @@ def test_act8_edges(session, cuda):
 @pytest.mark.parametrize("m,k,n,rank,c0,c1", [
     (1, 64, 256, 4, 0, 256), (33, 512, 700, 5, 100, 600), (128, 256, 160, 8, 0, 160), (300, 1024, 704, 64, 0, 704),
     (257, 2080, 1001, 33, 0, 1001), (515, 4096, 640, 16, 32, 616), (128, 32, 32, 1, 0, 32),
-    (1500, 1056, 2048, 32, 0, 2048)])
+    (1500, 1056, 2048, 32, 0, 2048), (30, 1248, 23, 1, 0, 23), (130, 3520, 1, 17, 0, 1), (77, 96, 1003, 3, 500, 513)])
 def test_backward_from_8_bits(session, cuda, m, k, n, rank, c0, c1, dtype):
     import torch
     packed, scales = _weights(k, n, 3)
