@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256) lora_xa_kernel(const float* __restrict__ 
         for (int j = 0; j < kXaCols; ++j) acc[r][j] = 0.0f;
     const int g = tid >> 4, q = tid & 15;
     for (int kb = blockIdx.z * kchunk; kb < min(K, (blockIdx.z + 1) * kchunk); kb += kXaChunk) {
-        const int kn = min(kXaChunk, K - kb);  // a multiple of 32 (K % 32 == 0)
+        const int kn = min(kXaChunk, K - kb);  // any length: the backward's K is the column count
         // stage X rows m0.. (zero past M) and A rows kb.. (zero past rank).
         // Aligned X goes by cp.async (16 bytes each, all of a thread's copies in
         // flight together), else by scalar loads.
@@ -233,7 +233,9 @@ __global__ void __launch_bounds__(256) lora_xa_kernel(const float* __restrict__ 
                 if (xvec) {
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
                 } else {
-                    *reinterpret_cast<float4*>(dst) = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3));
+                    *reinterpret_cast<float4*>(dst) =
+                        make_float4(__ldg(src), c4 + 1 < kn ? __ldg(src + 1) : 0.0f, c4 + 2 < kn ? __ldg(src + 2) : 0.0f,
+                                    c4 + 3 < kn ? __ldg(src + 3) : 0.0f);  // nothing past the row
                 }
             } else {
                 *reinterpret_cast<float4*>(dst) = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -179,6 +179,29 @@ def test_backward_from_8_bits_spreads_nan_and_steps(session, cuda):
     assert np.array_equal(out[1][0][keep], out[0][0][keep])
 
 
+@pytest.mark.parametrize("m,n", [(30, 23), (130, 1001), (5, 1), (64, 130)])
+def test_fp32_backward_with_rows_of_any_length(session, cuda, m, n):
+    """The fp32 backward where dY's rows are no whole 16 bytes: nothing behind a row (here NaN behind the last) takes
+    part.  dY and its last row's neighbour are one buffer, so nothing is read out of range either way."""
+    import torch
+    k, rank = 160, 4
+    packed, scales = _weights(k, n, 37)
+    rng = np.random.default_rng(n)
+    A, B = (rng.standard_normal(s).astype(np.float32) * 0.02 for s in ((k, rank), (rank, n)))
+    x = _randn((m, k), cuda, 1)
+    buf = torch.full((m * n + 4,), float("nan"), device=cuda)
+    dy = buf[:m * n].view(m, n)
+    dy.copy_(_randn((m, n), cuda, 2))
+    with session.weights(packed, scales, k, n) as h:
+        h.set_lora(A, B, float(rank))
+        h.lora_backward(x.data_ptr(), dy.data_ptr(), m)
+        _, _, da, db = h.get_lora(rank, grads=True)
+    X, D, A64, B64 = x.double(), dy.double(), torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()
+    for got, ref, S in ((da, X.T @ (D @ B64.T), X.abs().T @ (D.abs() @ B64.abs().T)),
+                        (db, (X @ A64).T @ D, (X.abs() @ A64.abs()).T @ D.abs())):
+        assert ((torch.from_numpy(got).to(cuda).double() - ref).abs() <= 2 * 2.0 ** -16 * S).all()
+
+
 # ------------------------------------------------------------------------------------------------------ dX of a layer --
 def _check_dx(got, dtype, ref, S):
     import torch
