@@ -188,7 +188,7 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
                                         void* stream);
 /* Softmax cross entropy of the logits z = X * dequant(W) over the handle's
  * columns (a whole vocabulary; a handle with an adapter attached is refused),
- * without keeping the logits:
+ * without keeping the logits (targets count from the handle's first column):
  *   lse[i] = log sum_v exp z[i][v],  loss[i] = lse[i] - z[i][targets[i]],
  *   dx[i] = row_scale[i] * (softmax(z[i]) - onehot(targets[i])) * dequant(W)^T.
  * x [m x k] and dx [m x k] of `dtype`, 16-byte aligned; targets int64 [m];

@@ -47,6 +47,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -713,11 +714,10 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
 template <bool TR, int PA, int PB, int EPI, bool WT>
 int gg_pairs() {
     using C = GgCfg<PA, PB, WT>;
-    static int cache[64];
-    static bool known[64];
+    static std::atomic<int> cache[64];  // pairs + 1; 0: not asked yet
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (known[dev]) return cache[dev];
+    if (const int known = cache[dev].load(std::memory_order_acquire)) return known - 1;
     auto kern = grad_gemm_kernel<TR, PA, PB, EPI, WT>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess) return 0;
     cudaFuncAttributes fa{};
@@ -736,8 +736,7 @@ int gg_pairs() {
     cfg.numAttrs = 1;
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) return 0;
-    cache[dev] = n;
-    known[dev] = true;
+    cache[dev].store(n + 1, std::memory_order_release);
     return n;
 }
 
@@ -745,7 +744,8 @@ template <bool TR, int PA, int PB, int EPI, bool WT>
 int gg_launch(const GradGemmArgs& a, cudaStream_t stream) {
     using C = GgCfg<PA, PB, WT>;
     auto kern = grad_gemm_kernel<TR, PA, PB, EPI, WT>;
-    const int cap = gg_pairs<TR, PA, PB, EPI, WT>();
+    int cap = gg_pairs<TR, PA, PB, EPI, WT>();
+    if (a.max_pairs > 0 && cap > a.max_pairs) cap = a.max_pairs;
     const long long units = static_cast<long long>(a.row_tiles) * a.col_tiles * a.splits;
     if (cap < 1 || units < 1 || units > (1ll << 30)) return static_cast<int>(cudaErrorInvalidConfiguration);
     cudaLaunchConfig_t cfg = {};

@@ -354,6 +354,7 @@ struct GradGemmArgs {
     float* smax;             // [col_tiles][ld_stat]
     float* ssum;             // [2 col_tiles][ld_stat]
     long long ld_stat;
+    int max_pairs;           // CTA pairs the launch may occupy (0: all)
     int* status;
 };
 int grad_gemm_pairs();  // co-resident CTA pairs on the current device

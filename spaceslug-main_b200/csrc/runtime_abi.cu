@@ -1368,10 +1368,11 @@ struct Carve {
     }
 };
 
-int pairs_or_throw() {
+// CTA pairs a training product of this handle may occupy.
+int grad_pairs(const spaceslug_q4_weights* w) {
     const int pairs = q4::grad_gemm_pairs();
     if (pairs < 1) throw CudaError("the training product does not fit this device");
-    return pairs;
+    return w->sm_budget > 0 ? std::min(pairs, std::max(1, w->sm_budget / 2)) : pairs;
 }
 
 // dX = dY W^T + s (dY B^T) A^T for at most kRowsKernelMax rows.
@@ -1396,7 +1397,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         return;
     }
     DeviceCtx& c = ctx_for(w->device);
-    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
+    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, pairs = grad_pairs(w);
     const size_t size = bf16 ? 2 : 4;
     // contraction: N padded to whole 64-wide stages, and one more stage for the adapter's G A^T
     const int wstages = (N + 63) / 64;
@@ -1507,6 +1508,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.lora_at = at;
         g.ld_at = static_cast<int>(ld_at);
         g.lora_stage = r > 0 ? wstages : -1;
+        g.max_pairs = pairs;
         g.status = c.status;
         check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, weights.from_planes, s), "dY W^T");
         if (g.splits > 1)
@@ -1550,11 +1552,12 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         return;
     }
     DeviceCtx& c = ctx_for(w->device);
-    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, pairs = pairs_or_throw();
+    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, pairs = grad_pairs(w);
     const size_t size = bf16 ? 2 : 4;
     const int tiles = (N + 255) / 256;
     const long long ld_p = static_cast<long long>(tiles) * 256;
-    const long long row_bytes = 2ll * planes * (dx ? ld_p : K);
+    // per row: the planes of X and of p~, and the partial sums of dX
+    const long long row_bytes = (2ll * planes + 1) * K + (dx ? 2ll * planes * ld_p + 4ll * K : 0);
     const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20));
     const TrainWeights weights(w, bf16, true, M, s);
     for (int m0 = 0; m0 < M; m0 += block) {
@@ -1605,6 +1608,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.smax = smax; g.ssum = ssum;
         g.ld_stat = mp;
         g.lora_stage = -1;
+        g.max_pairs = pairs;
         g.status = c.status;
         encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(K),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
