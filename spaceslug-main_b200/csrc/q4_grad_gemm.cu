@@ -784,18 +784,62 @@ int gg_launch_pdl(void (*kern)(Params...), unsigned grid, unsigned threads, cuda
 }
 __device__ __forceinline__ float gg_in(const float* p) { return *p; }
 __device__ __forceinline__ float gg_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void gg_in8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void gg_in8(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+// Eight columns as loaded: a batch of them is in flight before the first is used.
+template <typename T>
+struct GgRaw8;
+template <>
+struct GgRaw8<float> {
+    static constexpr int kBatch = 2;
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = *reinterpret_cast<const float4*>(p);
+        b = *(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <>
+struct GgRaw8<__nv_bfloat16> {
+    static constexpr int kBatch = 4;
+    uint4 q;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { q = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+    }
+};
+// f(p, v) for this thread's pieces of 8 columns p = thread, thread + 256, ...
+template <bool VEC, typename T, typename F>
+__device__ __forceinline__ void gg_row(const T* row, int cols, F&& f) {
+    const int pieces = (cols + 7) / 8;
+    if constexpr (VEC) {
+        using R = GgRaw8<T>;
+        for (int p0 = threadIdx.x; p0 < pieces; p0 += 256 * R::kBatch) {
+            R q[R::kBatch];
+#pragma unroll
+            for (int u = 0; u < R::kBatch; ++u)
+                if (p0 + 256 * u < pieces) q[u].load(row + (p0 + 256 * u) * 8);
+#pragma unroll
+            for (int u = 0; u < R::kBatch; ++u)
+                if (p0 + 256 * u < pieces) {
+                    float v[8];
+                    q[u].values(v);
+                    f(p0 + 256 * u, v);
+                }
+        }
+    } else {
+        for (int p = threadIdx.x; p < pieces; p += 256) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < cols ? gg_in(row + p * 8 + i) : 0.0f;
+            f(p, v);
+        }
     }
 }
 
@@ -810,7 +854,7 @@ __device__ __forceinline__ void gg_in8(const __nv_bfloat16* p, float (&v)[8]) {
 // The row is read twice, the second time from L1 / L2: keeping it in registers
 // (48 floats a thread) halves the blocks per SM and measured slower (24 against
 // 16 us at 4096 x 4096 bf16).
-template <typename T, int PA>
+template <typename T, int PA, bool VEC>
 __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     __shared__ float red[8];
     __shared__ float gs[64];
@@ -821,22 +865,11 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
     const long long* targets = after_wait(A.targets);
     const float* gpart = after_wait(A.gpart);
     const int* gexp = after_wait(A.gexp);
-    const bool vec = A.cols % 8 == 0;
     const int pieces = (A.cols + 7) / 8;
-    auto get = [&](int p, float (&v)[8]) {
-        if (vec) {
-            gg_in8(row + p * 8, v);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < A.cols ? gg_in(row + p * 8 + i) : 0.0f;
-        }
-    };
     float top = 0.0f, dot = 0.0f;
     const long long tgt = targets != nullptr ? targets[m] : -1;
     const bool want_dot = tgt >= 0 && tgt < A.N;
-    for (int p = threadIdx.x; p < pieces; p += 256) {
-        float v[8];
-        get(p, v);
+    gg_row<VEC>(row, A.cols, [&](int p, const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
         if (want_dot) {  // the target's logit, w = v s in fp32
@@ -847,7 +880,7 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
                 part = fmaf(v[i], static_cast<float>((static_cast<int>((q >> (4 * i)) & 15u) ^ 8) - 8), part);
             dot = fmaf(part, __ldg(A.scales + tgt * (A.cols / 32) + (p >> 2)), dot);
         }
-    }
+    });
     if (A.rank > 0 && threadIdx.x < 64) {
         float g = 0.0f;
         if (threadIdx.x < A.rank) {
@@ -907,11 +940,7 @@ __global__ void __launch_bounds__(256) cast_planes_kernel(const CastArgs A) {
         if constexpr (PA == 2)
             *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
     };
-    for (int p = threadIdx.x; p < pieces; p += 256) {
-        float v[8];
-        get(p, v);
-        put(p, v);
-    }
+    gg_row<VEC>(row, A.cols, put);
     const int end = static_cast<int>(A.ld / 8), gp = A.rank > 0 ? end - 8 : end;
     for (int p = pieces + threadIdx.x; p < end; p += 256) {
         float v[8];
@@ -1158,8 +1187,14 @@ int launch_weight_planes(const uint32_t* packed, const float* scales, const int*
 
 int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream) {
     if (a.M < 1 || a.ld % 8 != 0 || a.ld < a.cols || a.rank > 64) return static_cast<int>(cudaErrorInvalidValue);
-    if (bf16) return gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1>, static_cast<unsigned>(a.M), 256, stream, a);
-    if (planes == 2) return gg_launch_pdl(cast_planes_kernel<float, 2>, static_cast<unsigned>(a.M), 256, stream, a);
+    const bool vec = a.cols % 8 == 0;  // rows of whole 16-byte pieces
+    const unsigned grid = static_cast<unsigned>(a.M);
+    if (bf16)
+        return vec ? gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1, true>, grid, 256, stream, a)
+                   : gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1, false>, grid, 256, stream, a);
+    if (planes == 2)
+        return vec ? gg_launch_pdl(cast_planes_kernel<float, 2, true>, grid, 256, stream, a)
+                   : gg_launch_pdl(cast_planes_kernel<float, 2, false>, grid, 256, stream, a);
     return static_cast<int>(cudaErrorInvalidValue);
 }
 

@@ -1285,7 +1285,14 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 // Rows up to which the training products stream the weights on the CUDA cores
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
 constexpr int kRowsKernelMax = 8;
-constexpr long long kTrainScratch = 512ll << 20;  // bytes of operand planes per block of rows
+constexpr long long kTrainScratch = 1ll << 30;  // bytes of operand planes and partial sums per block of rows
+
+// Rows per block: as many as the scratch holds, in even blocks of whole tiles.
+int train_block(int M, long long row_bytes) {
+    const long long most = std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20);
+    const long long blocks = (M + most - 1) / most;
+    return static_cast<int>(((M + blocks - 1) / blocks + 255) / 256 * 256);
+}
 
 // Splits of the contraction of a product of `tiles` 256 x 256 tiles and
 // `chunks` accumulator chunks of `cost` cycles: the least of waves x (chunks
@@ -1405,7 +1412,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     const long long np = (static_cast<long long>(N) + 7) / 8 * 8;
     const bool gt = r > 0 && N >= 32 && N % (bf16 ? 8 : 4) == 0;  // G by the tensor-core passes
     const int rp = gt ? (bf16 ? q4::lora16_rp(r) : q4::lora_tc_rp(r)) : r;
-    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / (ld * 2 * planes) / 256 * 256, 256, 1 << 20));
+    const int block = train_block(M, ld * 2 * planes);
     const size_t b_at = r > 0 ? static_cast<size_t>(planes) * 64 * ld_at * 2 : 0, b_exp = r > 0 ? 64 * sizeof(int) : 0;
     const size_t b_bp = gt ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0;
     Carve fixed;
@@ -1558,7 +1565,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     const long long ld_p = static_cast<long long>(tiles) * 256;
     // per row: the planes of X and of p~, and the partial sums of dX
     const long long row_bytes = (2ll * planes + 1) * K + (dx ? 2ll * planes * ld_p + 4ll * K : 0);
-    const int block = static_cast<int>(std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20));
+    const int block = train_block(M, row_bytes);
     const TrainWeights weights(w, bf16, true, M, s);
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
