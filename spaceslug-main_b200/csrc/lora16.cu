@@ -360,35 +360,42 @@ struct L16FinishLaunch {
 
 // v[row][j] = sum over z of src[z][row][j] in order (or src[j][row] of a
 // row-major [r][R] source), written as the planes of a narrow operand or as a
-// gradient.  One block per 32 rows, transposed through shared memory.
-__global__ void __launch_bounds__(256) lora16_finish_kernel(const L16FinishLaunch F) {
-    __shared__ float tile[32][65];
+// gradient.  One block per 16 rows (few rows have many splits: a thread has two
+// sums at most, eight loads of each in flight), transposed through shared memory.
+constexpr int kL16FinRows = 16, kL16FinThreads = 512;
+__global__ void __launch_bounds__(kL16FinThreads) lora16_finish_kernel(const L16FinishLaunch F) {
+    __shared__ float tile[kL16FinRows][65];
     pdl_launch_dependents();
     pdl_wait();
     const bool second = F.count > 1 && static_cast<int>(blockIdx.x) >= F.blocks0;
     const Lora16Finish& f = F.f[second ? 1 : 0];
     const int rp = f.rp, R = f.R, r = f.r;
     const long long ld = f.ld;
-    const int r0 = (static_cast<int>(blockIdx.x) - (second ? F.blocks0 : 0)) * 32;
+    const float* src = after_wait(f.src);
+    const int r0 = (static_cast<int>(blockIdx.x) - (second ? F.blocks0 : 0)) * kL16FinRows;
     if (f.from_rows) {
-        for (int i = threadIdx.x; i < rp * 32; i += 256) {
-            const int j = i / 32, rr = i % 32, row = r0 + rr;
-            tile[rr][j] = row < R && j < r ? f.src[static_cast<size_t>(j) * f.pitch + row] : 0.0f;
+        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
+            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
+            tile[rr][j] = row < R && j < r ? src[static_cast<size_t>(j) * f.pitch + row] : 0.0f;
         }
     } else {
-        for (int i = threadIdx.x; i < 32 * rp; i += 256) {
+        for (int i = threadIdx.x; i < kL16FinRows * rp; i += kL16FinThreads) {
             const int rr = i / rp, j = i % rp, row = r0 + rr;
             float v = 0.0f;
-            if (row < R && j < r)
-                for (int z = 0; z < f.splits; ++z) v += f.src[(static_cast<size_t>(z) * R + row) * f.pitch + j];
+            if (row < R && j < r) {
+                const float* p = src + static_cast<size_t>(row) * f.pitch + j;
+                const size_t step = static_cast<size_t>(R) * f.pitch;
+#pragma unroll 8
+                for (int z = 0; z < f.splits; ++z) v += p[z * step];
+            }
             tile[rr][j] = v;
         }
     }
     __syncthreads();
     if (f.mode == kL16Planes16) {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(f.out);
-        for (int i = threadIdx.x; i < rp * 32; i += 256) {
-            const int j = i / 32, rr = i % 32, row = r0 + rr;
+        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
+            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
             if (row >= R) continue;
             const float v = tile[rr][j];
             const __nv_bfloat16 hi = __float2bfloat16_rn(v);
@@ -400,23 +407,23 @@ __global__ void __launch_bounds__(256) lora16_finish_kernel(const L16FinishLaunc
         }
     } else if (f.mode == kL16PlanesTf32) {
         float* out = static_cast<float*>(f.out);
-        for (int i = threadIdx.x; i < rp * 32; i += 256) {
-            const int j = i / 32, rr = i % 32, row = r0 + rr;
+        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
+            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
             if (row >= R) continue;
             const float v = tile[rr][j], h = to_tf32(v);
             out[static_cast<size_t>(j) * ld + row] = h;
             out[static_cast<size_t>(rp + j) * ld + row] = v - h;
         }
     } else if (f.mode == kL16Transposed) {
-        for (int i = threadIdx.x; i < r * 32; i += 256) {
-            const int j = i / 32, rr = i % 32, row = r0 + rr;
+        for (int i = threadIdx.x; i < r * kL16FinRows; i += kL16FinThreads) {
+            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
             if (row >= R) continue;
             const float v = f.s * tile[rr][j];
             static_cast<float*>(f.out)[static_cast<size_t>(j) * ld + row] = v;
             if (f.out2) f.out2[static_cast<size_t>(j) * ld + row] = v;
         }
     } else {
-        for (int i = threadIdx.x; i < 32 * r; i += 256) {
+        for (int i = threadIdx.x; i < kL16FinRows * r; i += kL16FinThreads) {
             const int rr = i / r, j = i % r, row = r0 + rr;
             if (row >= R) continue;
             const float v = f.s * tile[rr][j];
@@ -486,10 +493,11 @@ int launch_lora16_finish(const Lora16Finish* f, int count, cudaStream_t stream) 
         if (q.R < 1 || q.splits < 1 || q.r < 1 || q.rp < q.r || q.rp > 64 || !q.src || !q.out)
             return static_cast<int>(cudaErrorInvalidValue);
         F.f[i] = q;
-        if (i == 0) F.blocks0 = (q.R + 31) / 32;
-        blocks += (q.R + 31) / 32;
+        const int nb = (q.R + kL16FinRows - 1) / kL16FinRows;
+        if (i == 0) F.blocks0 = nb;
+        blocks += nb;
     }
-    return l16_launch(lora16_finish_kernel, static_cast<unsigned>(blocks), 256, 0, stream, F);
+    return l16_launch(lora16_finish_kernel, static_cast<unsigned>(blocks), kL16FinThreads, 0, stream, F);
 }
 
 }  // namespace q4

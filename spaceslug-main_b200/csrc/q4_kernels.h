@@ -318,7 +318,7 @@ int rows_wt_splits(int N, int K, int sm_count);
 // partial[splits][M][K] of sum_n d[m][n] w(k, n); with coef, d holds logits and stands for g (softmax - onehot)
 int launch_rows_wt(const void* d, bool bf16, const float* coef, const long long* targets, const uint32_t* packed,
                    const float* scales, float* partial, int splits, int M, int N, int K, cudaStream_t stream);
-// G[z][m][j] = sum over range z of n of dy[m][n] B[j][n], any M
+// G[z][m][j] = sum over range z of n of dy[m][n] B[j][n]
 int rows_proj_splits(int M, int N, int rank, int sm_count);
 int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int splits, int M, int N, int rank,
                      cudaStream_t stream);

@@ -4,7 +4,7 @@
 //   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n), and each 32 columns' max and sum of exponentials
 //   rows_loss_kernel     lse, loss and the rows' coefficients of the gradient
 //   rows_wt_kernel       dx[m][k] = sum_n d[m][n] w(k, n), d given or formed from z and the coefficients
-//   rows_proj_kernel     G[m][j]  = sum_n dy[m][n] B[j][n] (the adapter's side, any number of rows)
+//   rows_proj_kernel     G[m][j]  = sum_n dy[m][n] B[j][n] (the adapter's side)
 //   rows_finish_kernel   sums the splits of n in order, adds s G A^T, rounds once to the output's type
 //
 // w(k, n) = float(v) * scale as everywhere (vulkan-runtime/shaders/q4gemm.comp:104-122),

@@ -1410,11 +1410,11 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     const int wstages = (N + 63) / 64;
     const long long ld = 64ll * (wstages + (r > 0 ? 1 : 0)), ld_at = (static_cast<long long>(K) + 255) / 256 * 256;
     const long long np = (static_cast<long long>(N) + 7) / 8 * 8;
-    const bool gt = r > 0 && N >= 32 && N % (bf16 ? 8 : 4) == 0;  // G by the tensor-core passes
-    const int rp = gt ? (bf16 ? q4::lora16_rp(r) : q4::lora_tc_rp(r)) : r;
+    const int rp = bf16 ? q4::lora16_rp(r) : q4::lora_tc_rp(r);
+    const bool copy = r > 0 && N * size % 16 != 0;  // rows of dY that TMA cannot follow: copied for G's pass
     const int block = train_block(M, ld * 2 * planes);
     const size_t b_at = r > 0 ? static_cast<size_t>(planes) * 64 * ld_at * 2 : 0, b_exp = r > 0 ? 64 * sizeof(int) : 0;
-    const size_t b_bp = gt ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0;
+    const size_t b_bp = r > 0 ? static_cast<size_t>(rp) * np * (bf16 ? 6 : 8) : 0;
     Carve fixed;
     for (size_t b : {b_at, b_exp, b_bp}) fixed.add(b);
     Scratch fixed_mem(fixed.total, s);
@@ -1423,10 +1423,9 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     int* gexp = fixed.take<int>(b_exp);
     void* bp = fixed.take<void>(b_bp);
     const TrainWeights weights(w, bf16, false, M, s);
-    if (r > 0)
+    if (r > 0) {
         check_launch(q4::launch_lora_at(w->lora_a, at, gexp, w->col_exp + N, K, r, static_cast<int>(ld_at), planes, s),
                      "A^T planes");
-    if (gt) {
         const q4::Lora16Finish f{w->lora_b, 1, N, N, r, rp, bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32, 1, 1.0f, bp,
                                  nullptr, np};
         check_launch(q4::launch_lora16_finish(&f, 1, s), "B planes");
@@ -1447,45 +1446,48 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.out_rows = g.row_tiles * 256;
         g.plane_rows = mc;
         int gsplits = 1;
-        if (gt)
-            q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
-        else if (r > 0)
-            gsplits = q4::rows_proj_splits(mc, N, r, c.sm_count);
+        if (r > 0) q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
         const size_t b_x = static_cast<size_t>(planes) * mc * ld * 2, b_re = static_cast<size_t>(mc) * sizeof(int);
         const size_t b_part = g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0;
         const size_t b_g = r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0;
+        const size_t ld_d = (copy ? static_cast<size_t>(np) : static_cast<size_t>(N)) * size, b_d = copy ? ld_d * mc : 0;
         Carve cut;
-        for (size_t b : {b_x, b_re, b_part, b_g}) cut.add(b);
+        for (size_t b : {b_x, b_re, b_part, b_g, b_d}) cut.add(b);
         Scratch mem(cut.total, s);
         cut.base = static_cast<char*>(mem.p);
         void* x16 = cut.take<void>(b_x);
         int* rexp = cut.take<int>(b_re);
         float* part = cut.take<float>(b_part);
         float* gpart = cut.take<float>(b_g);
-        if (gt && bf16) {
+        const void* rows = d;
+        if (copy) {
+            void* to = cut.take<void>(b_d);
+            check(cudaMemcpy2DAsync(to, ld_d, d, N * size, N * size, static_cast<size_t>(mc), cudaMemcpyDeviceToDevice, s),
+                  "cudaMemcpy2DAsync (dY rows)");
+            rows = to;
+        }
+        if (r > 0 && bf16) {
             q4::Lora16Pass p{};
             p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
             q4::Lora16Problem& q = p.prob[0];
-            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
-                      static_cast<uint64_t>(N) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rows, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
+                      ld_d, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
             encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, bp, static_cast<uint64_t>(N),
                       static_cast<uint64_t>(3 * rp), static_cast<uint64_t>(np) * 2, 64, static_cast<uint32_t>(3 * rp),
                       CU_TENSOR_MAP_SWIZZLE_128B);
             q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
             check_launch(q4::launch_lora16_pass(p, s), "dY B^T");
-        } else if (gt) {
+        } else if (r > 0) {
             q4::LoraTcPass p{};
             p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
             q4::LoraTcProblem& q = p.prob[0];
-            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, d, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
-                      static_cast<uint64_t>(N) * 4, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+            encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, rows, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
+                      ld_d, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
             encode_2d(&q.tm_b, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, bp, static_cast<uint64_t>(N),
                       static_cast<uint64_t>(2 * rp), static_cast<uint64_t>(np) * 4, 32, static_cast<uint32_t>(2 * rp),
                       CU_TENSOR_MAP_SWIZZLE_128B);
             q.partial = gpart; q.R = mc; q.L = N; q.splits = gsplits;
             check_launch(q4::launch_lora_tc_pass(p, s), "dY B^T");
-        } else if (r > 0) {
-            check_launch(q4::launch_rows_proj(d, bf16, w->lora_b, gpart, gsplits, mc, N, r, s), "dY B^T");
         }
         q4::CastArgs ca{};
         ca.x = d; ca.out = x16; ca.row_exp = rexp;
