@@ -360,11 +360,13 @@ struct L16FinishLaunch {
 
 // v[row][j] = sum over z of src[z][row][j] in order (or src[j][row] of a
 // row-major [r][R] source), written as the planes of a narrow operand or as a
-// gradient.  One block per 16 rows (few rows have many splits: a thread has two
-// sums at most, eight loads of each in flight), transposed through shared memory.
-constexpr int kL16FinRows = 16, kL16FinThreads = 512;
+// gradient.  One block per ROWS rows, transposed through shared memory: 32 (whole
+// 128-byte lines of fp32 rows), or 16 where few rows have many splits (a thread
+// then has two sums at most, eight loads of each in flight).
+constexpr int kL16FinThreads = 512;
+template <int ROWS>
 __global__ void __launch_bounds__(kL16FinThreads) lora16_finish_kernel(const L16FinishLaunch F) {
-    __shared__ float tile[kL16FinRows][65];
+    __shared__ float tile[ROWS][65];
     pdl_launch_dependents();
     pdl_wait();
     const bool second = F.count > 1 && static_cast<int>(blockIdx.x) >= F.blocks0;
@@ -372,14 +374,14 @@ __global__ void __launch_bounds__(kL16FinThreads) lora16_finish_kernel(const L16
     const int rp = f.rp, R = f.R, r = f.r;
     const long long ld = f.ld;
     const float* src = after_wait(f.src);
-    const int r0 = (static_cast<int>(blockIdx.x) - (second ? F.blocks0 : 0)) * kL16FinRows;
+    const int r0 = (static_cast<int>(blockIdx.x) - (second ? F.blocks0 : 0)) * ROWS;
     if (f.from_rows) {
-        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
-            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
+        for (int i = threadIdx.x; i < rp * ROWS; i += kL16FinThreads) {
+            const int j = i / ROWS, rr = i % ROWS, row = r0 + rr;
             tile[rr][j] = row < R && j < r ? src[static_cast<size_t>(j) * f.pitch + row] : 0.0f;
         }
     } else {
-        for (int i = threadIdx.x; i < kL16FinRows * rp; i += kL16FinThreads) {
+        for (int i = threadIdx.x; i < ROWS * rp; i += kL16FinThreads) {
             const int rr = i / rp, j = i % rp, row = r0 + rr;
             float v = 0.0f;
             if (row < R && j < r) {
@@ -394,8 +396,8 @@ __global__ void __launch_bounds__(kL16FinThreads) lora16_finish_kernel(const L16
     __syncthreads();
     if (f.mode == kL16Planes16) {
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(f.out);
-        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
-            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
+        for (int i = threadIdx.x; i < rp * ROWS; i += kL16FinThreads) {
+            const int j = i / ROWS, rr = i % ROWS, row = r0 + rr;
             if (row >= R) continue;
             const float v = tile[rr][j];
             const __nv_bfloat16 hi = __float2bfloat16_rn(v);
@@ -407,23 +409,23 @@ __global__ void __launch_bounds__(kL16FinThreads) lora16_finish_kernel(const L16
         }
     } else if (f.mode == kL16PlanesTf32) {
         float* out = static_cast<float*>(f.out);
-        for (int i = threadIdx.x; i < rp * kL16FinRows; i += kL16FinThreads) {
-            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
+        for (int i = threadIdx.x; i < rp * ROWS; i += kL16FinThreads) {
+            const int j = i / ROWS, rr = i % ROWS, row = r0 + rr;
             if (row >= R) continue;
             const float v = tile[rr][j], h = to_tf32(v);
             out[static_cast<size_t>(j) * ld + row] = h;
             out[static_cast<size_t>(rp + j) * ld + row] = v - h;
         }
     } else if (f.mode == kL16Transposed) {
-        for (int i = threadIdx.x; i < r * kL16FinRows; i += kL16FinThreads) {
-            const int j = i / kL16FinRows, rr = i % kL16FinRows, row = r0 + rr;
+        for (int i = threadIdx.x; i < r * ROWS; i += kL16FinThreads) {
+            const int j = i / ROWS, rr = i % ROWS, row = r0 + rr;
             if (row >= R) continue;
             const float v = f.s * tile[rr][j];
             static_cast<float*>(f.out)[static_cast<size_t>(j) * ld + row] = v;
             if (f.out2) f.out2[static_cast<size_t>(j) * ld + row] = v;
         }
     } else {
-        for (int i = threadIdx.x; i < kL16FinRows * r; i += kL16FinThreads) {
+        for (int i = threadIdx.x; i < ROWS * r; i += kL16FinThreads) {
             const int rr = i / r, j = i % r, row = r0 + rr;
             if (row >= R) continue;
             const float v = f.s * tile[rr][j];
@@ -487,17 +489,26 @@ int launch_lora16_finish(const Lora16Finish* f, int count, cudaStream_t stream) 
     if (count < 1 || count > 2) return static_cast<int>(cudaErrorInvalidValue);
     L16FinishLaunch F{};
     F.count = count;
-    int blocks = 0;
+    int most = 0;
     for (int i = 0; i < count; ++i) {
         const Lora16Finish& q = f[i];
         if (q.R < 1 || q.splits < 1 || q.r < 1 || q.rp < q.r || q.rp > 64 || !q.src || !q.out)
             return static_cast<int>(cudaErrorInvalidValue);
         F.f[i] = q;
-        const int nb = (q.R + kL16FinRows - 1) / kL16FinRows;
-        if (i == 0) F.blocks0 = nb;
-        blocks += nb;
+        most = q.R > most ? q.R : most;
     }
-    return l16_launch(lora16_finish_kernel, static_cast<unsigned>(blocks), kL16FinThreads, 0, stream, F);
+    // 4096 x 4096 x 11008, rank 16: dA / dB in 6.5 us with 32 rows, 9.1 with 16;
+    // 32 x 1536 x 2328, rank 64: the whole backward 45 us with 16 rows (77 with
+    // 32 rows on 256 threads, one load in flight).
+    const int rows = most >= 2048 ? 32 : 16;
+    int blocks = 0;
+    for (int i = 0; i < count; ++i) {
+        blocks += (f[i].R + rows - 1) / rows;
+        if (i == 0) F.blocks0 = blocks;
+    }
+    return rows == 32
+               ? l16_launch(lora16_finish_kernel<32>, static_cast<unsigned>(blocks), kL16FinThreads, 0, stream, F)
+               : l16_launch(lora16_finish_kernel<16>, static_cast<unsigned>(blocks), kL16FinThreads, 0, stream, F);
 }
 
 }  // namespace q4
