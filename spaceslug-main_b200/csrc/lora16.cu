@@ -10,11 +10,19 @@
 // partial sums added in a fixed order afterwards (deterministic).
 //
 // Against the fp32 form: the wide operand needs no hi / lo split, so a stage
-// of 64 l is four MMAs (kind::f16 on bf16, M = 128, K = 16) instead of
-// thirty-two of the TF32 passes, and X crosses HBM in a byte per value.  The narrow operand enters
+// of 64 l is four MMAs (kind::f16 on bf16, M = 128, K = 16) instead of the
+// sixteen of the TF32 passes, and X crosses HBM in a byte per value.  The narrow operand enters
 // as three stacked bf16 planes (hi, mid, lo: 24 bits, exact), N = 3 RP, whose
 // sums the epilogue adds.  So every product is exact and the sums are fp32:
 // restarted every 64 l and added in registers, rounded to nearest.
+//
+// For ranks up to 16 an fp32 dY comes the same way (F32): its values as three
+// bf16 planes in tensor memory, 32 + 6 KB and twelve MMAs per stage, so that T
+// and G, dA and dB stay one launch each.  Higher ranks leave tensor memory no
+// room for that; their dY goes through lora_tc.cu.  (M x K x N, rank, the whole
+// backward this way and with lora_tc.cu: 128 x 64 x 256, 4: 22 and 28 us; 512 x
+// 4096 x 4096, 16: 32 and 43; 2048 x 4096 x 4096: 48 and 60; 4096 x 4096 x
+// 11008: 118 and 125.)
 //
 //  - T and G read the wide operand with its rows as rows of D: TMA boxes of
 //    128 rows x 64 l (bf16 128-byte swizzled, codes 64-byte swizzled).
@@ -44,14 +52,16 @@ constexpr int kL16L = 64;         // contraction elements per stage
 constexpr int kL16Threads = 512;  // warps: 0 TMA, 1-2 MMA, 4-7 epilogue, 8-15 split
 constexpr int kL16ATile = kL16Rows * kL16L * 2;
 
-template <int RP>
+template <int RP, bool F32>
 struct L16Cfg {
     static constexpr int kN = 3 * RP;
+    static constexpr int kATile = F32 ? 2 * kL16ATile : kL16ATile;
     static constexpr int kBTile = kN * kL16L * 2;  // 128-byte rows: 6, 12 or 24 KB
-    static constexpr int kStageBytes = kL16ATile + kBTile;
-    // tensor memory: two accumulator buffers of 3 RP columns, then 32 columns (64 bf16) per stage
+    static constexpr int kStageBytes = kATile + kBTile;
+    // tensor memory: two accumulator buffers of 3 RP columns, then per stage 32 columns (64 bf16) for each plane of Aop
     static constexpr int kACol = 2 * kN;
-    static constexpr int kTmemStages = (512 - kACol) / 32;
+    static constexpr int kACols = F32 ? 96 : 32;
+    static constexpr int kTmemStages = (512 - kACol) / kACols;
     static constexpr int kSmemStages = 200 * 1024 / kStageBytes;
     static constexpr int kStages0 = kSmemStages < kTmemStages ? kSmemStages : kTmemStages;
     // even: a slot then belongs to one group of split warps and one MMA warp,
@@ -105,9 +115,9 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t u0, uint32_t u1, float2 s
     return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
 }
 
-template <int RP, bool MN>
+template <int RP, bool MN, bool F32>
 __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_constant__ Lora16Pass P) {
-    using C = L16Cfg<RP>;
+    using C = L16Cfg<RP, F32>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -158,7 +168,8 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 const L16Unit w = l16_unit(P, u);
                 const Lora16Problem& pb = P.prob[w.pi];
-                const uint32_t bytes = (pb.act8 ? kL16ATile / 2 : kL16ATile) + C::kBTile;
+                const bool wide = F32 && pb.kind == kL16F32;
+                const uint32_t bytes = (pb.kind == kL16Act8 ? kL16ATile / 2 : wide ? 2 * kL16ATile : kL16ATile) + C::kBTile;
                 const int row0 = w.tile * kL16Rows;
                 for (int st = w.s0; st < w.s1; ++st, ++q) {
                     const int s = q % C::kStages;
@@ -174,8 +185,9 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
                         tma_load_2d(a, &pb.tm_a, full(s), row0, l0);
                     } else {
                         tma_load_2d(a, &pb.tm_a, full(s), l0, row0);
+                        if (wide) tma_load_2d(a + kL16ATile, &pb.tm_a, full(s), l0 + 32, row0);  // 32 fp32 per box row
                     }
-                    tma_load_2d(a + kL16ATile, &pb.tm_b, full(s), l0, 0);
+                    tma_load_2d(a + C::kATile, &pb.tm_b, full(s), l0, 0);
                 }
             }
             if (*abort_flag)
@@ -188,26 +200,36 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
             // -------------------------------- MMA: even and odd stages --
             const int par = warp - 1;
             constexpr uint32_t idesc = umma_idesc_f16(1u, kL16Rows, C::kN);
-            int total = 0;
-            for (int u = blockIdx.x; u < units; u += gridDim.x) {
-                const L16Unit w = l16_unit(P, u);
-                total += w.s1 - w.s0;
-            }
             const uint32_t dacc = tmem + static_cast<uint32_t>(par * C::kN);
-            int last = -1;
-            for (int q = par; q < total; q += 2) {
-                const int s = q % C::kStages;
-                if (q >= 2 && !mbar_wait(chunk_empty(par), ((q >> 1) - 1) & 1u, abort_flag, status, kStatusTimeoutMma))
-                    break;
-                if (!mbar_wait(split(s), (q / C::kStages) & 1u, abort_flag, status, kStatusTimeoutMma)) break;
-                tc_fence_after_sync();
-                const uint32_t bt = base + s * C::kStageBytes + kL16ATile;
-                const uint32_t at = tmem + static_cast<uint32_t>(C::kACol + 32 * s);
+            int last = -1, q = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const L16Unit w = l16_unit(P, u);
+                const bool wide = F32 && P.prob[w.pi].kind == kL16F32;
+                for (int st = w.s0; st < w.s1; ++st, ++q) {
+                    if ((q & 1) != par) continue;
+                    const int s = q % C::kStages;
+                    if ((q >= 2 &&
+                         !mbar_wait(chunk_empty(par), ((q >> 1) - 1) & 1u, abort_flag, status, kStatusTimeoutMma)) ||
+                        !mbar_wait(split(s), (q / C::kStages) & 1u, abort_flag, status, kStatusTimeoutMma)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t bt = base + s * C::kStageBytes + C::kATile;
+                    const uint32_t at = tmem + static_cast<uint32_t>(C::kACol + C::kACols * s);
 #pragma unroll
-                for (int kk = 0; kk < kL16L / 16; ++kk)
-                    umma_f16_ts(dacc, at + 8 * kk, umma_desc_k_sw128(bt + kk * 32), idesc, kk > 0 ? 1u : 0u);
-                umma_commit(empty(s));
-                last = q;
+                    for (int kk = 0; kk < kL16L / 16; ++kk) {
+                        const uint64_t bd = umma_desc_k_sw128(bt + kk * 32);
+                        umma_f16_ts(dacc, at + 8 * kk, bd, idesc, kk > 0 ? 1u : 0u);
+                        if (wide) {  // the mid and lo planes
+                            umma_f16_ts(dacc, at + 32 + 8 * kk, bd, idesc, 1u);
+                            umma_f16_ts(dacc, at + 64 + 8 * kk, bd, idesc, 1u);
+                        }
+                    }
+                    umma_commit(empty(s));
+                    last = q;
+                }
             }
             if (*abort_flag && last >= 0) mbar_drain(empty(last % C::kStages), (last / C::kStages) & 1u);
         }
@@ -272,7 +294,7 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
                 if ((q & 1) != par) continue;
                 const int s = q % C::kStages, l0 = st * kL16L;
                 float step0 = 0.0f, step1 = 0.0f;  // this thread's two step factors of the stage
-                if (pb.act8) {
+                if (pb.kind == kL16Act8) {
                     if constexpr (MN) {
                         // group of this warp's 32 rows of D, at l = l0 + lane and l0 + 32 + lane
                         const long long g = w.tile * (kL16Rows / 32) + quarter;
@@ -295,8 +317,37 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
                 }
                 tc_fence_after_sync();  // the MMAs that last read this stage's tensor memory have completed
                 const uint8_t* stage = smem + s * C::kStageBytes;
+                const uint32_t acol = t_lane + static_cast<uint32_t>(C::kACol + C::kACols * s);
                 uint32_t v[32];
-                if (pb.act8) {
+                if (F32 && pb.kind == kL16F32) {
+                    if constexpr (F32) {
+                        // 64 fp32 of this row, cut into bf16 hi, mid and lo parts of 8 bits each
+                        // (exact, and no value near the largest rounds up to infinity)
+                        float f[64];
+                        if constexpr (MN) {
+                            const float* col = reinterpret_cast<const float*>(stage) + row;  // l at 512 l
+#pragma unroll
+                            for (int l = 0; l < 64; ++l) f[l] = col[128 * l];
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) {  // two boxes of 32 l, 128-byte rows
+                                const float4 x = *reinterpret_cast<const float4*>(stage + (c >> 3) * kL16ATile + 128 * row +
+                                                                                  (((c & 7) ^ (row & 7)) << 4));
+                                f[4 * c] = x.x; f[4 * c + 1] = x.y; f[4 * c + 2] = x.z; f[4 * c + 3] = x.w;
+                            }
+                        }
+#pragma unroll
+                        for (int p = 0; p < 3; ++p) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                v[i] = __byte_perm(__float_as_uint(f[2 * i]), __float_as_uint(f[2 * i + 1]), 0x7632);
+                                f[2 * i] -= __uint_as_float(v[i] << 16);
+                                f[2 * i + 1] -= __uint_as_float(v[i] & 0xFFFF0000u);
+                            }
+                            if (p < 2) tmem_st32(acol + 32 * p, v);
+                        }
+                    }
+                } else if (pb.kind == kL16Act8) {
                     if constexpr (MN) {
                         steps[lane] = step0;
                         steps[32 + lane] = step1;
@@ -337,7 +388,7 @@ __global__ void __launch_bounds__(kL16Threads, 1) lora16_kernel(const __grid_con
                         v[4 * c + 3] = x.w;
                     }
                 }
-                tmem_st32(t_lane + static_cast<uint32_t>(C::kACol + 32 * s), v);
+                tmem_st32(acol + (F32 && pb.kind == kL16F32 ? 64 : 0), v);
                 tmem_st_wait();
                 tc_fence_before_sync();
                 __syncwarp();
@@ -450,10 +501,10 @@ int l16_launch(Kern kern, unsigned grid, int threads, int smem, cudaStream_t str
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, arg));
 }
 
-template <int RP, bool MN>
+template <int RP, bool MN, bool F32 = false>
 int l16_pass(const Lora16Pass& p, cudaStream_t stream) {
-    using C = L16Cfg<RP>;
-    auto kern = lora16_kernel<RP, MN>;
+    using C = L16Cfg<RP, F32>;
+    auto kern = lora16_kernel<RP, MN, F32>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemAlloc);
     if (e != cudaSuccess) return static_cast<int>(e);
     long long units = 0;
@@ -471,14 +522,18 @@ int lora16_stage() { return kL16L; }
 
 int launch_lora16_pass(const Lora16Pass& p, cudaStream_t stream) {
     if (p.count < 1 || p.count > 2 || p.sm_count < 1) return static_cast<int>(cudaErrorInvalidValue);
+    bool f32 = false;
     for (int i = 0; i < p.count; ++i) {
         const Lora16Problem& q = p.prob[i];
         if (q.R < 1 || q.L < 1 || q.splits < 1 || q.splits > (q.L + kL16L - 1) / kL16L || !q.partial ||
-            (q.act8 && (!q.exps || q.groups < 1)))
+            (q.kind == kL16Act8 && (!q.exps || q.groups < 1)) || (q.kind == kL16F32 && p.rp != 16))
             return static_cast<int>(cudaErrorInvalidValue);
+        f32 |= q.kind == kL16F32;
     }
     switch (p.rp) {
-        case 16: return p.mn_major ? l16_pass<16, true>(p, stream) : l16_pass<16, false>(p, stream);
+        case 16:
+            if (f32) return p.mn_major ? l16_pass<16, true, true>(p, stream) : l16_pass<16, false, true>(p, stream);
+            return p.mn_major ? l16_pass<16, true>(p, stream) : l16_pass<16, false>(p, stream);
         case 32: return p.mn_major ? l16_pass<32, true>(p, stream) : l16_pass<32, false>(p, stream);
         case 64: return p.mn_major ? l16_pass<64, true>(p, stream) : l16_pass<64, false>(p, stream);
         default: return static_cast<int>(cudaErrorInvalidValue);

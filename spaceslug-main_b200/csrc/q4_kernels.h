@@ -396,13 +396,15 @@ int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K,
 
 // LoRA gradients with wide operands exact in bf16 (lora16.cu): a problem is partial[split][row][rp] of D[R x r] = sum
 // over l < L of Aop[row][l] Bop[j][l].  tm_a: bf16 (K-major box 64 l x 128 rows, 128B swizzle; MN-major box 128 rows x
-// 64 l, unswizzled) or, with act8, int8 codes (64 l x 128 rows, 64B swizzle; 128 rows x 64 l, unswizzled) with their
-// step bytes exps [source row][groups]; tm_b: Bop's stacked bf16 planes, dims {L, 3 rp}, box 64 x 3 rp, 128B swizzle.
+// 64 l, unswizzled), int8 codes (64 l x 128 rows, 64B swizzle; 128 rows x 64 l, unswizzled) with their step bytes
+// exps [source row][groups], or fp32 (rp 16 only; 32 l x 128 rows, 128B swizzle; 128 rows x 64 l, unswizzled); tm_b:
+// Bop's stacked bf16 planes, dims {L, 3 rp}, box 64 x 3 rp, 128B swizzle.
+enum : int { kL16Bf16 = 0, kL16Act8 = 1, kL16F32 = 2 };
 struct Lora16Problem {
     CUtensorMap tm_a, tm_b;
     const uint8_t* exps;
     float* partial;
-    int R, L, splits, act8, groups;
+    int R, L, splits, kind, groups;
 };
 struct Lora16Pass {
     Lora16Problem prob[2];

@@ -1161,10 +1161,10 @@ const char* rows_error(const void* in, const void* out, int dtype, uint32_t m) {
 }
 
 // The adapter's gradients with X in 8 bits, into the handle (and to da, db):
-// all four products in bf16 passes (lora16.cu) when dY is bf16 too; for fp32 dY
-// the two products of X there and the two of dY in the TF32 passes of
-// lora_tc.cu.  TMA wants rows of dY whose length is a multiple of 16 bytes:
-// others are copied once into such rows.
+// all four products in the passes of lora16.cu, an fp32 dY with a rank up to 16
+// included; for fp32 dY with a higher rank the two products of X there and the
+// two of dY in the TF32 passes of lora_tc.cu.  TMA wants rows of dY whose length
+// is a multiple of 16 bytes: others are copied once into such rows.
 void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps, const void* dy, bool bf16,
                             int M, float* da, float* db, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
@@ -1173,6 +1173,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     auto round8 = [](int v) { return (static_cast<long long>(v) + 7) / 8 * 8; };
     const long long Kp = round8(K), Np = round8(N), Mp = round8(M);
     const size_t size = bf16 ? 2 : 4;
+    const bool one = bf16 || rp == 16;  // dY in the same passes as X
     const bool copy = N * size % 16 != 0;
     const size_t ld_y = (copy ? static_cast<size_t>(Np) : static_cast<size_t>(N)) * size;
     Scratch rows(copy ? ld_y * M : 0, s);
@@ -1184,7 +1185,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     const int R1[2] = {M, M}, L1[2] = {K, N}, R2[2] = {K, N}, L2[2] = {M, M};
     int s1[2], s2[2];  // splits of {T, G} and {dA, dB}
     const int st = q4::lora16_stage();
-    if (bf16) {
+    if (one) {
         q4::lora_tc_plan(2, R1, L1, c.sm_count, s1, st);
         q4::lora_tc_plan(2, R2, L2, c.sm_count, s2, st);
     } else {
@@ -1193,9 +1194,9 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
         q4::lora_tc_plan(1, R2, L2, c.sm_count, s2, st);
         q4::lora_tc_plan(1, R2 + 1, L2 + 1, c.sm_count, s2 + 1);
     }
-    const int rg = bf16 ? rp : rt;  // padded rank of the dY passes
+    const int rg = one ? rp : rt;  // padded rank of the dY passes
     // planes: A^T and G^T (bf16), B and T^T (bf16 or TF32); partial sums of both passes
-    const size_t pl16 = static_cast<size_t>(3) * rp * 2, plY = bf16 ? pl16 : static_cast<size_t>(2) * rt * 4;
+    const size_t pl16 = static_cast<size_t>(3) * rp * 2, plY = one ? pl16 : static_cast<size_t>(2) * rt * 4;
     auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     const size_t bA = up(pl16 * Kp), bG = up(pl16 * Mp), bB = up(plY * Np), bT = up(plY * Mp);
     const size_t pT = up(static_cast<size_t>(s1[0]) * M * rp * 4), pG = up(static_cast<size_t>(s1[1]) * M * rg * 4);
@@ -1223,13 +1224,14 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
         q.R = mn ? K : M;
         q.L = mn ? M : K;
         q.splits = splits;
-        q.act8 = 1;
+        q.kind = q4::kL16Act8;
         q.groups = G;
     };
-    auto y16_problem = [&](q4::Lora16Problem& q, bool mn, const void* plane, int splits, float* partial) {
+    auto y_problem = [&](q4::Lora16Problem& q, bool mn, const void* plane, int splits, float* partial) {
         q = {};
-        encode_2d(&q.tm_a, B16, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), ld_y,
-                  mn ? 128 : 64, mn ? 64 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
+        q.kind = bf16 ? q4::kL16Bf16 : q4::kL16F32;
+        encode_2d(&q.tm_a, bf16 ? B16 : F32, dy, static_cast<uint64_t>(N), static_cast<uint64_t>(M), ld_y,
+                  mn ? 128 : bf16 ? 64 : 32, mn ? 64 : 128, mn ? CU_TENSOR_MAP_SWIZZLE_NONE : SW);
         planes16(q, plane, mn ? M : N);
         q.partial = partial;
         q.R = mn ? N : M;
@@ -1255,7 +1257,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
         q.splits = splits;
         check_launch(q4::launch_lora_tc_pass(p, s), "lora pass (fp32 dY)");
     };
-    const int planesY = bf16 ? q4::kL16Planes16 : q4::kL16PlanesTf32;
+    const int planesY = one ? q4::kL16Planes16 : q4::kL16PlanesTf32;
     q4::Lora16Finish f[2];
     f[0] = {w->lora_a, 1, K, r, r, rp, q4::kL16Planes16, 0, 1.0f, at, nullptr, Kp};
     f[1] = {w->lora_b, 1, N, N, r, rg, planesY, 1, 1.0f, bt, nullptr, Np};
@@ -1264,19 +1266,19 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     p.rp = rp;
     p.sm_count = c.sm_count;
     p.status = c.status;
-    p.count = bf16 ? 2 : 1;
+    p.count = one ? 2 : 1;
     x_problem(p.prob[0], false, at, s1[0], partT);
-    if (bf16) y16_problem(p.prob[1], false, bt, s1[1], partG);
+    if (one) y_problem(p.prob[1], false, bt, s1[1], partG);
     check_launch(q4::launch_lora16_pass(p, s), "lora T / G pass");
-    if (!bf16) y32_pass(false, bt, s1[1], partG);
+    if (!one) y32_pass(false, bt, s1[1], partG);
     f[0] = {partT, s1[0], M, rp, r, rg, planesY, 0, 1.0f, tt, nullptr, Mp};
     f[1] = {partG, s1[1], M, rg, r, rp, q4::kL16Planes16, 0, 1.0f, gt, nullptr, Mp};
     check_launch(q4::launch_lora16_finish(f, 2, s), "lora T / G planes");
     p.mn_major = 1;
     x_problem(p.prob[0], true, gt, s2[0], partA);
-    if (bf16) y16_problem(p.prob[1], true, tt, s2[1], partB);
+    if (one) y_problem(p.prob[1], true, tt, s2[1], partB);
     check_launch(q4::launch_lora16_pass(p, s), "lora dA / dB pass");
-    if (!bf16) y32_pass(true, tt, s2[1], partB);
+    if (!one) y32_pass(true, tt, s2[1], partB);
     f[0] = {partA, s2[0], K, rp, r, rp, q4::kL16AsRows, 0, scale, w->lora_da, da, r};
     f[1] = {partB, s2[1], N, rg, r, rg, q4::kL16Transposed, 0, scale, w->lora_db, db, N};
     check_launch(q4::launch_lora16_finish(f, 2, s), "lora dA / dB");
