@@ -357,6 +357,29 @@ struct GradGemmArgs {
     int max_pairs;           // CTA pairs the launch may occupy (0: all)
     int* status;
 };
+// The same products for at most kFewRows rows (q4_few_rows.cu): blocks of 128 n x 128 k.
+constexpr int kFewRows = 64;
+struct FewRowsArgs {
+    CUtensorMap tm_a;        // f16 planes of the rows [planes * M][contraction], box 64 x few_rows_padded(M), 128B swizzle
+    CUtensorMap tm_w, tm_s;  // packed words and scales as in GradGemmArgs
+    const int* w_exp;        // the handle's power of two (device)
+    const int* row_exp;      // [M], or nullptr: fixed_exp for every row
+    int fixed_exp;
+    int M, N, K;
+    int tiles, splits;       // tiles of 128 n (logits) or 128 k, splits of the contraction
+    int blocks, chunk, chunks;  // blocks of 128 of the contraction, blocks per accumulator chunk, chunks
+    const float* coef;       // [chunks][ld_stat] factor of a row's chunk, or nullptr
+    const long long* targets;  // logits: [M]
+    float* smax;             // [tiles][ld_stat]
+    float* ssum;             // [4 tiles][ld_stat]
+    long long ld_stat;       // at least few_rows_padded(M)
+    void* out;               // logits with kGgProb: planes of p~ f16 [planes * M][ld_out]; transposed: fp32 [splits][M][K]
+    long long ld_out;
+    int sm_count;            // blocks the launch may occupy
+    int* status;
+};
+int few_rows_padded(int M);
+int launch_few_rows(const FewRowsArgs& a, int planes, int epi, cudaStream_t stream);
 int grad_gemm_pairs();  // co-resident CTA pairs on the current device
 int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_planes, cudaStream_t stream);
 // The weights' planes [N][K]: hi (f16), and 64 lo in e4m3 unless null.
@@ -385,9 +408,9 @@ struct CastArgs {
 };
 int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream);
 int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int K, cudaStream_t stream);
-// tile statistics -> chunk factors (in smax), row sums, loss and lse
+// tile statistics (`parts` sums per tile, 2 or 4) -> chunk factors (in smax), row sums, loss and lse
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
-                     float* loss, float* lse, int M, int N, int tiles, long long ld, cudaStream_t stream);
+                     float* loss, float* lse, int M, int N, int tiles, int parts, long long ld, cudaStream_t stream);
 int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,
                    const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream);

@@ -1287,6 +1287,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 // Rows up to which the training products stream the weights on the CUDA cores
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
 constexpr int kRowsKernelMax = 8;
+constexpr int kFewRowsCost = 560;  // shared-memory cycles of a block of 128 n x 128 k and plane of the weights
 constexpr long long kTrainScratch = 1ll << 30;  // bytes of operand planes and partial sums per block of rows
 
 // Rows per block: as many as the scratch holds, in even blocks of whole tiles.
@@ -1345,7 +1346,8 @@ struct TrainWeights {
                      "weight planes");
     }
     // tensor maps of the logits' or the transposed product
-    void encode(q4::GradGemmArgs& g, bool transposed) const {
+    template <typename Args>
+    void encode(Args& g, bool transposed) const {
         const uint64_t K = static_cast<uint64_t>(w->K), N = static_cast<uint64_t>(w->N);
         if (from_planes) {
             encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, planes.p, K, N, K * 2, 64, transposed ? 64 : 128,
@@ -1400,7 +1402,62 @@ void run_input_gradient_rows(spaceslug_q4_weights* w, const void* dy, void* dx, 
                  "dX");
 }
 
+// The products of up to kFewRows rows (q4_few_rows.cu): SMs they may occupy, and
+// the shared-memory cycles of a block, which the splits are weighed by.
+int few_rows_sms(const spaceslug_q4_weights* w, const DeviceCtx& c) {
+    return w->sm_budget > 0 ? std::min(c.sm_count, w->sm_budget) : c.sm_count;
+}
+
+// dX of up to kFewRows rows: planes of dY, the product in splits of n, and the
+// adapter's side in fp32 as for fewer rows.
+void run_input_gradient_few(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
+    DeviceCtx& c = ctx_for(w->device);
+    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, sms = few_rows_sms(w, c);
+    const long long ld = (static_cast<long long>(N) + 63) / 64 * 64;
+    const TrainWeights weights(w, bf16, false, M, s);
+    q4::FewRowsArgs g{};
+    g.M = M; g.N = N; g.K = K;
+    g.tiles = (K + 127) / 128;
+    g.blocks = (N + 127) / 128;
+    g.chunk = bf16 ? 4 : 2;  // truncated sums of 512 or 256 terms
+    g.chunks = (g.blocks + g.chunk - 1) / g.chunk;
+    g.splits = grad_splits(g.tiles, g.chunks, kFewRowsCost * planes * g.chunk, sms, static_cast<long long>(M) * K, true);
+    const int gsplits = r > 0 ? q4::rows_proj_splits(M, N, r, sms) : 0;
+    const size_t b_x = static_cast<size_t>(planes) * M * ld * 2, b_re = static_cast<size_t>(M) * sizeof(int);
+    const size_t b_part = static_cast<size_t>(g.splits) * M * K * 4, b_g = static_cast<size_t>(gsplits) * M * r * 4;
+    Carve cut;
+    for (size_t b : {b_x, b_re, b_part, b_g}) cut.add(b);
+    Scratch mem(cut.total, s);
+    cut.base = static_cast<char*>(mem.p);
+    void* x16 = cut.take<void>(b_x);
+    int* rexp = cut.take<int>(b_re);
+    float* part = cut.take<float>(b_part);
+    float* gpart = cut.take<float>(b_g);
+    if (r > 0) check_launch(q4::launch_rows_proj(dy, bf16, w->lora_b, gpart, gsplits, M, N, r, s), "dY B^T");
+    q4::CastArgs ca{};
+    ca.x = dy; ca.out = x16; ca.row_exp = rexp;
+    ca.M = M; ca.cols = N; ca.ld = ld;
+    check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "dY planes");
+    encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(ld),
+              static_cast<uint64_t>(planes) * M, static_cast<uint64_t>(ld) * 2, 64,
+              static_cast<uint32_t>(q4::few_rows_padded(M)), CU_TENSOR_MAP_SWIZZLE_128B);
+    weights.encode(g, true);
+    g.w_exp = w->col_exp + N;
+    g.row_exp = rexp;
+    g.out = part;
+    g.sm_count = sms;
+    g.status = c.status;
+    check_launch(q4::launch_few_rows(g, planes, q4::kGgF32, s), "dY W^T");
+    check_launch(q4::launch_rows_finish(part, g.splits, static_cast<long long>(M) * K, gpart, gsplits, w->lora_a, r,
+                                        r > 0 ? w->alpha / static_cast<float>(r) : 0.0f, dx, bf16, M, K, s),
+                 "dX");
+}
+
 void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
+    if (M > kRowsKernelMax && M <= q4::kFewRows) {
+        run_input_gradient_few(w, dy, dx, bf16, M, s);
+        return;
+    }
     if (M <= kRowsKernelMax) {
         run_input_gradient_rows(w, dy, dx, bf16, M, s);
         return;
@@ -1549,6 +1606,81 @@ void run_cross_entropy_rows(spaceslug_q4_weights* w, const void* x, bool bf16, c
                  "dX");
 }
 
+// Loss and gradient of up to kFewRows rows: the steps of run_cross_entropy with
+// the products of q4_few_rows.cu, whose tiles are 128 columns.
+void run_cross_entropy_few(spaceslug_q4_weights* w, const void* x, bool bf16, const long long* targets,
+                           const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
+    DeviceCtx& c = ctx_for(w->device);
+    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, sms = few_rows_sms(w, c), rp = q4::few_rows_padded(M);
+    const int tiles = (N + 127) / 128, ktiles = (K + 127) / 128;
+    const long long ld_p = static_cast<long long>(tiles) * 128;
+    const int splits =
+        dx ? grad_splits(ktiles, tiles, kFewRowsCost * planes, sms, static_cast<long long>(M) * K, true) : 0;
+    const TrainWeights weights(w, bf16, true, M, s);
+    const size_t b_x = static_cast<size_t>(planes) * M * K * 2, b_row = static_cast<size_t>(rp) * 4;
+    const size_t b_t = static_cast<size_t>(tiles) * rp * 4, b_prob = dx ? static_cast<size_t>(planes) * M * ld_p * 2 : 0;
+    const size_t b_part = static_cast<size_t>(splits) * M * K * 4;
+    Carve cut;
+    for (size_t b : {b_x, b_row, b_t, 4 * b_t, b_row, b_row, b_prob, b_part}) cut.add(b);
+    Scratch mem(cut.total, s);
+    cut.base = static_cast<char*>(mem.p);
+    void* x16 = cut.take<void>(b_x);
+    int* rexp = cut.take<int>(b_row);
+    float* smax = cut.take<float>(b_t);
+    float* ssum = cut.take<float>(4 * b_t);
+    float* zt = cut.take<float>(b_row);
+    float* total = cut.take<float>(b_row);
+    void* prob = cut.take<void>(b_prob);
+    float* part = cut.take<float>(b_part);
+    q4::CastArgs ca{};
+    ca.x = x; ca.out = x16; ca.row_exp = rexp;
+    ca.M = M; ca.cols = K; ca.ld = K;
+    ca.by_word = 1;
+    ca.targets = targets; ca.packed = w->packed; ca.scales = w->scales; ca.zt = zt; ca.N = N;
+    check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "X planes");
+    q4::FewRowsArgs g{};
+    g.M = M; g.N = N; g.K = K;
+    g.tiles = tiles;
+    g.splits = 1;
+    g.blocks = ktiles;
+    g.chunk = bf16 ? 4 : 2;  // truncated sums of 512 or 256 terms
+    g.chunks = (g.blocks + g.chunk - 1) / g.chunk;
+    g.w_exp = w->col_exp + N;
+    g.row_exp = rexp;
+    g.targets = targets;
+    g.smax = smax; g.ssum = ssum;
+    g.ld_stat = rp;
+    g.out = prob;
+    g.ld_out = ld_p;
+    g.sm_count = sms;
+    g.status = c.status;
+    weights.encode(g, false);
+    encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(K),
+              static_cast<uint64_t>(planes) * M, static_cast<uint64_t>(K) * 2, 64, static_cast<uint32_t>(rp),
+              CU_TENSOR_MAP_SWIZZLE_128B);
+    check_launch(q4::launch_few_rows(g, planes, dx ? q4::kGgProb : q4::kGgLoss, s), "logits");
+    check_launch(q4::launch_loss_rows(smax, ssum, zt, targets, total, loss, lse, M, N, tiles, 4, rp, s), "loss rows");
+    if (!dx) return;
+    q4::FewRowsArgs d = g;
+    d.tiles = ktiles;
+    d.splits = splits;
+    d.blocks = tiles;
+    d.chunk = 1;  // one 128-column tile of the logits: one factor per row
+    d.chunks = tiles;
+    d.row_exp = nullptr;
+    d.fixed_exp = 14;  // p~ carries 2^14
+    d.coef = smax;
+    d.out = part;
+    weights.encode(d, true);
+    encode_2d(&d.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob, static_cast<uint64_t>(ld_p),
+              static_cast<uint64_t>(planes) * M, static_cast<uint64_t>(ld_p) * 2, 64, static_cast<uint32_t>(rp),
+              CU_TENSOR_MAP_SWIZZLE_128B);
+    check_launch(q4::launch_few_rows(d, planes, q4::kGgF32, s), "P W^T");
+    check_launch(q4::launch_loss_dx(part, splits, M, total, loss, targets, row_scale, w->packed, w->scales, dx, bf16, M, N, K,
+                                    s),
+                 "dX");
+}
+
 // Loss and gradient.  Per block of rows: the f16 planes of X; the logits'
 // product, whose epilogue leaves each 256-column tile's max, sum and (for the
 // gradient) exp(z - max) as f16 planes; the rows' lse, loss and tile factors;
@@ -1560,6 +1692,10 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     const long long* targets = reinterpret_cast<const long long*>(targets64);
     if (M <= kRowsKernelMax) {
         run_cross_entropy_rows(w, x, bf16, targets, row_scale, loss, lse, dx, M, s);
+        return;
+    }
+    if (M <= q4::kFewRows) {
+        run_cross_entropy_few(w, x, bf16, targets, row_scale, loss, lse, dx, M, s);
         return;
     }
     DeviceCtx& c = ctx_for(w->device);
@@ -1635,7 +1771,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
             g.tm_out = g.tm_a;  // not read
         check_launch(q4::launch_grad_gemm(g, planes, dx ? q4::kGgProb : q4::kGgLoss, weights.from_planes, s), "logits");
         check_launch(q4::launch_loss_rows(smax, ssum, zt, targets + m0, total, loss + m0, lse ? lse + m0 : nullptr, mc, N,
-                                          tiles, mp, s),
+                                          tiles, 2, mp, s),
                      "loss rows");
         if (!dx) continue;
         q4::GradGemmArgs d = g;
