@@ -94,17 +94,6 @@ __device__ __forceinline__ L16Unit l16_unit(const Lora16Pass& P, int u) {
     return w;
 }
 
-// kind::f16 with A in tensor memory (two 16-bit elements per column).
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 __device__ __forceinline__ float step_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // Two codes (bytes with the sign bit flipped, i.e. code + 128) times their steps as a bf16 pair; exact.

@@ -8,22 +8,24 @@
 // q4_grad_gemm.cu, but with the operands' roles exchanged: the 128 lanes of the
 // accumulator are weights (128 n of the logits, 128 k of the transposed
 // product) and the rows are the MMA's N, so that a few rows cost a few columns
-// instead of a 256-row tile of zeros.  The operand image of a block of 128 n x
-// 128 k, two times 128 rows (n) of 64 k, 128-byte swizzled, is K-major for the
-// logits and MN-major for the transposed product, which contracts over n.
+// instead of a 256-row tile of zeros.  The rows' planes are stacked in N, [hi
+// rows; lo rows], so that both meet the weights' hi plane in one MMA.
 //
-// What bounds it then is the weights' way through shared memory: per block and
-// plane 32 KB written by the dequant warps and 32 KB read by the MMAs, 512
-// cycles at 128 bytes a cycle (two planes: 1024), against 10 KB from HBM.  The
-// rows' planes are stacked in N, [hi rows; lo rows], so that hi and lo of the
-// rows meet the weights' hi plane in one MMA.
+// The weights are then the MMA's A operand.  For the logits a thread's weights
+// are one lane's (its n) and go from registers to tensor memory; the transposed
+// product contracts over n and takes them from shared memory, MN-major (128 n x
+// 128 k as two images of 128 rows of 128 bytes, 128-byte swizzled).  There
+// shared memory is what bounds it: per block of 128 n x 128 k and plane of the
+// weights 32 KB written and 32 KB read at 128 bytes a cycle.  (With the logits'
+// operand there too, 32 x 2048 x 50000 fp32 logits took 43 us.)
 //
 // Roles (28 warps): warp 0 loads the rows' planes, warp 2 packed words and
 // scales (TMA), warp 1 issues the MMAs (M = 128, K = 16), warps 4-11 hold the
 // sums (thread = lane of the accumulator, half of the rows each) and run the
-// epilogue, warps 12-27 dequantise: two groups of eight take the blocks in
-// turn.  Numbers of slots are even, so a slot belongs to one group, which sees
-// every phase of its barriers.  Every wait is bounded (status word + abort flag).
+// epilogue, warps 12-27 dequantise: two groups of eight take the blocks of 128 x
+// 128 in turn.  The numbers of slots are even, so a slot belongs to one group,
+// which sees every phase of its barriers.  Every wait is bounded (status word +
+// abort flag).
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -39,28 +41,35 @@ namespace q4 {
 
 namespace {
 
-constexpr int kFrPlane = 128 * 128 * 2;  // one f16 plane of a block: [2 halves of k][128 n][64 k]
+constexpr int kFrPlane = 128 * 128 * 2;  // one f16 plane of a block in shared memory: [2 halves of k][128 n][64 k]
 constexpr int kFrEpiWarp0 = 4, kFrEpiWarps = 8, kFrDeqWarp0 = 12, kFrGroupWarps = 8;
 constexpr int kFrThreads = 32 * (kFrDeqWarp0 + 2 * kFrGroupWarps);
 
 // RP: padded rows; PA, PB: planes of the rows and of the weights.
-template <int RP, int PA, int PB>
+template <bool TR, int RP, int PA, int PB>
 struct FrCfg {
-    static constexpr int kHalf = PA * RP * 128;  // 64 of the contraction: PA * RP rows of 128 bytes
-    static constexpr int kStageBytes = PB * kFrPlane + 2 * kHalf;
-    static constexpr int kStages = PB == 1 ? 4 : 2;
-    static constexpr int kLimit = 232448 - 1024 - 4096;  // slack of the 1024-byte alignment; barriers and statistics
-    static constexpr int kRaw = kStages * kStageBytes + 4 * kGgRawBytes <= kLimit ? 4 : 2;
-    static_assert(kStages % 2 == 0 && kRaw % 2 == 0, "a slot belongs to one dequant group");
-    static constexpr int kRawOff = kStages * kStageBytes;
+    static constexpr int kHalf = PA * RP * 128;  // PA * RP rows of 64 of the contraction
+    static constexpr int kXBytes = 2 * kHalf;
+    static constexpr int kAcc = 2 * PA * RP;       // tensor memory columns of the two accumulators
+    // Slots of the weights' blocks: 128 KB of shared memory, or two of PB * 64 columns of tensor memory.
+    static constexpr int kWBytes = TR ? PB * kFrPlane : 0;
+    static constexpr int kW = TR ? 131072 / kWBytes : 2;
+    static constexpr int kRaw = !TR ? 8 : kXBytes > 16384 ? 2 : 4;
+    // The rows get what 223 KB leave: their loads have the latency of L2 to hide.
+    static constexpr int kX0 = (228352 - kW * kWBytes - kRaw * kGgRawBytes) / kXBytes, kX = kX0 < 8 ? kX0 : 8;
+    static_assert(kW % 2 == 0 && kRaw % 2 == 0 && kX >= 2, "a slot of weights belongs to one dequant group");
+    static constexpr int kXOff = kW * kWBytes;
+    static constexpr int kRawOff = kXOff + kX * kXBytes;
     static constexpr int kRedOff = kRawOff + kRaw * kGgRawBytes;  // [2 buffers][4 quarters][RP] floats
     static constexpr int kBarOff = kRedOff + 2 * 4 * RP * 4;
-    // full_x[S], full_w[S], empty[S], full_r[R], empty_r[R], acc_full[2], acc_empty[2], xch[2], done
-    static constexpr int kNumBars = 3 * kStages + 2 * kRaw + 7;
+    // full_x[X], empty_x[X], full_w[W], empty_w[W], full_r[R], empty_r[R], acc_full[2], acc_empty[2], xch[2], done
+    static constexpr int kNumBars = 2 * (kX + kW + kRaw) + 7;
     static constexpr int kMiscOff = kBarOff + kNumBars * 8;
     static constexpr int kSmem = kMiscOff + 16 + 1024;
     static_assert(kSmem <= 232448, "shared memory budget");
-    static constexpr uint32_t kTmemCols = 2 * PA * RP;  // 64, 128 or 256: two accumulators
+    static constexpr int kTmemUsed = kAcc + (TR ? 0 : kW * PB * 64);
+    static constexpr uint32_t kTmemCols = kTmemUsed <= 64 ? 64 : kTmemUsed <= 128 ? 128 : kTmemUsed <= 256 ? 256 : 512;
+    static_assert(kTmemUsed <= 512, "tensor memory");
 };
 
 struct FrUnit {
@@ -103,21 +112,24 @@ __device__ __forceinline__ float fr_reduce(const float (&v)[V], int lane) {
 
 template <bool TR, int RP, int PA, int PB, int EPI>
 __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_constant__ FewRowsArgs P) {
-    using C = FrCfg<RP, PA, PB>;
-    constexpr int ST = C::kStages, R = C::kRaw, NC = PA * RP;
+    using C = FrCfg<TR, RP, PA, PB>;
+    constexpr int SX = C::kX, SW = C::kW, R = C::kRaw, NC = PA * RP;
+    static_assert(TR || PB == 2, "the logits take hi and lo of the weights");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_base = smem_u32(smem_raw), base = (raw_base + 1023u) & ~1023u;
     uint8_t* smem = smem_raw + (base - raw_base);
     const uint32_t bar = base + C::kBarOff;
     auto full_x = [&](int s) { return bar + 8u * s; };
-    auto full_w = [&](int s) { return bar + 8u * (ST + s); };
-    auto empty = [&](int s) { return bar + 8u * (2 * ST + s); };
-    auto full_r = [&](int r) { return bar + 8u * (3 * ST + r); };
-    auto empty_r = [&](int r) { return bar + 8u * (3 * ST + R + r); };
-    auto acc_full = [&](int b) { return bar + 8u * (3 * ST + 2 * R + b); };
-    auto acc_empty = [&](int b) { return bar + 8u * (3 * ST + 2 * R + 2 + b); };
-    auto xch_bar = [&](int h) { return bar + 8u * (3 * ST + 2 * R + 4 + h); };
-    const uint32_t done_bar = bar + 8u * (3 * ST + 2 * R + 6);
+    auto empty_x = [&](int s) { return bar + 8u * (SX + s); };
+    auto full_w = [&](int s) { return bar + 8u * (2 * SX + s); };
+    auto empty_w = [&](int s) { return bar + 8u * (2 * SX + SW + s); };
+    auto full_r = [&](int r) { return bar + 8u * (2 * SX + 2 * SW + r); };
+    auto empty_r = [&](int r) { return bar + 8u * (2 * SX + 2 * SW + R + r); };
+    const uint32_t bar2 = bar + 8u * (2 * (SX + SW + R));
+    auto acc_full = [&](int b) { return bar2 + 8u * b; };
+    auto acc_empty = [&](int b) { return bar2 + 8u * (2 + b); };
+    auto xch_bar = [&](int h) { return bar2 + 8u * (4 + h); };
+    const uint32_t done_bar = bar2 + 8u * 6;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kMiscOff);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kMiscOff + 4);
 
@@ -125,10 +137,13 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
     const int units = P.tiles * P.splits;
     int* status = P.status;
     if (tid == 0) {
-        for (int s = 0; s < ST; ++s) {
+        for (int s = 0; s < SX; ++s) {
             mbar_init(full_x(s), 1);
+            mbar_init(empty_x(s), 1);
+        }
+        for (int s = 0; s < SW; ++s) {
             mbar_init(full_w(s), kFrGroupWarps);
-            mbar_init(empty(s), 1);
+            mbar_init(empty_w(s), 1);
         }
         for (int r = 0; r < R; ++r) {
             mbar_init(full_r(r), 1);
@@ -166,13 +181,13 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
                 const FrUnit w = fr_unit(P, u);
                 const int b1 = min(w.c1 * P.chunk, P.blocks);
                 for (int b = w.c0 * P.chunk; b < b1; ++b, ++q) {
-                    const int s = q % ST;
-                    if (!gg_wait(empty(s), ((q / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutProducer)) {
+                    const int s = q % SX;
+                    if (!gg_wait(empty_x(s), ((q / SX) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutProducer)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t dst = base + s * C::kStageBytes + PB * kFrPlane;
-                    mbar_arrive_expect_tx(full_x(s), 2 * C::kHalf);
+                    const uint32_t dst = base + C::kXOff + s * C::kXBytes;
+                    mbar_arrive_expect_tx(full_x(s), C::kXBytes);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -181,7 +196,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
                 }
             }
             if (*abort_flag)
-                for (int j = q > ST ? q - ST : 0; j < q; ++j) mbar_drain(full_x(j % ST), (j / ST) & 1u);
+                for (int j = q > SX ? q - SX : 0; j < q; ++j) mbar_drain(full_x(j % SX), (j / SX) & 1u);
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -229,28 +244,33 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
                     const int b1 = min((c + 1) * P.chunk, P.blocks);
                     uint32_t acc = 0;
                     for (int i = c * P.chunk; i < b1; ++i, ++q) {
-                        const int s = q % ST;
-                        const uint32_t ph = (q / ST) & 1u;
-                        if (!gg_wait(full_x(s), ph, abort_flag, status, kStatusTimeoutMma) ||
-                            !gg_wait(full_w(s), ph, abort_flag, status, kStatusTimeoutMma)) {
+                        const int x = q % SX, s = q % SW;
+                        if (!gg_wait(full_x(x), (q / SX) & 1u, abort_flag, status, kStatusTimeoutMma) ||
+                            !gg_wait(full_w(s), (q / SW) & 1u, abort_flag, status, kStatusTimeoutMma)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after_sync();
-                        const uint32_t at = base + s * C::kStageBytes, bt = at + PB * kFrPlane;
+                        [[maybe_unused]] const uint32_t at = base + s * C::kWBytes;
+                        const uint32_t bt = base + C::kXOff + x * C::kXBytes;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const uint64_t bd = umma_desc_k_sw128(bt + (j >> 2) * C::kHalf + (j & 3) * 32);
-                            auto wd = [&](int p) {
-                                const uint32_t a = at + p * kFrPlane;
-                                return TR ? gg_desc_mn_sw128(a + j * 2048, kFrPlane / 2)
-                                          : umma_desc_k_sw128(a + (j >> 2) * (kFrPlane / 2) + (j & 3) * 32);
-                            };
-                            umma_f16_ss(dacc, wd(0), bd, idesc, acc);
+                            if constexpr (TR) {
+                                umma_f16_ss(dacc, gg_desc_mn_sw128(at + j * 2048, kFrPlane / 2), bd, idesc, acc);
+                                if constexpr (PB == 2)
+                                    umma_f16_ss(dacc, gg_desc_mn_sw128(at + kFrPlane + j * 2048, kFrPlane / 2), bd, idesc_lo,
+                                                1u);
+                            } else {
+                                // a scale group (32 k) is 16 columns of hi, then 16 of lo
+                                const uint32_t a = tmem + static_cast<uint32_t>(C::kAcc + s * 128 + (j >> 1) * 32 + (j & 1) * 8);
+                                umma_f16_ts(dacc, a, bd, idesc, acc);
+                                umma_f16_ts(dacc, a + 16, bd, idesc_lo, 1u);
+                            }
                             acc = 1;
-                            if constexpr (PB == 2) umma_f16_ss(dacc, wd(1), bd, idesc_lo, 1u);
                         }
-                        umma_commit(empty(s));
+                        umma_commit(empty_w(s));
+                        umma_commit(empty_x(x));
                     }
                     if (ok) umma_commit(acc_full(b));
                 }
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
         __syncwarp();
     } else if (warp >= kFrDeqWarp0) {
         // ------------------------------------------------------- dequant --
-        // Thread t of a group: n = t % 128 of the block, 64 k t / 128: two scale groups of one n.
+        // Thread t of a group: n = t % 128 of the block, 64 k t / 128: two scale groups (32 k) of one n.
         const int group = (warp - kFrDeqWarp0) / kFrGroupWarps;
         const int t = tid - (kFrDeqWarp0 + group * kFrGroupWarps) * 32, row = t & 127, kh = t >> 7;
         const float cs = exp2i(*P.w_exp);
@@ -269,7 +289,6 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
         const uint32_t at0 = static_cast<uint32_t>(row * 64 + (((2 * kh) ^ rkey) << 4));
         const uint32_t at1 = static_cast<uint32_t>(row * 64 + (((2 * kh + 1) ^ rkey) << 4));
         const uint32_t ats = static_cast<uint32_t>(kGgRawWords + row * 16 + kh * 8);
-        const uint32_t out_row = static_cast<uint32_t>(kh * (kFrPlane / 2) + row * 128);
         int q = 0;
         bool ok = true;
         for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -277,7 +296,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
             const int b1 = min(w.c1 * P.chunk, P.blocks);
             for (int b = w.c0 * P.chunk; b < b1; ++b, ++q) {
                 if ((q & 1) != group) continue;
-                const int r = q % R, s = q % ST;
+                const int r = q % R, s = q % SW;
                 if (!gg_wait_warp(full_r(r), (q / R) & 1u, abort_flag, status, kStatusTimeoutDequant)) {
                     ok = false;
                     break;
@@ -288,26 +307,45 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
                 const float2 sc = *reinterpret_cast<const float2*>(raw + ats);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(empty_r(r));
-                if (!gg_wait_warp(empty(s), ((q / ST) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
+                if (!gg_wait_warp(empty_w(s), ((q / SW) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutDequant)) {
                     ok = false;
                     break;
                 }
-                uint8_t* dst = smem + s * C::kStageBytes + out_row;
+                if constexpr (!TR) tc_fence_after_sync();  // the MMAs that last read this slot have completed
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     __half2 s_hi, s_lo;
                     split_scale_f16((h == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
                     const uint32_t ww[4] = {words[h].x, words[h].y, words[h].z, words[h].w};
+                    if constexpr (TR) {
+                        uint8_t* dst = smem + s * C::kWBytes + kh * (kFrPlane / 2) + row * 128;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 hi, lo;
-                        gg_dequant<PB, false>(ww[i], s_hi, s_lo, hi, lo);
-                        const int o = ((4 * h + i) ^ (row & 7)) << 4;
-                        *reinterpret_cast<uint4*>(dst + o) = hi;
-                        if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kFrPlane + o) = lo;
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 hi, lo;
+                            gg_dequant<PB, false>(ww[i], s_hi, s_lo, hi, lo);
+                            const int o = ((4 * h + i) ^ (row & 7)) << 4;
+                            *reinterpret_cast<uint4*>(dst + o) = hi;
+                            if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kFrPlane + o) = lo;
+                        }
+                    } else {
+                        uint32_t v[32];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 hi, lo;
+                            gg_dequant<2, false>(ww[i], s_hi, s_lo, hi, lo);
+                            v[4 * i] = hi.x; v[4 * i + 1] = hi.y; v[4 * i + 2] = hi.z; v[4 * i + 3] = hi.w;
+                            v[16 + 4 * i] = lo.x; v[17 + 4 * i] = lo.y; v[18 + 4 * i] = lo.z; v[19 + 4 * i] = lo.w;
+                        }
+                        tmem_st32(tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) +
+                                      static_cast<uint32_t>(C::kAcc + s * 128 + (2 * kh + h) * 32), v);
                     }
                 }
-                fence_proxy_async_smem();
+                if constexpr (TR) {
+                    fence_proxy_async_smem();
+                } else {
+                    tmem_st_wait();
+                    tc_fence_before_sync();
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(full_w(s));
             }
@@ -427,7 +465,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
 
 template <bool TR, int RP, int PA, int PB, int EPI>
 int fr_launch(const FewRowsArgs& a, cudaStream_t stream) {
-    using C = FrCfg<RP, PA, PB>;
+    using C = FrCfg<TR, RP, PA, PB>;
     auto kern = few_rows_kernel<TR, RP, PA, PB, EPI>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
