@@ -685,7 +685,10 @@ int gg_launch_pdl(void (*kern)(Params...), unsigned grid, unsigned threads, cuda
 }
 __device__ __forceinline__ float gg_in(const float* p) { return *p; }
 __device__ __forceinline__ float gg_in(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-constexpr int kCastThreads = 128;  // per row: 2048 x 11008 bf16 takes 19 us, with 256 23 and with 512 30 (block-wide steps)
+// Threads per row of the cast: 2048 x 11008 bf16 takes 19 us with 128, 23 with
+// 256 and 30 with 512 (block-wide steps); up to kCastFew rows, a block per SM or
+// less, 512 (fp32, 32 x 11008: 6.8 us against 9.2; 128 x 11008: 5.6 against 8.1).
+constexpr int kCastThreads = 128, kCastThreadsFew = 512, kCastFew = 128;
 // Eight columns as loaded: a batch of them is in flight before the first is used.
 template <typename T>
 struct GgRaw8;
@@ -716,27 +719,27 @@ struct GgRaw8<__nv_bfloat16> {
         }
     }
 };
-// f(p, v) for this thread's pieces of 8 columns p = thread, thread + kCastThreads, ...
-template <bool VEC, typename T, typename F>
+// f(p, v) for this thread's pieces of 8 columns p = thread, thread + THREADS, ...
+template <int THREADS, bool VEC, typename T, typename F>
 __device__ __forceinline__ void gg_row(const T* row, int cols, F&& f) {
     const int pieces = (cols + 7) / 8;
     if constexpr (VEC) {
         using R = GgRaw8<T>;
-        for (int p0 = threadIdx.x; p0 < pieces; p0 += kCastThreads * R::kBatch) {
+        for (int p0 = threadIdx.x; p0 < pieces; p0 += THREADS * R::kBatch) {
             R q[R::kBatch];
 #pragma unroll
             for (int u = 0; u < R::kBatch; ++u)
-                if (p0 + kCastThreads * u < pieces) q[u].load(row + (p0 + kCastThreads * u) * 8);
+                if (p0 + THREADS * u < pieces) q[u].load(row + (p0 + THREADS * u) * 8);
 #pragma unroll
             for (int u = 0; u < R::kBatch; ++u)
-                if (p0 + kCastThreads * u < pieces) {
+                if (p0 + THREADS * u < pieces) {
                     float v[8];
                     q[u].values(v);
-                    f(p0 + kCastThreads * u, v);
+                    f(p0 + THREADS * u, v);
                 }
         }
     } else {
-        for (int p = threadIdx.x; p < pieces; p += kCastThreads) {
+        for (int p = threadIdx.x; p < pieces; p += THREADS) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = p * 8 + i < cols ? gg_in(row + p * 8 + i) : 0.0f;
@@ -756,9 +759,9 @@ __device__ __forceinline__ void gg_row(const T* row, int cols, F&& f) {
 // The row is read twice, the second time from L1 / L2: keeping it in registers
 // (48 floats a thread) halves the blocks per SM and measured slower (24 against
 // 16 us at 4096 x 4096 bf16).
-template <typename T, int PA, bool VEC>
-__global__ void __launch_bounds__(kCastThreads) cast_planes_kernel(const CastArgs A) {
-    __shared__ float red[kCastThreads / 32];
+template <typename T, int PA, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS) cast_planes_kernel(const CastArgs A) {
+    __shared__ float red[THREADS / 32];
     __shared__ float gs[64];
     pdl_launch_dependents();
     pdl_wait();
@@ -771,7 +774,7 @@ __global__ void __launch_bounds__(kCastThreads) cast_planes_kernel(const CastArg
     float top = 0.0f, dot = 0.0f;
     const long long tgt = targets != nullptr ? targets[m] : -1;
     const bool want_dot = tgt >= 0 && tgt < A.N;
-    gg_row<VEC>(row, A.cols, [&](int p, const float (&v)[8]) {
+    gg_row<THREADS, VEC>(row, A.cols, [&](int p, const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
         if (want_dot) {  // the target's logit, w = v s in fp32
@@ -796,7 +799,7 @@ __global__ void __launch_bounds__(kCastThreads) cast_planes_kernel(const CastArg
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
-    for (int i = 0; i < kCastThreads / 32; ++i) top = fmaxf(top, red[i]);
+    for (int i = 0; i < THREADS / 32; ++i) top = fmaxf(top, red[i]);
     int e = 0;
     if (top > 0.0f && isfinite(top)) {
         int e2;
@@ -812,7 +815,7 @@ __global__ void __launch_bounds__(kCastThreads) cast_planes_kernel(const CastArg
         __syncthreads();
         if (threadIdx.x == 0) {
             float z = 0.0f;
-            for (int i = 0; i < kCastThreads / 32; ++i) z += red[i];
+            for (int i = 0; i < THREADS / 32; ++i) z += red[i];
             A.zt[m] = z;
         }
     }
@@ -842,9 +845,9 @@ __global__ void __launch_bounds__(kCastThreads) cast_planes_kernel(const CastArg
         if constexpr (PA == 2)
             *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
     };
-    gg_row<VEC>(row, A.cols, put);
+    gg_row<THREADS, VEC>(row, A.cols, put);
     const int end = static_cast<int>(A.ld / 8), gp = A.rank > 0 ? end - 8 : end;
-    for (int p = pieces + threadIdx.x; p < end; p += kCastThreads) {
+    for (int p = pieces + threadIdx.x; p < end; p += THREADS) {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = p >= gp ? gs[(p - gp) * 8 + i] : 0.0f;
@@ -909,35 +912,43 @@ __global__ void __launch_bounds__(1024) min_exp_kernel(const int* __restrict__ c
 // logit: row max M2 with the target, S = sum over tiles of sums * 2^(tile max -
 // M2) + 2^(target - M2), the factor 2^(tile max - M2) of every tile in place of
 // its max, lse and loss.  The loss of a likely target is log1p(others /
-// target), which does not cancel.  32 rows x 32 lanes per block.
+// target), which does not cancel.  ROWS rows x 1024 / ROWS threads per block: 4
+// rows of few, whose tiles a few blocks would walk in turn, 32 of many, for
+// whole lines (32 rows of 391 tiles of 128 columns: 8.5 us with 4, 21 with 32;
+// 50000 columns in tiles of 256: 1024 rows 7.7 and 12.5 us, 2048 rows 12.6 and
+// 12.7, 4096 rows 19.8 and 12.7).
+constexpr int kLossRowsFew = 1024;
+template <int ROWS>
 __global__ void __launch_bounds__(1024) loss_rows_kernel(float* smax, const float* ssum, const float* zt,
                                                          const long long* targets,
                                                          float* __restrict__ total, float* __restrict__ loss,
                                                          float* __restrict__ lse, int M, int N, int tiles, int parts,
                                                          long long ld) {
-    __shared__ float part[32][33];
+    constexpr int kParts = 1024 / ROWS;
+    __shared__ float red[32][ROWS];
     pdl_launch_dependents();
     pdl_wait();
     smax = after_wait(smax);
     ssum = after_wait(ssum);
     zt = after_wait(zt);
     targets = after_wait(targets);
-    const int r = threadIdx.x & 31, p = threadIdx.x >> 5;
-    const int row = blockIdx.x * 32 + r;
+    const int r = threadIdx.x % ROWS, p = threadIdx.x / ROWS, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x * ROWS + r;
     const bool in = row < M;
     const long long t = in ? targets[row] : -1;
     const float t2 = t >= 0 && t < N ? zt[row] * 1.4426950408889634f : -INFINITY;
     float top = t2;
 #pragma unroll 4
-    for (int i = p; i < tiles && in; i += 32) top = fmaxf(top, smax[static_cast<size_t>(i) * ld + row]);
-    part[p][r] = top;
+    for (int i = p; i < tiles && in; i += kParts) top = fmaxf(top, smax[static_cast<size_t>(i) * ld + row]);
+    for (int o = 16; o >= ROWS; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    red[warp][r] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i][r]);
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, red[i][r]);
     __syncthreads();
     float sum = 0.0f;
 #pragma unroll 4
-    for (int i = p; i < tiles && in; i += 32) {
+    for (int i = p; i < tiles && in; i += kParts) {
         float* at = smax + static_cast<size_t>(i) * ld + row;
         const float f = exp2f(*at - top);
         const float* st = ssum + static_cast<size_t>(parts * i) * ld + row;
@@ -946,10 +957,11 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(float* smax, const floa
         sum += f * all;
         *at = f;
     }
-    part[p][r] = sum;
+    for (int o = 16; o >= ROWS; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    red[warp][r] = sum;
     __syncthreads();
     if (p != 0 || !in) return;
-    for (int i = 1; i < 32; ++i) sum += part[i][r];
+    for (int i = 1; i < 32; ++i) sum += red[i][r];
     const float et = exp2f(t2 - top), all = sum + et;
     total[row] = all;
     const float l = 0.69314718055994531f * (top + log2f(all));
@@ -1097,12 +1109,20 @@ int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t st
     if (a.M < 1 || a.ld % 8 != 0 || a.ld < a.cols || a.rank > 64) return static_cast<int>(cudaErrorInvalidValue);
     const bool vec = a.cols % 8 == 0;  // rows of whole 16-byte pieces
     const unsigned grid = static_cast<unsigned>(a.M);
+    auto launch = [&](auto few, auto wide, auto one, auto two) {
+        return a.M <= kCastFew ? (vec ? gg_launch_pdl(few, grid, kCastThreadsFew, stream, a)
+                                      : gg_launch_pdl(wide, grid, kCastThreadsFew, stream, a))
+                               : (vec ? gg_launch_pdl(one, grid, kCastThreads, stream, a)
+                                      : gg_launch_pdl(two, grid, kCastThreads, stream, a));
+    };
     if (bf16)
-        return vec ? gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1, true>, grid, kCastThreads, stream, a)
-                   : gg_launch_pdl(cast_planes_kernel<__nv_bfloat16, 1, false>, grid, kCastThreads, stream, a);
+        return launch(cast_planes_kernel<__nv_bfloat16, 1, true, kCastThreadsFew>,
+                      cast_planes_kernel<__nv_bfloat16, 1, false, kCastThreadsFew>,
+                      cast_planes_kernel<__nv_bfloat16, 1, true, kCastThreads>,
+                      cast_planes_kernel<__nv_bfloat16, 1, false, kCastThreads>);
     if (planes == 2)
-        return vec ? gg_launch_pdl(cast_planes_kernel<float, 2, true>, grid, kCastThreads, stream, a)
-                   : gg_launch_pdl(cast_planes_kernel<float, 2, false>, grid, kCastThreads, stream, a);
+        return launch(cast_planes_kernel<float, 2, true, kCastThreadsFew>, cast_planes_kernel<float, 2, false, kCastThreadsFew>,
+                      cast_planes_kernel<float, 2, true, kCastThreads>, cast_planes_kernel<float, 2, false, kCastThreads>);
     return static_cast<int>(cudaErrorInvalidValue);
 }
 
@@ -1113,8 +1133,11 @@ int launch_min_exp(const int* col_exp, const float* scales, int* out, int N, int
 
 int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long long* targets, float* total,
                      float* loss, float* lse, int M, int N, int tiles, int parts, long long ld, cudaStream_t stream) {
-    return gg_launch_pdl(loss_rows_kernel, static_cast<unsigned>((M + 31) / 32), 1024, stream, smax, ssum, zt, targets,
-                         total, loss, lse, M, N, tiles, parts, ld);
+    auto launch = [&](auto kern, int rows) {
+        return gg_launch_pdl(kern, static_cast<unsigned>((M + rows - 1) / rows), 1024, stream, smax, ssum, zt, targets, total,
+                             loss, lse, M, N, tiles, parts, ld);
+    };
+    return M <= kLossRowsFew ? launch(loss_rows_kernel<4>, 4) : launch(loss_rows_kernel<32>, 32);
 }
 
 int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,

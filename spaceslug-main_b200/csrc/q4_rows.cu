@@ -1,5 +1,6 @@
-// The training operators on the frozen int4 weights for one to eight rows, on
-// the CUDA cores in fp32: products that stream the packed weights once.
+// The training operators on the frozen int4 weights for one to eight rows (up to
+// a size; see rows_kernels_pay), on the CUDA cores in fp32: products that stream
+// the packed weights once.
 //
 //   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n), and each 32 columns' max and sum of exponentials
 //   rows_loss_kernel     lse, loss and the rows' coefficients of the gradient
@@ -204,9 +205,11 @@ __global__ void __launch_bounds__(512) rows_loss_kernel(const float* smax, const
 // rows' d values of 256 n at a time sit in shared memory: d itself, or with
 // `coef` (the loss) g p = coef[1] exp2(z2 - coef[0]) and coef[2] at the target.
 // The words of eight n per thread are in flight while d is staged.
+// Registers for two blocks per SM from three rows on: held to a quarter of them,
+// four rows of 4096 x 11008 took 58 us instead of 39.
 constexpr int kWtWords = 64, kWtParts = 4, kWtThreads = kWtWords * kWtParts, kWtTile = 128, kWtBatch = 8;
 template <int MR, typename T>
-__global__ void __launch_bounds__(kWtThreads, MR <= 4 ? 4 : 2) rows_wt_kernel(const T* d, const float* coef, const long long* targets,
+__global__ void __launch_bounds__(kWtThreads, MR <= 2 ? 4 : 2) rows_wt_kernel(const T* d, const float* coef, const long long* targets,
                                                              const uint32_t* __restrict__ packed,
                                                              const float* __restrict__ scales,
                                                              float* __restrict__ partial, int N, int K) {
@@ -364,18 +367,18 @@ __global__ void __launch_bounds__(256) rows_finish_kernel(const float* partial, 
     a = after_wait(a);
     const long long row = blockIdx.y;
     const int c = threadIdx.x & 127, h = threadIdx.x >> 7, k = blockIdx.x * 128 + c;
-    if (threadIdx.x < rank) {
-        float t = 0.0f;
-#pragma unroll 8
-        for (int z = 0; z < gsplits; ++z) t += g[(static_cast<size_t>(z) * M + row) * rank + threadIdx.x];
-        gs[threadIdx.x] = scale * t;
-    }
     float v = 0.0f;
     if (k < K) {
         const float* p = partial + row * K + k;
         const int z1 = h == 0 ? (splits + 1) / 2 : splits;
 #pragma unroll 8
         for (int z = h == 0 ? 0 : (splits + 1) / 2; z < z1; ++z) v += p[z * split_floats];
+    }
+    if (threadIdx.x < rank) {
+        float t = 0.0f;
+#pragma unroll 8
+        for (int z = 0; z < gsplits; ++z) t += g[(static_cast<size_t>(z) * M + row) * rank + threadIdx.x];
+        gs[threadIdx.x] = scale * t;
     }
     if (h == 1) half[c] = v;
     __syncthreads();

@@ -1286,7 +1286,15 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 
 // Rows up to which the training products stream the weights on the CUDA cores
 // (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
-constexpr int kRowsKernelMax = 8;
+// Up to 8 rows the CUDA-core kernels of q4_rows.cu, which cost a launch less but
+// more with every row, or those of q4_few_rows.cu, by rows x weights.  Measured
+// on B200 (us, q4_rows / q4_few_rows), dX of 4 rows: 2048 x 2048 15 / 17, 4096 x
+// 4096 25 / 25 in bf16 and 25 / 29 in fp32, 4096 x 11008 39 / 37 and 39 / 43; loss
+// and dX: 4 x 1024 x 8000 31 / 34 and 31 / 36, 8 x 1024 x 8000 37 / 32 and 37 / 34,
+// 2 x 1024 x 32003 50 / 48 and 50 / 57, 8 x 1024 x 32003 72 / 48 and 74 / 59.
+bool rows_kernels_pay(int M, const spaceslug_q4_weights* w, bool bf16) {
+    return M <= 8 && static_cast<double>(M) * w->N * w->K <= (bf16 ? 64e6 : 128e6);
+}
 constexpr int kFewRowsCost = 560;  // shared-memory cycles of a block of 128 n x 128 k and plane of the weights
 constexpr long long kTrainScratch = 1ll << 30;  // bytes of operand planes and partial sums per block of rows
 
@@ -1386,7 +1394,7 @@ int grad_pairs(const spaceslug_q4_weights* w) {
     return w->sm_budget > 0 ? std::min(pairs, std::max(1, w->sm_budget / 2)) : pairs;
 }
 
-// dX = dY W^T + s (dY B^T) A^T for at most kRowsKernelMax rows.
+// dX = dY W^T + s (dY B^T) A^T for at most 8 rows.
 void run_input_gradient_rows(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
     const int splits = q4::rows_wt_splits(w->N, w->K, c.sm_count), r = w->rank;
@@ -1454,11 +1462,11 @@ void run_input_gradient_few(spaceslug_q4_weights* w, const void* dy, void* dx, b
 }
 
 void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
-    if (M > kRowsKernelMax && M <= q4::kFewRows) {
+    if (M <= q4::kFewRows) {
         run_input_gradient_few(w, dy, dx, bf16, M, s);
         return;
     }
-    if (M <= kRowsKernelMax) {
+    if (rows_kernels_pay(M, w, bf16)) {
         run_input_gradient_rows(w, dy, dx, bf16, M, s);
         return;
     }
@@ -1586,7 +1594,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     }
 }
 
-// Loss and gradient of at most kRowsKernelMax rows, their logits in scratch.
+// Loss and gradient of at most 8 rows, their logits in scratch.
 void run_cross_entropy_rows(spaceslug_q4_weights* w, const void* x, bool bf16, const long long* targets,
                             const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
@@ -1690,7 +1698,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
                        const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     static_assert(sizeof(long long) == sizeof(int64_t), "targets are int64");
     const long long* targets = reinterpret_cast<const long long*>(targets64);
-    if (M <= kRowsKernelMax) {
+    if (rows_kernels_pay(M, w, bf16)) {
         run_cross_entropy_rows(w, x, bf16, targets, row_scale, loss, lse, dx, M, s);
         return;
     }

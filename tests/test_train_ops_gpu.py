@@ -525,6 +525,89 @@ def test_two_streams_and_two_graphs_at_once(session, cuda):
     assert session.device_status(0) == 0
 
 
+# ------------------------------------------------------------------------------------------------------------ few rows --
+# Up to 64 rows have kernels of their own, with fewer than nine from a size on: the bounds above hold for them as they are.
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,rank,c0,c1", [
+    (3, 6176, 8003, 2, 0, 8003), (8, 4128, 4099, 0, 0, 4099), (9, 32, 1, 1, 0, 1), (16, 96, 129, 0, 0, 129),
+    (17, 160, 1003, 8, 0, 1003), (31, 2080, 515, 0, 0, 515), (32, 4096, 130, 16, 0, 130), (33, 1056, 4099, 64, 0, 4099),
+    (63, 288, 77, 0, 0, 77), (64, 512, 2048, 5, 96, 1999), (64, 32, 40003, 3, 0, 40003), (65, 96, 300, 0, 0, 300)])
+def test_few_rows_input_gradient(session, cuda, m, k, n, rank, c0, c1, dtype):
+    test_input_gradient(session, cuda, m, k, n, rank, c0, c1, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n", [(3, 4096, 12001), (8, 2080, 9001), (9, 32, 1), (16, 288, 129), (17, 96, 40005),
+                                   (32, 128, 128), (33, 2080, 1003), (63, 1056, 257), (64, 288, 38500), (65, 64, 130)])
+def test_few_rows_cross_entropy(session, cuda, m, k, n, dtype):
+    test_cross_entropy(session, cuda, m, k, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_few_rows_in_every_setting(session, cuda, dtype):
+    """Held to a few SMs, on two streams at once, captured and replayed: the same results; a row of NaN or an ignored one
+    changes no other row."""
+    import torch
+    m, k, n = 40, 416, 5003
+    packed, scales = _weights(k, n, 53)
+    x, dy = _randn((m, k), cuda, 5).to(_dt(dtype)), _randn((m, n), cuda, 6).to(_dt(dtype))
+    t = torch.randint(0, n, (m,), device=cuda)
+    W, ones = _w64(packed, scales, k, n, cuda), torch.ones((m,), device=cuda)
+    st = [torch.cuda.Stream(cuda) for _ in range(2)]
+    new = lambda: [torch.full((m,), float("nan"), device=cuda), torch.full((m,), float("nan"), device=cuda),
+                   torch.full((m, k), float("nan"), device=cuda, dtype=x.dtype),
+                   torch.full((m, k), float("nan"), device=cuda, dtype=x.dtype)]
+
+    def run(h, o, s, x=x, t=t):
+        h.cross_entropy(x.data_ptr(), t.data_ptr(), o[0].data_ptr(), m, lse=o[1].data_ptr(), dx=o[2].data_ptr(),
+                        dtype=dtype, stream=s.cuda_stream)
+        h.input_gradient(dy.data_ptr(), o[3].data_ptr(), m, dtype=dtype, stream=s.cuda_stream)
+
+    with session.weights(packed, scales, k, n) as h:
+        for budget in (2, 7, 0):
+            h.set_sm_budget(budget)
+            o = new()
+            torch.cuda.synchronize()
+            run(h, o, st[0])
+            torch.cuda.synchronize()
+            _check_loss(dtype, (o[0], o[1], o[2]), _loss_ref(x, W, t, ones))
+            _check_dx(o[3], dtype, dy.double() @ W.T, dy.double().abs() @ W.abs().T)
+        outs = [new(), new()]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in range(2):
+                run(h, outs[i], st[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p in outs for a, b in zip(p, o))
+        graphs = []
+        for i in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st[i]):
+                run(h, outs[i], st[i])
+            graphs.append(g)
+        for p in outs:
+            for v in p:
+                v.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for i in range(2):
+                with torch.cuda.stream(st[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for p in outs for a, b in zip(p, o))
+        del graphs
+        hurt, ht = x.clone(), t.clone()
+        hurt[3, 7], ht[5] = float("nan"), -1
+        q = new()
+        torch.cuda.synchronize()
+        run(h, q, st[0], hurt, ht)
+        torch.cuda.synchronize()
+        keep = [i for i in range(m) if i not in (3, 5)]
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(q, o))
+        assert torch.isnan(q[0][3]) and torch.isnan(q[2][3]).all() and q[0][5] == 0 and not q[2][5].any()
+    assert session.device_status(0) == 0
+
+
 # ------------------------------------------------------------------------------------------------------------ refusals --
 def test_refusals(session, cuda):
     import torch
