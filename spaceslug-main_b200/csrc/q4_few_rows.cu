@@ -14,10 +14,15 @@
 // The weights are then the MMA's A operand.  For the logits a thread's weights
 // are one lane's (its n) and go from registers to tensor memory; the transposed
 // product contracts over n and takes them from shared memory, MN-major (128 n x
-// 128 k as two images of 128 rows of 128 bytes, 128-byte swizzled).  There
-// shared memory is what bounds it: per block of 128 n x 128 k and plane of the
-// weights 32 KB written and 32 KB read at 128 bytes a cycle.  (With the logits'
-// operand there too, 32 x 2048 x 50000 fp32 logits took 43 us.)
+// 128 k as two images of 128 rows of 128 bytes, 128-byte swizzled).  With the
+// logits' operand in shared memory too, fp32 logits of 32 x 2048 x 50000 took 72
+// us instead of 62.
+//
+// What bounds it is the dequantisation beside everything else an SM issues: a
+// block of 128 n x 128 k takes about 1500 cycles (logits) or 2000 (transposed,
+// fp32), with 61% and 48% of the issue slots, a fifth of the tensor pipe and a
+// quarter of HBM's bandwidth in use.  Tried and slower: stages of half a block,
+// a second MMA warp with an accumulator per block, one lane per warp polling.
 //
 // Roles (28 warps): warp 0 loads the rows' planes, warp 2 packed words and
 // scales (TMA), warp 1 issues the MMAs (M = 128, K = 16), warps 4-11 hold the
