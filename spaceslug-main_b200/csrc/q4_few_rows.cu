@@ -234,24 +234,24 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
             // ------------------------------------------------------- MMA --
             constexpr uint32_t major = TR ? (1u << 15) : 0u;  // A: MN-major
             constexpr uint32_t idesc = umma_idesc_f16(0u, 128, NC) | major, idesc_lo = umma_idesc_f16(0u, 128, RP) | major;
-            int q = 0, cq = 0;
+            int x = 0, s = 0, b = 0;           // slots, and the parities to wait for: counted along, not divided out
+            uint32_t xp = 0, sp = 0, ap = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 const FrUnit w = fr_unit(P, u);
-                for (int c = w.c0; c < w.c1 && ok; ++c, ++cq) {
-                    const int b = cq & 1;
-                    if (!gg_wait(acc_empty(b), ((cq >> 1) & 1u) ^ 1u, abort_flag, status, kStatusTimeoutMma)) {
+                int i = w.c0 * P.chunk;
+                const int end = min(w.c1 * P.chunk, P.blocks);
+                while (i < end && ok) {
+                    if (!gg_wait(acc_empty(b), ap, abort_flag, status, kStatusTimeoutMma)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after_sync();
                     const uint32_t dacc = tmem + static_cast<uint32_t>(b * NC);
-                    const int b1 = min((c + 1) * P.chunk, P.blocks);
                     uint32_t acc = 0;
-                    for (int i = c * P.chunk; i < b1; ++i, ++q) {
-                        const int x = q % SX, s = q % SW;
-                        if (!gg_wait(full_x(x), (q / SX) & 1u, abort_flag, status, kStatusTimeoutMma) ||
-                            !gg_wait(full_w(s), (q / SW) & 1u, abort_flag, status, kStatusTimeoutMma)) {
+                    for (const int stop = min(i + P.chunk, end); i < stop; ++i) {
+                        if (!gg_wait(full_w(s), sp, abort_flag, status, kStatusTimeoutMma) ||
+                            !gg_wait(full_x(x), xp, abort_flag, status, kStatusTimeoutMma)) {
                             ok = false;
                             break;
                         }
@@ -262,22 +262,26 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
                         for (int j = 0; j < 8; ++j) {
                             const uint64_t bd = umma_desc_k_sw128(bt + (j >> 2) * C::kHalf + (j & 3) * 32);
                             if constexpr (TR) {
-                                umma_f16_ss(dacc, gg_desc_mn_sw128(at + j * 2048, kFrPlane / 2), bd, idesc, acc);
+                                umma_f16_ss(dacc, gg_desc_mn_sw128(at + j * 2048, kFrPlane / 2), bd, idesc, j > 0 ? 1u : acc);
                                 if constexpr (PB == 2)
                                     umma_f16_ss(dacc, gg_desc_mn_sw128(at + kFrPlane + j * 2048, kFrPlane / 2), bd, idesc_lo,
                                                 1u);
                             } else {
                                 // a scale group (32 k) is 16 columns of hi, then 16 of lo
                                 const uint32_t a = tmem + static_cast<uint32_t>(C::kAcc + s * 128 + (j >> 1) * 32 + (j & 1) * 8);
-                                umma_f16_ts(dacc, a, bd, idesc, acc);
+                                umma_f16_ts(dacc, a, bd, idesc, j > 0 ? 1u : acc);
                                 umma_f16_ts(dacc, a + 16, bd, idesc_lo, 1u);
                             }
-                            acc = 1;
                         }
                         umma_commit(empty_w(s));
                         umma_commit(empty_x(x));
+                        acc = 1;
+                        if (++x == SX) x = 0, xp ^= 1u;
+                        if (++s == SW) s = 0, sp ^= 1u;
                     }
                     if (ok) umma_commit(acc_full(b));
+                    b ^= 1;
+                    if (b == 0) ap ^= 1u;
                 }
             }
             umma_commit(done_bar);  // tracks every MMA issued above
