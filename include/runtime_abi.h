@@ -165,7 +165,9 @@ int spaceslug_q4_weights_get_lora(const spaceslug_q4_weights* w, float* a_out, f
  * (magnitudes above 63.5 * 2^122, which would restore as an infinity: by up to
  * one), and the restored value is exact in bf16.  A group with an infinity or a NaN comes
  * back as NaN.  Device pointers, x and codes 16-byte aligned, asynchronous on
- * `stream`, m * k <= 2^40; works in CUDA graph capture. */
+ * `stream`, m * k <= 2^40; works in CUDA graph capture.  Here and in the calls
+ * below a buffer that a call writes may not overlap another of its buffers
+ * (refused). */
 int spaceslug_act8_pack_device(const void* x, int dtype, int8_t* codes, uint8_t* exps, uint32_t m, uint32_t k,
                                void* stream);
 /* x = codes * 2^(exps - 127), the values the backward uses. */
@@ -181,7 +183,7 @@ int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_
                                             const void* dy, int dtype, uint32_t m, float* da, float* db, void* stream);
 /* dX = dY * dequant(W)^T + (alpha / rank) * (dY * B^T) * A^T [m x k] for the
  * handle's columns and adapter (if one is attached), dY [m x (col_end -
- * col_begin)], both of `dtype`, 16-byte aligned; dx must not overlap dy.  For a
+ * col_begin)], both of `dtype`, 16-byte aligned, m <= 2^24.  For a
  * column shard dX is this shard's partial sum.  fp32 at fp32-level accuracy;
  * bf16 products of f16 operands summed in fp32, rounded once. */
 int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, int dtype, uint32_t m,
@@ -195,8 +197,8 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
  * row_scale fp32 [m] (the upstream gradient of each row's loss; NULL: all 1);
  * loss fp32 [m]; lse fp32 [m] or NULL; dx or NULL (the loss alone).  A negative
  * target takes its row out: loss 0, dx 0 (lse is still written).  A target past
- * the columns gives NaN in its row's loss and dx.  dx may be x itself.  Device
- * pointers, asynchronous on `stream`; scratch from the stream-ordered pool. */
+ * the columns gives NaN in its row's loss and dx.  dx may be x itself.  m <= 2^24;
+ * device pointers, asynchronous on `stream`; scratch from the stream-ordered pool. */
 int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, int dtype, const int64_t* targets,
                                        const float* row_scale, float* loss, float* lse, void* dx, uint32_t m,
                                        void* stream);

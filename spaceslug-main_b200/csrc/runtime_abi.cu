@@ -18,6 +18,7 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <stdexcept>
@@ -1144,6 +1145,25 @@ int pointer_device(const void* p) {
     return a.device;
 }
 
+// A buffer of a call: one that it writes may share no byte with any other.
+struct Span {
+    const void* p;
+    uint64_t bytes;
+    bool written;
+};
+bool spans_clash(std::initializer_list<Span> spans) {
+    for (const Span* a = spans.begin(); a != spans.end(); ++a)
+        for (const Span* b = a + 1; b != spans.end(); ++b) {
+            if (!a->p || !b->p || (!a->written && !b->written)) continue;
+            const uintptr_t x = reinterpret_cast<uintptr_t>(a->p), y = reinterpret_cast<uintptr_t>(b->p);
+            if (x < y ? y - x < a->bytes : x - y < b->bytes) return true;
+        }
+    return false;
+}
+uint64_t dtype_bytes(int dtype) { return dtype == SPACESLUG_BF16 ? 2 : 4; }
+bool aligned_to(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+constexpr char kOverlap[] = "a buffer that the call writes overlaps another";
+
 const char* act8_error(const void* x, int dtype, const void* codes, const void* exps, uint32_t m, uint32_t k) {
     if (!x || !codes || !exps) return "null pointer";
     if (dtype != SPACESLUG_F32 && dtype != SPACESLUG_BF16) return "dtype must be SPACESLUG_F32 or SPACESLUG_BF16";
@@ -1284,8 +1304,9 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     check_launch(q4::launch_lora16_finish(f, 2, s), "lora dA / dB");
 }
 
-// Rows up to which the training products stream the weights on the CUDA cores
-// (q4_rows.cu); above, the CTA-pair tensor-core kernel (q4_grad_gemm.cu).
+// The training products' kernels: up to 64 rows q4_few_rows.cu, above the CTA
+// pairs of q4_grad_gemm.cu (64 / 128 rows: fp32 dX of 4096 x 11008 66 / 95 us,
+// fp32 loss and dX of 2048 x 50000 141 / 249 us: twice 64 rows take no less).
 // Up to 8 rows the CUDA-core kernels of q4_rows.cu, which cost a launch less but
 // more with every row, or those of q4_few_rows.cu, by rows x weights.  Measured
 // on B200 (us, q4_rows / q4_few_rows), dX of 4 rows: 2048 x 2048 15 / 17, 4096 x
@@ -2483,6 +2504,9 @@ int spaceslug_q4_weights_lora_backward(spaceslug_q4_weights* w, const float* x, 
 int spaceslug_act8_pack_device(const void* x, int dtype, int8_t* codes, uint8_t* exps, uint32_t m, uint32_t k,
                                void* stream) {
     if (const char* e = act8_error(x, dtype, codes, exps, m, k)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    const uint64_t count = static_cast<uint64_t>(m) * k;
+    if (spans_clash({{x, count * dtype_bytes(dtype), false}, {codes, count, true}, {exps, count / 32, true}}))
+        return fail(SPACESLUG_INVALID_ARGUMENT, kOverlap);
     return guarded([&] {
         DeviceGuard dev(pointer_device(x));
         check_launch(q4::launch_act8_pack(x, dtype == SPACESLUG_BF16, codes, exps,
@@ -2495,6 +2519,9 @@ int spaceslug_act8_pack_device(const void* x, int dtype, int8_t* codes, uint8_t*
 int spaceslug_act8_unpack_device(const int8_t* codes, const uint8_t* exps, void* x, int dtype, uint32_t m, uint32_t k,
                                  void* stream) {
     if (const char* e = act8_error(x, dtype, codes, exps, m, k)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    const uint64_t count = static_cast<uint64_t>(m) * k;
+    if (spans_clash({{x, count * dtype_bytes(dtype), true}, {codes, count, false}, {exps, count / 32, false}}))
+        return fail(SPACESLUG_INVALID_ARGUMENT, kOverlap);
     return guarded([&] {
         DeviceGuard dev(pointer_device(x));
         check_launch(q4::launch_act8_unpack(codes, exps, x, dtype == SPACESLUG_BF16,
@@ -2510,6 +2537,14 @@ int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_
     if (const char* e = act8_error(dy, dtype, codes, exps, m, static_cast<uint32_t>(w->K)))
         return fail(SPACESLUG_INVALID_ARGUMENT, e);
     if (w->rank == 0) return fail(SPACESLUG_INVALID_ARGUMENT, "no LoRA adapter attached");
+    if (!aligned_to(da, 4) || !aligned_to(db, 4)) return fail(SPACESLUG_INVALID_ARGUMENT, "da and db must be 4-byte aligned");
+    const uint64_t mk = static_cast<uint64_t>(m) * w->K, mn = static_cast<uint64_t>(m) * w->N;
+    if (spans_clash({{codes, mk, false},
+                     {exps, mk / 32, false},
+                     {dy, mn * dtype_bytes(dtype), false},
+                     {da, static_cast<uint64_t>(w->K) * w->rank * 4, true},
+                     {db, static_cast<uint64_t>(w->N) * w->rank * 4, true}}))
+        return fail(SPACESLUG_INVALID_ARGUMENT, kOverlap);
     return guarded([&] {
         DeviceGuard dev(w->device);
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -2525,6 +2560,9 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
                                         void* stream) {
     if (!w || !dy || !dx) return fail(SPACESLUG_INVALID_ARGUMENT, "null pointer");
     if (const char* e = rows_error(dy, dx, dtype, m)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
+    if (spans_clash({{dy, static_cast<uint64_t>(m) * w->N * dtype_bytes(dtype), false},
+                     {dx, static_cast<uint64_t>(m) * w->K * dtype_bytes(dtype), true}}))
+        return fail(SPACESLUG_INVALID_ARGUMENT, kOverlap);
     return guarded([&] {
         DeviceGuard dev(w->device);
         run_input_gradient(w, dy, dx, dtype == SPACESLUG_BF16, static_cast<int>(m), static_cast<cudaStream_t>(stream));
@@ -2538,6 +2576,17 @@ int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, i
     if (!w || !x || !targets || !loss) return fail(SPACESLUG_INVALID_ARGUMENT, "null pointer");
     if (const char* e = rows_error(x, dx, dtype, m)) return fail(SPACESLUG_INVALID_ARGUMENT, e);
     if (w->rank != 0) return fail(SPACESLUG_INVALID_ARGUMENT, "cross entropy takes a handle without an adapter");
+    if (!aligned_to(targets, 8) || !aligned_to(row_scale, 4) || !aligned_to(loss, 4) || !aligned_to(lse, 4))
+        return fail(SPACESLUG_INVALID_ARGUMENT, "targets must be 8-byte, row_scale, loss and lse 4-byte aligned");
+    const uint64_t rows = static_cast<uint64_t>(m) * w->K * dtype_bytes(dtype), m4 = static_cast<uint64_t>(m) * 4;
+    if (spans_clash({{dx == x ? nullptr : x, rows, false},  // dx may be x itself
+                     {targets, 2 * m4, false},
+                     {row_scale, m4, false},
+                     {loss, m4, true},
+                     {lse, m4, true},
+                     {dx, rows, true}}) ||
+        (dx == x && spans_clash({{x, rows, false}, {loss, m4, true}, {lse, m4, true}})))
+        return fail(SPACESLUG_INVALID_ARGUMENT, kOverlap);
     return guarded([&] {
         DeviceGuard dev(w->device);
         run_cross_entropy(w, x, dtype == SPACESLUG_BF16, targets, row_scale, loss, lse, dx, static_cast<int>(m),

@@ -20,6 +20,17 @@ def test_act8_refuses(session, name, x, codes, exps, dtype, m, k):
     assert session._native().spaceslug_last_error()
 
 
+@pytest.mark.parametrize("name", ["spaceslug_act8_pack_device", "spaceslug_act8_unpack_device"])
+@pytest.mark.parametrize("x,codes,exps", [(C, C, B), (C, C + 64 * 96 * 2 - 16, B), (C + 64 * 96 - 16, C, B), (C, A, C + 5),
+                                          (C, A, C - 191)])
+def test_act8_refuses_overlap(session, name, x, codes, exps):
+    """64 x 96 bf16: x 12288 bytes, codes 6144, exps 192; what is written shares a byte with another buffer."""
+    f = session.raw(name)
+    args = (x, 1, codes, exps, 64, 96, None) if "unpack" not in name else (codes, exps, x, 1, 64, 96, None)
+    assert f(*args) == 1
+    assert b"overlaps" in session._native().spaceslug_last_error()
+
+
 def test_handle_calls_refuse_null(session):
     back, grad, loss = (session.raw("spaceslug_q4_weights_" + n) for n in
                         ("lora_backward_act8", "input_gradient", "cross_entropy"))

@@ -640,6 +640,51 @@ def test_refusals(session, cuda):
     assert not torch.cuda.is_current_stream_capturing() and session.device_status(0) == 0
 
 
+def test_refusals_of_overlap_and_alignment(session, cuda):
+    """Buffers that a call writes may share no byte with another (but dx may be x itself), and scalars lie on their own
+    size; neighbours are fine."""
+    import torch
+    k, n, m = 64, 96, 4
+    packed, scales = _weights(k, n, 29)
+    pool = torch.zeros((1 << 16,), device=cuda)
+    P = pool.data_ptr()
+    X, D, T, L, E, S = P, P + 4 * m * k, P + 8192, P + 16384, P + 20000, P + 24000
+    Q, G, A, B = P + 32768, P + 40000, P + 49152, P + 57344
+    grad, ce, back = (session.raw("spaceslug_q4_weights_" + s) for s in ("input_gradient", "cross_entropy", "lora_backward_act8"))
+
+    def clash(code):
+        return code == 1 and b"overlaps" in session._native().spaceslug_last_error()
+
+    with session.weights(packed, scales, k, n) as h:
+        w = h.handle
+        assert grad(w, D, D - 4 * m * k, 0, m, None) == 0  # dx ends where dy begins
+        for dx in (D, D - 4 * m * k + 16, D + 4 * m * n - 16):
+            assert clash(grad(w, D, dx, 0, m, None))
+        good = [X, 0, T, S, L, E, X, m, None]
+        assert ce(w, *good) == 0
+        for i, v in ((4, X), (4, T), (4, S), (5, L), (5, L + 12), (5, X + 4 * m * k - 4), (6, X + 16), (6, T), (4, T + 8 * m - 4)):
+            args = list(good)
+            args[i] = v
+            assert clash(ce(w, *args)), (i, v)
+        for i, v in ((2, T + 4), (3, S + 2), (4, L + 1), (5, E + 2)):
+            args = list(good)
+            args[i] = v
+            assert ce(w, *args) == 1 and b"aligned" in session._native().spaceslug_last_error()
+        h.set_lora(np.zeros((k, 2), np.float32), np.zeros((2, n), np.float32), 2.0)
+        good = [Q, G, D, 0, m, A, B, None]
+        assert back(w, *good) == 0
+        for i, v in ((5, D), (5, Q + 16), (5, G), (6, A), (6, A + 4 * (2 * k - 1)), (6, D + 4 * (m * n - 1))):
+            args = list(good)
+            args[i] = v
+            assert clash(back(w, *args)), (i, v)
+        for i in (5, 6):
+            args = list(good)
+            args[i] += 2
+            assert back(w, *args) == 1 and b"aligned" in session._native().spaceslug_last_error()
+    torch.cuda.synchronize()
+    assert session.device_status(0) == 0
+
+
 # ------------------------------------------------------------------------------------------------------ used together --
 def _net(session, k, hidden, vocab, rank, seed):
     rng = np.random.default_rng(seed)
