@@ -19,9 +19,9 @@
 // us instead of 62.
 //
 // What bounds it is the dequantisation beside everything else an SM issues: a
-// block of 128 n x 128 k takes about 1500 cycles (logits) or 2000 (transposed,
-// fp32), with 61% and 48% of the issue slots, a fifth of the tensor pipe and a
-// quarter of HBM's bandwidth in use.  Tried and slower: stages of half a block,
+// block of 128 n x 128 k takes about 1600 cycles (logits) or 1900 (transposed,
+// fp32), with 60% and 57% of the issue slots, a fifth of the tensor pipe and a
+// quarter of HBM's bandwidth in use (32 x 2048 x 50000: 47 and 52 us, ncu).  Tried and slower: stages of half a block,
 // a second MMA warp with an accumulator per block, one lane per warp polling.
 //
 // Roles (28 warps): warp 0 loads the rows' planes, warp 2 packed words and

@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(256) rows_proj_kernel(const T* dy, const float
     }
 }
 
+__device__ __forceinline__ void prefetch_l1(const float* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
+
 // One row's 128 k per block (blockIdx.y: row): the splits' sum, half of them
 // per thread of a pair of warps, each in order; and with an adapter
 // scale * (sum of G's ranges) A^T.
@@ -358,7 +360,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) rows_finish_kernel(const float* partial, int splits, long long split_floats,
                                                           const float* g, int gsplits, const float* a, int rank,
                                                           float scale, T* __restrict__ out, int M, int K) {
-    __shared__ float gs[64];
+    __shared__ float gp[4][64], gs[64];
     __shared__ float half[128];
     pdl_launch_dependents();
     pdl_wait();
@@ -367,6 +369,17 @@ __global__ void __launch_bounds__(256) rows_finish_kernel(const float* partial, 
     a = after_wait(a);
     const long long row = blockIdx.y;
     const int c = threadIdx.x & 127, h = threadIdx.x >> 7, k = blockIdx.x * 128 + c;
+    if (rank > 0) {
+        // every fourth range of G per thread, and this thread's row of A on its way before either is needed
+        const int j = threadIdx.x & 63, q = threadIdx.x >> 6;
+        if (h == 0 && k < K) prefetch_l1(a + static_cast<size_t>(k) * rank);
+        float t = 0.0f;
+        if (j < rank) {
+#pragma unroll 8
+            for (int z = q; z < gsplits; z += 4) t += g[(static_cast<size_t>(z) * M + row) * rank + j];
+        }
+        gp[q][j] = t;
+    }
     float v = 0.0f;
     if (k < K) {
         const float* p = partial + row * K + k;
@@ -374,14 +387,13 @@ __global__ void __launch_bounds__(256) rows_finish_kernel(const float* partial, 
 #pragma unroll 8
         for (int z = h == 0 ? 0 : (splits + 1) / 2; z < z1; ++z) v += p[z * split_floats];
     }
-    if (threadIdx.x < rank) {
-        float t = 0.0f;
-#pragma unroll 8
-        for (int z = 0; z < gsplits; ++z) t += g[(static_cast<size_t>(z) * M + row) * rank + threadIdx.x];
-        gs[threadIdx.x] = scale * t;
-    }
     if (h == 1) half[c] = v;
     __syncthreads();
+    if (rank > 0) {
+        const int j = threadIdx.x;
+        if (j < 64) gs[j] = scale * ((gp[0][j] + gp[1][j]) + (gp[2][j] + gp[3][j]));
+        __syncthreads();
+    }
     if (h == 1 || k >= K) return;
     v += half[c];
     if (rank > 0) {

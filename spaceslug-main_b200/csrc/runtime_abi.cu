@@ -1483,12 +1483,12 @@ void run_input_gradient_few(spaceslug_q4_weights* w, const void* dy, void* dx, b
 }
 
 void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
-    if (M <= q4::kFewRows) {
-        run_input_gradient_few(w, dy, dx, bf16, M, s);
-        return;
-    }
     if (rows_kernels_pay(M, w, bf16)) {
         run_input_gradient_rows(w, dy, dx, bf16, M, s);
+        return;
+    }
+    if (M <= q4::kFewRows) {
+        run_input_gradient_few(w, dy, dx, bf16, M, s);
         return;
     }
     DeviceCtx& c = ctx_for(w->device);
