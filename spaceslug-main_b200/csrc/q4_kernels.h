@@ -323,7 +323,7 @@ int rows_proj_splits(int M, int N, int rank, int sm_count);
 int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int splits, int M, int N, int rank,
                      cudaStream_t stream);
 // out [M][K] = sum in order of the splits (split_floats apart) + scale (sum of G's ranges) A^T (A [K][rank]; rank 0:
-// none), any M without an adapter
+// none) for a few rows (M is the grid's y)
 int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, int gsplits,
                        const float* a, int rank, float scale, void* out, bool bf16, int M, int K, cudaStream_t stream);
 // The large products of training through the frozen weights (q4_grad_gemm.cu).  Epilogues: the logits' tile statistics
@@ -414,6 +414,9 @@ int launch_loss_rows(float* smax, const float* ssum, const float* zt, const long
 int launch_loss_dx(const float* partial, int splits, long long out_rows, const float* total, const float* loss,
                    const long long* targets, const float* row_scale, const uint32_t* packed, const float* scales, void* dx, bool bf16, int M,
                    int N, int K, cudaStream_t stream);
+// out [count] (fp32 or bf16; count % 4 == 0) = sum in order of `splits` runs of fp32, split_floats apart
+int launch_sum_splits(const float* partial, int splits, long long split_floats, void* out, bool bf16, long long count,
+                      cudaStream_t stream);
 int launch_lora_at(const float* a, void* at, int* gexp, const int* w_exp, int K, int rank, int ld, int planes,
                    cudaStream_t stream);
 

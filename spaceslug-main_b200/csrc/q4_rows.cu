@@ -498,18 +498,12 @@ int launch_rows_proj(const void* dy, bool bf16, const float* b, float* g, int sp
 
 int launch_rows_finish(const float* partial, int splits, long long split_floats, const float* g, int gsplits,
                        const float* a, int rank, float scale, void* out, bool bf16, int M, int K, cudaStream_t stream) {
-    int rc = 0;
-    for (int m0 = 0; m0 < M && rc == 0; m0 += 32768) {  // rows are blockIdx.y
-        const int mc = M - m0 < 32768 ? M - m0 : 32768;
-        if (rank > 0 && m0 > 0) return static_cast<int>(cudaErrorInvalidValue);  // an adapter here has few rows
-        const dim3 grid(static_cast<unsigned>((K + 127) / 128), static_cast<unsigned>(mc));
-        const long long at = static_cast<long long>(m0) * K;
-        rc = bf16 ? rows_launch(rows_finish_kernel<__nv_bfloat16>, grid, 256, stream, partial + at, splits, split_floats, g,
-                                gsplits, a, rank, scale, static_cast<__nv_bfloat16*>(out) + at, mc, K)
-                  : rows_launch(rows_finish_kernel<float>, grid, 256, stream, partial + at, splits, split_floats, g, gsplits,
-                                a, rank, scale, static_cast<float*>(out) + at, mc, K);
-    }
-    return rc;
+    if (M < 1 || M > 32768) return static_cast<int>(cudaErrorInvalidValue);
+    const dim3 grid(static_cast<unsigned>((K + 127) / 128), static_cast<unsigned>(M));
+    return bf16 ? rows_launch(rows_finish_kernel<__nv_bfloat16>, grid, 256, stream, partial, splits, split_floats, g, gsplits,
+                              a, rank, scale, static_cast<__nv_bfloat16*>(out), M, K)
+                : rows_launch(rows_finish_kernel<float>, grid, 256, stream, partial, splits, split_floats, g, gsplits, a, rank,
+                              scale, static_cast<float*>(out), M, K);
 }
 
 }  // namespace q4

@@ -1609,8 +1609,8 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.status = c.status;
         check_launch(q4::launch_grad_gemm(g, planes, direct16 ? q4::kGgBf16 : q4::kGgF32, weights.from_planes, s), "dY W^T");
         if (g.splits > 1)
-            check_launch(q4::launch_rows_finish(part, g.splits, static_cast<long long>(g.out_rows) * K, nullptr, 0, nullptr,
-                                                0, 0.0f, out, bf16, mc, K, s),
+            check_launch(q4::launch_sum_splits(part, g.splits, static_cast<long long>(g.out_rows) * K, out, bf16,
+                                               static_cast<long long>(mc) * K, s),
                          "dX");
     }
 }
