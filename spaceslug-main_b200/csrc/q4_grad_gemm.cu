@@ -1012,15 +1012,17 @@ __global__ void __launch_bounds__(256) loss_dx_kernel(const float* partial, int 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
         if (t >= 0) {
+            const bool in = t < N;  // the target's weights are on their way while the splits are added
+            const uint32_t q = in ? __ldg(packed + t * (K / 8) + k / 8) : 0u;
+            const float s = in ? __ldg(scales + t * (K / 32) + k / 32) : 0.0f;
+#pragma unroll 4
             for (int z = 0; z < splits; ++z) {
                 const float4* p = reinterpret_cast<const float4*>(partial + (z * out_rows + row) * K + k);
                 const float4 a = p[0], b = p[1];
                 v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
                 v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
             }
-            if (t < N) {
-                const uint32_t q = packed[t * (K / 8) + k / 8];
-                const float s = scales[t * (K / 32) + k / 32];
+            if (in) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int nib = static_cast<int>((q >> (4 * i)) & 15u);
