@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint4 hi, lo;
-                            gg_dequant<PB, false>(ww[i], s_hi, s_lo, hi, lo);
+                            gg_dequant<PB>(ww[i], s_hi, s_lo, hi, lo);
                             const int o = ((4 * h + i) ^ (row & 7)) << 4;
                             *reinterpret_cast<uint4*>(dst + o) = hi;
                             if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kFrPlane + o) = lo;
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kFrThreads, 1) few_rows_kernel(const __grid_co
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             uint4 hi, lo;
-                            gg_dequant<2, false>(ww[i], s_hi, s_lo, hi, lo);
+                            gg_dequant<2>(ww[i], s_hi, s_lo, hi, lo);
                             v[4 * i] = hi.x; v[4 * i + 1] = hi.y; v[4 * i + 2] = hi.z; v[4 * i + 3] = hi.w;
                             v[16 + 4 * i] = lo.x; v[17 + 4 * i] = lo.y; v[18 + 4 * i] = lo.z; v[19 + 4 * i] = lo.w;
                         }

@@ -29,12 +29,6 @@ __device__ __forceinline__ uint64_t gg_desc_mn_sw128(uint32_t addr, uint32_t lbo
     return d;
 }
 
-// Two f16 as two e4m3 bytes (round to nearest, clamped to +-448).
-__device__ __forceinline__ uint32_t gg_e4m3x2(__half2 v) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&v)));
-    return r;
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -81,8 +75,7 @@ __device__ __forceinline__ void gg_ld_wait(uint32_t (&r)[16]) {
 // accumulator's columns, undone by the epilogue's choice of registers.
 // hi = RN16(v s_hi + RN16(v s_lo)) as in dequant_word_f16x2, lo = (v s_hi -
 // hi) + RN16(v s_lo), whose bracket is exact, so hi + lo is v s to 2^-22.
-// With LO8, lo is 64 times that in e4m3: eight bytes in lo.x and lo.y.
-template <int PB, bool LO8>
+template <int PB>
 __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_lo, uint4& hi, uint4& lo) {
     const __half2 sixteenth = __half2half2(__ushort_as_half(0x2C00u));  // 1/16
     const __half2 bias0 = __half2half2(__ushort_as_half(0xE408u));      // -1032: 1024 + (v + 8)
@@ -100,15 +93,11 @@ __device__ __forceinline__ void gg_dequant(uint32_t q, __half2 s_hi, __half2 s_l
         h[b] = *reinterpret_cast<const uint32_t*>(&w);
         if constexpr (PB == 2) {
             const __half2 r = __hadd2(__hfma2(v, s_hi, __hneg2(w)), c);
-            if constexpr (LO8) {
-                l[b] = gg_e4m3x2(__hmul2(r, __half2half2(__ushort_as_half(0x5400u))));  // 64 r
-            } else {
-                l[b] = *reinterpret_cast<const uint32_t*>(&r);
-            }
+            l[b] = *reinterpret_cast<const uint32_t*>(&r);
         }
     }
     hi = make_uint4(h[0], h[1], h[2], h[3]);
-    if constexpr (PB == 2) lo = LO8 ? make_uint4(l[0] | (l[1] << 16), l[2] | (l[3] << 16), 0, 0) : make_uint4(l[0], l[1], l[2], l[3]);
+    if constexpr (PB == 2) lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 // Place of k (0..7) in that order.
 __host__ __device__ constexpr int gg_place(int k) { return k < 4 ? 2 * k : 2 * (k - 4) + 1; }

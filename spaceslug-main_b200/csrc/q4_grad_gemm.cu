@@ -17,12 +17,11 @@
 // handle.  PA, PB planes each: 1 = the value rounded once to 11 bits, 2 = hi
 // and lo, 22 bits.  (1, 1): bf16 in and out, whose 8 bits are exact in f16,
 // so only w is rounded (2^-12) below the output's own 2^-9.  (1, 2): logits
-// of bf16 x, products to 2^-22, because the loss is fp32.  (2, 2): fp32 (hi
+// of bf16 x, products to 2^-22, because the loss is fp32 (with the lo product
+// in fp8 the logits' product took a quarter less, but logits were right to 7e-6
+// of their norm only, where a plain 32-bit product has 3e-7).  (2, 2): fp32 (hi
 // hi + hi lo + lo hi).  One scale for the whole handle loses nothing that
-// shows: columns 2^-28 below the largest still have 11 bits.  In (1, 2) the lo
-// product only has to be right to a few bits (it is 2^-12 of the whole), so it
-// runs in fp8 at half the cost: e4m3 copies of the rows and of 64 lo, whose
-// 2^-4 leaves logits right to about 2^-16 of their terms.  The target's own
+// shows: columns 2^-28 below the largest still have 11 bits.  The target's own
 // logit comes from an fp32 product and its term is kept out of the sums, so
 // that a loss near zero keeps its digits.
 //
@@ -80,12 +79,8 @@ struct GgCfg {
     static constexpr int kThreads = WT ? 384 : 640;
     static constexpr int kEpiWarp0 = WT ? 4 : 12;
     static constexpr int kRegsLaunch = WT ? 0 : kGgRegsLaunch;  // least the launch must have
-    // (1, 2): the lo plane of w in fp8, against an fp8 copy of the rows
-    static constexpr bool kLo8 = PA == 1 && PB == 2;
-    static constexpr int kA8 = PA * kGgTile;                       // fp8 rows: 128 x 64 bytes
-    static constexpr int kB = kA8 + (kLo8 ? kGgTile / 2 : 0);      // w hi
-    static constexpr int kBLo = kB + kGgTile;                      // w lo (f16, or 128 x 64 bytes of fp8)
-    static constexpr int kStageBytes = kLo8 ? kBLo + kGgTile / 2 : (PA + PB) * kGgTile;
+    static constexpr int kB = PA * kGgTile;  // w hi, then w lo
+    static constexpr int kStageBytes = (PA + PB) * kGgTile;
     static constexpr int kStages = PA + PB == 2 ? (WT ? 6 : 5) : PA + PB == 3 ? (WT ? 4 : 3) : 2;
     static constexpr int kOutOff = kStages * kStageBytes;
     static constexpr int kRawOff = kOutOff + kGgEpiWarps * kGgOutBytes;
@@ -103,26 +98,6 @@ struct GgCfg {
     static_assert(kSmem <= 232448, "shared memory budget");
 };
 
-// K-major operand of 64-byte rows (64 fp8), 64-byte swizzled: 8-row atoms of 512 bytes.
-__device__ __forceinline__ uint64_t gg_desc_k_sw64(uint32_t addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(1u) << 16;
-    d |= static_cast<uint64_t>(512u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(4u) << 61;  // SWIZZLE_64B
-    return d;
-}
-// Pair MMA on e4m3 operands (K = 32), fp32 accumulate.
-__device__ __forceinline__ void umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 template <int R>
 __device__ __forceinline__ void regs_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
@@ -251,16 +226,13 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                                                      at ? 64 * p : st * kGgBK);
                         } else {
                             tma_load_2d_pair(b, &P.tm_w, fx, st * kGgBK, tile0);
-                            if constexpr (PB == 2)
-                                tma_load_2d_pair(base + s * C::kStageBytes + C::kBLo, &P.tm_s, fx, st * kGgBK, tile0);
+                            if constexpr (PB == 2) tma_load_2d_pair(b + kGgTile, &P.tm_s, fx, st * kGgBK, tile0);
                         }
                     }
 #pragma unroll
                     for (int p = 0; p < PA; ++p)
                         tma_load_2d_pair(base + s * C::kStageBytes + p * kGgTile, &P.tm_a, fx, st * kGgBK,
                                          p * P.plane_rows + m0);
-                    if constexpr (C::kLo8)
-                        tma_load_2d_pair(base + s * C::kStageBytes + C::kA8, &P.tm_a8, fx, st * kGgBK, m0);
                 }
             }
             if (*abort_flag && leader)
@@ -316,14 +288,6 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                         }
                         tc_fence_after_sync();
                         const uint32_t at = base + s * C::kStageBytes, bt = at + C::kB;
-                        if constexpr (C::kLo8) {
-#pragma unroll
-                            for (int kk = 0; kk < kGgBK / 32; ++kk) {
-                                umma_f8_ss_pair(dacc, gg_desc_k_sw64(at + C::kA8 + kk * 32),
-                                                gg_desc_k_sw64(at + C::kBLo + kk * 32), idesc, acc);
-                                acc = 1;
-                            }
-                        }
                         auto mma = [&](int pa, int pb, int kk) {
                             const uint64_t ad = umma_desc_k_sw128(at + pa * kGgTile + kk * 32);
                             const uint64_t bd = TR ? gg_desc_mn_sw128(bt + pb * kGgTile + kk * 2048, kGgTile / 2)
@@ -334,7 +298,7 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
 #pragma unroll
                         for (int kk = 0; kk < kGgBK / 16; ++kk) {
                             if constexpr (PA == 2) mma(1, 0, kk);
-                            if constexpr (PB == 2 && !C::kLo8) mma(0, 1, kk);
+                            if constexpr (PB == 2) mma(0, 1, kk);
                             mma(0, 0, kk);
                         }
                         umma_commit_pair_both(empty(s), 0x3);
@@ -412,21 +376,12 @@ __global__ void __launch_bounds__(WT ? 384 : 640, 1) grad_gemm_kernel(const __gr
                             split_scale_f16((h == 0 ? sc.x : sc.y) * cs, s_hi, s_lo);
                             const uint32_t words[4] = {q[h].x, q[h].y, q[h].z, q[h].w};
 #pragma unroll
-                            for (int i = 0; i < 4; i += 2) {
-                                uint4 hi0, hi1, lo0, lo1;
-                                gg_dequant<PB, C::kLo8>(words[i], s_hi, s_lo, hi0, lo0);
-                                gg_dequant<PB, C::kLo8>(words[i + 1], s_hi, s_lo, hi1, lo1);
-                                const int o0 = ((4 * h + i) ^ (row & 7)) << 4, o1 = ((4 * h + i + 1) ^ (row & 7)) << 4;
-                                *reinterpret_cast<uint4*>(dst + o0) = hi0;
-                                *reinterpret_cast<uint4*>(dst + o1) = hi1;
-                                if constexpr (C::kLo8) {  // 64-byte rows: a 16-byte piece holds two words
-                                    *reinterpret_cast<uint4*>(smem + s * C::kStageBytes + C::kBLo + row * 64 +
-                                                              (((2 * h + i / 2) ^ ((row >> 1) & 3)) << 4)) =
-                                        make_uint4(lo0.x, lo0.y, lo1.x, lo1.y);
-                                } else if constexpr (PB == 2) {
-                                    *reinterpret_cast<uint4*>(dst + kGgTile + o0) = lo0;
-                                    *reinterpret_cast<uint4*>(dst + kGgTile + o1) = lo1;
-                                }
+                            for (int i = 0; i < 4; ++i) {
+                                uint4 hi, lo;
+                                gg_dequant<PB>(words[i], s_hi, s_lo, hi, lo);
+                                const int o = ((4 * h + i) ^ (row & 7)) << 4;
+                                *reinterpret_cast<uint4*>(dst + o) = hi;
+                                if constexpr (PB == 2) *reinterpret_cast<uint4*>(dst + kGgTile + o) = lo;
                             }
                         }
                     }
@@ -759,8 +714,7 @@ __device__ __forceinline__ void gg_row_each(const T* row, int cols, int end, F&&
 // are the row's G = s dY B^T (the sum of its partial products) times 2^gexp[j],
 // the exponents that A^T's planes were scaled down by, so that G A^T is 64
 // more terms of the same contraction; the row's exponent covers them too.
-// For the loss it also forms the target's logit in fp32, and (bf16) the e4m3
-// copy of the row.
+// For the loss it also forms the target's logit in fp32.
 // The row is read twice, the second time from L1 / L2: keeping it in registers
 // (48 floats a thread) halves the blocks per SM and measured slower (24 against
 // 16 us at 4096 x 4096 bf16).
@@ -843,14 +797,6 @@ __global__ void __launch_bounds__(THREADS) cast_planes_kernel(const CastArgs A) 
             }
         }
         *reinterpret_cast<uint4*>(hi + p * 8) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (PA == 1 && A.out8 != nullptr) {  // the row * 2^(e - 6) in e4m3, to go with 64 w_lo
-            const __half2 down = __half2half2(__ushort_as_half(0x2400u));  // 1/64
-            uint32_t q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = gg_e4m3x2(__hmul2(*reinterpret_cast<const __half2*>(&h[i]), down));
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(A.out8) + m * A.ld + p * 8) =
-                make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-        }
         if constexpr (PA == 2)
             *reinterpret_cast<uint4*>(hi + static_cast<long long>(A.M) * A.ld + p * 8) = make_uint4(l[0], l[1], l[2], l[3]);
     };
@@ -876,11 +822,11 @@ __global__ void __launch_bounds__(THREADS) cast_planes_kernel(const CastArgs A) 
 // The dequantised planes [N][K] of a handle's weights, in the dequantised
 // words' order: what the products' dequant warps write to shared memory, once
 // for all row tiles.  Four words per thread, a block apart.
-template <bool LO8>
+template <bool LO>
 __global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __restrict__ packed,
                                                             const float* __restrict__ scales,
                                                             const int* __restrict__ w_exp, __half* __restrict__ hi,
-                                                            uint2* __restrict__ lo8, long long words) {
+                                                            __half* __restrict__ lo, long long words) {
     pdl_launch_dependents();
     const float cs = exp2i(*w_exp);
     const long long i0 = static_cast<long long>(blockIdx.x) * 1024 + threadIdx.x;
@@ -900,9 +846,9 @@ __global__ void __launch_bounds__(256) weight_planes_kernel(const uint32_t* __re
         __half2 s_hi, s_lo;
         split_scale_f16(s[u] * cs, s_hi, s_lo);
         uint4 h, l;
-        gg_dequant<LO8 ? 2 : 1, LO8>(q[u], s_hi, s_lo, h, l);
+        gg_dequant<LO ? 2 : 1>(q[u], s_hi, s_lo, h, l);
         reinterpret_cast<uint4*>(hi)[i] = h;
-        if constexpr (LO8) lo8[i] = make_uint2(l.x, l.y);
+        if constexpr (LO) reinterpret_cast<uint4*>(lo)[i] = l;
     }
 }
 
@@ -1138,21 +1084,19 @@ int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_plane
     return static_cast<int>(cudaErrorInvalidValue);
 }
 
-int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo8, int N, int K,
+int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo, int N, int K,
                          cudaStream_t stream) {
     const long long words = static_cast<long long>(N) * (K / 8);
     const unsigned blocks = static_cast<unsigned>((words + 1023) / 1024);
-    if (lo8 == nullptr)
-        return gg_launch_pdl(weight_planes_kernel<false>, blocks, 256, stream, packed, scales, w_exp, static_cast<__half*>(hi),
-                             static_cast<uint2*>(lo8), words);
-    return gg_launch_pdl(weight_planes_kernel<true>, blocks, 256, stream, packed, scales, w_exp, static_cast<__half*>(hi),
-                         static_cast<uint2*>(lo8), words);
+    auto kern = lo == nullptr ? weight_planes_kernel<false> : weight_planes_kernel<true>;
+    return gg_launch_pdl(kern, blocks, 256, stream, packed, scales, w_exp, static_cast<__half*>(hi),
+                         static_cast<__half*>(lo), words);
 }
 
 int launch_cast_planes(const CastArgs& a, bool bf16, int planes, cudaStream_t stream) {
     if (a.M < 1 || a.ld % 8 != 0 || a.ld < a.cols || a.rank > 64) return static_cast<int>(cudaErrorInvalidValue);
     const bool vec = a.cols % 8 == 0;  // rows of whole 16-byte pieces
-    if (!vec && (a.targets != nullptr || a.by_word || a.out8 != nullptr)) return static_cast<int>(cudaErrorInvalidValue);
+    if (!vec && (a.targets != nullptr || a.by_word)) return static_cast<int>(cudaErrorInvalidValue);
     const unsigned grid = static_cast<unsigned>(a.M);
     auto launch = [&](auto few, auto wide, auto one, auto two) {
         return a.M <= kCastFew ? (vec ? gg_launch_pdl(few, grid, kCastThreadsFew, stream, a)

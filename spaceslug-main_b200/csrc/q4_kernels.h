@@ -332,11 +332,10 @@ int launch_rows_finish(const float* partial, int splits, long long split_floats,
 enum : int { kGgLoss = 0, kGgProb = 1, kGgF32 = 2, kGgBf16 = 3 };
 struct GradGemmArgs {
     CUtensorMap tm_a;        // f16 planes of the rows: [planes * plane_rows][contraction], box 64 x 128, 128B swizzle
-    CUtensorMap tm_a8;       // logits of one plane: the rows in e4m3 [rows][contraction], box 64 x 128, 64B swizzle
     CUtensorMap tm_out;      // p~ planes or the output: box 128 bytes x 32 rows, 128B swizzle (not read by kGgLoss)
     // Weights as packed words uint32 [N][K/8] (tm_w, box 16 x 128, 64B swizzle) and scales fp32 [N][groups] (tm_s, rows
-    // of 16-byte multiples, box 4 x 128); or, of one row plane, from planes [N][K]: f16 hi (tm_w), 128B swizzle, box
-    // 64 x 128 (logits, and lo as e4m3: tm_s, 64B swizzle) or 64 x 64 (transposed, and A^T's plane: tm_at, box 64 x 64).
+    // of 16-byte multiples, box 4 x 128); or, of one row plane, from f16 planes [N][K], 128B swizzle: hi (tm_w) and, for
+    // the logits, lo (tm_s), box 64 x 128, or hi, box 64 x 64 (transposed, and A^T's plane: tm_at, box 64 x 64).
     CUtensorMap tm_w;
     CUtensorMap tm_s;
     CUtensorMap tm_at;
@@ -382,16 +381,15 @@ int few_rows_padded(int M);
 int launch_few_rows(const FewRowsArgs& a, int planes, int epi, cudaStream_t stream);
 int grad_gemm_pairs();  // co-resident CTA pairs on the current device
 int launch_grad_gemm(const GradGemmArgs& a, int planes, int epi, bool from_planes, cudaStream_t stream);
-// The weights' planes [N][K]: hi (f16), and 64 lo in e4m3 unless null.
-int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo8, int N, int K,
+// The weights' f16 planes [N][K]: hi, and lo unless null.
+int launch_weight_planes(const uint32_t* packed, const float* scales, const int* w_exp, void* hi, void* lo, int N, int K,
                          cudaStream_t stream);
 // f16 planes [planes][M][ld] of fp32 (2 planes) or bf16 (1) rows scaled by 2^row_exp; by_word: each 8 columns in the
 // order 0 4 1 5 2 6 3 7; with an adapter (rank > 0) the last 64 columns hold gscale * sum of gpart [gsplits][M][gpitch].
-// targets (logits): the target column's logit of each row in fp32 to zt, and to out8 the e4m3 copy of bf16 rows.
+// targets (logits): the target column's logit of each row in fp32 to zt.
 struct CastArgs {
     const void* x;
     void* out;
-    void* out8;
     const long long* targets;
     const uint32_t* packed;
     const float* scales;

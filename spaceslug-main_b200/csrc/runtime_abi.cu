@@ -1364,14 +1364,14 @@ constexpr int kPlaneRows = 2048;
 struct TrainWeights {
     spaceslug_q4_weights* w;
     bool from_planes;
-    Scratch planes;  // hi [N][K] f16, and for the logits 64 lo [N][K] e4m3
-    void* lo8 = nullptr;
+    Scratch planes;  // hi [N][K] f16, and for the logits lo [N][K]
+    void* lo = nullptr;
     TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s)
         : w(h), from_planes(bf16 && M >= kPlaneRows),
-          planes(from_planes ? static_cast<size_t>(h->N) * h->K * (logits ? 3 : 2) : 0, s) {
+          planes(from_planes ? static_cast<size_t>(h->N) * h->K * (logits ? 4 : 2) : 0, s) {
         if (!from_planes) return;
-        if (logits) lo8 = static_cast<char*>(planes.p) + static_cast<size_t>(w->N) * w->K * 2;
-        check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, planes.p, lo8, w->N, w->K, s),
+        if (logits) lo = static_cast<char*>(planes.p) + static_cast<size_t>(w->N) * w->K * 2;
+        check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, planes.p, lo, w->N, w->K, s),
                      "weight planes");
     }
     // tensor maps of the logits' or the transposed product
@@ -1383,7 +1383,7 @@ struct TrainWeights {
                       CU_TENSOR_MAP_SWIZZLE_128B);
             g.tm_s = g.tm_w;  // not read by the transposed product
             if (!transposed)
-                encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_UINT8, lo8, K, N, K, 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
+                encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, lo, K, N, K * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
             return;
         }
         const uint64_t G = K / 32, Gp = (G + 3) / 4 * 4;
@@ -1733,12 +1733,12 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
     const int tiles = (N + 255) / 256;
     const long long ld_p = static_cast<long long>(tiles) * 256;
     // per row: the planes of X and of p~, and the partial sums of dX
-    const long long row_bytes = (2ll * planes + 1) * K + (dx ? 2ll * planes * ld_p + 4ll * K : 0);
+    const long long row_bytes = 2ll * planes * K + (dx ? 2ll * planes * ld_p + 4ll * K : 0);
     const int block = train_block(M, row_bytes);
     const TrainWeights weights(w, bf16, true, M, s);
     for (int m0 = 0; m0 < M; m0 += block) {
         const int mc = std::min(block, M - m0), mp = (mc + 255) / 256 * 256;
-        const size_t b_x = static_cast<size_t>(planes) * mc * K * 2, b_x8 = bf16 ? static_cast<size_t>(mc) * K : 0;
+        const size_t b_x = static_cast<size_t>(planes) * mc * K * 2;
         const size_t b_re = static_cast<size_t>(mc) * sizeof(int), b_t = static_cast<size_t>(tiles) * mp * 4;
         const size_t b_row = static_cast<size_t>(mp) * 4, b_prob = dx ? static_cast<size_t>(planes) * mp * ld_p * 2 : 0;
         const int splits = dx ? grad_splits(static_cast<long long>(mp / 256) * ((K + 255) / 256), tiles,
@@ -1746,11 +1746,10 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
                               : 0;
         const size_t b_part = static_cast<size_t>(splits) * mp * K * 4;
         Carve cut;
-        for (size_t b : {b_x, b_x8, b_re, b_t, 2 * b_t, b_row, b_row, b_prob, b_part}) cut.add(b);
+        for (size_t b : {b_x, b_re, b_t, 2 * b_t, b_row, b_row, b_prob, b_part}) cut.add(b);
         Scratch mem(cut.total, s);
         cut.base = static_cast<char*>(mem.p);
         void* x16 = cut.take<void>(b_x);
-        void* x8 = cut.take<void>(b_x8);
         int* rexp = cut.take<int>(b_re);
         float* smax = cut.take<float>(b_t);
         float* ssum = cut.take<float>(2 * b_t);
@@ -1763,7 +1762,6 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         ca.out = x16; ca.row_exp = rexp;
         ca.M = mc; ca.cols = K; ca.ld = K;
         ca.by_word = 1;
-        ca.out8 = x8;
         ca.targets = targets + m0; ca.packed = w->packed; ca.scales = w->scales; ca.zt = zt; ca.N = N;
         check_launch(q4::launch_cast_planes(ca, bf16, planes, s), "X planes");
         q4::GradGemmArgs g{};
@@ -1788,10 +1786,6 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
         g.status = c.status;
         encode_2d(&g.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x16, static_cast<uint64_t>(K),
                   static_cast<uint64_t>(planes) * mc, static_cast<uint64_t>(K) * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-        g.tm_a8 = g.tm_a;  // not read without an e4m3 copy
-        if (bf16)
-            encode_2d(&g.tm_a8, CU_TENSOR_MAP_DATA_TYPE_UINT8, x8, static_cast<uint64_t>(K), static_cast<uint64_t>(mc),
-                      static_cast<uint64_t>(K), 64, 128, CU_TENSOR_MAP_SWIZZLE_64B);
         if (dx)
             encode_2d(&g.tm_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, prob, static_cast<uint64_t>(ld_p),
                       static_cast<uint64_t>(planes) * mp, static_cast<uint64_t>(ld_p) * 2, 64, 32,

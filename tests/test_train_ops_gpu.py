@@ -4,10 +4,8 @@ gradient, softmax cross entropy over a vocabulary) against 64-bit restatements.
 Tolerances.  S = sum |a||b| over a product's terms, in 64 bits.
   fp32: operands to 2^-21, and sums of rounded terms whose chains are at most 255 long: |error| <= 2^-16 S.
   bf16: one operand rounded to f16 (2^-11 of each term), the result to bf16 (2^-8 of it): 2^-11 S + 2^-8 |y| + 2^-16 S.
-Logits are held to the fp32 bound for both types: dz = 2^-16 max_v S (bf16: what W's f16 part leaves is multiplied in
-fp8, off by at most 2^-11 (2^-4 + 2^-4) = 2^-14 of a term and of random sign, so by 2^-14 S / sqrt(k), which is below
-2^-16 S from k = 16 on).  Then lse is off by dz + 2^-20 (1 + |lse|), a loss
-by twice that, a probability by 2 dz + 2^-16 of itself.
+Logits are held to the fp32 bound for both types: dz = 2^-16 max_v S (bf16 rows are exact and W enters as f16 hi and lo).
+Then lse is off by dz + 2^-20 (1 + |lse|), a loss by twice that, a probability by 2 dz + 2^-16 of itself.
 """
 from __future__ import annotations
 
@@ -774,4 +772,26 @@ def test_training_step(session, cuda, m):
     del graph
     for h in (*hs, hv):
         h.close()
+    assert session.device_status(0) == 0
+
+
+# --------------------------------------------------------------------------------------- found faults and their mends --
+@pytest.mark.parametrize("m", [1, 8, 9, 64, 65, 300, 2100])
+def test_logits_of_bf16_rows_at_every_row_count(session, cuda, m):
+    """One column and no target: lse is the logit itself.  w = 2^-6 (1 + 2^-12 + 2^-16) is f16 hi + lo without a rest and
+    the rows are exact too, so all 2 x 64 products are exact; a sum that cuts each at 2^-24 of S = |z| is off by at most
+    2^-17 S, the ways to log2 and back by 2^-21.  (lo and the row in e4m3, 1.0625 each, would be off by 2^-15.)"""
+    import torch
+    k = 64
+    packed = np.full((1, k // 8), 0x11111111, np.uint32)
+    scales = np.full((1, k // 32), 2.0 ** -6 * (1 + 2.0 ** -12 + 2.0 ** -16), np.float32)
+    x = torch.full((m, k), 1.0625, device=cuda) * torch.exp2(torch.arange(m, device=cuda).float() % 9 - 4)[:, None]
+    x = x.bfloat16()
+    none, loss = torch.full((m,), -1, dtype=torch.int64, device=cuda), torch.empty((m,), device=cuda)
+    lse, dx = torch.empty((m,), device=cuda), torch.empty_like(x)
+    z = x.double() @ _w64(packed, scales, k, 1, cuda)[:, 0]
+    with session.weights(packed, scales, k, 1) as h:
+        for d in (0, dx.data_ptr()):
+            h.cross_entropy(x.data_ptr(), none.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=d, dtype="bf16")
+            assert ((lse.double() - z).abs() <= 1.0625 * 2.0 ** -17 * z).all(), float(((lse.double() - z).abs() / z).max())
     assert session.device_status(0) == 0
