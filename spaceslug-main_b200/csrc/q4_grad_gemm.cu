@@ -1018,6 +1018,7 @@ __global__ void __launch_bounds__(256) sum_splits_kernel(const float* partial, i
     }
 }
 
+constexpr int kGgNoColumn = -512;  // 2^-512 of any finite fp32 value is 0
 // One block per rank j < 64: f16 planes [planes][64][ld] of A^T's row j times
 // 2^E_j, E_j such that its largest magnitude lies in [2^13, 2^14) (k in the
 // dequantised words' order, zeros past K and past the rank), and the exponent
@@ -1045,7 +1046,8 @@ __global__ void __launch_bounds__(256) lora_at_kernel(const float* a, __half* __
         frexpf(top, &e2);
         e = min(max(14 - e2, -120), 120);
     }
-    if (threadIdx.x == 0) gexp[j] = *w_exp - e;
+    // a column of zeros: G's column, which meets nothing, shrinks to 0 and has no say in its row's exponent
+    if (threadIdx.x == 0) gexp[j] = top > 0.0f ? *w_exp - e : kGgNoColumn;
     const float s = exp2i(e);
 #pragma unroll 4
     for (int i = threadIdx.x; i < ld; i += 256) {

@@ -795,3 +795,36 @@ def test_logits_of_bf16_rows_at_every_row_count(session, cuda, m):
             h.cross_entropy(x.data_ptr(), none.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=d, dtype="bf16")
             assert ((lse.double() - z).abs() <= 1.0625 * 2.0 ** -17 * z).all(), float(((lse.double() - z).abs() / z).max())
     assert session.device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [40, 65, 300, 2050])
+@pytest.mark.parametrize("zero", ["all", "one", "one_row"])
+def test_input_gradient_with_zero_columns_of_a(session, cuda, m, zero, dtype):
+    """Ranks whose column of A is zero (a pruned rank; an adapter that starts from A = 0) add nothing to dX and cost its
+    other terms no bits, however large their row of B; one nonzero element makes the column count."""
+    import torch
+    k, n, rank = 256, 4096, 4
+    packed, scales = _weights(k, n, 61, 0.0005, 0.001)
+    rng = np.random.default_rng(m)
+    A = (rng.standard_normal((k, rank)) * 1e-4).astype(np.float32)
+    B = rng.standard_normal((rank, n)).astype(np.float32)
+    B[1] *= 1e3
+    if zero == "all":
+        A[:] = 0.0
+    else:
+        A[:, 1] = 0.0
+        if zero == "one_row":
+            A[17, 1] = 1e-6
+    dy = _randn((m, n), cuda, 5).to(_dt(dtype))
+    dx, bare = (torch.full((m, k), float("nan"), device=cuda, dtype=_dt(dtype)) for _ in range(2))
+    with session.weights(packed, scales, k, n) as h:
+        h.input_gradient(dy.data_ptr(), bare.data_ptr(), m, dtype=dtype)
+        h.set_lora(A, B, 2.0 * rank)
+        h.input_gradient(dy.data_ptr(), dx.data_ptr(), m, dtype=dtype)
+    W, D = _w64(packed, scales, k, n, cuda), dy.double()
+    A64, B64 = torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()
+    ref, S = D @ W.T, D.abs() @ W.abs().T
+    _check_dx(bare, dtype, ref, S)
+    _check_dx(dx, dtype, ref + 2.0 * (D @ B64.T) @ A64.T, S + 2 * 2.0 * (D.abs() @ B64.abs().T) @ A64.abs().T)
+    assert session.device_status(0) == 0
