@@ -190,7 +190,7 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
                                         void* stream);
 /* Softmax cross entropy of the logits z = X * dequant(W) over the handle's
  * columns (a whole vocabulary; a handle with an adapter attached is refused),
- * without keeping the logits (targets count from the handle's first column):
+ * keeping no logits past the call (targets count from the handle's first column):
  *   lse[i] = log sum_v exp z[i][v],  loss[i] = lse[i] - z[i][targets[i]],
  *   dx[i] = row_scale[i] * (softmax(z[i]) - onehot(targets[i])) * dequant(W)^T.
  * x [m x k] and dx [m x k] of `dtype`, 16-byte aligned; targets int64 [m];
@@ -198,7 +198,13 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
  * loss fp32 [m]; lse fp32 [m] or NULL; dx or NULL (the loss alone).  A negative
  * target takes its row out: loss 0, dx 0 (lse is still written).  A target past
  * the columns gives NaN in its row's loss and dx.  dx may be x itself.  m <= 2^24;
- * device pointers, asynchronous on `stream`; scratch from the stream-ordered pool. */
+ * device pointers, asynchronous on `stream`.  Scratch, here and for
+ * input_gradient, from the stream-ordered pool (which keeps it for later calls):
+ * the logits live there for a block of rows at a time, as fp32 (m <= 8) or as the
+ * f16 planes of exp(z - max), up to about 1 GiB for a block; from 2048 bf16
+ * rows on the weights' f16 planes, 2 bytes per weight (4 for the loss), unless
+ * that is more than 4 GiB or cannot be had: then the packed words are unpacked
+ * for every row tile, about a tenth slower. */
 int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, int dtype, const int64_t* targets,
                                        const float* row_scale, float* loss, float* lse, void* dx, uint32_t m,
                                        void* stream);
@@ -270,6 +276,11 @@ int spaceslug_q4_device_status(int device);
  * entry points) or spaceslug_q4_device_status reports it (asynchronous ones).
  * Synchronises the device first.  For tests of the timeout path only. */
 int spaceslug_q4_debug_wait_test(uint64_t wait_limit_ns, int stall);
+/* Test hook: the bytes of scratch that a block of rows of
+ * spaceslug_q4_weights_input_gradient and _cross_entropy may take (a block is
+ * 256 rows at least), and those of the weights' planes (more: they are read as
+ * words); 0: 2^30 and 2^32, the most.  For the whole process, from the next call on. */
+int spaceslug_q4_debug_train_scratch(uint64_t row_bytes, uint64_t weight_bytes);
 
 /* Number of kernels this library has launched since load (all devices). */
 uint64_t spaceslug_q4_launch_count(void);

@@ -1317,11 +1317,14 @@ bool rows_kernels_pay(int M, const spaceslug_q4_weights* w, bool bf16) {
     return M <= 8 && static_cast<double>(M) * w->N * w->K <= (bf16 ? 64e6 : 128e6);
 }
 constexpr int kFewRowsCost = 560;  // shared-memory cycles of a block of 128 n x 128 k and plane of the weights
-constexpr long long kTrainScratch = 1ll << 30;  // bytes of operand planes and partial sums per block of rows
+// Most bytes of a training call's scratch: the rows' operand planes and partial sums of one block of rows, and the
+// weights' planes (spaceslug_q4_debug_train_scratch sets less).
+constexpr long long kTrainRowBytes = 1ll << 30, kTrainWeightBytes = 4ll << 30;
+std::atomic<long long> g_train_row_bytes{kTrainRowBytes}, g_train_weight_bytes{kTrainWeightBytes};
 
 // Rows per block: as many as the scratch holds, in even blocks of whole tiles.
 int train_block(int M, long long row_bytes) {
-    const long long most = std::clamp<long long>(kTrainScratch / row_bytes / 256 * 256, 256, 1 << 20);
+    const long long most = std::clamp<long long>(g_train_row_bytes.load() / row_bytes / 256 * 256, 256, 1 << 20);
     const long long blocks = (M + most - 1) / most;
     return static_cast<int>(((M + blocks - 1) / blocks + 255) / 256 * 256);
 }
@@ -1355,21 +1358,26 @@ void encode_grad_out(CUtensorMap* map, const void* out, uint64_t rows, int K) {
 // The weights of one training call: the handle's words and scales, dequantised
 // by the products themselves, or, where many row tiles would each do that
 // again, planes that one kernel writes into scratch first.  Measured on B200
-// (planes / words): bf16 dX at k = 4096, n = 11008: 113 / 98 us at 1024 rows, 207
-// / 199 at 1536, 192 / 196 at 2048, 363 / 406 at 4096; bf16 loss at k = 4096, n =
-// 32000: 689 / 654, 980 / 961, 1248 / 1291 and 2409 / 2541 us.  fp32 products,
+// (planes / words): bf16 dX at k = 4096, n = 11008: 102 / 100 us at 1024 rows, 152
+// / 156 at 1536, 164 / 177 at 2048, 307 / 347 at 4096; bf16 loss and dX at k =
+// 4096, n = 32000: 680 / 660, 1022 / 1026, 1300 / 1400 and 2330 / 2550 us.  fp32 products,
 // three MMAs per weight, are not bound by the dequantisation: 5337 / 5131 us at
 // 4096 rows, words always.
 constexpr int kPlaneRows = 2048;
 struct TrainWeights {
     spaceslug_q4_weights* w;
-    bool from_planes;
+    bool from_planes = false;
     Scratch planes;  // hi [N][K] f16, and for the logits lo [N][K]
     void* lo = nullptr;
-    TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s)
-        : w(h), from_planes(bf16 && M >= kPlaneRows),
-          planes(from_planes ? static_cast<size_t>(h->N) * h->K * (logits ? 4 : 2) : 0, s) {
-        if (!from_planes) return;
+    TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s) : w(h), planes(0, s) {
+        const long long bytes = static_cast<long long>(h->N) * h->K * (logits ? 4 : 2);
+        if (!bf16 || M < kPlaneRows || bytes > g_train_weight_bytes.load()) return;
+        if (cudaMallocAsync(&planes.p, static_cast<size_t>(bytes), s) != cudaSuccess) {  // the words need no memory
+            planes.p = nullptr;
+            cudaGetLastError();
+            return;
+        }
+        from_planes = true;
         if (logits) lo = static_cast<char*>(planes.p) + static_cast<size_t>(w->N) * w->K * 2;
         check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, planes.p, lo, w->N, w->K, s),
                      "weight planes");
@@ -2692,6 +2700,14 @@ int spaceslug_q4_debug_wait_test(uint64_t wait_limit_ns, int stall) {
         check(static_cast<cudaError_t>(q4::gemv_imma_set_wait_test(lim, st)), "set the IMMA GEMV test hook");
         return SPACESLUG_OK;
     });
+}
+
+int spaceslug_q4_debug_train_scratch(uint64_t row_bytes, uint64_t weight_bytes) {
+    if (row_bytes > static_cast<uint64_t>(kTrainRowBytes) || weight_bytes > static_cast<uint64_t>(kTrainWeightBytes))
+        return fail(SPACESLUG_INVALID_ARGUMENT, "at most 2^30 and 2^32 bytes");
+    g_train_row_bytes = row_bytes ? static_cast<long long>(row_bytes) : kTrainRowBytes;
+    g_train_weight_bytes = weight_bytes ? static_cast<long long>(weight_bytes) : kTrainWeightBytes;
+    return SPACESLUG_OK;
 }
 
 uint64_t spaceslug_q4_launch_count(void) { return g_launches.load(); }

@@ -47,3 +47,9 @@ def test_binding_names_element_types(session):
 
 def test_capabilities_list_the_training_calls(session):
     assert {"act8_checkpoint", "lora_training_act8", "q4_input_gradient", "q4_cross_entropy"} <= set(session.capabilities())
+
+
+def test_scratch_hook_bounds(session):
+    hook = session.raw("spaceslug_q4_debug_train_scratch")
+    assert hook((1 << 30) + 1, 0) == 1 and hook(0, (1 << 32) + 1) == 1
+    assert hook(1, 1) == 0 and hook(0, 0) == 0

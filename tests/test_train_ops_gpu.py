@@ -828,3 +828,70 @@ def test_input_gradient_with_zero_columns_of_a(session, cuda, m, zero, dtype):
     _check_dx(bare, dtype, ref, S)
     _check_dx(dx, dtype, ref + 2.0 * (D @ B64.T) @ A64.T, S + 2 * 2.0 * (D.abs() @ B64.abs().T) @ A64.abs().T)
     assert session.device_status(0) == 0
+
+
+@pytest.fixture
+def scratch(session):
+    hook = session.raw("spaceslug_q4_debug_train_scratch")
+    yield lambda rows, weights: hook(rows, weights)
+    assert hook(0, 0) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("weights", [0, 1])  # from 2048 bf16 rows: from planes, and from words
+@pytest.mark.parametrize("m,k,n,rank", [(257, 96, 300, 0), (515, 160, 1003, 5), (700, 288, 515, 33), (2100, 416, 130, 16)])
+def test_input_gradient_in_blocks_of_rows(session, cuda, scratch, m, k, n, rank, weights, dtype):
+    """Blocks of 256 rows and a ragged last one, with the bounds of one block."""
+    assert scratch(1, weights) == 0
+    test_input_gradient(session, cuda, m, k, n, rank, 0, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("weights", [0, 1])
+@pytest.mark.parametrize("m,k,n", [(257, 96, 300), (515, 160, 1003), (700, 288, 257), (2100, 416, 515)])
+def test_cross_entropy_in_blocks_of_rows(session, cuda, scratch, m, k, n, weights, dtype):
+    """The same for the loss: with lse, row_scale, ignored rows, dx in place of x, and the loss alone."""
+    assert scratch(1, weights) == 0
+    test_cross_entropy(session, cuda, m, k, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_blocks_of_rows_captured_on_two_streams(session, cuda, scratch, dtype):
+    """Two graphs of calls in three blocks, replayed side by side: the results of an eager call, which are those of one
+    block for the loss (whose logits are not split)."""
+    import torch
+    m, k, n = 600, 160, 1003
+    packed, scales = _weights(k, n, 67)
+    x, dy = _randn((m, k), cuda, 5).to(_dt(dtype)), _randn((m, n), cuda, 6).to(_dt(dtype))
+    t = torch.randint(0, n, (m,), device=cuda)
+    new = lambda: [torch.full((m,), float("nan"), device=cuda), torch.full((m,), float("nan"), device=cuda),
+                   torch.full_like(x, float("nan")), torch.full_like(x, float("nan"))]
+    st = [torch.cuda.Stream(cuda) for _ in range(2)]
+    with session.weights(packed, scales, k, n) as h:
+        def run(o, s):
+            h.cross_entropy(x.data_ptr(), t.data_ptr(), o[0].data_ptr(), m, lse=o[1].data_ptr(), dx=o[2].data_ptr(),
+                            dtype=dtype, stream=s.cuda_stream)
+            h.input_gradient(dy.data_ptr(), o[3].data_ptr(), m, dtype=dtype, stream=s.cuda_stream)
+
+        whole, ref, outs = new(), new(), [new(), new()]
+        torch.cuda.synchronize()
+        run(whole, st[0])
+        torch.cuda.synchronize()
+        assert scratch(1, 0) == 0
+        run(ref, st[0])
+        torch.cuda.synchronize()
+        assert torch.equal(ref[0], whole[0]) and torch.equal(ref[1], whole[1])
+        graphs = []
+        for i in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st[i]):
+                run(outs[i], st[i])
+            graphs.append(g)
+        for _ in range(5):
+            for i in range(2):
+                with torch.cuda.stream(st[i]):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, ref))
+        del graphs
+    assert session.device_status(0) == 0
