@@ -321,7 +321,10 @@ int spaceslug_q4_weights_run_push(spaceslug_q4_weights* w, const float* x, float
                                   float* const* peer_y, uint32_t npeers, void* stream);
 /* Caps the SMs a GEMM launch of this handle occupies (0: all, else >= 2), so
  * that kernels on other streams (an exchange running beside the GEMM) find
- * free SMs.  Decode-sized launches (m <= 8) ignore it. */
+ * free SMs.  Decode-sized launches (m <= 8) ignore it.  Of the training calls
+ * lora_backward_act8, input_gradient and cross_entropy keep their persistent
+ * launches (the products and the adapter's passes) to it; their short ones
+ * (casts, planes, sums, statistics), m <= 8 and lora_backward ignore it. */
 int spaceslug_q4_weights_set_sm_budget(spaceslug_q4_weights* w, uint32_t sms);
 /* Stores rows [0, rows) x columns [0, width) of the pitched fp32 block at
  * `src` (row pitch ld floats) to the same offsets in npeers (<= 7) peer-mapped

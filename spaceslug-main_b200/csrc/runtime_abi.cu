@@ -1180,6 +1180,11 @@ const char* rows_error(const void* in, const void* out, int dtype, uint32_t m) {
     return nullptr;
 }
 
+// SMs that a persistent launch of this handle may occupy.
+int budget_sms(const spaceslug_q4_weights* w, const DeviceCtx& c) {
+    return w->sm_budget > 0 ? std::min(c.sm_count, w->sm_budget) : c.sm_count;
+}
+
 // The adapter's gradients with X in 8 bits, into the handle (and to da, db):
 // all four products in the passes of lora16.cu, an fp32 dY with a rank up to 16
 // included; for fp32 dY with a higher rank the two products of X there and the
@@ -1189,6 +1194,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
                             int M, float* da, float* db, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
     const int K = w->K, N = w->N, r = w->rank, rp = q4::lora16_rp(r), rt = q4::lora_tc_rp(r), G = K / 32;
+    const int sms = budget_sms(w, c);
     const float scale = w->alpha / static_cast<float>(r);
     auto round8 = [](int v) { return (static_cast<long long>(v) + 7) / 8 * 8; };
     const long long Kp = round8(K), Np = round8(N), Mp = round8(M);
@@ -1206,13 +1212,13 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     int s1[2], s2[2];  // splits of {T, G} and {dA, dB}
     const int st = q4::lora16_stage();
     if (one) {
-        q4::lora_tc_plan(2, R1, L1, c.sm_count, s1, st);
-        q4::lora_tc_plan(2, R2, L2, c.sm_count, s2, st);
+        q4::lora_tc_plan(2, R1, L1, sms, s1, st);
+        q4::lora_tc_plan(2, R2, L2, sms, s2, st);
     } else {
-        q4::lora_tc_plan(1, R1, L1, c.sm_count, s1, st);
-        q4::lora_tc_plan(1, R1 + 1, L1 + 1, c.sm_count, s1 + 1);
-        q4::lora_tc_plan(1, R2, L2, c.sm_count, s2, st);
-        q4::lora_tc_plan(1, R2 + 1, L2 + 1, c.sm_count, s2 + 1);
+        q4::lora_tc_plan(1, R1, L1, sms, s1, st);
+        q4::lora_tc_plan(1, R1 + 1, L1 + 1, sms, s1 + 1);
+        q4::lora_tc_plan(1, R2, L2, sms, s2, st);
+        q4::lora_tc_plan(1, R2 + 1, L2 + 1, sms, s2 + 1);
     }
     const int rg = one ? rp : rt;  // padded rank of the dY passes
     // planes: A^T and G^T (bf16), B and T^T (bf16 or TF32); partial sums of both passes
@@ -1262,7 +1268,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
         q4::LoraTcPass p{};
         p.count = 1;
         p.rp = rt;
-        p.sm_count = c.sm_count;
+        p.sm_count = sms;
         p.status = c.status;
         p.mn_major = mn ? 1 : 0;
         q4::LoraTcProblem& q = p.prob[0];
@@ -1284,7 +1290,7 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
     check_launch(q4::launch_lora16_finish(f, 2, s), "lora A / B planes");
     q4::Lora16Pass p{};
     p.rp = rp;
-    p.sm_count = c.sm_count;
+    p.sm_count = sms;
     p.status = c.status;
     p.count = one ? 2 : 1;
     x_problem(p.prob[0], false, at, s1[0], partT);
@@ -1439,17 +1445,11 @@ void run_input_gradient_rows(spaceslug_q4_weights* w, const void* dy, void* dx, 
                  "dX");
 }
 
-// The products of up to kFewRows rows (q4_few_rows.cu): SMs they may occupy, and
-// the shared-memory cycles of a block, which the splits are weighed by.
-int few_rows_sms(const spaceslug_q4_weights* w, const DeviceCtx& c) {
-    return w->sm_budget > 0 ? std::min(c.sm_count, w->sm_budget) : c.sm_count;
-}
-
 // dX of up to kFewRows rows: planes of dY, the product in splits of n, and the
 // adapter's side in fp32 as for fewer rows.
 void run_input_gradient_few(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
-    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, sms = few_rows_sms(w, c);
+    const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, sms = budget_sms(w, c);
     const long long ld = (static_cast<long long>(N) + 63) / 64 * 64;
     const TrainWeights weights(w, bf16, false, M, s);
     q4::FewRowsArgs g{};
@@ -1501,6 +1501,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
     }
     DeviceCtx& c = ctx_for(w->device);
     const int N = w->N, K = w->K, r = w->rank, planes = bf16 ? 1 : 2, pairs = grad_pairs(w);
+    const int sms = budget_sms(w, c);
     const size_t size = bf16 ? 2 : 4;
     // contraction: N padded to whole 64-wide stages, and one more stage for the adapter's G A^T
     const int wstages = (N + 63) / 64;
@@ -1542,7 +1543,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         g.out_rows = g.row_tiles * 256;
         g.plane_rows = mc;
         int gsplits = 1;
-        if (r > 0) q4::lora_tc_plan(1, &mc, &N, c.sm_count, &gsplits, bf16 ? q4::lora16_stage() : 32);
+        if (r > 0) q4::lora_tc_plan(1, &mc, &N, sms, &gsplits, bf16 ? q4::lora16_stage() : 32);
         const size_t b_x = static_cast<size_t>(planes) * mc * ld * 2, b_re = static_cast<size_t>(mc) * sizeof(int);
         const size_t b_part = g.splits > 1 ? static_cast<size_t>(g.splits) * g.out_rows * K * 4 : 0;
         const size_t b_g = r > 0 ? static_cast<size_t>(gsplits) * mc * rp * 4 : 0;
@@ -1564,7 +1565,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
         }
         if (r > 0 && bf16) {
             q4::Lora16Pass p{};
-            p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
+            p.count = 1; p.rp = rp; p.sm_count = sms; p.status = c.status;
             q4::Lora16Problem& q = p.prob[0];
             encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rows, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
                       ld_d, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -1575,7 +1576,7 @@ void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool 
             check_launch(q4::launch_lora16_pass(p, s), "dY B^T");
         } else if (r > 0) {
             q4::LoraTcPass p{};
-            p.count = 1; p.rp = rp; p.sm_count = c.sm_count; p.status = c.status;
+            p.count = 1; p.rp = rp; p.sm_count = sms; p.status = c.status;
             q4::LoraTcProblem& q = p.prob[0];
             encode_2d(&q.tm_a, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, rows, static_cast<uint64_t>(N), static_cast<uint64_t>(mc),
                       ld_d, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -1648,7 +1649,7 @@ void run_cross_entropy_rows(spaceslug_q4_weights* w, const void* x, bool bf16, c
 void run_cross_entropy_few(spaceslug_q4_weights* w, const void* x, bool bf16, const long long* targets,
                            const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     DeviceCtx& c = ctx_for(w->device);
-    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, sms = few_rows_sms(w, c), rp = q4::few_rows_padded(M);
+    const int N = w->N, K = w->K, planes = bf16 ? 1 : 2, sms = budget_sms(w, c), rp = q4::few_rows_padded(M);
     const int tiles = (N + 127) / 128, ktiles = (K + 127) / 128;
     const long long ld_p = static_cast<long long>(tiles) * 128;
     const int splits =

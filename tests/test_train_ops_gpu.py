@@ -9,6 +9,8 @@ Then lse is off by dz + 2^-20 (1 + |lse|), a loss by twice that, a probability b
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -894,4 +896,80 @@ def test_blocks_of_rows_captured_on_two_streams(session, cuda, scratch, dtype):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for o in outs for a, b in zip(o, ref))
         del graphs
+    assert session.device_status(0) == 0
+
+
+class _KernelNode(ctypes.Structure):  # CUDA_KERNEL_NODE_PARAMS of the driver API
+    _fields_ = [("func", ctypes.c_void_p), ("grid", ctypes.c_uint * 3), ("block", ctypes.c_uint * 3),
+                ("shared", ctypes.c_uint), ("params", ctypes.c_void_p), ("extra", ctypes.c_void_p),
+                ("kern", ctypes.c_void_p), ("ctx", ctypes.c_void_p)]
+
+
+def _persistent_grids(call, stream):
+    """Blocks of the launches that call() makes with more than half an SM's shared memory each, in order of capture."""
+    import torch
+    g = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(g, stream=stream):
+        call()
+    cu, raw, count, out = ctypes.CDLL("libcuda.so.1"), ctypes.c_void_p(g.raw_cuda_graph()), ctypes.c_size_t(0), []
+    assert cu.cuGraphGetNodes(raw, None, ctypes.byref(count)) == 0
+    nodes = (ctypes.c_void_p * count.value)()
+    assert cu.cuGraphGetNodes(raw, nodes, ctypes.byref(count)) == 0
+    for node in nodes:
+        kind, p = ctypes.c_int(-1), _KernelNode()
+        assert cu.cuGraphNodeGetType(ctypes.c_void_p(node), ctypes.byref(kind)) == 0
+        if kind.value == 0:
+            assert cu.cuGraphKernelNodeGetParams_v2(ctypes.c_void_p(node), ctypes.byref(p)) == 0
+            if p.shared > 114 * 1024:
+                out.append(p.grid[0])
+    return out
+
+
+@pytest.mark.parametrize("dtype,rank", [("f32", 8), ("f32", 33), ("bf16", 8), ("bf16", 64)])
+@pytest.mark.parametrize("m", [40, 600])
+def test_persistent_launches_keep_to_the_sm_budget(session, cuda, m, dtype, rank):
+    """Every launch of a training call that takes an SM's shared memory for itself, the adapter's passes among them, has
+    as many blocks as the budget allows at most, and more without one; the results hold their bounds."""
+    import torch
+    k, n = 1056, 4099
+    packed, scales = _weights(k, n, 71)
+    rng = np.random.default_rng(3)
+    A, B = (rng.standard_normal(s).astype(np.float32) * 0.02 for s in ((k, rank), (rank, n)))
+    x, dy = _randn((m, k), cuda, 1), _randn((m, n), cuda, 2).to(_dt(dtype))
+    codes, exps, back = _act8(session, x, "f32")
+    xs = x.to(dy.dtype)
+    t, loss = torch.randint(0, n, (m,), device=cuda), torch.empty((m,), device=cuda)
+    dx, dl = torch.empty_like(xs), torch.empty_like(xs)
+    da, db = torch.empty((k, rank), device=cuda), torch.empty((rank, n), device=cuda)
+    st = torch.cuda.Stream(cuda)
+    W, D, A64, B64 = _w64(packed, scales, k, n, cuda), dy.double(), *(torch.from_numpy(v).to(cuda).double() for v in (A, B))
+    X = back.double()
+    with session.weights(packed, scales, k, n) as h, session.weights(packed, scales, k, n) as head:
+        h.set_lora(A, B, 2.0 * rank)
+        calls = dict(
+            back=lambda s: h.lora_backward_act8(codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m, dtype=dtype,
+                                                da=da.data_ptr(), db=db.data_ptr(), stream=s),
+            dx=lambda s: h.input_gradient(dy.data_ptr(), dx.data_ptr(), m, dtype=dtype, stream=s),
+            loss=lambda s: head.cross_entropy(xs.data_ptr(), t.data_ptr(), loss.data_ptr(), m, dx=dl.data_ptr(),
+                                              dtype=dtype, stream=s))
+        for call in calls.values():  # first calls allocate
+            call(0)
+        torch.cuda.synchronize()
+        for name, call in calls.items():
+            for budget in (6, 0):
+                h.set_sm_budget(budget)
+                head.set_sm_budget(budget)
+                grids = _persistent_grids(lambda: call(st.cuda_stream), st)
+                assert len(grids) >= (1 if name == "dx" else 2), (name, grids)
+                if budget:
+                    assert max(grids) <= budget, (name, grids)
+                else:
+                    assert max(grids) > 6, (name, grids)
+        h.set_sm_budget(6)
+        calls["back"](0)
+        calls["dx"](0)
+    _check_dx(dx, dtype, D @ W.T + 2.0 * (D @ B64.T) @ A64.T, D.abs() @ W.abs().T + 4.0 * (D.abs() @ B64.abs().T) @ A64.abs().T)
+    for got, ref, S in ((da, 2.0 * X.T @ (D @ B64.T), 2.0 * X.abs().T @ (D.abs() @ B64.abs().T)),
+                        (db, 2.0 * (X @ A64).T @ D, 2.0 * (X.abs() @ A64.abs()).T @ D.abs())):
+        assert ((got.double() - ref).abs() <= 2 * 2.0 ** -16 * S).all()
     assert session.device_status(0) == 0
