@@ -204,7 +204,9 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
  * f16 planes of exp(z - max), up to about 1 GiB for a block; from 2048 bf16
  * rows on the weights' f16 planes, 2 bytes per weight (4 for the loss), unless
  * that is more than 4 GiB or cannot be had: then the packed words are unpacked
- * for every row tile, about a tenth slower. */
+ * for every row tile, about a tenth slower.  Where k % 128 != 0 the first of
+ * these calls with more than 8 rows that is not captured gives the handle a copy
+ * of its scales in rows of 16-byte multiples, and waits for it. */
 int spaceslug_q4_weights_cross_entropy(spaceslug_q4_weights* w, const void* x, int dtype, const int64_t* targets,
                                        const float* row_scale, float* loss, float* lse, void* dx, uint32_t m,
                                        void* stream);

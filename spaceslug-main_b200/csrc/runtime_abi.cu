@@ -954,7 +954,10 @@ struct spaceslug_q4_weights {
     uint32_t col_begin = 0, n_total = 0;
     uint32_t* packed = nullptr;
     float* scales = nullptr;
-    float* scales_pad = nullptr;  // scales with rows of 16-byte multiples (training products, k % 128 != 0)
+    // Scales with rows of 16-byte multiples, as TMA asks where k % 128 != 0: made by the first training product that
+    // needs them (padded_scales), so that a handle that only infers does not hold them.
+    float* scales_pad = nullptr;
+    std::mutex pad_mu;
     int* col_exp = nullptr;
     float* lora_a = nullptr;
     float* lora_b = nullptr;
@@ -985,19 +988,10 @@ struct spaceslug_q4_weights {
     int adam_step = 0;
 };
 
-// What the training products need beside a handle's words and scales, laid out
-// once: the least column exponent (one power of two for the whole handle) and,
-// where k % 128 != 0, a copy of the scales whose rows are 16-byte multiples, as
-// TMA asks.  On the context's stream.
+// What the training products need beside a handle's words and scales from its
+// start: the least column exponent (one power of two for the whole handle).
 void prepare_training(spaceslug_q4_weights* w, cudaStream_t s) {
     check_launch(q4::launch_min_exp(w->col_exp, w->scales, w->col_exp + w->N, w->N, w->K, s), "min_exp");
-    const size_t G = static_cast<size_t>(w->K) / 32, Gp = (G + 3) / 4 * 4;
-    if (G == Gp) return;
-    check(cudaMalloc(&w->scales_pad, w->N * Gp * 4), "cudaMalloc padded scales");
-    check(cudaMemsetAsync(w->scales_pad, 0, w->N * Gp * 4, s), "cudaMemset padded scales");
-    check(cudaMemcpy2DAsync(w->scales_pad, Gp * 4, w->scales, G * 4, G * 4, static_cast<size_t>(w->N),
-                            cudaMemcpyDeviceToDevice, s),
-          "cudaMemcpy2D padded scales");
 }
 
 // Caller holds the device's host_mu (or owns the handle exclusively).
@@ -1375,18 +1369,54 @@ struct TrainWeights {
     bool from_planes = false;
     Scratch planes;  // hi [N][K] f16, and for the logits lo [N][K]
     void* lo = nullptr;
-    TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s) : w(h), planes(0, s) {
-        const long long bytes = static_cast<long long>(h->N) * h->K * (logits ? 4 : 2);
-        if (!bf16 || M < kPlaneRows || bytes > g_train_weight_bytes.load()) return;
+    const float* scales = nullptr;  // not from planes: rows of 16-byte multiples
+    Scratch own_scales;
+    TrainWeights(spaceslug_q4_weights* h, bool bf16, bool logits, int M, cudaStream_t s)
+        : w(h), planes(0, s), own_scales(0, s) {
+        if (!take_planes(bf16, logits, M, s)) scales = padded_scales(s);
+    }
+    bool take_planes(bool bf16, bool logits, int M, cudaStream_t s) {
+        const long long bytes = static_cast<long long>(w->N) * w->K * (logits ? 4 : 2);
+        if (!bf16 || M < kPlaneRows || bytes > g_train_weight_bytes.load()) return false;
         if (cudaMallocAsync(&planes.p, static_cast<size_t>(bytes), s) != cudaSuccess) {  // the words need no memory
             planes.p = nullptr;
             cudaGetLastError();
-            return;
+            return false;
         }
         from_planes = true;
         if (logits) lo = static_cast<char*>(planes.p) + static_cast<size_t>(w->N) * w->K * 2;
         check_launch(q4::launch_weight_planes(w->packed, w->scales, w->col_exp + w->N, planes.p, lo, w->N, w->K, s),
                      "weight planes");
+        return true;
+    }
+    // The handle's padded scales.  The first call makes them and waits, so that calls on any stream may read them; a
+    // call that is captured before that (no allocation there) copies them within its graph.
+    const float* padded_scales(cudaStream_t s) {
+        const size_t G = static_cast<size_t>(w->K) / 32, Gp = (G + 3) / 4 * 4, N = static_cast<size_t>(w->N);
+        if (G == Gp) return w->scales;
+        auto pad = [&](void* to) {
+            check(cudaMemcpy2DAsync(to, Gp * 4, w->scales, G * 4, G * 4, N, cudaMemcpyDeviceToDevice, s),
+                  "cudaMemcpy2D padded scales");
+        };
+        std::lock_guard<std::mutex> lk(w->pad_mu);
+        if (w->scales_pad) return w->scales_pad;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            check(cudaMallocAsync(&own_scales.p, N * Gp * 4, s), "cudaMallocAsync padded scales");
+            pad(own_scales.p);
+            return static_cast<const float*>(own_scales.p);
+        }
+        void* made = nullptr;
+        check(cudaMalloc(&made, N * Gp * 4), "cudaMalloc padded scales");
+        try {
+            pad(made);
+            check(cudaStreamSynchronize(s), "cudaStreamSynchronize");
+        } catch (...) {
+            cudaFree(made);
+            throw;
+        }
+        return w->scales_pad = static_cast<float*>(made);
     }
     // tensor maps of the logits' or the transposed product
     template <typename Args>
@@ -1401,7 +1431,6 @@ struct TrainWeights {
             return;
         }
         const uint64_t G = K / 32, Gp = (G + 3) / 4 * 4;
-        const float* scales = w->scales_pad ? w->scales_pad : w->scales;
         encode_2d(&g.tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT32, w->packed, K / 8, N, K / 2, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B);
         encode_2d(&g.tm_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, scales, G, N, Gp * 4, 4, 128, CU_TENSOR_MAP_SWIZZLE_NONE);
     }

@@ -973,3 +973,68 @@ def test_persistent_launches_keep_to_the_sm_budget(session, cuda, m, dtype, rank
                         (db, 2.0 * (X @ A64).T @ D, 2.0 * (X.abs() @ A64.abs()).T @ D.abs())):
         assert ((got.double() - ref).abs() <= 2 * 2.0 ** -16 * S).all()
     assert session.device_status(0) == 0
+
+
+def test_a_handle_that_only_infers_holds_its_weights_alone(session, cuda):
+    """k % 128 != 0: 16 + 4 bytes of words and scales and 4 of exponents per column of 32 k; the training products' padded
+    scales (16 more) come with the first call that needs them."""
+    import torch
+    k, n = 32, 1 << 20
+    packed, scales = np.zeros((n, k // 8), np.uint32), np.full((n, 1), 0.01, np.float32)
+    session.weights(packed, scales, k, n).close()  # staging buffers
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info(cuda)[0]
+    with session.weights(packed, scales, k, n) as h:
+        assert free - torch.cuda.mem_get_info(cuda)[0] <= 24 * n + 4 * (2 << 20)  # blocks of 2 MiB
+        assert h.n == n
+
+
+@pytest.mark.parametrize("k", [32, 96, 416])
+@pytest.mark.parametrize("first", ["captured", "eager", "two_streams"])
+def test_first_training_call_of_a_handle(session, cuda, k, first):
+    """The padded scales of a first call: captured (its graph makes its own, and so does a second graph), eager, or from
+    two streams at once; the same results each way, and a graph of before works beside the handle's copy."""
+    import torch
+    m, n = 20, 777
+    packed, scales = _weights(k, n, 73)
+    dy, x = _randn((m, n), cuda, 1), _randn((m, k), cuda, 2)
+    t = torch.randint(0, n, (m,), device=cuda)
+    W = _w64(packed, scales, k, n, cuda)
+    ref = _loss_ref(x, W, t, torch.ones((m,), device=cuda))
+    st = [torch.cuda.Stream(cuda) for _ in range(2)]
+    new = lambda: [torch.full((m, k), float("nan"), device=cuda), torch.full((m, k), float("nan"), device=cuda),
+                   torch.full((m,), float("nan"), device=cuda), torch.full((m,), float("nan"), device=cuda)]
+    outs = [new(), new()]
+    torch.cuda.synchronize()
+    with session.weights(packed, scales, k, n) as h:
+        def run(o, s):
+            h.input_gradient(dy.data_ptr(), o[0].data_ptr(), m, stream=s.cuda_stream)
+            h.cross_entropy(x.data_ptr(), t.data_ptr(), o[2].data_ptr(), m, lse=o[3].data_ptr(), dx=o[1].data_ptr(),
+                            stream=s.cuda_stream)
+
+        graphs = []
+        if first == "captured":
+            for o, s in zip(outs, st):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    run(o, s)
+                graphs.append(g)
+            for g, s in zip(graphs, st):
+                with torch.cuda.stream(s):
+                    g.replay()
+        else:
+            for o, s in zip(outs, st if first == "two_streams" else st[:1] * 2):
+                run(o, s)
+        torch.cuda.synchronize()
+        after = new()
+        run(after, st[0])
+        for g, s in zip(graphs, st):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o in (*outs, after):
+            _check_dx(o[0], "f32", dy.double() @ W.T, dy.double().abs() @ W.abs().T)
+            _check_loss("f32", (o[2], o[3], o[1]), ref)
+            assert all(torch.equal(a, b) for a, b in zip(o, after))
+        del graphs
+    assert session.device_status(0) == 0
