@@ -1,6 +1,6 @@
 // The training operators on the frozen int4 weights for one to eight rows (up to
-// a size; see rows_kernels_pay), on the CUDA cores in fp32: products that stream
-// the packed weights once.
+// a size; see rows_pay_dx and rows_pay_loss), on the CUDA cores in fp32: products
+// that stream the packed weights once.
 //
 //   rows_logits_kernel   z[m][n]  = sum_k x[m][k] w(k, n), and each 32 columns' max and sum of exponentials
 //   rows_loss_kernel     lse, loss and the rows' coefficients of the gradient

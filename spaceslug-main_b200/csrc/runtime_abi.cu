@@ -1308,13 +1308,43 @@ void run_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const 
 // pairs of q4_grad_gemm.cu (64 / 128 rows: fp32 dX of 4096 x 11008 66 / 95 us,
 // fp32 loss and dX of 2048 x 50000 141 / 249 us: twice 64 rows take no less).
 // Up to 8 rows the CUDA-core kernels of q4_rows.cu, which cost a launch less but
-// more with every row, or those of q4_few_rows.cu, by rows x weights.  Measured
-// on B200 (us, q4_rows / q4_few_rows), dX of 4 rows: 2048 x 2048 15 / 17, 4096 x
-// 4096 25 / 25 in bf16 and 25 / 29 in fp32, 4096 x 11008 39 / 37 and 39 / 43; loss
-// and dX: 4 x 1024 x 8000 31 / 34 and 31 / 36, 8 x 1024 x 8000 37 / 32 and 37 / 34,
-// 2 x 1024 x 32003 50 / 48 and 50 / 57, 8 x 1024 x 32003 72 / 48 and 74 / 59.
-bool rows_kernels_pay(int M, const spaceslug_q4_weights* w, bool bf16) {
-    return M <= 8 && static_cast<double>(M) * w->N * w->K <= (bf16 ? 64e6 : 128e6);
+// more with every row, or those of q4_few_rows.cu.  Measured on B200 for 1 to 8
+// rows, both types, nine sizes of 2^20 to 131e6 weights from HBM, in CUDA graphs
+// (us, q4_rows / q4_few_rows).  For dX the rules take the faster or one within a
+// tenth of it, but for 3 fp32 rows of 1024 x 8000 (13.6 / 11.8; short k: the final
+// sum has few blocks for many splits) and 4 bf16 rows of 4096 x 4096 with an adapter
+// (17.0 / 19.1).
+//
+// dX without an adapter, bf16: 6 and 8 rows of 2048 x 2048 9.5 / 10.0 and 11.1 /
+// 10.0, 2 and 3 of 4096 x 4096 11.5 / 12.6 and 13.4 / 12.7, 1 and 2 of 4096 x 11008
+// 21.1 / 21.9 and 22.4 / 21.7, 1 of 2048 x 32000 29.4 / 26.7; fp32, whose two planes
+// cost q4_few_rows.cu more: 8 of 2048 x 2048 11.1 / 11.2, 5 and 6 of 4096 x 4096 15.1 /
+// 15.8 and 16.3 / 15.6, 4 and 5 of 4096 x 11008 26.8 / 28.1 and 30.0 / 28.0, 3 and 4 of
+// 4096 x 32000 61.9 / 62.5 and 65.0 / 62.3.  With an adapter of rank 16, bf16: 2 and
+// 3 of 2048 x 2048 10.7 / 12.2 and 13.2 / 12.5, 1 of 4096 x 4096 16.4 / 16.2, of 4096 x
+// 11008 30.8 / 26.8; fp32: 5 and 8 of 1024 x 8000 17.4 / 16.8 and 21.6 / 17.9, 6 and 8
+// of 4096 x 4096 20.9 / 22.1 and 23.1 / 22.1, 5 and 6 of 4096 x 11008 35.4 / 36.0 and
+// 37.9 / 36.1, 1 of 2048 x 32000 50.7 / 44.5.
+bool rows_pay_dx(int M, const spaceslug_q4_weights* w, bool bf16) {
+    const double size = static_cast<double>(w->N) * w->K;
+    double most;  // rows
+    if (w->rank > 0)
+        most = bf16 ? 8.4e6 / size : size > 48e6 ? 0.0 : std::max(5.0, (w->K < 2048 ? 34e6 : 118e6) / size);
+    else
+        most = bf16 ? (size > 48e6 ? 0.0 : std::max(2.0, 24e6 / size)) : std::max(4.0, 34e6 / size);
+    return M <= 8 && M <= most;
+}
+// Loss, with dX or alone (the same kernels, for the same loss): q4_few_rows.cu's
+// logits have one CTA per 128 columns, so that a short vocabulary leaves SMs idle.
+// Loss and dX, bf16 and fp32: 8 rows of 11008 x 4096 93 / 94 and 94 / 104, 8 of 4096 x
+// 4096 42 / 42 and 42 / 45, 5 and 8 of 1024 x 8000 23.9 / 24.8, 24.1 / 26.3 and 29.9 /
+// 25.1, 30.2 / 26.9, 1 of 4096 x 11008 48 / 53 and 48 / 59, 2 60 / 53 and 61 / 59, 1 of
+// 1024 x 32003 42.5 / 39.9 and 42.8 / 46.3, of 2048 x 32000 69 / 60 and 69 / 74.  Alone:
+// 8 of 1024 x 8000 13.5 / 15.2 and 13.8 / 15.7, 1 of 4096 x 11008 23 / 31 and 23 / 32, of
+// 1024 x 32003 17.5 / 22.6 and 17.7 / 25.7; the loss alone loses most to the shared
+// rule with 6 bf16 rows of 1024 x 8000, 11.9 / 15.0, and 1 fp32 row of 4096 x 32000, 48 / 62.
+bool rows_pay_loss(int M, const spaceslug_q4_weights* w, bool bf16, int sm_count) {
+    return M <= 8 && (w->N <= 32 * sm_count || static_cast<double>(M) * w->N * w->K <= (bf16 ? 48e6 : 66e6));
 }
 constexpr int kFewRowsCost = 560;  // shared-memory cycles of a block of 128 n x 128 k and plane of the weights
 // Most bytes of a training call's scratch: the rows' operand planes and partial sums of one block of rows, and the
@@ -1520,7 +1550,7 @@ void run_input_gradient_few(spaceslug_q4_weights* w, const void* dy, void* dx, b
 }
 
 void run_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, bool bf16, int M, cudaStream_t s) {
-    if (rows_kernels_pay(M, w, bf16)) {
+    if (rows_pay_dx(M, w, bf16)) {
         run_input_gradient_rows(w, dy, dx, bf16, M, s);
         return;
     }
@@ -1757,7 +1787,7 @@ void run_cross_entropy(spaceslug_q4_weights* w, const void* x, bool bf16, const 
                        const float* row_scale, float* loss, float* lse, void* dx, int M, cudaStream_t s) {
     static_assert(sizeof(long long) == sizeof(int64_t), "targets are int64");
     const long long* targets = reinterpret_cast<const long long*>(targets64);
-    if (rows_kernels_pay(M, w, bf16)) {
+    if (rows_pay_loss(M, w, bf16, ctx_for(w->device).sm_count)) {
         run_cross_entropy_rows(w, x, bf16, targets, row_scale, loss, lse, dx, M, s);
         return;
     }

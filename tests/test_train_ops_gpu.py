@@ -1038,3 +1038,19 @@ def test_first_training_call_of_a_handle(session, cuda, k, first):
             assert all(torch.equal(a, b) for a, b in zip(o, after))
         del graphs
     assert session.device_status(0) == 0
+
+
+# One to eight rows run on either of two sets of kernels, by type, rows, size and adapter: sizes on both sides of the rules.
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,rank", [
+    (1, 1056, 8003, 3), (2, 1056, 8003, 0), (3, 1056, 8003, 0), (8, 2080, 2051, 16), (8, 2080, 2051, 0), (5, 4128, 4099, 16),
+    (7, 4128, 4099, 64), (2, 4128, 11011, 0), (4, 4128, 12003, 0), (1, 32, 3, 2), (8, 96, 70001, 0)])
+def test_one_to_eight_rows_input_gradient(session, cuda, m, k, n, rank, dtype):
+    test_input_gradient(session, cuda, m, k, n, rank, 0, n, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n", [(1, 1056, 32003), (1, 2080, 32003), (2, 1056, 32003), (8, 4128, 4099), (8, 1056, 4736),
+                                   (8, 1056, 4737), (6, 1056, 8003), (1, 32, 70001), (8, 32, 300001)])
+def test_one_to_eight_rows_cross_entropy(session, cuda, m, k, n, dtype):
+    test_cross_entropy(session, cuda, m, k, n, dtype)
