@@ -1054,3 +1054,121 @@ def test_one_to_eight_rows_input_gradient(session, cuda, m, k, n, rank, dtype):
                                    (8, 1056, 4737), (6, 1056, 8003), (1, 32, 70001), (8, 32, 300001)])
 def test_one_to_eight_rows_cross_entropy(session, cuda, m, k, n, dtype):
     test_cross_entropy(session, cuda, m, k, n, dtype)
+
+
+def _linear_with_adapter(m):
+    """Inputs whose adapter weighs more than the weights."""
+    k, n, rank = 512, 320, 8
+    rng = np.random.default_rng(97 + m)
+    A, B, u, dy = ((rng.standard_normal(s) * f).astype(np.float32) for s, f in
+                   (((k, rank), 0.2), ((rank, n), 0.2), ((m, k), 1.0), ((m, n), 1.0)))
+    return k, n, rank, A, B, u, dy
+
+
+@pytest.mark.parametrize("m", [4, 40, 300])
+def test_input_gradient_is_the_transpose_of_the_layer_with_its_adapter(session, cuda, m):
+    """<dY, f(u)> = <dX, u> per row, f by the fp32 decode path in calls of four rows: both sides to 2^-16 of S = sum |dY|
+    |u| (|W| + s |A| |B|), and the adapter's part ten times that over the rows."""
+    import torch
+    k, n, rank, A, B, u, dy = _linear_with_adapter(m)
+    packed, scales = _weights(k, n, 23)
+    W = _w64(packed, scales, k, n, cuda)
+    A64, B64, U, D = (torch.from_numpy(v).to(cuda).double() for v in (A, B, u, dy))
+    u, dy = torch.from_numpy(u).to(cuda), torch.from_numpy(dy).to(cuda)
+    y, dx = torch.empty((m, n), device=cuda), torch.empty((m, k), device=cuda)
+    with session.weights(packed, scales, k, n) as h:
+        h.set_lora(A, B, 2.0 * rank)
+        for i in range(0, m, 4):
+            h.run(u[i:].data_ptr(), y[i:].data_ptr(), 4)
+        h.input_gradient(dy.data_ptr(), dx.data_ptr(), m)
+    tol = 2 * 2.0 ** -16 * (D.abs() * (U.abs() @ W.abs() + 2 * 2.0 * (U.abs() @ A64.abs()) @ B64.abs())).sum(1)
+    adapter = (D * (2.0 * (U @ A64) @ B64)).sum(1).abs()
+    assert adapter.norm() >= 10 * tol.norm()
+    assert ((D * y.double()).sum(1) - (dx.double() * U).sum(1)).abs().le(tol).all()
+    assert session.device_status(0) == 0
+
+
+@pytest.mark.parametrize("m", [6, 40, 200, 2300])
+def test_training_step_in_bf16(session, cuda, m):
+    """The step of test_training_step with bf16 activations and gradients between the calls (the forward takes and gives
+    fp32: the caller casts), each call against 64 bits, and once more as a replayed graph with other inputs."""
+    import torch
+    k, hidden, vocab, rank = 256, 384, 1000, 8
+    layers, head = _net(session, k, hidden, vocab, rank, 83)
+    hs = []
+    for packed, scales, kk, nn, A, B in layers:
+        h = session.weights(packed, scales, kk, nn)
+        h.set_lora(A, B, 2.0 * rank)
+        hs.append(h)
+    hv = session.weights(*head)
+    st, b16 = torch.cuda.Stream(cuda), torch.bfloat16
+    x = _randn((m, k), cuda, 15).to(b16)
+    t = torch.randint(0, vocab, (m,), device=cuda)
+    scale = torch.full((m,), 1.0 / m, device=cuda)
+    xf, y1, y2 = torch.empty((m, k), device=cuda), torch.empty((m, hidden), device=cuda), torch.empty((m, k), device=cuda)
+    h1, h2 = torch.empty((m, hidden), device=cuda, dtype=b16), torch.empty((m, k), device=cuda, dtype=b16)
+    c1, e1 = torch.empty((m, k), dtype=torch.int8, device=cuda), torch.empty((m, k // 32), dtype=torch.uint8, device=cuda)
+    c2, e2 = torch.empty((m, hidden), dtype=torch.int8, device=cuda), torch.empty((m, hidden // 32), dtype=torch.uint8, device=cuda)
+    loss, lse = torch.empty((m,), device=cuda), torch.empty((m,), device=cuda)
+    d2, d1 = torch.empty((m, k), device=cuda, dtype=b16), torch.empty((m, hidden), device=cuda, dtype=b16)
+    g = [(torch.empty((kk, rank), device=cuda), torch.empty((rank, nn), device=cuda)) for _, _, kk, nn, _, _ in layers]
+
+    def step():
+        s = st.cuda_stream
+        session.act8_pack_device(x.data_ptr(), c1.data_ptr(), e1.data_ptr(), m, k, dtype="bf16", stream=s)
+        xf.copy_(x)
+        hs[0].run(xf.data_ptr(), y1.data_ptr(), m, s)
+        h1.copy_(y1)
+        session.act8_pack_device(h1.data_ptr(), c2.data_ptr(), e2.data_ptr(), m, hidden, dtype="bf16", stream=s)
+        hs[1].run(y1.data_ptr(), y2.data_ptr(), m, s)
+        h2.copy_(y2)
+        hv.cross_entropy(h2.data_ptr(), t.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=d2.data_ptr(),
+                         row_scale=scale.data_ptr(), dtype="bf16", stream=s)
+        hs[1].lora_backward_act8(c2.data_ptr(), e2.data_ptr(), d2.data_ptr(), m, dtype="bf16", da=g[1][0].data_ptr(),
+                                 db=g[1][1].data_ptr(), stream=s)
+        hs[1].input_gradient(d2.data_ptr(), d1.data_ptr(), m, dtype="bf16", stream=s)
+        hs[0].lora_backward_act8(c1.data_ptr(), e1.data_ptr(), d1.data_ptr(), m, dtype="bf16", da=g[0][0].data_ptr(),
+                                 db=g[0][1].data_ptr(), stream=s)
+
+    W = [_w64(p, s, kk, nn, cuda) for p, s, kk, nn, _, _ in layers]
+    AB = [(torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()) for *_, A, B in layers]
+    Wv = _w64(*head, cuda)
+
+    def check():
+        torch.cuda.synchronize()
+        rl, rloss, rdx, Sdx, S = _loss_ref(h2, Wv, t, scale)
+        _check_loss("bf16", (loss, lse, None), (rl, rloss, rdx, Sdx, S))
+        # As _check_loss, and what f16 leaves of a p far below its tile's largest: 2^14 p / max p is kept in steps of 2^-24
+        # at least, so p is off by 2^-25 / 2^14 = 2^-39 of that largest, which is at most 1.  With logits as far apart as
+        # these (loss 30 and more) it shows where neither the likely token's nor the target's weight is nonzero.
+        tol = (2 * 2.0 ** -16 * S[:, None] + 2.0 ** -16 + 2.0 ** -10) * Sdx + 2.0 ** -8 * rdx.abs() + 1e-37
+        tol += 2.0 ** -39 * scale[:, None].double() * Wv.abs().sum(1)
+        assert ((d2.double() - rdx).abs() <= tol).all(), float(((d2.double() - rdx).abs() / tol).max())
+        X1 = c1.double() * torch.exp2(e1.double() - 127).repeat_interleave(32, 1)
+        X2 = c2.double() * torch.exp2(e2.double() - 127).repeat_interleave(32, 1)
+        for X, D, (A, B), (da, db) in ((X2, d2.double(), AB[1], g[1]), (X1, d1.double(), AB[0], g[0])):
+            for got, ref, S in ((da, 2.0 * X.T @ (D @ B.T), 2.0 * X.abs().T @ (D.abs() @ B.abs().T)),
+                                (db, 2.0 * (X @ A).T @ D, 2.0 * (X.abs() @ A.abs()).T @ D.abs())):
+                assert ((got.double() - ref).abs() <= 2 * 2.0 ** -16 * S).all()
+        D, (A, B) = d2.double(), AB[1]
+        _check_dx(d1, "bf16", D @ W[1].T + 2.0 * (D @ B.T) @ A.T, D.abs() @ W[1].abs().T + 4.0 * (D.abs() @ B.abs().T) @ A.abs().T)
+        # 8-bit copies: half a step per element
+        assert ((X2 - h1.double()).abs() <= torch.exp2(e2.double() - 128).repeat_interleave(32, 1)).all()
+
+    with torch.cuda.stream(st):
+        step()
+        check()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            step()
+        x.copy_(_randn((m, k), cuda, 16))
+        t.copy_(torch.randint(0, vocab, (m,), device=cuda))
+        for v in (loss, lse, d2, d1):
+            v.fill_(float("nan"))
+        st.synchronize()
+        graph.replay()
+        check()
+    del graph
+    for h in (*hs, hv):
+        h.close()
+    assert session.device_status(0) == 0
