@@ -1172,3 +1172,141 @@ def test_training_step_in_bf16(session, cuda, m):
     for h in (*hs, hv):
         h.close()
     assert session.device_status(0) == 0
+
+
+# --------------------------------------------------------------------------------------- calls at the documented edges --
+def test_act8_edges_in_bf16(session, cuda):
+    """The edges of test_act8_edges that bf16 has, with step bytes that begin at an odd address."""
+    import torch
+    rows = np.zeros((9, 64), np.float32)
+    rows[0, :3] = 127.0, -127.0, 0.5
+    rows[1, :3] = 127.5, 1.0, 3.0
+    rows[2, :2] = 3.3895313892515355e38, 1.0  # the largest bf16
+    rows[3, :2] = 2.0 ** -126, -(2.0 ** -133)
+    rows[4, 1], rows[4, 40] = np.inf, 3.0
+    rows[5, 33], rows[5, 2] = np.nan, -5.0
+    rows[6, :4] = 64.0, 63.5, 62.5, -61.5
+    rows[7, :] = -0.0
+    rows[8, :] = 2.0 ** 100
+    x = torch.from_numpy(rows).to(cuda).bfloat16()
+    codes = torch.full((9, 64), 77, dtype=torch.int8, device=cuda)
+    room, back = torch.full((1 + 18 + 5,), 99, dtype=torch.uint8, device=cuda), torch.empty_like(x)
+    session.act8_pack_device(x.data_ptr(), codes.data_ptr(), room.data_ptr() + 1, 9, 64, dtype="bf16")
+    session.act8_unpack_device(codes.data_ptr(), room.data_ptr() + 1, back.data_ptr(), 9, 64, dtype="bf16")
+    c, e = _act8_oracle(x.float().cpu().numpy())
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(room[1:19].cpu().numpy().reshape(9, 2), e)
+    assert room[0] == 99 and (room[19:] == 99).all()
+    bad = np.repeat(e == 255, 32, 1)
+    b = back.double().cpu().numpy()
+    assert bad.sum() == 2 * 32 and np.isnan(b[bad]).all()
+    assert np.array_equal(b[~bad], (c * np.exp2(e.astype(np.float64) - 127).repeat(32, 1))[~bad])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [5, 40, 300])
+def test_cross_entropy_targets_at_the_ends_of_int64(session, cuda, m, dtype):
+    """The least int64 takes a row out, the greatest (and one that is the column count past 2^32) is past the columns."""
+    import torch
+    k, n = 64, 300
+    packed, scales = _weights(k, n, 89)
+    x = _randn((m, k), cuda, 1).to(_dt(dtype))
+    t = torch.randint(0, n, (m,), device=cuda)
+    t[1], t[3], t[4] = -2 ** 63, 2 ** 63 - 1, 2 ** 32 + 7
+    loss, lse, dx = torch.empty((m,), device=cuda), torch.empty((m,), device=cuda), torch.empty_like(x)
+    with session.weights(packed, scales, k, n) as h:
+        h.cross_entropy(x.data_ptr(), t.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=dx.data_ptr(), dtype=dtype)
+    assert torch.isnan(loss[3:5]).all() and torch.isnan(dx[3:5]).all() and loss[1] == 0 and not dx[1].any()
+    keep = torch.tensor([i for i in range(m) if i not in (3, 4)], device=cuda)
+    ref = [v[keep] for v in _loss_ref(x, _w64(packed, scales, k, n, cuda), torch.where(t >= n, 0, t), torch.ones((m,), device=cuda))]
+    _check_loss(dtype, (loss[keep], lse[keep], dx[keep]), ref)
+    assert session.device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [3, 40, 300, 2050])
+def test_zero_and_negative_scales(session, cuda, m, dtype):
+    """A handle of zeros (a uniform softmax, no gradient; dX from the adapter alone) and one with negative scales."""
+    import torch
+    k, n, rank = 96, 515, 3
+    packed, scales = _weights(k, n, 91)
+    rng = np.random.default_rng(5)
+    A, B = (rng.standard_normal(s).astype(np.float32) * 0.1 for s in ((k, rank), (rank, n)))
+    A64, B64 = torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()
+    x, dy = _randn((m, k), cuda, 1).to(_dt(dtype)), _randn((m, n), cuda, 2).to(_dt(dtype))
+    t, ones = torch.randint(0, n, (m,), device=cuda), torch.ones((m,), device=cuda)
+    loss, lse, dl, dx = torch.empty((m,), device=cuda), torch.empty((m,), device=cuda), torch.empty_like(x), torch.empty_like(x)
+    signs = np.where(rng.random(scales.shape) < 0.5, -1.0, 1.0).astype(np.float32)
+    for sc in (np.zeros_like(scales), scales * signs):
+        W = _w64(packed, sc, k, n, cuda)
+        with session.weights(packed, sc, k, n) as h:
+            h.cross_entropy(x.data_ptr(), t.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=dl.data_ptr(), dtype=dtype)
+            h.set_lora(A, B, 2.0 * rank)
+            h.input_gradient(dy.data_ptr(), dx.data_ptr(), m, dtype=dtype)
+        _check_loss(dtype, (loss, lse, dl), _loss_ref(x, W, t, ones))
+        D = dy.double()
+        _check_dx(dx, dtype, D @ W.T + 2.0 * (D @ B64.T) @ A64.T, D.abs() @ W.abs().T + 4.0 * (D.abs() @ B64.abs().T) @ A64.abs().T)
+        if not sc.any():
+            assert not dl.any()
+    assert session.device_status(0) == 0
+
+
+def test_buffers_of_more_than_2_31_elements(session, cuda):
+    """70001 rows of 32800 (and 65 of the last rows against 64 bits): bytes and elements past 32 bits in X, its 8-bit form,
+    dY and dX of every training call."""
+    import torch
+    m, wide, few, rank = 70001, 32800, 32, 2
+    last = slice(m - 65, m)
+    big = torch.empty((m, wide), dtype=torch.bfloat16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    for i in range(0, m, 10000):
+        big[i:i + 10000] = torch.randn(big[i:i + 10000].shape, device=cuda, generator=gen)
+    t = torch.randint(0, few, (m,), device=cuda)
+    codes, exps = torch.empty((m, wide), dtype=torch.int8, device=cuda), torch.empty((m, wide // 32), dtype=torch.uint8, device=cuda)
+    out = torch.zeros_like(big)
+    session.act8_pack_device(big.data_ptr(), codes.data_ptr(), exps.data_ptr(), m, wide, dtype="bf16")
+    session.act8_unpack_device(codes.data_ptr(), exps.data_ptr(), out.data_ptr(), m, wide, dtype="bf16")
+    c, e = _act8_oracle(big[last].float().cpu().numpy())
+    assert np.array_equal(codes[last].cpu().numpy(), c) and np.array_equal(exps[last].cpu().numpy(), e)
+    for i in range(0, m, 10000):
+        step = torch.exp2(exps[i:i + 10000].float() - 127).repeat_interleave(32, 1)
+        assert torch.equal(out[i:i + 10000].float(), codes[i:i + 10000].float() * step)
+        assert ((out[i:i + 10000].float() - big[i:i + 10000].float()).abs() <= step / 2).all()
+    rng = np.random.default_rng(3)
+    # X wide: the adapter's gradients (every row counts) and the loss
+    packed, scales = _weights(wide, few, 93)
+    A, B = (rng.standard_normal(s).astype(np.float32) * 0.02 for s in ((wide, rank), (rank, few)))
+    dy = _randn((m, few), cuda, 4).bfloat16()
+    da, db = torch.empty((wide, rank), device=cuda), torch.empty((rank, few), device=cuda)
+    loss, lse = torch.empty((m,), device=cuda), torch.empty((m,), device=cuda)
+    with session.weights(packed, scales, wide, few) as h:
+        h.cross_entropy(big.data_ptr(), t.data_ptr(), loss.data_ptr(), m, lse=lse.data_ptr(), dx=out.data_ptr(), dtype="bf16")
+        h.set_lora(A, B, float(rank))
+        h.lora_backward_act8(codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m, dtype="bf16", da=da.data_ptr(), db=db.data_ptr())
+    ref = _loss_ref(big[last], _w64(packed, scales, wide, few, cuda), t[last], torch.ones((65,), device=cuda))
+    _check_loss("bf16", (loss[last], lse[last], out[last]), ref)
+    A64, B64 = torch.from_numpy(A).to(cuda).double(), torch.from_numpy(B).to(cuda).double()
+    ra, Sa, rb, Sb = torch.zeros_like(A64), torch.zeros_like(A64), torch.zeros_like(B64), torch.zeros_like(B64)
+    for i in range(0, m, 5000):
+        X = codes[i:i + 5000].double() * torch.exp2(exps[i:i + 5000].double() - 127).repeat_interleave(32, 1)
+        D = dy[i:i + 5000].double()
+        ra += X.T @ (D @ B64.T)
+        rb += (X @ A64).T @ D
+        X.abs_()
+        Sa += X.T @ (D.abs() @ B64.abs().T)
+        Sb += (X @ A64.abs()).T @ D.abs()
+    for got, r, S in ((da, ra, Sa), (db, rb, Sb)):
+        assert ((got.double() - r).abs() <= 2 * 2.0 ** -16 * S).all()
+    del codes, exps
+    # dY wide, in blocks of rows; then dX wide
+    packed, scales = _weights(few, wide, 95)
+    dx = torch.empty((m, few), dtype=torch.bfloat16, device=cuda)
+    with session.weights(packed, scales, few, wide) as h:
+        h.input_gradient(big.data_ptr(), dx.data_ptr(), m, dtype="bf16")
+    W, D = _w64(packed, scales, few, wide, cuda), big[last].double()
+    _check_dx(dx[last], "bf16", D @ W.T, D.abs() @ W.abs().T)
+    packed, scales = _weights(wide, few, 93)
+    with session.weights(packed, scales, wide, few) as h:
+        h.input_gradient(dy.data_ptr(), out.data_ptr(), m, dtype="bf16")
+    W, D = _w64(packed, scales, wide, few, cuda), dy[last].double()
+    _check_dx(out[last], "bf16", D @ W.T, D.abs() @ W.abs().T)
+    assert session.device_status(0) == 0
