@@ -185,7 +185,10 @@ int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_
  * handle's columns and adapter (if one is attached), dY [m x (col_end -
  * col_begin)], both of `dtype`, 16-byte aligned, m <= 2^24.  For a
  * column shard dX is this shard's partial sum.  fp32 at fp32-level accuracy;
- * bf16 products of f16 operands summed in fp32, rounded once. */
+ * bf16 products of f16 operands (W rounded to 11 bits) summed in fp32, rounded
+ * once.  Above 8 rows operands are kept down to 2^-39 of the largest of their
+ * row, or of all weights.  A row of dY with an infinity or a NaN gives a row of
+ * infinities and NaN (which of the two may differ from exact arithmetic's). */
 int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy, void* dx, int dtype, uint32_t m,
                                         void* stream);
 /* Softmax cross entropy of the logits z = X * dequant(W) over the handle's
@@ -197,7 +200,9 @@ int spaceslug_q4_weights_input_gradient(spaceslug_q4_weights* w, const void* dy,
  * row_scale fp32 [m] (the upstream gradient of each row's loss; NULL: all 1);
  * loss fp32 [m]; lse fp32 [m] or NULL; dx or NULL (the loss alone).  A negative
  * target takes its row out: loss 0, dx 0 (lse is still written).  A target past
- * the columns gives NaN in its row's loss and dx.  dx may be x itself.  m <= 2^24;
+ * the columns gives NaN in its row's loss and dx.  dx may be x itself.  loss and
+ * lse at fp32-level accuracy in both types; in dx a probability counts down to
+ * 2^-39 of the largest of its 256 columns.  m <= 2^24;
  * device pointers, asynchronous on `stream`.  Scratch, here and for
  * input_gradient, from the stream-ordered pool (which keeps it for later calls):
  * the logits live there for a block of rows at a time, as fp32 (m <= 8) or as the

@@ -20,9 +20,9 @@
 // bf16 planes in tensor memory, 32 + 6 KB and twelve MMAs per stage, so that T
 // and G, dA and dB stay one launch each.  Higher ranks leave tensor memory no
 // room for that; their dY goes through lora_tc.cu.  (M x K x N, rank, the whole
-// backward this way and with lora_tc.cu: 128 x 64 x 256, 4: 22 and 28 us; 512 x
-// 4096 x 4096, 16: 32 and 43; 2048 x 4096 x 4096: 48 and 60; 4096 x 4096 x
-// 11008: 118 and 125.)
+// backward in a CUDA graph this way and with lora_tc.cu: 128 x 64 x 256, 4: 12.9
+// and 18.2 us; 7 x 4096 x 4096, 16: 21.0 and 27.2; 512 x 4096 x 4096: 23.6 and 32.1;
+// 2048 x 4096 x 4096: 39.4 and 47.9; 4096 x 4096 x 11008: 109 and 115.)
 //
 //  - T and G read the wide operand with its rows as rows of D: TMA boxes of
 //    128 rows x 64 l (bf16 128-byte swizzled, codes 64-byte swizzled).

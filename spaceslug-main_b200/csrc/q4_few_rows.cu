@@ -15,13 +15,13 @@
 // are one lane's (its n) and go from registers to tensor memory; the transposed
 // product contracts over n and takes them from shared memory, MN-major (128 n x
 // 128 k as two images of 128 rows of 128 bytes, 128-byte swizzled).  With the
-// logits' operand in shared memory too, fp32 logits of 32 x 2048 x 50000 took 72
-// us instead of 62.
+// logits' operand in shared memory too, the fp32 loss of 32 x 2048 x 50000 (its
+// cast and statistics included, calls in a loop) took 72 us instead of 62.
 //
 // What bounds it is the dequantisation beside everything else an SM issues: a
 // block of 128 n x 128 k takes about 1600 cycles (logits) or 1900 (transposed,
 // fp32), with 60% and 57% of the issue slots, a fifth of the tensor pipe and a
-// quarter of HBM's bandwidth in use (32 x 2048 x 50000: 47 and 52 us, ncu).  Tried and slower: stages of half a block,
+// quarter of HBM's bandwidth in use (32 x 2048 x 50000: 48 and 53 us by ncu, one launch).  Tried and slower: stages of half a block,
 // a second MMA warp with an accumulator per block, one lane per warp polling.
 //
 // Roles (28 warps): warp 0 loads the rows' planes, warp 2 packed words and

@@ -990,10 +990,11 @@ def test_a_handle_that_only_infers_holds_its_weights_alone(session, cuda):
 
 
 @pytest.mark.parametrize("k", [32, 96, 416])
-@pytest.mark.parametrize("first", ["captured", "eager", "two_streams"])
+@pytest.mark.parametrize("first", ["captured", "eager", "two_streams", "two_threads"])
 def test_first_training_call_of_a_handle(session, cuda, k, first):
     """The padded scales of a first call: captured (its graph makes its own, and so does a second graph), eager, or from
-    two streams at once; the same results each way, and a graph of before works beside the handle's copy."""
+    two streams or threads at once; the same results each way, and a graph of before works beside the handle's copy."""
+    import threading
     import torch
     m, n = 20, 777
     packed, scales = _weights(k, n, 73)
@@ -1022,6 +1023,12 @@ def test_first_training_call_of_a_handle(session, cuda, k, first):
             for g, s in zip(graphs, st):
                 with torch.cuda.stream(s):
                     g.replay()
+        elif first == "two_threads":
+            threads = [threading.Thread(target=run, args=v) for v in zip(outs, st)]
+            for v in threads:
+                v.start()
+            for v in threads:
+                v.join()
         else:
             for o, s in zip(outs, st if first == "two_streams" else st[:1] * 2):
                 run(o, s)
