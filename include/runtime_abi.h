@@ -144,7 +144,9 @@ int spaceslug_q4_weights_lora_backward(spaceslug_q4_weights* w, const float* x, 
 int spaceslug_q4_weights_lora_sgd(spaceslug_q4_weights* w, float learning_rate, void* stream);
 /* AdamW with decoupled weight decay and bias-corrected moments (kept in the
  * handle; set_lora resets them):  m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,
- * p -= lr * ((m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps) + wd * p). */
+ * p -= lr * ((m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps) + wd * p).  t counts on
+ * the device: each replay of a captured call is a step (of the captured
+ * rates).  The first call allocates the moments and is refused in a capture. */
 int spaceslug_q4_weights_lora_adamw(spaceslug_q4_weights* w, float learning_rate, float beta1, float beta2, float eps,
                                     float weight_decay, void* stream);
 /* Host copies of the adapter and its last gradients (any output may be NULL);
@@ -178,7 +180,8 @@ int spaceslug_act8_unpack_device(const int8_t* codes, const uint8_t* exps, void*
  * 16-byte aligned.  The gradients (fp32) stay in the handle as there; da
  * [k x rank] and db [rank x columns], where given (device pointers), receive a
  * copy.  The first backward of a handle allocates its gradients: make it before
- * any stream capture. */
+ * any stream capture.  A captured graph names the handle's buffers: after
+ * set_lora it must be captured again. */
 int spaceslug_q4_weights_lora_backward_act8(spaceslug_q4_weights* w, const int8_t* codes, const uint8_t* exps,
                                             const void* dy, int dtype, uint32_t m, float* da, float* db, void* stream);
 /* dX = dY * dequant(W)^T + (alpha / rank) * (dY * B^T) * A^T [m x k] for the

@@ -16,7 +16,6 @@
 // [C][r] (dA).  sgd_kernel / adamw_kernel update a parameter array in place.
 #include <cuda_runtime.h>
 
-#include <cmath>
 #include <cstdint>
 
 #include "q4_kernels.h"
@@ -88,10 +87,19 @@ __global__ void __launch_bounds__(256) sgd_kernel(float* __restrict__ p, const f
 }
 
 // AdamW (decoupled weight decay), bias-corrected moments; c1 = 1 - beta1^t, c2 = 1 - beta2^t.
+// The step count t and its bias corrections 1 - beta^t, kept on the device so
+// that a step in a replayed CUDA graph counts as one.
+__global__ void adamw_step_kernel(AdamWState* state, float beta1, float beta2) {
+    const int t = ++state->t;
+    state->c1 = 1.0f - static_cast<float>(pow(static_cast<double>(beta1), static_cast<double>(t)));
+    state->c2 = 1.0f - static_cast<float>(pow(static_cast<double>(beta2), static_cast<double>(t)));
+}
+
 __global__ void __launch_bounds__(256) adamw_kernel(float* __restrict__ p, const float* __restrict__ g,
                                                     float* __restrict__ m1, float* __restrict__ m2, float lr,
-                                                    float beta1, float beta2, float eps, float wd, float c1, float c2,
-                                                    long long count) {
+                                                    float beta1, float beta2, float eps, float wd,
+                                                    const AdamWState* __restrict__ state, long long count) {
+    const float c1 = state->c1, c2 = state->c2;
     const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= count) return;
     const float gi = g[i];
@@ -155,12 +163,15 @@ int launch_sgd(float* p, const float* g, float lr, long long count, cudaStream_t
     return static_cast<int>(cudaGetLastError());
 }
 
+int launch_adamw_step(AdamWState* state, float beta1, float beta2, cudaStream_t stream) {
+    adamw_step_kernel<<<1, 1, 0, stream>>>(state, beta1, beta2);
+    return static_cast<int>(cudaGetLastError());
+}
+
 int launch_adamw(float* p, const float* g, float* m1, float* m2, float lr, float beta1, float beta2, float eps,
-                 float wd, int step, long long count, cudaStream_t stream) {
+                 float wd, const AdamWState* state, long long count, cudaStream_t stream) {
     if (count <= 0) return 0;
-    const float c1 = 1.0f - std::pow(beta1, static_cast<float>(step));
-    const float c2 = 1.0f - std::pow(beta2, static_cast<float>(step));
-    adamw_kernel<<<blocks(count, 256), 256, 0, stream>>>(p, g, m1, m2, lr, beta1, beta2, eps, wd, c1, c2, count);
+    adamw_kernel<<<blocks(count, 256), 256, 0, stream>>>(p, g, m1, m2, lr, beta1, beta2, eps, wd, state, count);
     return static_cast<int>(cudaGetLastError());
 }
 

@@ -269,8 +269,15 @@ struct LoraTcFinalize {
 };
 int launch_lora_tc_finalize(const LoraTcFinalize* f, int count, int rp, cudaStream_t stream);
 int launch_sgd(float* p, const float* g, float lr, long long count, cudaStream_t stream);
+// AdamW's step count and bias corrections on the device: launch_adamw_step counts one step, launch_adamw updates `count`
+// parameters by it.
+struct AdamWState {
+    int t;
+    float c1, c2;
+};
+int launch_adamw_step(AdamWState* state, float beta1, float beta2, cudaStream_t stream);
 int launch_adamw(float* p, const float* g, float* m1, float* m2, float lr, float beta1, float beta2, float eps,
-                 float wd, int step, long long count, cudaStream_t stream);
+                 float wd, const AdamWState* state, long long count, cudaStream_t stream);
 // fp32 GEMM on tcgen05 with 3xTF32 (sgemm_tc.cu).  The operands are first
 // split into TF32 hi / lo planes in K-major layout ([out_rows][ld] fp32, K
 // contiguous): launch_split_planes writes the planes of a row-major

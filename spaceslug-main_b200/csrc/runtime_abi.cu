@@ -984,8 +984,7 @@ struct spaceslug_q4_weights {
     // training state (allocated on first use, reset by set_lora)
     float* lora_da = nullptr;
     float* lora_db = nullptr;
-    float* adam = nullptr;  // first and second moments of A then of B: 2 * (K*r + r*N)
-    int adam_step = 0;
+    float* adam = nullptr;  // first and second moments of A then of B: 2 * (K*r + r*N), and the step count (AdamWState)
 };
 
 // What the training products need beside a handle's words and scales from its
@@ -2150,7 +2149,6 @@ int spaceslug_q4_weights_set_lora(spaceslug_q4_weights* w, const float* lora_a, 
         cudaFree(w->lora_db);
         cudaFree(w->adam);
         w->lora_a = w->lora_b = w->lora_da = w->lora_db = w->adam = nullptr;
-        w->adam_step = 0;
         w->rank = 0;
         if (rank == 0) return SPACESLUG_OK;
         // lora_b is the full [rank x n_total] matrix; keep the handle's columns.
@@ -2682,15 +2680,22 @@ int spaceslug_q4_weights_lora_adamw(spaceslug_q4_weights* w, float learning_rate
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
         const long long na = static_cast<long long>(w->K) * w->rank, nb = static_cast<long long>(w->rank) * w->N;
         if (!w->adam) {
-            check(cudaMalloc(&w->adam, static_cast<size_t>(2 * (na + nb)) * 4), "cudaMalloc AdamW moments");
-            check(cudaMemsetAsync(w->adam, 0, static_cast<size_t>(2 * (na + nb)) * 4, s), "cudaMemset moments");
+            // captured, the zeros would be written again by every replay
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            check(cudaStreamIsCapturing(s, &capture), "cudaStreamIsCapturing");
+            if (capture != cudaStreamCaptureStatusNone)
+                return fail(SPACESLUG_INVALID_ARGUMENT, "the first AdamW step allocates its moments: make it before a capture");
+            const size_t bytes = static_cast<size_t>(2 * (na + nb)) * 4 + sizeof(q4::AdamWState);
+            check(cudaMalloc(&w->adam, bytes), "cudaMalloc AdamW moments");
+            check(cudaMemsetAsync(w->adam, 0, bytes, s), "cudaMemset moments");
         }
-        ++w->adam_step;
+        auto* state = reinterpret_cast<q4::AdamWState*>(w->adam + 2 * (na + nb));
+        check_launch(q4::launch_adamw_step(state, beta1, beta2, s), "adamw step");
         check_launch(q4::launch_adamw(w->lora_a, w->lora_da, w->adam, w->adam + na, learning_rate, beta1, beta2, eps,
-                                      weight_decay, w->adam_step, na, s),
+                                      weight_decay, state, na, s),
                      "adamw A");
         check_launch(q4::launch_adamw(w->lora_b, w->lora_db, w->adam + 2 * na, w->adam + 2 * na + nb, learning_rate,
-                                      beta1, beta2, eps, weight_decay, w->adam_step, nb, s),
+                                      beta1, beta2, eps, weight_decay, state, nb, s),
                      "adamw B");
         return SPACESLUG_OK;
     });

@@ -1317,3 +1317,48 @@ def test_buffers_of_more_than_2_31_elements(session, cuda):
     W, D = _w64(packed, scales, wide, few, cuda), dy[last].double()
     _check_dx(out[last], "bf16", D @ W.T, D.abs() @ W.abs().T)
     assert session.device_status(0) == 0
+
+
+def test_a_captured_adamw_step_counts_its_replays(session, cuda):
+    """Backward and AdamW replayed four times after two eager steps against six eager steps of another handle: the same
+    adapter bit for bit, and a first step refused in a capture, which goes on."""
+    import torch
+    m, k, n, rank = 40, 96, 130, 4
+    packed, scales = _weights(k, n, 103)
+    rng = np.random.default_rng(4)
+    A, B = (rng.standard_normal(s).astype(np.float32) * 0.1 for s in ((k, rank), (rank, n)))
+    codes, exps, _ = _act8(session, _randn((m, k), cuda, 1), "f32")
+    dy = _randn((m, n), cuda, 2)
+    st = torch.cuda.Stream(cuda)
+    with session.weights(packed, scales, k, n) as h, session.weights(packed, scales, k, n) as g:
+        def step(w, lr=1e-2):
+            w.lora_backward_act8(codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m, stream=st.cuda_stream)
+            w.lora_adamw(lr, stream=st.cuda_stream)
+
+        adamw = session.raw("spaceslug_q4_weights_lora_adamw")
+        for w in (h, g):
+            w.set_lora(A, B, 2.0 * rank)
+        torch.cuda.synchronize()
+        for _ in range(6):
+            step(g)
+        h.lora_backward_act8(codes.data_ptr(), exps.data_ptr(), dy.data_ptr(), m, stream=st.cuda_stream)
+        first = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first, stream=st):
+            dy.mul_(1.0)
+            assert adamw(h.handle, 1e-2, 0.9, 0.999, 1e-8, 0.0, st.cuda_stream) == 1
+        assert b"before a capture" in session._native().spaceslug_last_error()
+        step(h)
+        step(h)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            step(h)
+        with torch.cuda.stream(st):
+            for _ in range(4):
+                graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(h.get_lora(rank), g.get_lora(rank)):
+            assert a is None or np.array_equal(a, b)
+        # six steps of one constant-sign gradient move a parameter by about six rates
+        assert np.abs(h.get_lora(rank)[0] - A).max() > 5e-2
+        del first, graph
+    assert session.device_status(0) == 0
