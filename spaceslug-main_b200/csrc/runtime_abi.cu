@@ -1419,33 +1419,24 @@ struct TrainWeights {
         return true;
     }
     // The handle's padded scales.  The first call makes them and waits, so that calls on any stream may read them; a
-    // call that is captured before that (no allocation there) copies them within its graph.
+    // call that is captured before that copies them within its graph.  (Stream-ordered memory: no allocation that
+    // another thread's capture would forbid.)
     const float* padded_scales(cudaStream_t s) {
         const size_t G = static_cast<size_t>(w->K) / 32, Gp = (G + 3) / 4 * 4, N = static_cast<size_t>(w->N);
         if (G == Gp) return w->scales;
-        auto pad = [&](void* to) {
-            check(cudaMemcpy2DAsync(to, Gp * 4, w->scales, G * 4, G * 4, N, cudaMemcpyDeviceToDevice, s),
-                  "cudaMemcpy2D padded scales");
-        };
         std::lock_guard<std::mutex> lk(w->pad_mu);
         if (w->scales_pad) return w->scales_pad;
+        check(cudaMallocAsync(&own_scales.p, N * Gp * 4, s), "cudaMallocAsync padded scales");
+        check(cudaMemcpy2DAsync(own_scales.p, Gp * 4, w->scales, G * 4, G * 4, N, cudaMemcpyDeviceToDevice, s),
+              "cudaMemcpy2D padded scales");
+        const float* made = static_cast<const float*>(own_scales.p);
         cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(s, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
-            cudaGetLastError();
-            check(cudaMallocAsync(&own_scales.p, N * Gp * 4, s), "cudaMallocAsync padded scales");
-            pad(own_scales.p);
-            return static_cast<const float*>(own_scales.p);
-        }
-        void* made = nullptr;
-        check(cudaMalloc(&made, N * Gp * 4), "cudaMalloc padded scales");
-        try {
-            pad(made);
-            check(cudaStreamSynchronize(s), "cudaStreamSynchronize");
-        } catch (...) {
-            cudaFree(made);
-            throw;
-        }
-        return w->scales_pad = static_cast<float*>(made);
+        check(cudaStreamIsCapturing(s, &capture), "cudaStreamIsCapturing");
+        if (capture != cudaStreamCaptureStatusNone) return made;
+        check(cudaStreamSynchronize(s), "cudaStreamSynchronize");
+        w->scales_pad = static_cast<float*>(own_scales.p);
+        own_scales.p = nullptr;  // the handle's now
+        return made;
     }
     // tensor maps of the logits' or the transposed product
     template <typename Args>
